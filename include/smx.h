@@ -195,6 +195,70 @@ SMX_API int smx_sample(const float *logits_dev, int n, const int32_t *context_de
                        const smx_sampling *params, double u, float *probs_dev, int32_t *token_dev,
                        void *stream);
 
+/* ---- serving operators: 8-bit KV cache, attention over it, drafted tokens ----------------------
+ * For hosts that keep their own forward pass and serve several sequences.  The reference has no counterpart:
+ * its caches are fp32 (TransformerModel.cs:476-506), one per session, and it decodes one token at a time.
+ *
+ * A cache holds n_slots sequences of up to ctx positions on the current device.  A row, the head_dim
+ * values of one position's K or V in one KV head, is kept as one Q8Tensor block (Q8Tensor.cs:72-128):
+ * scale = max |x| / 127 (fp32), codes = the integers nearest to x / scale, ties to even.  A row that holds a
+ * NaN or an infinity reads back as NaN in every element.  head_dim: a multiple of 8 up to 256.  The
+ * memory's layout is the library's own.  Calls on one cache are ordered by their streams as accesses to
+ * one buffer are; the library holds no other state for them, and every call can be captured into a graph. */
+typedef struct smx_kv_cache smx_kv_cache;
+SMX_API int smx_kv_cache_create(int n_slots, int n_kv_head, int head_dim, int ctx, smx_kv_cache **out);
+/* Any of the pointers may be NULL; bytes: device memory of the cache. */
+SMX_API int smx_kv_cache_info(const smx_kv_cache *c, int *n_slots, int *n_kv_head, int *head_dim, int *ctx,
+                              int64_t *bytes);
+SMX_API int smx_kv_cache_destroy(smx_kv_cache *c);
+/* Writes the rows of n_tok tokens: token t's K at k_dev + t * k_stride and V at v_dev + t * v_stride, each
+ * [n_kv_head][head_dim] (strides in floats, so both may lie in the rows of a fused projection), to position
+ * pos_dev[t] of slot slots_dev[t].  A token whose slot or position the cache does not have (-1, say, in
+ * a padded batch) is not written.  A place named twice in one call is left with undefined contents. */
+SMX_API int smx_kv_append(smx_kv_cache *c, const float *k_dev, int64_t k_stride, const float *v_dev, int64_t v_stride,
+                          const int32_t *slots_dev, const int32_t *pos_dev, int n_tok, void *stream);
+/* Reads rows back: k_dev, v_dev [n_tok][n_kv_head][head_dim].  Places that the cache does not have, and
+ * positions never written, give zeros. */
+SMX_API int smx_kv_read(const smx_kv_cache *c, const int32_t *slots_dev, const int32_t *pos_dev, int n_tok, float *k_dev,
+                        float *v_dev, void *stream);
+/* Bytes of work memory that an attention call of these sizes needs (prefix_len 0: smx_attention_cached). */
+SMX_API int smx_attention_work_bytes(const smx_kv_cache *c, int n_seq, int n_q, int n_head, int prefix_len, int max_len,
+                                     int64_t *bytes);
+/* Attention of the last n_q tokens of each of n_seq sequences over the cache (MultiHeadAttention.cs:676-844 with
+ * the exponential itself in place of FastExp).  Sequence b's positions are the first lens_dev[b] of slot
+ * slots_dev[b], its n_q tokens (already appended) among them; token i sees all up to itself, the first
+ * lens_dev[b] - n_q + 1 + i.  One token each: decode; several: drafted tokens.  q: token i of sequence b at
+ * q_dev + (b * n_q + i) * q_stride, [n_head][head_dim]; out_dev [n_seq][n_q][n_head][head_dim]; scores
+ * are scaled by 1 / sqrt(head_dim); n_head a multiple of n_kv_head.  max_len: at least every length (a
+ * greater one counts as max_len); a tight bound saves workgroups.  A row that sees nothing, and the rows
+ * of a sequence whose slot the cache does not have, are zeros.  work_dev: smx_attention_work_bytes bytes,
+ * free for other use when the call's work is done; calls that may overlap, replays of captured graphs among
+ * them, need one each. */
+SMX_API int smx_attention_cached(const smx_kv_cache *c, const float *q_dev, int64_t q_stride, float *out_dev, int n_seq,
+                                 int n_q, int n_head, const int32_t *slots_dev, const int32_t *lens_dev, int max_len,
+                                 void *work_dev, int64_t work_bytes, void *stream);
+/* The same for sequences that begin with one prefix: every token sees the first prefix_len positions of slot
+ * prefix_slot, then its sequence's own (lens_dev counts those alone and may be 0).  The prefix is read
+ * once for all of them. */
+SMX_API int smx_attention_shared(const smx_kv_cache *c, const float *q_dev, int64_t q_stride, float *out_dev, int n_seq,
+                                 int n_q, int n_head, int prefix_slot, int prefix_len, const int32_t *slots_dev,
+                                 const int32_t *lens_dev, int max_len, void *work_dev, int64_t work_bytes, void *stream);
+/* Verification of drafted tokens against the target model (speculative decoding).  Of sequence b, with
+ * n = lens_dev[b] drafted tokens (at most n_draft; n_draft for all when lens_dev is NULL): target_dev holds the
+ * n_draft + 1 rows of probabilities p_i (vocab floats, rows target_stride apart; smx_sample's probs are such a
+ * row), draft_dev the n_draft rows q_i that the tokens tokens_dev[b][i] were drawn from (NULL: tokens
+ * chosen without a distribution, q_i = 1 at the token).  Token x_i is accepted if u_accept_dev[b][i] * q_i(x_i) <
+ * p_i(x_i), up to the first that is not; then one token is drawn: at a refused one from max(p_i - q_i, 0)
+ * (from p_i where nothing is left of that), otherwise from p_n, as the lowest token of positive weight at
+ * which the running sum exceeds u_draw_dev[b] times the whole.  Uniform numbers in [0, 1).  out_dev
+ * [n_seq][n_draft + 1]: the accepted tokens, the drawn one (-1 if every weight is 0), then -1;
+ * accepted_dev [n_seq]: how many were accepted.  A negative length marks an empty place: -1 throughout,
+ * none accepted.  A NaN probability counts as 0, a token outside the vocabulary is refused. */
+SMX_API int smx_verify_draft(const float *target_dev, int64_t target_stride, const float *draft_dev, int64_t draft_stride,
+                             const int32_t *tokens_dev, const int32_t *lens_dev, const float *u_accept_dev,
+                             const float *u_draw_dev, int n_seq, int n_draft, int vocab, int32_t *out_dev,
+                             int32_t *accepted_dev, void *stream);
+
 /* ---- model / session level --------------------------------------------------------------- */
 typedef struct smx_context smx_context;
 typedef struct smx_model smx_model;

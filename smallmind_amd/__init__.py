@@ -2,7 +2,8 @@
 
 Layers (see include/smx.h for the C-ABI the reference's C# code would bind):
   quantization  IWeightTensor mirror (GpuWeightTensor) + dequant / quantize / norm / RoPE /
-                softmax / attention / activation operators
+                softmax / attention / activation operators; 8-bit KV cache (GpuKvCache) with
+                batched and shared-prefix attention, verification of drafted tokens
   model         GpuTransformerModel (TransformerModel.Forward + KV cache) and
                 GpuInferenceSession (prefill + greedy decode on the device)
   synthetic     seeded workloads of the benchmark configurations
@@ -14,7 +15,7 @@ from . import _lib
 _lib.load()
 
 from .model import GpuContext, GpuInferenceSession, GpuTransformerModel, ModelConfig  # noqa: E402
-from .quantization import GgufTensorType, GpuWeightTensor, SmxError  # noqa: E402
+from .quantization import GgufTensorType, GpuKvCache, GpuWeightTensor, SmxError  # noqa: E402
 
 __all__ = ["GpuContext", "GpuInferenceSession", "GpuTransformerModel", "ModelConfig",
-           "GgufTensorType", "GpuWeightTensor", "SmxError"]
+           "GgufTensorType", "GpuKvCache", "GpuWeightTensor", "SmxError"]

@@ -36,6 +36,8 @@ EXPORTS = [
     "smx_smq_read_config", "smx_smq_pack", "smx_sample",
     "smx_session_generate_sampled", "smx_batcher_create", "smx_batcher_add", "smx_batcher_add_sampled", "smx_batcher_remove",
     "smx_batcher_count", "smx_batcher_step", "smx_batcher_destroy",
+    "smx_kv_cache_create", "smx_kv_cache_info", "smx_kv_cache_destroy", "smx_kv_append", "smx_kv_read",
+    "smx_attention_work_bytes", "smx_attention_cached", "smx_attention_shared", "smx_verify_draft",
 ]
 
 
@@ -129,6 +131,15 @@ def load() -> ctypes.CDLL:
         "smx_argmax": (i32, [vp, i32, vp, vp]),
         "smx_stream_read": (i32, [vp, u64, vp]),
         "smx_sample": (i32, [vp, i32, vp, i32, ctypes.POINTER(SamplingC), ctypes.c_double, vp, vp, vp]),
+        "smx_kv_cache_create": (i32, [i32, i32, i32, i32, pp]),
+        "smx_kv_cache_info": (i32, [vp, vp, vp, vp, vp, vp]),
+        "smx_kv_cache_destroy": (i32, [vp]),
+        "smx_kv_append": (i32, [vp, vp, i64, vp, i64, vp, vp, i32, vp]),
+        "smx_kv_read": (i32, [vp, vp, vp, i32, vp, vp, vp]),
+        "smx_attention_work_bytes": (i32, [vp, i32, i32, i32, i32, i32, ctypes.POINTER(ctypes.c_int64)]),
+        "smx_attention_cached": (i32, [vp, vp, i64, vp, i32, i32, i32, vp, vp, i32, vp, i64, vp]),
+        "smx_attention_shared": (i32, [vp, vp, i64, vp, i32, i32, i32, i32, i32, vp, vp, i32, vp, i64, vp]),
+        "smx_verify_draft": (i32, [vp, i64, vp, i64, vp, vp, vp, vp, i32, i32, i32, vp, vp, vp]),
         "smx_context_create": (i32, [i32, pp]),
         "smx_context_destroy": (i32, [vp]),
         "smx_model_create": (i32, [vp, ctypes.POINTER(ModelConfigC), pp]),

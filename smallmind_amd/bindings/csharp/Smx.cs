@@ -91,6 +91,28 @@ namespace SmallMind.Backends.Rocm
         [DllImport(Lib)] public static extern int smx_sample(float* logitsDev, int n, int* contextDev, int nContext,
             in Sampling p, double u, float* probsDev, int* tokenDev, IntPtr stream);
 
+        // 8-bit KV cache, attention over it, verification of drafted tokens (device pointers)
+        [DllImport(Lib)] public static extern int smx_kv_cache_create(int nSlots, int nKvHead, int headDim, int ctx,
+            out IntPtr cache);
+        [DllImport(Lib)] public static extern int smx_kv_cache_info(IntPtr cache, int* nSlots, int* nKvHead, int* headDim,
+            int* ctx, long* bytes);
+        [DllImport(Lib)] public static extern int smx_kv_cache_destroy(IntPtr cache);
+        [DllImport(Lib)] public static extern int smx_kv_append(IntPtr cache, float* kDev, long kStride, float* vDev,
+            long vStride, int* slotsDev, int* posDev, int nTok, IntPtr stream);
+        [DllImport(Lib)] public static extern int smx_kv_read(IntPtr cache, int* slotsDev, int* posDev, int nTok,
+            float* kDev, float* vDev, IntPtr stream);
+        [DllImport(Lib)] public static extern int smx_attention_work_bytes(IntPtr cache, int nSeq, int nQ, int nHead,
+            int prefixLen, int maxLen, out long bytes);
+        [DllImport(Lib)] public static extern int smx_attention_cached(IntPtr cache, float* qDev, long qStride,
+            float* outDev, int nSeq, int nQ, int nHead, int* slotsDev, int* lensDev, int maxLen, void* workDev,
+            long workBytes, IntPtr stream);
+        [DllImport(Lib)] public static extern int smx_attention_shared(IntPtr cache, float* qDev, long qStride,
+            float* outDev, int nSeq, int nQ, int nHead, int prefixSlot, int prefixLen, int* slotsDev, int* lensDev,
+            int maxLen, void* workDev, long workBytes, IntPtr stream);
+        [DllImport(Lib)] public static extern int smx_verify_draft(float* targetDev, long targetStride, float* draftDev,
+            long draftStride, int* tokensDev, int* lensDev, float* uAcceptDev, float* uDrawDev, int nSeq, int nDraft,
+            int vocab, int* outDev, int* acceptedDev, IntPtr stream);
+
         // model and sessions
         [DllImport(Lib)] public static extern int smx_context_create(int device, out IntPtr ctx);
         [DllImport(Lib)] public static extern int smx_context_destroy(IntPtr ctx);

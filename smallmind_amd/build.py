@@ -22,11 +22,14 @@ HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 # prefill 62.6-63.1K -> 66.1-66.4K tok/s, configs[4] +2.2 %; same results).
 MFMA_VGPR = ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]
 
-# (source, object name, extra flags); the GEMV is built once per block format so its
-# instantiations compile in parallel.
+# (source, object name, extra flags); the GEMV is built once per block format, the attention
+# over the 8-bit cache once per row width, so their instantiations compile in parallel.
 SOURCES = [("k_quant.hip", "k_quant", []), ("k_ops.hip", "k_ops", []), ("runtime.cpp", "runtime", []),
            ("gemv_dispatch.cpp", "gemv_dispatch", []), ("k_qgemm.hip", "k_qgemm", MFMA_VGPR),
-           ("k_attn_prefill.hip", "k_attn_prefill", MFMA_VGPR), ("gguf.cpp", "gguf", []), ("smq.cpp", "smq", []), ("host_common.cpp", "host_common", []), ("k_sample.hip", "k_sample", [])] + [
+           ("k_attn_prefill.hip", "k_attn_prefill", MFMA_VGPR), ("gguf.cpp", "gguf", []), ("smq.cpp", "smq", []), ("host_common.cpp", "host_common", []), ("k_sample.hip", "k_sample", []),
+           ("k_kvcache.hip", "k_kvcache", []), ("k_attn_q8_join.hip", "k_attn_q8_join", []), ("k_verify.hip", "k_verify", []),
+           ("kv_ops.cpp", "kv_ops", [])] + [
+           ("k_attn_q8.hip", f"k_attn_q8_w{w}", [f"-DSMX_ATTN_W={w}", *MFMA_VGPR]) for w in range(32, 257, 32)] + [
            ("k_gemv.hip", f"k_gemv_f{f}", [f"-DSMX_GEMV_FMT={f}"]) for f in range(9)] + [
            ("k_qgemm_tile.hip", f"k_qgemm_tile_f{f}", [f"-DSMX_TILE_FMT={f}", *MFMA_VGPR]) for f in (0, 1, 2, 3, 4, 7, 8)]
 

@@ -1,0 +1,123 @@
+// k_attn_q8_join.hip -- the plan of the attention over the 8-bit KV cache and the sum of its parts.
+#include <math.h>
+
+#include "smx_attn_q8.h"
+#include "smx_device.h"
+#include "smx_internal.h"
+
+namespace smx {
+
+namespace {
+
+// One thread per output element: out = sum_s 2^(m_s - M) acc_s / sum_s 2^(m_s - M) l_s over the parts s that
+// have weight, M their largest m.  Rows of a sequence without a slot are 0.
+__global__ __launch_bounds__(256) void k_attn_q8_join(const AttnQ8Args a)
+{
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= a.n_rows * a.hd) return;
+    const int64_t row = i / a.hd;
+    const int d = (int)(i - row * a.hd);
+    const int seq = (int)(row / ((int64_t)a.n_q * a.n_head));
+    float o = 0.0f, l = 0.0f, top = -__builtin_huge_valf();
+    if ((unsigned)a.slots[seq] < (unsigned)a.n_slots) {
+        for (int s = 0; s < a.parts; s++) top = fmaxf(top, a.part_ml[(s * a.n_rows + row) * 2]);
+        for (int s = 0; s < a.parts; s++) {
+            const float *ml = a.part_ml + (s * a.n_rows + row) * 2;
+            const float m = ml[0], ls = ml[1];
+            if (ls == 0.0f) continue;
+            const float f = __builtin_amdgcn_exp2f(m - top);
+            l += ls * f;
+            o += a.part_acc[(s * a.n_rows + row) * a.hd + d] * f;
+        }
+    }
+    a.out[i] = l == 0.0f ? 0.0f : o / l;
+}
+
+// Chunks of a length that make about `want` workgroups of `units` rows of workgroups: whole multiples of
+// four tiles, one for each wave of a workgroup.
+void cut(int len, int64_t units, int64_t want, int *chunk, int *splits)
+{
+    const int unit = 4 * kKvTile, most = (len + unit - 1) / unit;
+    int64_t n = (want + units - 1) / units;
+    n = n < 1 ? 1 : n > most ? most : n;
+    *chunk = n == 0 ? unit : (int)(((int64_t)len + n - 1) / n + unit - 1) / unit * unit;
+    *splits = (len + *chunk - 1) / *chunk;
+}
+
+// A single part writes the outputs itself, unless it is the prefix, which knows no slots.
+bool attn_q8_direct(const AttnQ8Plan &p) { return p.parts == 1 && p.own_splits == 1; }
+
+}  // namespace
+
+#define SMX_W(w) hipError_t launch_attn_q8_w##w(const AttnQ8Args &a, int mt_own, int mt_pre, unsigned blocks, hipStream_t s);
+SMX_W(32) SMX_W(64) SMX_W(96) SMX_W(128) SMX_W(160) SMX_W(192) SMX_W(224) SMX_W(256)
+#undef SMX_W
+
+AttnQ8Plan attn_q8_plan(const KvView &c, int n_seq, int n_q, int n_head, int prefix_len, int max_len)
+{
+    AttnQ8Plan p{};
+    const int64_t group = n_head / c.n_kv, own_rows = n_q * group, pre_rows = n_seq * own_rows;
+    // two blocks of rows share a wave's codes
+    const bool two = c.w <= 128 ? kAttnQ8TwoBlocks<128> : kAttnQ8TwoBlocks<256>;
+    p.mt_own = two && own_rows > 16 ? 2 : 1;
+    p.mt_pre = two && pre_rows > 16 ? 2 : 1;
+    p.own_blocks = (int)((own_rows + 16 * p.mt_own - 1) / (16 * p.mt_own));
+    p.pre_blocks = (int)((pre_rows + 16 * p.mt_pre - 1) / (16 * p.mt_pre));
+    const int64_t own_units = (int64_t)n_seq * c.n_kv * p.own_blocks, pre_units = (int64_t)c.n_kv * p.pre_blocks;
+    cut(max_len, own_units, 2048, &p.own_chunk, &p.own_splits);
+    cut(prefix_len, pre_units, 2048, &p.pre_chunk, &p.pre_splits);
+    p.parts = p.own_splits + p.pre_splits;
+    p.pre_wgs = pre_units * p.pre_splits;
+    p.blocks = p.pre_wgs + own_units * p.own_splits;
+    const int64_t rows = (int64_t)n_seq * n_q * n_head;
+    p.work_bytes = attn_q8_direct(p) ? 0 : p.parts * rows * (int64_t)(c.hd + 2) * 4;
+    return p;
+}
+
+hipError_t launch_attn_q8(const KvView &c, const AttnQ8Plan &p, const float *q, int64_t q_stride, float *out, int n_seq,
+                          int n_q, int n_head, int prefix_slot, int prefix_len, const int32_t *slots, const int32_t *lens,
+                          int max_len, void *work, hipStream_t s)
+{
+    AttnQ8Args a{};
+    a.q = q;
+    a.out = out;
+    a.cache = c.base;
+    a.head_bytes = (size_t)c.tiles * kv_tile_bytes(c.w);
+    a.slots = slots;
+    a.lens = lens;
+    a.n_rows = (int64_t)n_seq * n_q * n_head;
+    a.part_acc = (float *)work;
+    a.part_ml = work ? (float *)work + p.parts * a.n_rows * c.hd : nullptr;
+    a.q_stride = q_stride;
+    a.scale_log2e = (float)(1.4426950408889634 / sqrt((double)c.hd));
+    a.q_vec = ((uintptr_t)q & 15) == 0 && q_stride % 4 == 0;
+    a.n_slots = c.n_slots;
+    a.n_seq = n_seq;
+    a.n_q = n_q;
+    a.n_head = n_head;
+    a.n_kv = c.n_kv;
+    a.hd = c.hd;
+    a.max_len = max_len;
+    a.own_chunk = p.own_chunk;
+    a.own_splits = p.own_splits;
+    a.own_blocks = p.own_blocks;
+    a.prefix_slot = prefix_slot;
+    a.prefix_len = prefix_len;
+    a.pre_chunk = p.pre_chunk;
+    a.pre_splits = p.pre_splits;
+    a.pre_wgs = (int)p.pre_wgs;
+    a.parts = p.parts;
+    a.direct = attn_q8_direct(p);
+    if (p.blocks) {
+        hipError_t e = hipErrorInvalidValue;
+#define SMX_W(w) case w: e = launch_attn_q8_w##w(a, p.mt_own, p.mt_pre, (unsigned)p.blocks, s); break;
+        switch (c.w) { SMX_W(32) SMX_W(64) SMX_W(96) SMX_W(128) SMX_W(160) SMX_W(192) SMX_W(224) SMX_W(256) }
+#undef SMX_W
+        if (e != hipSuccess) return e;
+    }
+    if (a.direct) return hipSuccess;
+    k_attn_q8_join<<<(unsigned)((a.n_rows * c.hd + 255) / 256), 256, 0, s>>>(a);
+    return hipGetLastError();
+}
+
+}  // namespace smx

@@ -1,0 +1,43 @@
+// smx_attn_q8.h -- arguments of the attention over the 8-bit KV cache.  The kernel is built once per
+// row width (k_attn_q8.hip); the plan, the dispatch and the joining of parts are in k_attn_q8_join.hip.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "smx_kvcache.h"
+
+namespace smx {
+
+// Whether a wave may take two 16-row blocks at rows of this width: wider ones leave registers for one.
+template <int W>
+constexpr bool kAttnQ8TwoBlocks = W <= 128;
+
+struct AttnQ8Args {
+    const float *q;             // token t, head h at t * q_stride + h * hd
+    float *out;                 // [n_seq * n_q][n_head][hd]
+    const uint8_t *cache;
+    size_t head_bytes;          // of one (slot, KV head)
+    const int32_t *slots, *lens;
+    float *part_ml, *part_acc;  // [parts][n_rows][2], [parts][n_rows][hd]
+    int64_t q_stride, n_rows;   // n_rows = n_seq * n_q * n_head
+    float scale_log2e;          // log2(e) / sqrt(hd)
+    int q_vec;                  // rows of q may be read as float4
+    int n_slots, n_seq, n_q, n_head, n_kv, hd;
+    int max_len, own_chunk, own_splits, own_blocks;
+    int prefix_slot, prefix_len, pre_chunk, pre_splits, pre_wgs;
+    int parts;                  // pre_splits + own_splits
+    int direct;                 // a single part of the sequences' own positions: it writes the outputs
+};
+
+// How a call is cut up.
+struct AttnQ8Plan {
+    int mt_own, mt_pre;         // 16-row blocks per wave
+    int own_chunk, own_splits, own_blocks;
+    int pre_chunk, pre_splits, pre_blocks;
+    int parts;
+    int64_t blocks, pre_wgs;    // workgroups of the launch
+    int64_t work_bytes;         // of the parts (0 where none are kept)
+};
+
+}  // namespace smx

@@ -9,6 +9,8 @@
 #include <string>
 
 #include "../../include/smx.h"
+#include "smx_attn_q8.h"
+#include "smx_kvcache.h"
 
 namespace smx {
 
@@ -349,6 +351,23 @@ hipError_t launch_attention_tokens(const float *q, int64_t q_stride, float *cons
                                    uint8_t *out_parts = nullptr, XpSums sums = XpSums{});   // sums: hd >= 32
 hipError_t launch_argmax_rows(const float *x, int n, int64_t stride, int M, int32_t *tok_next,
                               int32_t *tok_pos, int32_t *const *tok_arr, hipStream_t s);
+
+// ---- 8-bit KV cache (smx_kvcache.h), attention over it, verification of drafted tokens ---------
+hipError_t launch_kv_append(const KvView &c, const float *k, int64_t k_stride, const float *v, int64_t v_stride,
+                            const int32_t *slots, const int32_t *pos, int n_tok, hipStream_t s);
+// k, v: [n_tok][n_kv][hd]
+hipError_t launch_kv_read(const KvView &c, const int32_t *slots, const int32_t *pos, int n_tok, float *k, float *v,
+                          hipStream_t s);
+// How a call is cut up (the same for every content of slots and lens), and the call with work of
+// plan.work_bytes bytes.
+AttnQ8Plan attn_q8_plan(const KvView &c, int n_seq, int n_q, int n_head, int prefix_len, int max_len);
+hipError_t launch_attn_q8(const KvView &c, const AttnQ8Plan &plan, const float *q, int64_t q_stride, float *out,
+                          int n_seq, int n_q, int n_head, int prefix_slot, int prefix_len, const int32_t *slots,
+                          const int32_t *lens, int max_len, void *work, hipStream_t s);
+// p: n_seq * (n_draft + 1) rows, q (may be null): n_seq * n_draft rows
+hipError_t launch_verify(const float *p, int64_t p_stride, const float *q, int64_t q_stride, const int32_t *draft,
+                         const int32_t *lens, const float *u_accept, const float *u_draw, int n_seq, int n_draft,
+                         int vocab, int32_t *tokens, int32_t *accepted, hipStream_t s);
 
 // ---- errors and block geometry (host_common.cpp) ------------------------------------------
 void set_error(const std::string &msg);

@@ -286,6 +286,182 @@ def sample(logits, u: float, context=None, temperature: float = 1.0, top_k: int 
     return int(out.item()), probs
 
 
+# ---- serving operators: 8-bit KV cache, attention over it, drafted tokens ------------------------
+def _on_device(device, *tensors):
+    """Checks that the tensors are on `device` and makes it current (a context manager)."""
+    for t in tensors:
+        if t is not None and t.device != device:
+            raise ValueError(f"operands must be on {device}, not {t.device}")
+    torch = _torch()
+    return _SAME_DEVICE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+
+class _SameDevice:
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *exc):
+        return False
+
+
+_SAME_DEVICE = _SameDevice()
+
+
+def _int32(t, n: int, what: str):
+    if t.dtype != _torch().int32 or not t.is_contiguous() or t.numel() != n:
+        raise ValueError(f"{what} must be a contiguous int32 tensor of {n} elements")
+    return t
+
+
+def _rows(t, heads: int, head_dim: int, what: str) -> int:
+    """The distance between the [heads][head_dim] rows of t [..., heads, head_dim], which may lie in the
+    rows of a wider matrix (a fused projection)."""
+    if t.dtype != _torch().float32 or t.dim() < 3 or t.shape[-2:] != (heads, head_dim):
+        raise ValueError(f"{what} must be float32 [..., {heads}, {head_dim}], is {t.dtype} {tuple(t.shape)}")
+    row = heads * head_dim
+    if t.numel() == 0:
+        return row
+    lead, strides = t.shape[:-2], t.stride()
+    ok = (strides[-1] == 1 or head_dim == 1) and (strides[-2] == head_dim or heads == 1)
+    step, n = None, 1
+    for size, st in zip(reversed(lead), reversed(strides[:-2])):
+        if size == 1:
+            continue
+        if step is None:
+            step = st
+        elif st != n * step:
+            ok = False
+        n *= size
+    step = row if step is None else step
+    if not ok or step < row:
+        raise ValueError(f"{what}: tokens must be evenly spaced rows of contiguous heads")
+    return step
+
+
+class GpuKvCache:
+    """An 8-bit KV cache of n_slots sequences of up to ctx positions (smx_kv_cache_*): every row of
+    head_dim values is kept as one Q8Tensor block, codes and an fp32 scale (Q8Tensor.cs:72-128).
+    head_dim: a multiple of 8 up to 256.  Lives on `device` (default: the current one)."""
+
+    def __init__(self, n_slots: int, n_kv_head: int, head_dim: int, ctx: int, device=None):
+        self._h = ctypes.c_void_p()
+        torch = _torch()
+        with torch.cuda.device(device if device is not None else torch.cuda.current_device()):
+            self.device = torch.device("cuda", torch.cuda.current_device())
+            call("smx_kv_cache_create", n_slots, n_kv_head, head_dim, ctx, ctypes.byref(self._h))
+        self.n_slots, self.n_kv_head, self.head_dim, self.ctx = n_slots, n_kv_head, head_dim, ctx
+
+    @property
+    def nbytes(self) -> int:
+        b = ctypes.c_int64()
+        call("smx_kv_cache_info", self._h, None, None, None, None, ctypes.byref(b))
+        return b.value
+
+    def append(self, k, v, slots, pos):
+        """Writes token t's rows k[t], v[t] ([n_tok, n_kv_head, head_dim] float32, possibly slices of a fused
+        projection) to position pos[t] of slot slots[t] (int32).  Places the cache does not have (-1) are
+        skipped; a place named twice is left with undefined contents."""
+        n = slots.numel()
+        ks, vs = _rows(k, self.n_kv_head, self.head_dim, "k"), _rows(v, self.n_kv_head, self.head_dim, "v")
+        if k.numel() != v.numel() or k.numel() != n * self.n_kv_head * self.head_dim:
+            raise ValueError(f"k and v must hold one row per token ({n})")
+        with _on_device(self.device, k, v, _int32(slots, n, "slots"), _int32(pos, n, "pos")):
+            if n:
+                call("smx_kv_append", self._handle(), k.data_ptr(), ks, v.data_ptr(), vs, slots.data_ptr(),
+                     pos.data_ptr(), n, _stream())
+
+    def read(self, slots, pos):
+        """(k, v), each [n_tok, n_kv_head, head_dim] float32: the values the cache holds at these places (zeros
+        at places it does not have)."""
+        torch, n = _torch(), slots.numel()
+        with _on_device(self.device, _int32(slots, n, "slots"), _int32(pos, n, "pos")):
+            k = torch.empty((n, self.n_kv_head, self.head_dim), dtype=torch.float32, device=self.device)
+            v = torch.empty_like(k)
+            if n:
+                call("smx_kv_read", self._handle(), slots.data_ptr(), pos.data_ptr(), n, k.data_ptr(), v.data_ptr(),
+                     _stream())
+        return k, v
+
+    def _handle(self):
+        if not self._h.value:
+            raise ValueError("the cache is closed")
+        return self._h
+
+    def close(self):
+        if getattr(self, "_h", None) and self._h.value and _lib._lib is not None:
+            _lib._lib.smx_kv_cache_destroy(self._h)
+            self._h = ctypes.c_void_p()
+
+    def __del__(self):
+        self.close()
+
+
+def _attention_q8(q, cache, prefix, slots, lens, max_len, name):
+    torch = _torch()
+    if q.dim() != 4:
+        raise ValueError("q must be [n_seq, n_q, n_head, head_dim]")
+    n_seq, n_q, n_head, hd = q.shape
+    stride = _rows(q, n_head, cache.head_dim, "q")
+    max_len = cache.ctx if max_len is None else max_len
+    with _on_device(cache.device, q, _int32(slots, n_seq, "slots"), _int32(lens, n_seq, "lens")):
+        out = torch.empty((n_seq, n_q, n_head, hd), dtype=torch.float32, device=cache.device)
+        h, need = cache._handle(), ctypes.c_int64()
+        call("smx_attention_work_bytes", h, n_seq, n_q, n_head, prefix[1] if prefix else 0, max_len, ctypes.byref(need))
+        work = torch.empty(need.value, dtype=torch.uint8, device=cache.device) if need.value else None
+        call(name, h, q.data_ptr(), stride, out.data_ptr(), n_seq, n_q, n_head, *prefix, slots.data_ptr(), lens.data_ptr(),
+             max_len, work.data_ptr() if need.value else None, need.value, _stream())
+    return out
+
+
+def attention_cached(q, cache: GpuKvCache, slots, lens, max_len: int | None = None):
+    """Attention of the last n_q tokens of n_seq sequences over an 8-bit cache (smx_attention_cached).
+    q [n_seq, n_q, n_head, head_dim] float32 (tokens may be rows of a fused projection); sequence b's
+    positions are the first lens[b] of slot slots[b] (int32 on the device), its n_q tokens the last of them,
+    each seeing all up to itself.  max_len: an upper bound of lens (default: ctx); a tight one is faster.
+    Returns [n_seq, n_q, n_head, head_dim]; zeros for rows that see nothing and for slots the cache does not
+    have."""
+    return _attention_q8(q, cache, (), slots, lens, max_len, "smx_attention_cached")
+
+
+def attention_shared(q, cache: GpuKvCache, prefix_slot: int, prefix_len: int, slots, lens, max_len: int | None = None):
+    """attention_cached for sequences that all begin with the first prefix_len positions of slot prefix_slot,
+    which are read once for all of them; slots and lens describe what each sequence has of its own, possibly
+    nothing (smx_attention_shared)."""
+    return _attention_q8(q, cache, (int(prefix_slot), int(prefix_len)), slots, lens, max_len, "smx_attention_shared")
+
+
+def verify_draft(target, draft, tokens, u_accept, u_draw, lens=None):
+    """Verification of drafted tokens (speculative decoding; smx_verify_draft).  target [n_seq, n_draft + 1,
+    vocab] and draft [n_seq, n_draft, vocab]: the probabilities of the target and of the draft model (draft
+    None: tokens chosen without a distribution); tokens [n_seq, n_draft] int32; u_accept [n_seq, n_draft] and
+    u_draw [n_seq]: uniform numbers in [0, 1); lens [n_seq] int32: drafted tokens per sequence (default:
+    n_draft, negative: an empty place).  Returns (out [n_seq, n_draft + 1], accepted [n_seq]) int32: the
+    accepted tokens, one drawn token, then -1."""
+    torch = _torch()
+    if target.dim() != 3 or target.shape[1] < 1:
+        raise ValueError("target must be [n_seq, n_draft + 1, vocab]")
+    n_seq, n_draft, vocab = target.shape[0], target.shape[1] - 1, target.shape[2]
+    ts = _rows(target.unsqueeze(-2), 1, vocab, "target")
+    ds = 0
+    if draft is not None:
+        if draft.shape != (n_seq, n_draft, vocab):
+            raise ValueError(f"draft must be {(n_seq, n_draft, vocab)}, is {tuple(draft.shape)}")
+        ds = _rows(draft.unsqueeze(-2), 1, vocab, "draft")
+    for u, shape, what in ((u_accept, (n_seq, n_draft), "u_accept"), (u_draw, (n_seq,), "u_draw")):
+        if tuple(u.shape) != shape or u.dtype != torch.float32 or not u.is_contiguous():
+            raise ValueError(f"{what} must be contiguous float32 {shape}")
+    if lens is not None:
+        _int32(lens, n_seq, "lens")
+    with _on_device(target.device, draft, _int32(tokens, n_seq * n_draft, "tokens"), u_accept, u_draw, lens):
+        out = torch.empty((n_seq, n_draft + 1), dtype=torch.int32, device=target.device)
+        accepted = torch.empty(n_seq, dtype=torch.int32, device=target.device)
+        call("smx_verify_draft", target.data_ptr(), ts, None if draft is None else draft.data_ptr(), ds,
+             tokens.data_ptr(), None if lens is None else lens.data_ptr(), u_accept.data_ptr(), u_draw.data_ptr(), n_seq,
+             n_draft, vocab, out.data_ptr(), accepted.data_ptr(), _stream())
+    return out, accepted
+
+
 __all__ = ["GgufTensorType", "GpuWeightTensor", "SmxError", "dequantize", "quantize", "fill_normal",
            "rmsnorm", "layernorm", "rope_tables", "rope_", "scale_mask_softmax_", "attention_decode",
-           "silu_mul", "gelu", "argmax", "sample", "row_bytes", "BLOCK_ELEMS", "BLOCK_BYTES"]
+           "silu_mul", "gelu", "argmax", "sample", "row_bytes", "BLOCK_ELEMS", "BLOCK_BYTES", "GpuKvCache",
+           "attention_cached", "attention_shared", "verify_draft"]

@@ -1,0 +1,622 @@
+"""The 8-bit KV cache, the attention over it and the verification of drafted tokens on the GPU, against
+plain 64-bit forms."""
+import ctypes
+
+import numpy as np
+import pytest
+
+from tests import kv_reference as R
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def Q(gpu):
+    from smallmind_amd import quantization
+    return quantization
+
+
+def dev(a, dtype=None):
+    import torch
+    return torch.from_numpy(np.ascontiguousarray(a if dtype is None else np.asarray(a, dtype))).cuda()
+
+
+def i32(a):
+    return dev(a, np.int32)
+
+
+# ---- rows written and read back -------------------------------------------------------------------
+def places(kind, n, slots, ctx, rng):
+    """n distinct places of a cache as callers come with them."""
+    if kind == "run":           # a prompt behind an odd number of positions
+        return np.full(n, slots - 1), 3 + np.arange(n)
+    if kind == "aligned":
+        return np.full(n, 0), np.arange(n)
+    if kind == "batch":         # a token for each of many sequences, positions all over
+        return np.arange(n) % slots, (np.arange(n) // slots * 5 + 7 * (np.arange(n) % slots)) % ctx
+    if kind == "runs":          # several tokens for each of several sequences
+        return np.arange(n) // 5 % slots, (np.arange(n) % 5 + 1 + 5 * (np.arange(n) // 5 // slots)) % ctx
+    p = rng.permutation(slots * ctx)[:n]
+    return p // ctx, p % ctx
+
+
+@pytest.mark.parametrize("hd", [8, 16, 32, 40, 64, 80, 96, 128, 136, 160, 192, 208, 224, 256])
+@pytest.mark.parametrize("kind,n", [("run", 1), ("run", 131), ("aligned", 64), ("batch", 17), ("runs", 93), ("random", 150)])
+def test_rows_come_back_as_they_were_encoded(Q, hd, kind, n):
+    rng = np.random.default_rng(hd * 1000 + n)
+    kv, slots, ctx = 3, 19, 150
+    s, p = places(kind, n, slots, ctx, rng)
+    assert len({(a, b) for a, b in zip(s.tolist(), p.tolist())}) == n
+    k = (rng.normal(0, 1, (n, kv, hd)) * np.exp2(rng.integers(-20, 20, (n, kv, 1)))).astype(np.float32)
+    v = rng.normal(0, 2, (n, kv, hd)).astype(np.float32)
+    c = Q.GpuKvCache(slots, kv, hd, ctx)
+    c.append(dev(k), dev(v), i32(s), i32(p))
+    all_s, all_p = np.repeat(np.arange(slots), ctx), np.tile(np.arange(ctx), slots)
+    gk, gv = c.read(i32(all_s), i32(all_p))
+    ek, ev = np.zeros((slots, ctx, kv, hd), np.float32), np.zeros((slots, ctx, kv, hd), np.float32)
+    ek[s, p], ev[s, p] = R.held(k), R.held(v)
+    assert np.array_equal(gk.cpu().numpy().reshape(ek.shape), ek)
+    assert np.array_equal(gv.cpu().numpy().reshape(ev.shape), ev)
+    c.close()
+
+
+def test_places_that_the_cache_does_not_have(Q):
+    rng = np.random.default_rng(3)
+    c = Q.GpuKvCache(2, 2, 64, 70)
+    s = np.array([0, -1, 2, 1, 1, 1, 0, 0, 2**31 - 1, -2**31])
+    p = np.array([5, 5, 5, -1, 70, 69, 6, 2**31 - 1, 0, -2**31])
+    k, v = (rng.normal(0, 1, (10, 2, 64)).astype(np.float32) for _ in range(2))
+    c.append(dev(k), dev(v), i32(s), i32(p))
+    ok = [0, 5, 6]
+    gk, gv = c.read(i32(s), i32(p))
+    for g, x in ((gk, k), (gv, v)):
+        e = np.zeros_like(x)
+        e[ok] = R.held(x[ok])
+        assert np.array_equal(g.cpu().numpy(), e)
+    gk, _ = c.read(i32(np.repeat([0, 1], 70)), i32(np.tile(np.arange(70), 2)))
+    assert int((gk.abs().sum((1, 2)) > 0).sum()) == 3
+    c.close()
+
+
+def test_values_next_to_a_border(Q):
+    """Multiples and halves of a step and their neighbours in fp32, for scales of every size."""
+    rows = []
+    for top in (127.0, 1.0, 3.7e-3, 2.0 ** -120, 127 * 2.0 ** -149, 190 * 2.0 ** -149, 2.0 ** -149, 3.0e38, 1e-30, 88.3):
+        top = np.float32(top)
+        step = np.float32(np.float64(top) / 127)
+        h = ((np.arange(-126, 126) + 0.5) * np.float64(step)).astype(np.float32)
+        h = np.concatenate([h, np.nextafter(h, np.float32(np.inf)), np.nextafter(h, np.float32(-np.inf)),
+                            (np.arange(-126, 127) * np.float64(step)).astype(np.float32)])
+        h = np.clip(h, -top, top)
+        h = np.concatenate([h, np.zeros(-len(h) % 63, np.float32)]).reshape(-1, 63)
+        rows.append(np.concatenate([np.full((len(h), 1), top, np.float32), h], 1))
+    x = np.concatenate(rows)[:, None]
+    n = len(x)
+    c = Q.GpuKvCache(1, 1, 64, n)
+    c.append(dev(x), dev(-x), i32(np.zeros(n)), i32(np.arange(n)))
+    k, v = c.read(i32(np.zeros(n)), i32(np.arange(n)))
+    assert np.array_equal(k.cpu().numpy(), R.held(x)) and np.array_equal(v.cpu().numpy(), R.held(-x))
+    c.close()
+
+
+def test_rows_that_are_not_finite(Q):
+    rng = np.random.default_rng(8)
+    x = rng.normal(0, 1, (6, 2, 64)).astype(np.float32)
+    x[1, 0, 63], x[2, 1, 0], x[4, 0, 5], x[5, :, :] = np.nan, np.inf, -np.inf, 0.0
+    c = Q.GpuKvCache(1, 2, 64, 64)
+    c.append(dev(x), dev(x), i32(np.zeros(6)), i32(np.arange(6)))
+    k, v = c.read(i32(np.zeros(6)), i32(np.arange(6)))
+    e = R.held(x)
+    assert np.isnan(e[1, 0]).all() and not np.isnan(e[1, 1]).any()
+    assert np.array_equal(k.cpu().numpy(), e, equal_nan=True) and np.array_equal(v.cpu().numpy(), e, equal_nan=True)
+    c.close()
+
+
+@pytest.mark.parametrize("hd,off", [(64, 0), (64, 1), (40, 3), (128, 2)])
+def test_rows_of_a_fused_projection(Q, hd, off):
+    import torch
+    rng = np.random.default_rng(hd + off)
+    n, heads, kv = 70, 4, 2
+    width = (heads + 2 * kv) * hd + 5
+    buf = dev(rng.normal(0, 1, n * width + off).astype(np.float32))
+    f = buf[off:].view(n, width)
+    k, v = f[:, heads * hd:(heads + kv) * hd].unflatten(1, (kv, hd)), f[:, (heads + kv) * hd:(heads + 2 * kv) * hd].unflatten(1, (kv, hd))
+    c = Q.GpuKvCache(1, kv, hd, n)
+    at = i32(np.arange(n))
+    c.append(k, v, torch.zeros_like(at), at)
+    gk, gv = c.read(torch.zeros_like(at), at)
+    assert np.array_equal(gk.cpu().numpy(), R.held(k.cpu().numpy())) and np.array_equal(gv.cpu().numpy(), R.held(v.cpu().numpy()))
+    c.close()
+
+
+def test_a_cache_of_more_than_4_gib(Q):
+    import torch
+    rng = np.random.default_rng(4)
+    c = Q.GpuKvCache(9, 8, 128, 262144)     # 4.9 GB
+    assert c.nbytes > (1 << 32)
+    s, p = np.array([8, 8, 8, 0, 7, 8, 8]), np.array([262143, 262142, 0, 262143, 100000, 131072, 200001])
+    k, v = (rng.normal(0, 1, (7, 8, 128)).astype(np.float32) for _ in range(2))
+    c.append(dev(k), dev(v), i32(s), i32(p))
+    gk, gv = c.read(i32(s), i32(p))
+    assert np.array_equal(gk.cpu().numpy(), R.held(k)) and np.array_equal(gv.cpu().numpy(), R.held(v))
+    # attention over all of the last slot: the zeros of the positions never written weigh equally
+    q = rng.normal(0, 1, (1, 1, 8, 128)).astype(np.float32)
+    out = Q.attention_cached(dev(q), c, i32([8]), i32([262144])).cpu().numpy()
+    hk, hv = R.held(k).astype(np.float64), R.held(v).astype(np.float64)
+    for h in range(8):
+        rows = [0, 1, 2, 5, 6]
+        w = np.exp(hk[rows, h] @ q[0, 0, h].astype(np.float64) / np.sqrt(128))
+        ref = w @ hv[rows, h] / (w.sum() + 262144 - len(rows))
+        # weights and their sum: 262144 terms in fp32 parts of 64 positions and more
+        assert np.abs(out[0, 0, h] - ref).max() <= 1e-3 * np.abs(ref).max()
+    c.close()
+    torch.cuda.empty_cache()
+
+
+# ---- attention ------------------------------------------------------------------------------------
+class Filled:
+    """A cache whose slots hold random rows, and what they stand for."""
+
+    def __init__(self, Q, slots, kv, hd, ctx, seed, spread=1.0):
+        rng = np.random.default_rng(seed)
+        self.k = rng.normal(0, spread, (slots, ctx, kv, hd)).astype(np.float32)
+        self.v = (rng.normal(0, 1, (slots, ctx, kv, hd)) * np.exp2(rng.integers(-3, 4, (slots, ctx, kv, 1)))).astype(np.float32)
+        self.cache = Q.GpuKvCache(slots, kv, hd, ctx)
+        n = slots * ctx
+        self.cache.append(dev(self.k.reshape(n, kv, hd)), dev(self.v.reshape(n, kv, hd)), i32(np.repeat(np.arange(slots), ctx)),
+                          i32(np.tile(np.arange(ctx), slots)))
+        self.hk, self.hv = R.held(self.k), R.held(self.v)
+
+
+def reference(f, q, slots, lens, prefix=None, max_len=None):
+    n_seq, n_q, H, hd = q.shape
+    kv = f.k.shape[2]
+    G = H // kv
+    out, bound = np.zeros(q.shape), np.zeros((n_seq, n_q, H))
+    for b in range(n_seq):
+        if not 0 <= slots[b] < f.k.shape[0]:
+            continue
+        n = max(0, min(int(lens[b]), f.k.shape[1] if max_len is None else max_len))
+        for h in range(kv):
+            k, v = f.hk[slots[b], :n, h], f.hv[slots[b], :n, h]
+            P = 0
+            if prefix:
+                P = prefix[1]
+                k, v = np.concatenate([f.hk[prefix[0], :P, h], k]), np.concatenate([f.hv[prefix[0], :P, h], v])
+            for i in range(n_q):
+                vis = np.zeros((G, P + n), bool)
+                vis[:, :P + max(0, n - n_q + 1 + i)] = True
+                o, e = R.attention(q[b, i, h * G:(h + 1) * G], k, v, vis)
+                out[b, i, h * G:(h + 1) * G], bound[b, i, h * G:(h + 1) * G] = o, e
+    return out, bound
+
+
+def close(got, want):
+    ref, bound = want
+    err = np.abs(got.cpu().numpy().astype(np.float64) - ref).max(-1)
+    assert (err <= bound).all(), (float((err - bound).max()), np.unravel_index((err - bound).argmax(), err.shape))
+
+
+@pytest.mark.parametrize("hd", [8, 32, 40, 64, 80, 96, 128, 160, 192, 224, 256])
+@pytest.mark.parametrize("group,n_q", [(1, 1), (3, 1), (8, 1), (1, 5), (5, 4), (4, 9), (20, 1), (7, 11)])
+def test_attention_cached(Q, hd, group, n_q):
+    f = Filled(Q, 7, 2, hd, 330, hd + group + n_q)
+    rng = np.random.default_rng(hd * group + n_q)
+    lens = np.array([1, 64, 0, 330, 65, 256, 63])
+    slots = np.array([6, 0, 1, 2, 3, 4, 5])
+    q = rng.normal(0, 1.3, (7, n_q, 2 * group, hd)).astype(np.float32)
+    got = Q.attention_cached(dev(q), f.cache, i32(slots), i32(lens))
+    close(got, reference(f, q, slots, lens))
+    assert not got[2].any()
+    f.cache.close()
+
+
+@pytest.mark.parametrize("hd", [32, 64, 80, 128, 256])
+@pytest.mark.parametrize("group,n_q,n_seq", [(1, 1, 1), (1, 1, 5), (4, 1, 9), (2, 3, 7), (8, 4, 3)])
+@pytest.mark.parametrize("P", [1, 64, 129, 600])
+def test_attention_shared(Q, hd, group, n_q, n_seq, P):
+    f = Filled(Q, n_seq + 1, 2, hd, 600, hd + group + n_q + P)
+    rng = np.random.default_rng(hd * group + n_q + P)
+    lens = np.array([0, 70, 1, 300, 64, 5, 0, 11, 2])[:n_seq]
+    slots = np.arange(n_seq)[::-1].copy()
+    q = rng.normal(0, 1.3, (n_seq, n_q, 2 * group, hd)).astype(np.float32)
+    got = Q.attention_shared(dev(q), f.cache, n_seq, P, i32(slots), i32(lens), 300)
+    close(got, reference(f, q, slots, lens, (n_seq, P)))
+    f.cache.close()
+
+
+def test_attention_over_a_prefix_alone_and_over_none(Q):
+    f = Filled(Q, 4, 2, 64, 500, 9)
+    rng = np.random.default_rng(1)
+    q = rng.normal(0, 1, (3, 2, 8, 64)).astype(np.float32)
+    slots, lens = np.array([0, -1, 2]), np.array([400, 400, 7])
+    for P in (100, 500):
+        close(Q.attention_shared(dev(q), f.cache, 3, P, i32(slots), i32(lens), 0), reference(f, q, slots, lens, (3, P), 0))
+    a = Q.attention_shared(dev(q), f.cache, 3, 0, i32(slots), i32(lens))
+    b = Q.attention_cached(dev(q), f.cache, i32(slots), i32(lens))
+    assert bool((a == b).all()) and not b[1].any()
+    assert not Q.attention_cached(dev(q), f.cache, i32(slots), i32(lens), 0).any()
+    f.cache.close()
+
+
+def test_attention_of_many_lengths_of_one_sequence(Q):
+    f = Filled(Q, 1, 1, 64, 1300, 12)
+    rng = np.random.default_rng(2)
+    lens = np.array([1, 2, 15, 16, 17, 31, 33, 48, 62, 63, 64, 65, 127, 128, 129, 255, 256, 257, 511, 513, 1023, 1025, 1299, 1300,
+                     5000, -3])
+    q = rng.normal(0, 2, (len(lens), 1, 2, 64)).astype(np.float32)
+    slots = np.zeros(len(lens), int)
+    close(Q.attention_cached(dev(q), f.cache, i32(slots), i32(lens)), reference(f, q, slots, lens))
+    close(Q.attention_cached(dev(q), f.cache, i32(slots), i32(lens), 100), reference(f, q, slots, lens, None, 100))
+    f.cache.close()
+
+
+@pytest.mark.parametrize("spread", [0.0, 1e-12, 6.0, 300.0])
+def test_attention_of_flat_and_sharp_scores(Q, spread):
+    f = Filled(Q, 2, 2, 64, 700, 21, spread)
+    rng = np.random.default_rng(5)
+    q = rng.normal(0, 2, (2, 3, 4, 64)).astype(np.float32)
+    slots, lens = np.array([0, 1]), np.array([700, 401])
+    close(Q.attention_cached(dev(q), f.cache, i32(slots), i32(lens)), reference(f, q, slots, lens))
+    close(Q.attention_shared(dev(q), f.cache, 1, 300, i32(slots), i32(lens)), reference(f, q, slots, lens, (1, 300)))
+    f.cache.close()
+
+
+def test_values_and_queries_of_very_different_sizes(Q):
+    """Rows of V from 2^-40 to 2^40 beside one another, queries with one element far above the rest, tiny and
+    huge ones: every row within its bound, which goes by the largest value that the row sees."""
+    rng = np.random.default_rng(6)
+    n, hd = 200, 64
+    k = rng.normal(0, 1, (n, 1, hd)).astype(np.float32)
+    v = (rng.normal(0, 1, (n, 1, hd)) * np.exp2(rng.integers(-40, 41, (n, 1, 1)))).astype(np.float32)
+    f = Filled(Q, 1, 1, hd, n, 0)
+    f.cache.append(dev(k), dev(v), i32(np.zeros(n)), i32(np.arange(n)))
+    f.hk[0], f.hv[0] = R.held(k), R.held(v)
+    q = rng.normal(0, 1, (5, 1, 1, hd)).astype(np.float32)
+    q[1, 0, 0, 3] = 40.0
+    q[2] *= 1e-30
+    q[3] = 0.0
+    q[4] *= 1e-42
+    slots, lens = np.zeros(5, int), np.array([n, n, n, 70, 3])
+    close(Q.attention_cached(dev(q), f.cache, i32(slots), i32(lens)), reference(f, q, slots, lens))
+    f.cache.close()
+
+
+def test_what_is_not_seen_does_not_count(Q):
+    """NaN rows behind a sequence's length, in other slots, and at a drafted token that only later ones see."""
+    f = Filled(Q, 3, 2, 64, 200, 31)
+    nan = np.full((1, 2, 64), np.nan, np.float32)
+    for p in (150, 151, 199):
+        f.cache.append(dev(nan), dev(nan), i32([0]), i32([p]))
+    f.cache.append(dev(nan), dev(nan), i32([1]), i32([0]))
+    f.cache.append(dev(f.k[2, 88:89]), dev(nan), i32([2]), i32([88]))
+    rng = np.random.default_rng(7)
+    q = rng.normal(0, 1, (2, 4, 4, 64)).astype(np.float32)
+    slots, lens = np.array([0, 2]), np.array([150, 90])
+    got = Q.attention_cached(dev(q), f.cache, i32(slots), i32(lens)).cpu()
+    ref, bound = reference(f, q, slots, lens)
+    close(got[:1], (ref[:1], bound[:1]))
+    close(got[1:, :2], (ref[1:, :2], bound[1:, :2]))        # these see positions 0 .. 87
+    assert got[1, 2:].isnan().all()
+    # a prefix with a NaN reaches every row, one behind its length none
+    assert Q.attention_shared(dev(q), f.cache, 1, 10, i32(slots), i32(lens)).isnan().all()
+    assert not Q.attention_shared(dev(q), f.cache, 0, 150, i32([2, 2]), i32([40, 3])).isnan().any()
+    f.cache.close()
+
+
+def test_a_query_that_is_not_finite_stays_alone(Q):
+    f = Filled(Q, 2, 2, 64, 100, 33)
+    rng = np.random.default_rng(8)
+    q = rng.normal(0, 1, (2, 2, 8, 64)).astype(np.float32)
+    slots, lens = np.array([0, 1]), np.array([100, 1])
+    ref, bound = reference(f, q, slots, lens)
+    q[0, 1, 3, 7], q[0, 0, 0, 0], q[1, 0, 2, 2] = np.inf, np.nan, np.nan
+    got = Q.attention_cached(dev(q), f.cache, i32(slots), i32(lens)).cpu()
+    assert got[0, 1, 3].isnan().all() and got[0, 0, 0].isnan().all()
+    assert not got[1, 0].any()          # sees nothing
+    ok = np.ones((2, 2, 8), bool)
+    ok[0, 1, 3] = ok[0, 0, 0] = False
+    err = np.abs(got.numpy() - ref).max(-1)
+    assert (err[ok] <= bound[ok]).all()
+    f.cache.close()
+
+
+@pytest.mark.parametrize("off", [0, 1, 2])
+def test_queries_in_the_rows_of_a_fused_projection(Q, off):
+    f = Filled(Q, 4, 2, 64, 90, 35)
+    rng = np.random.default_rng(9)
+    width = (8 + 4) * 64 + off
+    buf = dev(rng.normal(0, 1, 4 * 3 * width + off).astype(np.float32))[off:].view(4, 3, width)
+    q = buf[:, :, :512].unflatten(2, (8, 64))
+    slots, lens = np.arange(4), np.array([90, 3, 44, 70])
+    close(Q.attention_cached(q, f.cache, i32(slots), i32(lens)), reference(f, q.cpu().numpy(), slots, lens))
+    f.cache.close()
+
+
+def test_rows_behind_the_outputs_and_the_work_memory_stay(Q):
+    import torch
+
+    from smallmind_amd._lib import call
+    f = Filled(Q, 3, 2, 64, 600, 36)
+    q = torch.randn(3, 2, 8, 64, device="cuda")
+    slots, lens = i32([0, 1, 2]), i32([600, 0, 77])
+    need = ctypes.c_int64()
+    call("smx_attention_work_bytes", f.cache._h, 3, 2, 8, 500, 600, ctypes.byref(need))
+    assert need.value > 0
+    out = torch.full((q.numel() + 512,), 7.5, device="cuda")
+    work = torch.full((need.value + 256,), 91, dtype=torch.uint8, device="cuda")
+    call("smx_attention_shared", f.cache._h, q.data_ptr(), 512, out.data_ptr(), 3, 2, 8, 2, 500, slots.data_ptr(),
+         lens.data_ptr(), 600, work.data_ptr(), need.value, None)
+    torch.cuda.synchronize()
+    assert bool((out[q.numel():] == 7.5).all()) and bool((work[need.value:] == 91).all())
+    want = Q.attention_shared(q, f.cache, 2, 500, slots, lens)
+    assert bool((out[:q.numel()] == want.reshape(-1)).all())
+    f.cache.close()
+
+
+def test_refusals(Q):
+    import torch
+
+    from smallmind_amd._lib import load
+    L = load()
+    c = Q.GpuKvCache(2, 2, 64, 128)
+    t = torch.zeros(4096, device="cuda")
+    i = torch.zeros(64, dtype=torch.int32, device="cuda")
+    n = ctypes.c_int64()
+
+    def cached(**k):
+        a = dict(q=t.data_ptr(), stride=256, out=t.data_ptr(), n_seq=2, n_q=1, n_head=4, slots=i.data_ptr(), lens=i.data_ptr(),
+                 max_len=128, work=None, bytes=0)
+        a.update(k)
+        return L.smx_attention_cached(c._h, *a.values(), None)
+
+    def shared(slot, length, **k):
+        a = dict(q=t.data_ptr(), stride=256, out=t.data_ptr(), n_seq=2, n_q=1, n_head=4, slot=slot, length=length,
+                 slots=i.data_ptr(), lens=i.data_ptr(), max_len=128, work=None, bytes=0)
+        a.update(k)
+        return L.smx_attention_shared(c._h, *a.values(), None)
+
+    for bad in (dict(q=None), dict(out=None), dict(slots=None), dict(lens=None), dict(stride=255), dict(n_seq=0), dict(n_q=0),
+                dict(n_head=0), dict(n_head=5), dict(max_len=-1), dict(max_len=129), dict(q=t.data_ptr() + 2)):
+        assert cached(**bad) == -1, bad
+    assert cached(n_seq=2**30, n_head=64, stride=64 * 64) == -5
+    assert shared(2, 10) == -1 and shared(-1, 10) == -1 and shared(0, 129) == -1 and shared(0, -1) == -1
+    assert shared(0, 10) == -1 and b"work" in L.smx_last_error()
+    assert shared(0, 10, work=t.data_ptr(), bytes=16) == -1
+    assert L.smx_attention_work_bytes(c._h, 1, 1, 3, 0, 128, ctypes.byref(n)) == -1
+    ap = lambda **k: L.smx_kv_append(c._h, *{**dict(k=t.data_ptr(), ks=128, v=t.data_ptr(), vs=128, s=i.data_ptr(),  # noqa: E731
+                                                   p=i.data_ptr(), n=1), **k}.values(), None)
+    for bad in (dict(k=None), dict(v=None), dict(s=None), dict(p=None), dict(ks=127), dict(vs=127), dict(n=-1), dict(k=t.data_ptr() + 1)):
+        assert ap(**bad) == -1, bad
+    assert ap(n=0) == 0
+    with pytest.raises(ValueError):
+        c.append(torch.zeros(3, 2, 64, device="cuda"), torch.zeros(3, 2, 64, device="cuda"), i[:2], i[:2])
+    with pytest.raises(ValueError):
+        c.append(torch.zeros(2, 2, 64, device="cuda").half(), torch.zeros(2, 2, 64, device="cuda"), i[:2], i[:2])
+    with pytest.raises(ValueError):
+        c.append(torch.zeros(2, 64, 2, device="cuda").transpose(1, 2), torch.zeros(2, 2, 64, device="cuda"), i[:2], i[:2])
+    with pytest.raises(ValueError):
+        c.append(torch.zeros(2, 2, 64), torch.zeros(2, 2, 64, device="cuda"), i[:2], i[:2])
+    with pytest.raises(ValueError):
+        Q.attention_cached(torch.zeros(2, 1, 4, 64, device="cuda"), c, i[:2].long(), i[:2])
+    with pytest.raises(ValueError):
+        Q.attention_cached(torch.zeros(2, 1, 4, 32, device="cuda"), c, i[:2], i[:2])
+    with pytest.raises(ValueError):
+        Q.attention_cached(torch.zeros(2, 1, 1, 4, 64, device="cuda")[0], c, i[:2], i[:2])
+    c.close()
+    with pytest.raises(ValueError):
+        c.read(i[:1], i[:1])
+    with pytest.raises(Q.SmxError):
+        Q.GpuKvCache(1, 1, 63, 64)
+
+
+def test_calls_on_other_streams_and_again(Q):
+    """The same call gives the same bits, on any stream, with other calls in flight."""
+    import torch
+    f = Filled(Q, 6, 2, 128, 900, 41)
+    q = torch.randn(5, 2, 8, 128, device="cuda")
+    slots, lens = i32(np.arange(5)), i32([900, 1, 333, 64, 257])
+    want = Q.attention_shared(q, f.cache, 5, 700, slots, lens)
+    plain = Q.attention_cached(q, f.cache, slots, lens)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    got = []
+    for _ in range(4):
+        for s in streams:
+            with torch.cuda.stream(s):
+                got.append((Q.attention_shared(q, f.cache, 5, 700, slots, lens), Q.attention_cached(q, f.cache, slots, lens)))
+    torch.cuda.synchronize()
+    assert all(bool((a == want).all()) and bool((b == plain).all()) for a, b in got)
+    f.cache.close()
+
+
+def test_captured_steps_replay(Q):
+    """Two captured graphs, each writing a token of its sequences and attending, replayed in turn with eager work
+    between: lengths and positions are read on the device, so every replay is the next step."""
+    import torch
+    rng = np.random.default_rng(50)
+    hd, kv, H, n = 64, 2, 6, 3
+    f = Filled(Q, 2 * n + 1, kv, hd, 320, 51)
+    steps = 5
+    xk, xv = (rng.normal(0, 1, (2, steps, n, kv, hd)).astype(np.float32) for _ in range(2))
+    xq = rng.normal(0, 1, (2, steps, n, 1, H, hd)).astype(np.float32)
+    start = np.array([[63, 0, 310], [127, 255, 5]])
+    state = []
+    for gi in range(2):
+        st = dict(k=dev(xk[gi, 0]), v=dev(xv[gi, 0]), q=dev(xq[gi, 0]), slots=i32(np.arange(n) + gi * n), pos=i32(start[gi]),
+                  lens=i32(start[gi] + 1))
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.stream(s):
+            Q.attention_shared(st["q"], f.cache, 2 * n, 300, st["slots"], st["lens"])
+        torch.cuda.synchronize()
+        with torch.cuda.graph(g, stream=s):
+            f.cache.append(st["k"], st["v"], st["slots"], st["pos"])
+            st["out"] = Q.attention_shared(st["q"], f.cache, 2 * n, 300, st["slots"], st["lens"])
+            st["pos"].add_(1)
+            st["lens"].add_(1)
+        st["graph"] = g
+        state.append(st)
+    for step in range(steps):
+        for gi, st in enumerate(state):
+            st["k"].copy_(dev(xk[gi, step]))
+            st["v"].copy_(dev(xv[gi, step]))
+            st["q"].copy_(dev(xq[gi, step]))
+            st["graph"].replay()
+        Q.attention_cached(state[0]["q"], f.cache, state[0]["slots"], state[0]["lens"])     # eager work between replays
+        torch.cuda.synchronize()
+        for gi, st in enumerate(state):
+            sl = np.arange(n) + gi * n
+            f.hk[sl, start[gi] + step], f.hv[sl, start[gi] + step] = R.held(xk[gi, step]), R.held(xv[gi, step])
+            close(st["out"], reference(f, xq[gi, step], sl, start[gi] + step + 1, (2 * n, 300)))
+    f.cache.close()
+
+
+# ---- verification of drafted tokens ---------------------------------------------------------------
+def drafts(rng, n_seq, n_draft, vocab, zeros=False):
+    lg = rng.normal(0, 2.5, (n_seq, n_draft + 1, vocab))
+    ld = lg[:, :n_draft] + rng.normal(0, 0.7, (n_seq, n_draft, vocab))
+    soft = lambda x: np.exp(x - x.max(-1, keepdims=True)) / np.exp(x - x.max(-1, keepdims=True)).sum(-1, keepdims=True)  # noqa: E731
+    p, q = soft(lg), soft(ld)
+    if zeros:       # as top-k leaves them
+        p, q = np.where(p > p.mean(-1, keepdims=True), p, 0.0), np.where(q > q.mean(-1, keepdims=True), q, 0.0)
+    p, q = p.astype(np.float32), q.astype(np.float32)
+    x = np.array([[rng.choice(vocab, p=q[b, i].astype(np.float64) / q[b, i].astype(np.float64).sum()) for i in range(n_draft)]
+                  for b in range(n_seq)], np.int32).reshape(n_seq, n_draft)
+    return p, q, x, rng.random((n_seq, n_draft), dtype=np.float32), rng.random(n_seq, dtype=np.float32)
+
+
+def check_verify(Q, p, q, x, ua, ud, lens=None):
+    vocab = p.shape[2]
+    out, acc = Q.verify_draft(dev(p), None if q is None else dev(q), dev(x), dev(ua), dev(ud), None if lens is None else i32(lens))
+    eo, ea = R.verify(p, q, x, ua, ud, lens, vocab)
+    assert np.array_equal(acc.cpu().numpy(), ea), (acc.cpu().numpy(), ea)
+    assert np.array_equal(out.cpu().numpy(), eo), (out.cpu().numpy(), eo)
+    return out, acc
+
+
+@pytest.mark.parametrize("vocab", [1, 2, 63, 64, 65, 1000, 1024, 1025, 16384, 16385, 50257, 70001])
+@pytest.mark.parametrize("n_seq,n_draft", [(1, 1), (3, 4), (7, 2)])
+def test_verify_draft(Q, vocab, n_seq, n_draft):
+    rng = np.random.default_rng(vocab + n_seq)
+    for zeros in (False, True) if vocab > 2 else (False,):
+        p, q, x, ua, ud = drafts(rng, n_seq, n_draft, vocab, zeros)
+        check_verify(Q, p, q, x, ua, ud)
+        check_verify(Q, p, None, x, ua, ud)
+        lens = rng.integers(-1, n_draft + 2, n_seq)
+        check_verify(Q, p, q, x, ua, ud, lens)
+    ua[:] = 0.0
+    ud[:] = 0.0
+    check_verify(Q, p, q, x, ua, ud)
+    ud[:] = np.float32(1 - 2.0 ** -24)
+    check_verify(Q, p, q, x, ua, ud)
+
+
+def test_verify_many_drafts_and_none(Q):
+    rng = np.random.default_rng(2)
+    p, q, x, ua, ud = drafts(rng, 4, 70, 33)
+    check_verify(Q, p, np.minimum(q, p[:, :70]), x, np.minimum(ua, 0.5), ud)     # long accepted runs
+    check_verify(Q, p, q, x, ua, ud, np.array([70, 65, 64, 0]))
+    e = np.zeros((4, 0, 33), np.float32)
+    check_verify(Q, p[:, :1], e, x[:, :0], ua[:, :0], ud)
+    check_verify(Q, p[:, :1], None, x[:, :0], ua[:, :0], ud)
+
+
+def test_verify_of_odd_probabilities(Q):
+    rng = np.random.default_rng(5)
+    p, q, x, ua, ud = drafts(rng, 12, 2, 300)
+    ua[:] = 0.999
+    q[0], p[0, :2] = q[0], q[0]                 # equal: ratio 1 accepts
+    p[1, 0, x[1, 0]] = 0.0                      # refused; drawn from the difference
+    p[2, 0] = q[2, 0] * np.float32(0.5)         # refused with nothing left of the difference: drawn from p
+    p[3, 0] = 0.0                               # no weight at all
+    p[4, 0, ::3] = np.nan
+    q[5, 0, ::2] = np.nan
+    x[6, 0], x[7, 0], x[8, 0] = -5, 300, 2**31 - 1
+    p[9, 0], p[9, 0, 299] = 0.0, 1.0            # everything on the last token
+    p[10, 0], p[10, 0, 0] = 0.0, 1.0
+    p[11, 0] = np.float32(1.0 / 300)
+    out, acc = check_verify(Q, p, q, x, ua, ud)
+    assert acc[3] == 0 and out[3].tolist() == [-1, -1, -1]
+    check_verify(Q, p, None, x, ua, ud)
+
+
+def test_verify_rows_of_wider_matrices_and_unaligned(Q):
+    rng = np.random.default_rng(6)
+    p, q, x, ua, ud = drafts(rng, 3, 3, 777)
+    wp, wq = np.zeros((3, 4, 800), np.float32), np.zeros((3, 3, 901), np.float32)
+    wp[:, :, 1:778], wq[:, :, 3:780] = p, q
+    out, acc = Q.verify_draft(dev(wp)[:, :, 1:778], dev(wq)[:, :, 3:780], dev(x), dev(ua), dev(ud))
+    eo, ea = R.verify(p, q, x, ua, ud, None, 777)
+    assert np.array_equal(out.cpu().numpy(), eo) and np.array_equal(acc.cpu().numpy(), ea)
+    with pytest.raises(ValueError):
+        Q.verify_draft(dev(p), dev(q)[:, :2], dev(x), dev(ua), dev(ud))
+    with pytest.raises(ValueError):
+        Q.verify_draft(dev(p).transpose(1, 2), None, dev(x), dev(ua), dev(ud))
+    with pytest.raises(ValueError):
+        Q.verify_draft(dev(p), dev(q), dev(x), dev(ua).double(), dev(ud))
+
+
+# ---- a run of them together -----------------------------------------------------------------------
+def test_speculative_serving_over_a_shared_prompt(Q):
+    """Three chats behind one prompt: in every round each drafts tokens, writes their rows, the target attends over
+    prompt and chat for all of them at once, its probabilities verify the drafts, and the lengths move on by what
+    was accepted.  Every round is replayed in 64 bits from what the cache holds."""
+    import torch
+    rng = np.random.default_rng(77)
+    n, H, kv, hd, V, D, P = 3, 8, 2, 64, 200, 3, 190
+    d = H * hd
+    emb = rng.normal(0, 1, (V, (H + 2 * kv) * hd)).astype(np.float32)         # the fused projection of each token
+    head = rng.normal(0, 0.6, (d, V)).astype(np.float32)
+    cache = Q.GpuKvCache(n + 1, kv, hd, 256)
+    prompt = rng.integers(0, V, P)
+    tk = lambda t: np.asarray(t)  # noqa: E731
+    E = dev(emb)
+
+    def rows(tokens):
+        f = E[dev(tk(tokens).reshape(-1), np.int64)]
+        return f[:, :d].unflatten(1, (H, hd)), f[:, d:d + kv * hd].unflatten(1, (kv, hd)), f[:, d + kv * hd:].unflatten(1, (kv, hd))
+
+    _, k, v = rows(prompt)
+    cache.append(k, v, i32(np.full(P, n)), i32(np.arange(P)))
+    f = type("F", (), {})()
+    f.k = np.zeros((n + 1, 256, kv, hd), np.float32)
+    f.hk, f.hv = f.k.copy(), f.k.copy()
+    put = lambda s, p, t: (f.hk.__setitem__((s, p), R.held(emb[t, d:d + kv * hd].reshape(kv, hd))),  # noqa: E731
+                           f.hv.__setitem__((s, p), R.held(emb[t, d + kv * hd:].reshape(kv, hd))))
+    for p, t in enumerate(prompt):
+        put(n, p, t)
+    last, lens = rng.integers(0, V, n), np.zeros(n, int)
+    slots = np.arange(n)
+    accepted_all = 0
+    for _ in range(6):
+        draft_p = rng.dirichlet(np.full(V, 0.3), (n, D)).astype(np.float32)
+        x = np.array([[rng.choice(V, p=draft_p[b, i].astype(np.float64) / draft_p[b, i].astype(np.float64).sum())
+                       for i in range(D)] for b in range(n)], np.int32)
+        ua, ud = rng.random((n, D), dtype=np.float32), rng.random(n, dtype=np.float32)
+        toks = np.concatenate([last[:, None], x], 1)
+        q, k, v = rows(toks)
+        pos = lens[:, None] + np.arange(D + 1)
+        cache.append(k, v, i32(np.repeat(slots, D + 1)), i32(pos.reshape(-1)))
+        new = i32(lens + D + 1)
+        out = Q.attention_shared(q.reshape(n, D + 1, H, hd), cache, n, P, i32(slots), new, 256)
+        for b in range(n):
+            for i in range(D + 1):
+                put(b, lens[b] + i, toks[b, i])
+        close(out, reference(f, q.reshape(n, D + 1, H, hd).cpu().numpy(), slots, lens + D + 1, (n, P)))
+        logits = out.reshape(n, D + 1, d) @ dev(head)
+        probs = torch.empty_like(logits)
+        for b in range(n):
+            for i in range(D + 1):
+                probs[b, i] = Q.sample(logits[b, i].contiguous(), 0.5, temperature=0.9, top_k=60)[1]
+        # drafts from the target's own neighbourhood, so that some are taken
+        mix = (0.5 * probs[:, :D] + 0.5 * dev(draft_p)).contiguous()
+        got, acc = Q.verify_draft(probs, mix, dev(x), dev(ua), dev(ud))
+        eo, ea = R.verify(probs.cpu().numpy(), mix.cpu().numpy(), x, ua, ud, None, V)
+        assert np.array_equal(got.cpu().numpy(), eo) and np.array_equal(acc.cpu().numpy(), ea)
+        accepted_all += int(ea.sum())
+        lens = lens + 1 + ea                     # the refused drafts' places are written over by the next round
+        last = eo[np.arange(n), ea]
+        assert (last >= 0).all()
+    cache.close()
