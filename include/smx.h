@@ -232,7 +232,7 @@ SMX_API int smx_attention_work_bytes(const smx_kv_cache *c, int n_seq, int n_q, 
  * are scaled by 1 / sqrt(head_dim); n_head a multiple of n_kv_head.  max_len: at least every length (a
  * greater one counts as max_len); a tight bound saves workgroups.  A row that sees nothing, and the rows
  * of a sequence whose slot the cache does not have, are zeros.  work_dev: smx_attention_work_bytes bytes,
- * free for other use when the call's work is done; calls that may overlap, replays of captured graphs among
+ * 16-byte aligned, free for other use when the call's work is done; calls that may overlap, replays of captured graphs among
  * them, need one each. */
 SMX_API int smx_attention_cached(const smx_kv_cache *c, const float *q_dev, int64_t q_stride, float *out_dev, int n_seq,
                                  int n_q, int n_head, const int32_t *slots_dev, const int32_t *lens_dev, int max_len,

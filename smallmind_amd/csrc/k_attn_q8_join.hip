@@ -9,28 +9,39 @@ namespace smx {
 
 namespace {
 
-// One thread per output element: out = sum_s 2^(m_s - M) acc_s / sum_s 2^(m_s - M) l_s over the parts s that
-// have weight, M their largest m.  Rows of a sequence without a slot are 0.
+// Four dims of a row per thread: out = sum_s 2^(m_s - M) acc_s / sum_s 2^(m_s - M) l_s over the parts s that have
+// weight, M their largest m so far.  Rows of a sequence without a slot are 0.
 __global__ __launch_bounds__(256) void k_attn_q8_join(const AttnQ8Args a)
 {
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i >= a.n_rows * a.hd) return;
-    const int64_t row = i / a.hd;
-    const int d = (int)(i - row * a.hd);
+    const int per = a.hd / 4;
+    if (i >= a.n_rows * per) return;
+    const int64_t row = i / per;
+    const int d = 4 * (int)(i - row * per);
     const int seq = (int)(row / ((int64_t)a.n_q * a.n_head));
-    float o = 0.0f, l = 0.0f, top = -__builtin_huge_valf();
-    if ((unsigned)a.slots[seq] < (unsigned)a.n_slots) {
-        for (int s = 0; s < a.parts; s++) top = fmaxf(top, a.part_ml[(s * a.n_rows + row) * 2]);
-        for (int s = 0; s < a.parts; s++) {
-            const float *ml = a.part_ml + (s * a.n_rows + row) * 2;
-            const float m = ml[0], ls = ml[1];
-            if (ls == 0.0f) continue;
-            const float f = __builtin_amdgcn_exp2f(m - top);
-            l += ls * f;
-            o += a.part_acc[(s * a.n_rows + row) * a.hd + d] * f;
-        }
+    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    float l = 0.0f, top = -__builtin_huge_valf();
+    const bool active = (unsigned)a.slots[seq] < (unsigned)a.n_slots;
+#pragma unroll 4
+    for (int s = 0; s < a.parts; s++) {
+        const float2 ml = *(const float2 *)(a.part_ml + (s * a.n_rows + row) * 2);
+        const float4 v = *(const float4 *)(a.part_acc + (s * a.n_rows + row) * a.hd + d);
+        if (ml.y == 0.0f) continue;   // a part without weight may hold anything in v
+        const float up = fmaxf(top, ml.x);
+        // (-inf - -inf where nothing but NaN has been seen: the sum is NaN already)
+        const float f = __builtin_amdgcn_exp2f(ml.x - up), g = l == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(top - up);
+        top = up;
+        l = l * g + ml.y * f;
+        o.x = o.x * g + v.x * f, o.y = o.y * g + v.y * f, o.z = o.z * g + v.z * f, o.w = o.w * g + v.w * f;
     }
-    a.out[i] = l == 0.0f ? 0.0f : o / l;
+    const float inv = !active || l == 0.0f ? 0.0f : 1.0f / l;
+    float *dst = a.out + row * a.hd + d;
+    if (!active) o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (a.out_vec) {
+        *(float4 *)dst = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+    } else {
+        dst[0] = o.x * inv, dst[1] = o.y * inv, dst[2] = o.z * inv, dst[3] = o.w * inv;
+    }
 }
 
 // Chunks of a length that make about `want` workgroups of `units` rows of workgroups: whole multiples of
@@ -49,7 +60,7 @@ bool attn_q8_direct(const AttnQ8Plan &p) { return p.parts == 1 && p.own_splits =
 
 }  // namespace
 
-#define SMX_W(w) hipError_t launch_attn_q8_w##w(const AttnQ8Args &a, int mt_own, int mt_pre, unsigned blocks, hipStream_t s);
+#define SMX_W(w) hipError_t launch_attn_q8_w##w(const AttnQ8Args &a, AttnQ8Pre pre, int mt_pre, unsigned blocks, hipStream_t s);
 SMX_W(32) SMX_W(64) SMX_W(96) SMX_W(128) SMX_W(160) SMX_W(192) SMX_W(224) SMX_W(256)
 #undef SMX_W
 
@@ -57,15 +68,19 @@ AttnQ8Plan attn_q8_plan(const KvView &c, int n_seq, int n_q, int n_head, int pre
 {
     AttnQ8Plan p{};
     const int64_t group = n_head / c.n_kv, own_rows = n_q * group, pre_rows = n_seq * own_rows;
-    // two blocks of rows share a wave's codes
-    const bool two = c.w <= 128 ? kAttnQ8TwoBlocks<128> : kAttnQ8TwoBlocks<256>;
-    p.mt_own = two && own_rows > 16 ? 2 : 1;
-    p.mt_pre = two && pre_rows > 16 ? 2 : 1;
-    p.own_blocks = (int)((own_rows + 16 * p.mt_own - 1) / (16 * p.mt_own));
-    p.pre_blocks = (int)((pre_rows + 16 * p.mt_pre - 1) / (16 * p.mt_pre));
+    p.own_blocks = (int)((own_rows + 15) / 16);
+    p.mt_pre = 1;
+    if (prefix_len > 0) {
+        // one block of rows: nothing to share; from there on the tiles are turned into fp16 once for all waves,
+        // and two blocks per wave share what it reads of them
+        p.pre = pre_rows > 16 ? PRE_ROWS : PRE_STREAM;
+        if (pre_rows > 64 && (c.w <= 128 ? kAttnQ8TwoBlocks<128> : kAttnQ8TwoBlocks<256>)) p.mt_pre = 2;
+        const int block = p.pre == PRE_ROWS ? 64 * p.mt_pre : 16;
+        p.pre_blocks = (int)((pre_rows + block - 1) / block);
+    }
     const int64_t own_units = (int64_t)n_seq * c.n_kv * p.own_blocks, pre_units = (int64_t)c.n_kv * p.pre_blocks;
     cut(max_len, own_units, 2048, &p.own_chunk, &p.own_splits);
-    cut(prefix_len, pre_units, 2048, &p.pre_chunk, &p.pre_splits);
+    if (prefix_len > 0) cut(prefix_len, pre_units, p.pre == PRE_ROWS ? 512 : 2048, &p.pre_chunk, &p.pre_splits);
     p.parts = p.own_splits + p.pre_splits;
     p.pre_wgs = pre_units * p.pre_splits;
     p.blocks = p.pre_wgs + own_units * p.own_splits;
@@ -91,6 +106,7 @@ hipError_t launch_attn_q8(const KvView &c, const AttnQ8Plan &p, const float *q, 
     a.q_stride = q_stride;
     a.scale_log2e = (float)(1.4426950408889634 / sqrt((double)c.hd));
     a.q_vec = ((uintptr_t)q & 15) == 0 && q_stride % 4 == 0;
+    a.out_vec = ((uintptr_t)out & 15) == 0;
     a.n_slots = c.n_slots;
     a.n_seq = n_seq;
     a.n_q = n_q;
@@ -110,13 +126,13 @@ hipError_t launch_attn_q8(const KvView &c, const AttnQ8Plan &p, const float *q, 
     a.direct = attn_q8_direct(p);
     if (p.blocks) {
         hipError_t e = hipErrorInvalidValue;
-#define SMX_W(w) case w: e = launch_attn_q8_w##w(a, p.mt_own, p.mt_pre, (unsigned)p.blocks, s); break;
+#define SMX_W(w) case w: e = launch_attn_q8_w##w(a, p.pre, p.mt_pre, (unsigned)p.blocks, s); break;
         switch (c.w) { SMX_W(32) SMX_W(64) SMX_W(96) SMX_W(128) SMX_W(160) SMX_W(192) SMX_W(224) SMX_W(256) }
 #undef SMX_W
         if (e != hipSuccess) return e;
     }
     if (a.direct) return hipSuccess;
-    k_attn_q8_join<<<(unsigned)((a.n_rows * c.hd + 255) / 256), 256, 0, s>>>(a);
+    k_attn_q8_join<<<(unsigned)((a.n_rows * (c.hd / 4) + 255) / 256), 256, 0, s>>>(a);
     return hipGetLastError();
 }
 

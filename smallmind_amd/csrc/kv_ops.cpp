@@ -70,7 +70,8 @@ int attend(const smx_kv_cache *c, const float *q, int64_t q_stride, float *out, 
         SMX_FAIL(SMX_EINVAL, "%s: prefix_slot %d of %d slots", fn, prefix_slot, c->view.n_slots);
     if (q_stride < (int64_t)n_head * c->view.hd)
         SMX_FAIL(SMX_EINVAL, "%s: q_stride %lld is less than n_head * head_dim", fn, (long long)q_stride);
-    if (((uintptr_t)q | (uintptr_t)out | (uintptr_t)work) & 3) SMX_FAIL(SMX_EINVAL, "%s: misaligned pointer", fn);
+    if (((uintptr_t)q | (uintptr_t)out) & 3) SMX_FAIL(SMX_EINVAL, "%s: misaligned pointer", fn);
+    if ((uintptr_t)work & 15) SMX_FAIL(SMX_EINVAL, "%s: the work memory must be 16-byte aligned", fn);
     if (plan.work_bytes > 0 && (!work || work_bytes < plan.work_bytes))
         SMX_FAIL(SMX_EINVAL, "%s: needs %lld bytes of work memory, has %lld", fn, (long long)plan.work_bytes,
                  (long long)(work ? work_bytes : 0));

@@ -9,9 +9,12 @@
 
 namespace smx {
 
-// Whether a wave may take two 16-row blocks at rows of this width: wider ones leave registers for one.
+// Whether a wave may take two 16-row blocks of a prefix's rows at this width: wider ones leave registers for one.
 template <int W>
 constexpr bool kAttnQ8TwoBlocks = W <= 128;
+
+// How the rows go through the prefix (k_attn_q8.hip).
+enum AttnQ8Pre { PRE_NONE, PRE_STREAM, PRE_ROWS };
 
 struct AttnQ8Args {
     const float *q;             // token t, head h at t * q_stride + h * hd
@@ -22,7 +25,7 @@ struct AttnQ8Args {
     float *part_ml, *part_acc;  // [parts][n_rows][2], [parts][n_rows][hd]
     int64_t q_stride, n_rows;   // n_rows = n_seq * n_q * n_head
     float scale_log2e;          // log2(e) / sqrt(hd)
-    int q_vec;                  // rows of q may be read as float4
+    int q_vec, out_vec;         // q, out may be read and written as float4
     int n_slots, n_seq, n_q, n_head, n_kv, hd;
     int max_len, own_chunk, own_splits, own_blocks;
     int prefix_slot, prefix_len, pre_chunk, pre_splits, pre_wgs;
@@ -32,7 +35,8 @@ struct AttnQ8Args {
 
 // How a call is cut up.
 struct AttnQ8Plan {
-    int mt_own, mt_pre;         // 16-row blocks per wave
+    int mt_pre;                 // 16-row blocks per wave (PRE_ROWS)
+    AttnQ8Pre pre;
     int own_chunk, own_splits, own_blocks;
     int pre_chunk, pre_splits, pre_blocks;
     int parts;
