@@ -53,6 +53,7 @@ constexpr int NC = W / 64;               // 64-wide pieces of a K row: 16 bytes 
 constexpr bool TAIL = W % 64 != 0;       // and a 32-wide one: 8 bytes per lane
 constexpr int NK = W / 32;               // matrix instructions along a K row
 constexpr int ND = W / 16;               // 16-dim groups of the output
+constexpr int NW = 4;                    // waves of a workgroup
 constexpr float kNegInf = -__builtin_huge_valf();
 constexpr float kLeast = 7.8886090522101181e-31f;   // 2^-100: no power of two below it is used as a scale
 
@@ -145,10 +146,10 @@ struct RowRef {          // a row of the batch
     int token, head;     // token: sequence * n_q + i
 };
 
-// Joining of the four waves' sums.
+// Joining of a workgroup's NW waves' sums.
 struct Shared {
-    float m[4][16], l[4][16];
-    float acc[4][16][W + 4];
+    float m[NW][16], l[NW][16];
+    float acc[NW][16][W + 4];
 };
 
 // The rows' queries as the second operands of K q^T, and c in the units of their products.
@@ -357,7 +358,7 @@ struct Running {
     }
 };
 
-// stream: the four waves take the tiles of positions [p0, p1) in turn; vis_of(row): positions that the row
+// stream: the NW waves take the tiles of positions [p0, p1) in turn; vis_of(row): positions that the row
 // sees, counted from the slot's first, min_vis at least.
 template <typename RowOf, typename VisOf>
 __device__ __forceinline__ void stream(const AttnQ8Args &a, Shared &S, const uint8_t *cache, int p0, int p1, int min_vis,
@@ -367,12 +368,6 @@ __device__ __forceinline__ void stream(const AttnQ8Args &a, Shared &S, const uin
     const int n_tiles = (p1 - p0 + kKvTile - 1) / kKvTile;
     constexpr size_t REC = kv_tile_bytes(W);
 
-    half8 qh[1][NK], ql[1][NK];
-    Running<1> R;
-    R.clear();
-    load_q<1>(a, qh, ql, R.c, g, col, row_of);
-    const int vis = row_of(col).valid ? vis_of(col) : 0;
-
     const uint8_t *rec = cache + (size_t)(p0 / kKvTile + wave) * REC;
     KTile kt;
     VTile vt;
@@ -380,9 +375,15 @@ __device__ __forceinline__ void stream(const AttnQ8Args &a, Shared &S, const uin
         load_k(kt, rec, g, col);
         load_v(vt, rec, g, col);
     }
+    half8 qh[1][NK], ql[1][NK];
+    Running<1> R;
+    R.clear();
+    load_q<1>(a, qh, ql, R.c, g, col, row_of);
+    const int vis = row_of(col).valid ? vis_of(col) : 0;
+
     // tiles that every row sees all of, then the rest: the same code with and without the bounds
     const auto go = [&](int &tile, int end, auto whole) {
-        for (; tile < end; tile += 4) {
+        for (; tile < end; tile += NW) {
             const float *scales = (const float *)(rec + 2 * kKvTile * W);
             float4v ks[4], vs[4];
 #pragma unroll
@@ -391,8 +392,8 @@ __device__ __forceinline__ void stream(const AttnQ8Args &a, Shared &S, const uin
                 vs[t] = *(const float4v *)(scales + kKvTile + 16 * t + 4 * g);
             }
             const float vone = scales[kKvTile + lane];
-            rec += 4 * REC;
-            const bool more = tile + 4 < n_tiles;
+            rec += NW * REC;
+            const bool more = tile + NW < n_tiles;
             float4v x[1][4];
             scores<1>(x, qh, ql, [&](int t, int n) {
                 if (TAIL && n == NK - 1) return halves(kt.b[t][0], kt.b[t][1]);
@@ -422,21 +423,21 @@ __device__ __forceinline__ void stream(const AttnQ8Args &a, Shared &S, const uin
     __syncthreads();
 }
 
-// Joins the four waves' sums and writes the rows: the outputs, or with more parts to come the part's
+// Joins the waves' sums and writes the rows: the outputs, or with more parts to come the part's
 // maximum (in powers of two), sum and weighted sums.
 template <typename RowOf>
 __device__ __forceinline__ void finish(const AttnQ8Args &a, Shared &S, int part, RowOf row_of)
 {
-    for (int i = threadIdx.x; i < 16 * (W / 4); i += 256) {
+    for (int i = threadIdx.x; i < 16 * (W / 4); i += 64 * NW) {
         const int row = i / (W / 4), d = 4 * (i % (W / 4));
         const RowRef r = row_of(row);
         if (!r.valid || d >= a.hd) continue;
         float top = kNegInf, sum = 0.0f;
 #pragma unroll
-        for (int w = 0; w < 4; w++) top = fmaxf(top, S.m[w][row]);
+        for (int w = 0; w < NW; w++) top = fmaxf(top, S.m[w][row]);
         float4v o = {0, 0, 0, 0};
 #pragma unroll
-        for (int w = 0; w < 4; w++) {
+        for (int w = 0; w < NW; w++) {
             // a wave without a visible position has the sum 0 (and one that saw NaN a NaN)
             const float f = S.m[w][row] == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(S.m[w][row] - top);
             if (S.l[w][row] == 0.0f) continue;
@@ -552,9 +553,10 @@ __device__ __forceinline__ void rows(const AttnQ8Args &a, Tiles &S, const uint8_
     }
 }
 
-// PRE, MTP: how the prefix is gone through, and 16-row blocks per wave there; the sequences' own positions: stream.
+// PRE, MTP: how the prefix is gone through, and 16-row blocks per wave there; the sequences' own positions:
+// stream.
 template <AttnQ8Pre PRE, int MTP>
-__global__ __launch_bounds__(256, W <= 128 ? 2 : 1) void k_attn_q8(const AttnQ8Args a)
+__global__ __launch_bounds__(64 * NW, W <= 64 && MTP == 1 ? 3 : W <= 128 ? 2 : 1) void k_attn_q8(const AttnQ8Args a)
 {
     union Mem {
         Shared own;
@@ -599,7 +601,7 @@ __global__ __launch_bounds__(256, W <= 128 ? 2 : 1) void k_attn_q8(const AttnQ8A
     const int part = a.pre_splits + split;
     if (p0 >= p1) {
         // nothing here: zeros, or a part without weight
-        for (int i = threadIdx.x; i < 16 * W; i += 256) {
+        for (int i = threadIdx.x; i < 16 * W; i += 64 * NW) {
             const int row = i / W, d = i % W;
             const RowRef r = row_of(row);
             if (!r.valid || d >= a.hd) continue;
@@ -623,12 +625,13 @@ __global__ __launch_bounds__(256, W <= 128 ? 2 : 1) void k_attn_q8(const AttnQ8A
 
 #define SMX_LAUNCH_NAME_(w) launch_attn_q8_w##w
 #define SMX_LAUNCH_NAME(w) SMX_LAUNCH_NAME_(w)
-hipError_t SMX_LAUNCH_NAME(SMX_ATTN_W)(const AttnQ8Args &a, AttnQ8Pre pre, int mt_pre, unsigned blocks, hipStream_t s)
+hipError_t SMX_LAUNCH_NAME(SMX_ATTN_W)(const AttnQ8Args &a, const AttnQ8Plan &p, hipStream_t s)
 {
-    if (pre == PRE_NONE) k_attn_q8<PRE_NONE, 1><<<blocks, 256, 0, s>>>(a);
-    else if (pre == PRE_STREAM) k_attn_q8<PRE_STREAM, 1><<<blocks, 256, 0, s>>>(a);
-    else if (mt_pre == 1) k_attn_q8<PRE_ROWS, 1><<<blocks, 256, 0, s>>>(a);
-    else if constexpr (kAttnQ8TwoBlocks<SMX_ATTN_W>) k_attn_q8<PRE_ROWS, 2><<<blocks, 256, 0, s>>>(a);
+    const unsigned blocks = (unsigned)p.blocks;
+    if (p.pre == PRE_NONE) k_attn_q8<PRE_NONE, 1><<<blocks, 64 * NW, 0, s>>>(a);
+    else if (p.pre == PRE_STREAM) k_attn_q8<PRE_STREAM, 1><<<blocks, 64 * NW, 0, s>>>(a);
+    else if (p.mt_pre == 1) k_attn_q8<PRE_ROWS, 1><<<blocks, 64 * NW, 0, s>>>(a);
+    else if constexpr (kAttnQ8Narrow<SMX_ATTN_W>) k_attn_q8<PRE_ROWS, 2><<<blocks, 64 * NW, 0, s>>>(a);
     else return hipErrorInvalidValue;
     return hipGetLastError();
 }

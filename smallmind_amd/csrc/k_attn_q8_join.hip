@@ -9,38 +9,72 @@ namespace smx {
 
 namespace {
 
-// Four dims of a row per thread: out = sum_s 2^(m_s - M) acc_s / sum_s 2^(m_s - M) l_s over the parts s that have
-// weight, M their largest m so far.  Rows of a sequence without a slot are 0.
+// out = sum_s 2^(m_s - M) acc_s / sum_s 2^(m_s - M) l_s over the parts s that have weight, M their largest m.
+// What bounds it is the latency of the parts' loads, so a thread takes four dims of every PP-th part of a row,
+// requested four at a time, and PP threads join theirs through LDS in a fixed order.  Rows of a sequence
+// without a slot are 0.
+struct Joined {
+    float4 o;
+    float l, top;
+};
+
+__device__ __forceinline__ void join(Joined &a, float4 v, float l, float m)
+{
+    if (l == 0.0f) return;   // a part without weight may hold anything in v
+    const float up = fmaxf(a.top, m);
+    // (-inf - -inf where nothing but NaN has been seen: the sum is NaN already)
+    const float f = __builtin_amdgcn_exp2f(m - up), g = a.l == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(a.top - up);
+    a.top = up;
+    a.l = a.l * g + l * f;
+    a.o.x = a.o.x * g + v.x * f, a.o.y = a.o.y * g + v.y * f;
+    a.o.z = a.o.z * g + v.z * f, a.o.w = a.o.w * g + v.w * f;
+}
+
+template <int PP>
 __global__ __launch_bounds__(256) void k_attn_q8_join(const AttnQ8Args a)
 {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    constexpr int R = 256 / PP;   // threads of a block that each have other outputs
+    __shared__ Joined S[PP > 1 ? PP - 1 : 1][PP > 1 ? R : 1];
+    const int lane = threadIdx.x % R, pp = threadIdx.x / R;
+    const int64_t i = (int64_t)blockIdx.x * R + lane;
     const int per = a.hd / 4;
-    if (i >= a.n_rows * per) return;
-    const int64_t row = i / per;
-    const int d = 4 * (int)(i - row * per);
-    const int seq = (int)(row / ((int64_t)a.n_q * a.n_head));
-    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    float l = 0.0f, top = -__builtin_huge_valf();
-    const bool active = (unsigned)a.slots[seq] < (unsigned)a.n_slots;
-#pragma unroll 4
-    for (int s = 0; s < a.parts; s++) {
-        const float2 ml = *(const float2 *)(a.part_ml + (s * a.n_rows + row) * 2);
-        const float4 v = *(const float4 *)(a.part_acc + (s * a.n_rows + row) * a.hd + d);
-        if (ml.y == 0.0f) continue;   // a part without weight may hold anything in v
-        const float up = fmaxf(top, ml.x);
-        // (-inf - -inf where nothing but NaN has been seen: the sum is NaN already)
-        const float f = __builtin_amdgcn_exp2f(ml.x - up), g = l == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(top - up);
-        top = up;
-        l = l * g + ml.y * f;
-        o.x = o.x * g + v.x * f, o.y = o.y * g + v.y * f, o.z = o.z * g + v.z * f, o.w = o.w * g + v.w * f;
+    const bool in = i < a.n_rows * per;
+    const int64_t row = in ? i / per : 0;
+    const int d = in ? 4 * (int)(i - row * per) : 0;
+    Joined J{make_float4(0.0f, 0.0f, 0.0f, 0.0f), 0.0f, -__builtin_huge_valf()};
+    for (int s0 = pp; s0 < a.parts; s0 += 4 * PP) {
+        float2 ml[4];
+        float4 v[4];
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const int s = min(s0 + k * PP, a.parts - 1);
+            ml[k] = *(const float2 *)(a.part_ml + (s * a.n_rows + row) * 2);
+            v[k] = *(const float4 *)(a.part_acc + (s * a.n_rows + row) * a.hd + d);
+        }
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+            if (s0 + k * PP < a.parts) join(J, v[k], ml[k].y, ml[k].x);
     }
-    const float inv = !active || l == 0.0f ? 0.0f : 1.0f / l;
+    if constexpr (PP > 1) {
+        if (pp > 0) S[pp - 1][lane] = J;
+        __syncthreads();
+        if (pp > 0) return;
+#pragma unroll
+        for (int k = 0; k < PP - 1; k++) {
+            const Joined &T = S[k][lane];
+            join(J, T.o, T.l, T.top);
+        }
+    }
+    if (!in) return;
+    const int seq = (int)(row / ((int64_t)a.n_q * a.n_head));
+    const bool active = (unsigned)a.slots[seq] < (unsigned)a.n_slots;
+    const float inv = !active || J.l == 0.0f ? 0.0f : 1.0f / J.l;
+    if (!active) J.o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     float *dst = a.out + row * a.hd + d;
-    if (!active) o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     if (a.out_vec) {
-        *(float4 *)dst = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+        *(float4 *)dst = make_float4(J.o.x * inv, J.o.y * inv, J.o.z * inv, J.o.w * inv);
     } else {
-        dst[0] = o.x * inv, dst[1] = o.y * inv, dst[2] = o.z * inv, dst[3] = o.w * inv;
+        dst[0] = J.o.x * inv, dst[1] = J.o.y * inv, dst[2] = J.o.z * inv, dst[3] = J.o.w * inv;
     }
 }
 
@@ -60,7 +94,7 @@ bool attn_q8_direct(const AttnQ8Plan &p) { return p.parts == 1 && p.own_splits =
 
 }  // namespace
 
-#define SMX_W(w) hipError_t launch_attn_q8_w##w(const AttnQ8Args &a, AttnQ8Pre pre, int mt_pre, unsigned blocks, hipStream_t s);
+#define SMX_W(w) hipError_t launch_attn_q8_w##w(const AttnQ8Args &a, const AttnQ8Plan &p, hipStream_t s);
 SMX_W(32) SMX_W(64) SMX_W(96) SMX_W(128) SMX_W(160) SMX_W(192) SMX_W(224) SMX_W(256)
 #undef SMX_W
 
@@ -68,19 +102,20 @@ AttnQ8Plan attn_q8_plan(const KvView &c, int n_seq, int n_q, int n_head, int pre
 {
     AttnQ8Plan p{};
     const int64_t group = n_head / c.n_kv, own_rows = n_q * group, pre_rows = n_seq * own_rows;
+    const bool narrow = c.w <= 128 ? kAttnQ8Narrow<128> : kAttnQ8Narrow<256>;
     p.own_blocks = (int)((own_rows + 15) / 16);
     p.mt_pre = 1;
     if (prefix_len > 0) {
         // one block of rows: nothing to share; from there on the tiles are turned into fp16 once for all waves,
         // and two blocks per wave share what it reads of them
         p.pre = pre_rows > 16 ? PRE_ROWS : PRE_STREAM;
-        if (pre_rows > 64 && (c.w <= 128 ? kAttnQ8TwoBlocks<128> : kAttnQ8TwoBlocks<256>)) p.mt_pre = 2;
+        if (pre_rows > 64 && narrow) p.mt_pre = 2;
         const int block = p.pre == PRE_ROWS ? 64 * p.mt_pre : 16;
         p.pre_blocks = (int)((pre_rows + block - 1) / block);
     }
     const int64_t own_units = (int64_t)n_seq * c.n_kv * p.own_blocks, pre_units = (int64_t)c.n_kv * p.pre_blocks;
-    cut(max_len, own_units, 2048, &p.own_chunk, &p.own_splits);
-    if (prefix_len > 0) cut(prefix_len, pre_units, p.pre == PRE_ROWS ? 512 : 2048, &p.pre_chunk, &p.pre_splits);
+    cut(max_len, own_units, 512, &p.own_chunk, &p.own_splits);
+    if (prefix_len > 0) cut(prefix_len, pre_units, 256, &p.pre_chunk, &p.pre_splits);
     p.parts = p.own_splits + p.pre_splits;
     p.pre_wgs = pre_units * p.pre_splits;
     p.blocks = p.pre_wgs + own_units * p.own_splits;
@@ -126,13 +161,17 @@ hipError_t launch_attn_q8(const KvView &c, const AttnQ8Plan &p, const float *q, 
     a.direct = attn_q8_direct(p);
     if (p.blocks) {
         hipError_t e = hipErrorInvalidValue;
-#define SMX_W(w) case w: e = launch_attn_q8_w##w(a, p.pre, p.mt_pre, (unsigned)p.blocks, s); break;
+#define SMX_W(w) case w: e = launch_attn_q8_w##w(a, p, s); break;
         switch (c.w) { SMX_W(32) SMX_W(64) SMX_W(96) SMX_W(128) SMX_W(160) SMX_W(192) SMX_W(224) SMX_W(256) }
 #undef SMX_W
         if (e != hipSuccess) return e;
     }
     if (a.direct) return hipSuccess;
-    k_attn_q8_join<<<(unsigned)((a.n_rows * (c.hd / 4) + 255) / 256), 256, 0, s>>>(a);
+    // about four parts per thread
+    const int64_t n = a.n_rows * (c.hd / 4);
+    if (p.parts <= 4) k_attn_q8_join<1><<<(unsigned)((n + 255) / 256), 256, 0, s>>>(a);
+    else if (p.parts <= 16) k_attn_q8_join<4><<<(unsigned)((n + 63) / 64), 256, 0, s>>>(a);
+    else k_attn_q8_join<16><<<(unsigned)((n + 15) / 16), 256, 0, s>>>(a);
     return hipGetLastError();
 }
 

@@ -9,9 +9,9 @@
 
 namespace smx {
 
-// Whether a wave may take two 16-row blocks of a prefix's rows at this width: wider ones leave registers for one.
+// Rows of up to 128 leave registers for two 16-row blocks of a prefix's rows per wave, and for two waves per SIMD.
 template <int W>
-constexpr bool kAttnQ8TwoBlocks = W <= 128;
+constexpr bool kAttnQ8Narrow = W <= 128;
 
 // How the rows go through the prefix (k_attn_q8.hip).
 enum AttnQ8Pre { PRE_NONE, PRE_STREAM, PRE_ROWS };
