@@ -43,6 +43,7 @@ namespace smx {
 namespace {
 
 typedef _Float16 half2v __attribute__((ext_vector_type(2)));
+typedef _Float16 half4v __attribute__((ext_vector_type(4)));
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef float float4v __attribute__((ext_vector_type(4)));
 typedef uint32_t uint4v __attribute__((ext_vector_type(4)));
@@ -53,7 +54,6 @@ constexpr int NC = W / 64;               // 64-wide pieces of a K row: 16 bytes 
 constexpr bool TAIL = W % 64 != 0;       // and a 32-wide one: 8 bytes per lane
 constexpr int NK = W / 32;               // matrix instructions along a K row
 constexpr int ND = W / 16;               // 16-dim groups of the output
-constexpr int NW = 4;                    // waves of a workgroup
 constexpr float kNegInf = -__builtin_huge_valf();
 constexpr float kLeast = 7.8886090522101181e-31f;   // 2^-100: no power of two below it is used as a scale
 
@@ -77,11 +77,22 @@ __device__ __forceinline__ float pow2_above(float f)
     return __uint_as_float((__float_as_uint(f) + 0x7FFFFFu) & 0x7F800000u);
 }
 
+// Brings a tile's V scales, a position's per lane, below 2^14 by a power of two that grows with them; returns what
+// sums in the old power's units are multiplied with.  (NaN scales stay NaN and do not count.)
+struct VUnit {
+    float up = kLeast;   // the power of two, at least every scale so far
+    __device__ __forceinline__ float take(float &scale);
+};
+
 // Two values as fp16 parts: h the nearest, l what is left.
 __device__ __forceinline__ void split(float a, float b, half2v &h, half2v &l)
 {
     h = half2v{(_Float16)a, (_Float16)b};
-    l = half2v{(_Float16)__builtin_fmaf((float)h[0], -1.0f, a), (_Float16)__builtin_fmaf((float)h[1], -1.0f, b)};
+    // a - h exactly, h read as fp16 by the same instruction (written as such, the compiler converts h first)
+    float ra, rb;
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(ra) : "v"(h), "v"(a));
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(rb) : "v"(h), "v"(b));
+    l = half2v{(_Float16)ra, (_Float16)rb};
 }
 
 __device__ __forceinline__ void put(half8 &v, int at, half2v h) { v[at] = h[0], v[at + 1] = h[1]; }
@@ -91,6 +102,12 @@ __device__ __forceinline__ float max_groups(float v)   // over the four lanes of
     float2 p = swap32(v, v);
     v = fmaxf(p.x, p.y);
     p = swap16(v, v);
+    return fmaxf(p.x, p.y);
+}
+
+__device__ __forceinline__ float max_halves(float v)   // of lanes l and l ^ 32
+{
+    const float2 p = swap32(v, v);
     return fmaxf(p.x, p.y);
 }
 
@@ -112,8 +129,32 @@ __device__ __forceinline__ float sum_groups(float v)
 }
 
 // Keeps the compiler from moving instructions across: without it, it fetches all operands of a tile before
-// the first product and runs out of registers.
+// the first product and runs out of registers, or fetches them right where they are used and waits.
 __device__ __forceinline__ void here() { __builtin_amdgcn_sched_barrier(0); }
+
+// A wave-uniform flag that the compiler takes for a new one at every use: a loop that asks for it is not copied for
+// each of its values.
+__device__ __forceinline__ bool asked(int flag)
+{
+    asm volatile("" : "+v"(flag));
+    return __builtin_amdgcn_readfirstlane(flag) != 0;
+}
+
+// Orders a wave's own accesses to LDS: what some lanes write, others read.
+__device__ __forceinline__ void wave_fence()
+{
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
+__device__ __forceinline__ float VUnit::take(float &scale)
+{
+    const float was = up;
+    up = fmaxf(up, pow2_above(max_lanes(fmaxf(scale, kLeast))));
+    const float down = __uint_as_float((254u << 23) - __float_as_uint(up));   // 1 / up
+    scale *= 16384.0f * down;
+    return was * down;
+}
 
 struct KTile {
     uint4v a[4][NC > 0 ? NC : 1];
@@ -146,219 +187,213 @@ struct RowRef {          // a row of the batch
     int token, head;     // token: sequence * n_q + i
 };
 
-// Joining of a workgroup's NW waves' sums.
-struct Shared {
-    float m[NW][16], l[NW][16];
-    float acc[NW][16][W + 4];
+// id / group: the product with the rounded reciprocal is off by less than 2^-20 (id < 2^28, group < 2^16) and the half
+// keeps it that far from whole numbers.
+__device__ __forceinline__ int by_group(int id, double inv_group) { return (int)(((double)id + 0.5) * inv_group); }
+
+
+// Sixteen rows' queries on their way from memory, read row by row, to the lanes of the second operands of K q^T.
+// The 16-byte chunks of row r are permuted by r, so that 16 lanes reading one chunk of 16 rows meet few bank conflicts.
+struct QRows {
+    float4v c[16][W / 4];
 };
 
-// The rows' queries as the second operands of K q^T, and c in the units of their products.
-template <int MT, typename RowOf>
-__device__ __forceinline__ void load_q(const AttnQ8Args &a, half8 (&qh)[MT][NK], half8 (&ql)[MT][NK], float (&c)[MT], int g,
-                                       int col, RowOf row_of)
+// Chunks of rows, `count` threads from `first` on; rows that do not exist and dims beyond head_dim are 0.
+template <typename RowOf>
+__device__ __forceinline__ void bring_q(const AttnQ8Args &a, QRows &S, int first, int count, RowOf row_of)
 {
-#pragma unroll
-    for (int mt = 0; mt < MT; mt++) {
-        const RowRef r = row_of(16 * mt + col);
-        const float *q = a.q + (int64_t)r.token * a.q_stride + (int64_t)r.head * a.hd;
-        float f[NK][8];
-        uint32_t top = 0;
-#pragma unroll
-        for (int n = 0; n < NK; n++) {
-            // the dims of this lane's bytes: 16 g + 8 (n % 2) of piece n / 2, 8 g of the 32-wide one
-            const int d = TAIL && n == NK - 1 ? 64 * NC + 8 * g : 64 * (n >> 1) + 16 * g + 8 * (n & 1);
-            const bool in = r.valid && d < a.hd;   // head_dim is a multiple of 8
+    for (int i = first; i < 16 * (W / 4); i += count) {
+        const int row = i / (W / 4), ch = i % (W / 4);
+        const RowRef r = row_of(row);
+        float4v f = {0, 0, 0, 0};
+        if (r.valid && 4 * ch < a.hd) {
+            const float *q = a.q + (int64_t)r.token * a.q_stride + (int64_t)r.head * a.hd + 4 * ch;
             if (a.q_vec) {
-                float4v u = {0, 0, 0, 0}, v = {0, 0, 0, 0};
-                if (in) u = *(const float4v *)(q + d), v = *(const float4v *)(q + d + 4);
-#pragma unroll
-                for (int e = 0; e < 4; e++) f[n][e] = u[e], f[n][4 + e] = v[e];
+                f = *(const float4v *)q;
             } else {
 #pragma unroll
-                for (int e = 0; e < 8; e++) f[n][e] = in ? q[d + e] : 0.0f;
+                for (int e = 0; e < 4; e++) f[e] = q[e];
             }
-#pragma unroll
-            for (int e = 0; e < 8; e++) top = max(top, __float_as_uint(f[n][e]) & 0x7FFFFFFFu);
         }
-        const float amax = max_groups(__uint_as_float(min(top, 0x7F7FFFFFu)));
-        const bool bad = max_groups(top > 0x7F7FFFFFu ? 1.0f : 0.0f) > 0.0f;   // a NaN or infinity: the row is NaN
-        const float unit = amax > kLeast ? __uint_as_float(__float_as_uint(amax) & 0x7F800000u) : kLeast;   // 2^e
-        const float mul = bad ? __uint_as_float(0x7FC00000u) : __uint_as_float((268u << 23) - __float_as_uint(unit));   // 2^14 / unit
-        c[mt] = a.scale_log2e * (unit * (1.0f / 16384.0f));
-#pragma unroll
-        for (int n = 0; n < NK; n++)
-#pragma unroll
-            for (int e = 0; e < 8; e += 2) {
-                half2v h, l;
-                split(f[n][e] * mul, f[n][e + 1] * mul, h, l);
-                put(qh[mt][n], e, h);
-                put(ql[mt][n], e, l);
-            }
+        S.c[row][ch ^ (row & 7)] = f;
     }
 }
 
+// The power of two that a row of q is brought to the range of fp16 with, and c in the units of the products.
+struct QScale {
+    float mul, c;
+};
+// amax: the largest finite element; bad: the row holds a NaN or an infinity, and becomes NaN.
+__device__ __forceinline__ QScale q_scale(const AttnQ8Args &a, float amax, bool bad)
+{
+    const float unit = amax > kLeast ? __uint_as_float(__float_as_uint(amax) & 0x7F800000u) : kLeast;   // 2^e
+    const float mul = __uint_as_float((268u << 23) - __float_as_uint(unit));                            // 2^14 / unit
+    return QScale{bad ? __uint_as_float(0x7FC00000u) : mul, a.scale_log2e * (unit * (1.0f / 16384.0f))};
+}
+
+// The operands of the rows in S, and c.
+__device__ __forceinline__ void take_q(const AttnQ8Args &a, const QRows &S, half8 (&qh)[NK], half8 (&ql)[NK], float &c, int g, int col)
+{
+    float4v f[NK][2];
+    uint32_t top = 0;
+#pragma unroll
+    for (int n = 0; n < NK; n++) {
+        // the dims of this lane's bytes: 16 g + 8 (n % 2) of piece n / 2, 8 g of the 32-wide one
+        const int d = TAIL && n == NK - 1 ? 64 * NC + 8 * g : 64 * (n >> 1) + 16 * g + 8 * (n & 1);
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+            f[n][j] = S.c[col][(d / 4 + j) ^ (col & 7)];
+#pragma unroll
+            for (int e = 0; e < 4; e++) top = max(top, __float_as_uint(f[n][j][e]) & 0x7FFFFFFFu);
+        }
+    }
+    const QScale q = q_scale(a, max_groups(__uint_as_float(min(top, 0x7F7FFFFFu))), max_groups(top > 0x7F7FFFFFu ? 1.0f : 0.0f) > 0.0f);
+    c = q.c;
+#pragma unroll
+    for (int n = 0; n < NK; n++)
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) {
+            half2v h, l;
+            split(f[n][e >> 2][e & 3] * q.mul, f[n][e >> 2][(e & 3) + 1] * q.mul, h, l);
+            put(qh[n], e, h);
+            put(ql[n], e, l);
+        }
+}
+
 // x = K q^T of a tile; k_of(t, n): the codes of positions 16 t .. as operand n along the row.  The operands of
-// the next n are made ready beside the products of this one; the products of four position groups lie
-// between two that add to the same sum.
-template <int MT, typename KOf>
-__device__ __forceinline__ void scores(float4v (&x)[MT][4], const half8 (&qh)[MT][NK], const half8 (&ql)[MT][NK], KOf k_of)
+// the next n are made ready (LDS: requested) before the products of this one; the products of four
+// position groups lie between two that add to the same sum.
+template <bool LDS, typename KOf>
+__device__ __forceinline__ void scores(float4v (&x)[4], const half8 (&qh)[NK], const half8 (&ql)[NK], KOf k_of)
 {
     half8 k[2][4];
 #pragma unroll
     for (int t = 0; t < 4; t++) {
         k[0][t] = k_of(t, 0);
-#pragma unroll
-        for (int mt = 0; mt < MT; mt++) x[mt][t] = float4v{0, 0, 0, 0};
+        x[t] = float4v{0, 0, 0, 0};
     }
 #pragma unroll
     for (int n = 0; n < NK; n++) {
         if (n + 1 < NK) {
 #pragma unroll
             for (int t = 0; t < 4; t++) k[(n + 1) & 1][t] = k_of(t, n + 1);
+            if (LDS) here();
         }
 #pragma unroll
-        for (int mt = 0; mt < MT; mt++)
+        for (int t = 0; t < 4; t++) x[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[n & 1][t], qh[n], x[t], 0, 0, 0);
 #pragma unroll
-            for (int t = 0; t < 4; t++)
-                x[mt][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[n & 1][t], qh[mt][n], x[mt][t], 0, 0, 0);
-#pragma unroll
-        for (int mt = 0; mt < MT; mt++)
-#pragma unroll
-            for (int t = 0; t < 4; t++)
-                x[mt][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[n & 1][t], ql[mt][n], x[mt][t], 0, 0, 0);
+        for (int t = 0; t < 4; t++) x[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[n & 1][t], ql[n], x[t], 0, 0, 0);
         here();
     }
 }
 
 // acc += V^T w^T of a tile; v_of(n, kb): the codes of dims 16 n .. at the positions of half kb.  Two groups
-// of dims at a time, the next two made ready beside their products.
-template <int MT, typename VOf>
-__device__ __forceinline__ void weigh(float4v (&acc)[MT][ND], const half8 (&ph)[MT][2], const half8 (&pl)[MT][2], VOf v_of)
+// of dims at a time (ND is even), the next two made ready before their products.
+template <bool LDS, typename VOf>
+__device__ __forceinline__ void weigh(float4v (&acc)[ND], const half8 (&ph)[2], const half8 (&pl)[2], VOf v_of)
 {
     half8 v[2][2][2];
 #pragma unroll
     for (int j = 0; j < 4; j++) v[0][j >> 1][j & 1] = v_of(j >> 1, j & 1);
 #pragma unroll
-    for (int n0 = 0; n0 < ND; n0 += 2) {   // (ND is even)
+    for (int n0 = 0; n0 < ND; n0 += 2) {
         const int b = (n0 >> 1) & 1;
         if (n0 + 2 < ND) {
 #pragma unroll
             for (int j = 0; j < 4; j++) v[b ^ 1][j >> 1][j & 1] = v_of(n0 + 2 + (j >> 1), j & 1);
+            if (LDS) here();
         }
 #pragma unroll
         for (int kb = 0; kb < 2; kb++) {
 #pragma unroll
-            for (int mt = 0; mt < MT; mt++)
+            for (int n = 0; n < 2; n++)
+                acc[n0 + n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[b][n][kb], ph[kb], acc[n0 + n], 0, 0, 0);
 #pragma unroll
-                for (int n = 0; n < 2; n++)
-                    acc[mt][n0 + n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[b][n][kb], ph[mt][kb], acc[mt][n0 + n], 0, 0, 0);
-#pragma unroll
-            for (int mt = 0; mt < MT; mt++)
-#pragma unroll
-                for (int n = 0; n < 2; n++)
-                    acc[mt][n0 + n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[b][n][kb], pl[mt][kb], acc[mt][n0 + n], 0, 0, 0);
+            for (int n = 0; n < 2; n++)
+                acc[n0 + n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[b][n][kb], pl[kb], acc[n0 + n], 0, 0, 0);
         }
         here();
     }
 }
 
-// The running softmax of MT blocks of rows.
-template <int MT>
+// The running softmax of a block of rows, a row per column of 16 lanes.
 struct Running {
     // m: the largest x so far; mc: c m as rounded, the exponent that acc and l are relative to
-    float m[MT], mc[MT], l[MT], c[MT];
-    float vref;   // power of two, at least every V scale so far: acc is relative to 2^-14 of it
-    float4v acc[MT][ND];
+    float m = kNegInf, mc = kNegInf, l = 0.0f, c;
+    float4v acc[ND];
 
-    __device__ __forceinline__ void clear()
+    __device__ __forceinline__ Running()
     {
-        vref = kLeast;
 #pragma unroll
-        for (int mt = 0; mt < MT; mt++) {
-            m[mt] = mc[mt] = kNegInf;
-            l[mt] = 0.0f;
-#pragma unroll
-            for (int n = 0; n < ND; n++) acc[mt][n] = float4v{0, 0, 0, 0};
-        }
+        for (int n = 0; n < ND; n++) acc[n] = float4v{0, 0, 0, 0};
     }
 
     // One tile: x (K q^T) becomes the weights' parts, acc and l move to the new maximum.  ks(t), vs(t): the
-    // scales of this lane's positions, vone: the V scale of position `lane`.  With WHOLE every position counts
-    // for every row; otherwise the tile's first `left` exist and row block mt sees its first vis[mt]; what is
-    // not seen weighs nothing whatever its scales hold.
+    // scales of this lane's positions, those of V as VUnit left them; vdown: what it returned.  With WHOLE every
+    // position counts for every row; otherwise the row sees the tile's first `vis`; what is not seen weighs
+    // nothing whatever its scales hold.
     template <bool WHOLE, typename KsOf, typename VsOf>
-    __device__ __forceinline__ void step(float4v (&x)[MT][4], KsOf ks, VsOf vs, float vone, half8 (&ph)[MT][2],
-                                         half8 (&pl)[MT][2], int left, const int (&vis)[MT], int lane)
+    __device__ __forceinline__ void step(float4v (&x)[4], KsOf ks, VsOf vs, float vdown, half8 (&ph)[2], half8 (&pl)[2], int vis,
+                                         int g)
     {
-        const int g = lane >> 4;
+        float top = m;
 #pragma unroll
         for (int t = 0; t < 4; t++) {
-            const float4v k = ks(t);
+            x[t] *= ks(t);
 #pragma unroll
-            for (int mt = 0; mt < MT; mt++) {
-                x[mt][t] *= k;
-                if constexpr (!WHOLE) {
-#pragma unroll
-                    for (int i = 0; i < 4; i++)
-                        if (16 * t + 4 * g + i >= vis[mt]) x[mt][t][i] = kNegInf;
-                }
+            for (int i = 0; i < 4; i++) {
+                if (!WHOLE && 16 * t + 4 * g + i >= vis) x[t][i] = kNegInf;
+                top = fmaxf(top, x[t][i]);
             }
         }
-        if (!WHOLE && lane >= left) vone = 0.0f;
-        const float vnew = fmaxf(vref, pow2_above(max_lanes(fmaxf(vone, kLeast))));
-        const float vmul = __uint_as_float((268u << 23) - __float_as_uint(vnew));   // 2^14 / vnew
-        const float vdown = vref * (vmul * (1.0f / 16384.0f));
-        vref = vnew;
-        float now[MT], sum[MT];
+        top = max_groups(top);
+        // (a row that has seen nothing yet: x = -inf against 0)
+        const float now = top == kNegInf ? 0.0f : top * c;
+        const float alpha = __builtin_amdgcn_exp2f(mc - now);
+        if (top != kNegInf) m = top, mc = now;
+        const float down = alpha * vdown;
+        if (__any(down != 1.0f)) {
 #pragma unroll
-        for (int mt = 0; mt < MT; mt++) {
-            float top = m[mt];
-#pragma unroll
-            for (int t = 0; t < 4; t++)
-#pragma unroll
-                for (int i = 0; i < 4; i++) top = fmaxf(top, x[mt][t][i]);
-            top = max_groups(top);
-            // (a row that has seen nothing yet: x = -inf against 0)
-            now[mt] = top == kNegInf ? 0.0f : top * c[mt];
-            const float alpha = __builtin_amdgcn_exp2f(mc[mt] - now[mt]);
-            if (top != kNegInf) m[mt] = top, mc[mt] = now[mt];
-            l[mt] *= alpha;
-            sum[mt] = 0.0f;
-            const float down = alpha * vdown;
-            if (__any(down != 1.0f)) {
-#pragma unroll
-                for (int n = 0; n < ND; n++) acc[mt][n] *= down;
-            }
+            for (int n = 0; n < ND; n++) acc[n] *= down;
         }
+        float sum = 0.0f;
 #pragma unroll
         for (int t = 0; t < 4; t++) {
-            const float4v v = vs(t) * vmul;
+            const float4v v = vs(t);
+            float w[4];
 #pragma unroll
-            for (int mt = 0; mt < MT; mt++) {
-                float w[4];
+            for (int i = 0; i < 4; i++) {
+                const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(x[t][i], c, -now));
+                sum += p;
+                w[i] = p * v[i];
+                if (!WHOLE && 16 * t + 4 * g + i >= vis) w[i] = 0.0f;
+            }
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(x[mt][t][i], c[mt], -now[mt]));
-                    sum[mt] += p;
-                    w[i] = p * v[i];
-                    if (!WHOLE && 16 * t + 4 * g + i >= vis[mt]) w[i] = 0.0f;
-                }
-#pragma unroll
-                for (int i = 0; i < 4; i += 2) {
-                    half2v h, r;
-                    split(w[i], w[i + 1], h, r);
-                    put(ph[mt][t >> 1], 4 * (t & 1) + i, h);
-                    put(pl[mt][t >> 1], 4 * (t & 1) + i, r);
-                }
+            for (int i = 0; i < 4; i += 2) {
+                half2v h, r;
+                split(w[i], w[i + 1], h, r);
+                put(ph[t >> 1], 4 * (t & 1) + i, h);
+                put(pl[t >> 1], 4 * (t & 1) + i, r);
             }
             here();
         }
-#pragma unroll
-        for (int mt = 0; mt < MT; mt++) l[mt] += sum[mt];
+        l = l * alpha + sum;
     }
 };
 
-// stream: the NW waves take the tiles of positions [p0, p1) in turn; vis_of(row): positions that the row
+// Memory of four waves that work on one unit: first the queries, then the joining of the waves' sums.
+struct Shared {
+    union {
+        QRows q;
+        struct {
+            float m[4][16], l[4][16];
+            float acc[4][16][W + 4];
+        };
+    };
+    float scale[4][2][kKvTile];   // of a wave's tile, K and V
+};
+
+// stream: the four waves take the tiles of positions [p0, p1) in turn; vis_of(row): positions that the row
 // sees, counted from the slot's first, min_vis at least.
 template <typename RowOf, typename VisOf>
 __device__ __forceinline__ void stream(const AttnQ8Args &a, Shared &S, const uint8_t *cache, int p0, int p1, int min_vis,
@@ -371,55 +406,67 @@ __device__ __forceinline__ void stream(const AttnQ8Args &a, Shared &S, const uin
     const uint8_t *rec = cache + (size_t)(p0 / kKvTile + wave) * REC;
     KTile kt;
     VTile vt;
+    float kone = 0.0f, vone = 0.0f;
+    VUnit unit;
+    float (*scale)[kKvTile] = S.scale[wave];
+    const auto load_scales = [&]() {
+        const float *p = (const float *)(rec + 2 * kKvTile * W) + lane;
+        kone = p[0], vone = p[kKvTile];
+    };
     if (wave < n_tiles) {
         load_k(kt, rec, g, col);
         load_v(vt, rec, g, col);
+        load_scales();
     }
-    half8 qh[1][NK], ql[1][NK];
-    Running<1> R;
-    R.clear();
-    load_q<1>(a, qh, ql, R.c, g, col, row_of);
+    half8 qh[NK], ql[NK];
+    Running R;
+    bring_q(a, S.q, threadIdx.x, 256, row_of);
+    __syncthreads();
+    take_q(a, S.q, qh, ql, R.c, g, col);
     const int vis = row_of(col).valid ? vis_of(col) : 0;
 
     // tiles that every row sees all of, then the rest: the same code with and without the bounds
     const auto go = [&](int &tile, int end, auto whole) {
-        for (; tile < end; tile += NW) {
-            const float *scales = (const float *)(rec + 2 * kKvTile * W);
-            float4v ks[4], vs[4];
-#pragma unroll
-            for (int t = 0; t < 4; t++) {
-                ks[t] = *(const float4v *)(scales + 16 * t + 4 * g);
-                vs[t] = *(const float4v *)(scales + kKvTile + 16 * t + 4 * g);
-            }
-            const float vone = scales[kKvTile + lane];
-            rec += NW * REC;
-            const bool more = tile + NW < n_tiles;
-            float4v x[1][4];
-            scores<1>(x, qh, ql, [&](int t, int n) {
+        for (; tile < end; tile += 4) {
+            // a position's scales per lane, to be read by the lanes whose x belongs to it
+            const int at = p0 + tile * kKvTile;
+            if (!decltype(whole)::value && lane >= p1 - at) vone = 0.0f;
+            const float vdown = unit.take(vone);
+            scale[0][lane] = kone;
+            scale[1][lane] = vone;
+            wave_fence();
+            rec += 4 * REC;
+            const bool more = tile + 4 < n_tiles;
+            float4v x[4];
+            scores<false>(x, qh, ql, [&](int t, int n) {
                 if (TAIL && n == NK - 1) return halves(kt.b[t][0], kt.b[t][1]);
                 return halves(kt.a[t][n >> 1][2 * (n & 1)], kt.a[t][n >> 1][2 * (n & 1) + 1]);
             });
             if (more) load_k(kt, rec, g, col);
-            const int at = p0 + tile * kKvTile;
-            const int seen[1] = {vis - at};
-            half8 ph[1][2], pl[1][2];
+            half8 ph[2], pl[2];
             R.template step<decltype(whole)::value>(
-                x, [&](int t) { return ks[t]; }, [&](int t) { return vs[t]; }, vone, ph, pl, p1 - at, seen, lane);
-            weigh<1>(R.acc, ph, pl, [&](int n, int kb) { return halves(vt.a[n][2 * kb], vt.a[n][2 * kb + 1]); });
-            if (more) load_v(vt, rec, g, col);
+                x, [&](int t) { return *(const float4v *)&scale[0][16 * t + 4 * g]; },
+                [&](int t) { return *(const float4v *)&scale[1][16 * t + 4 * g]; }, vdown, ph, pl, vis - at, g);
+            weigh<false>(R.acc, ph, pl, [&](int n, int kb) { return halves(vt.a[n][2 * kb], vt.a[n][2 * kb + 1]); });
+            if (more) {
+                load_v(vt, rec, g, col);
+                load_scales();
+            }
+            wave_fence();
         }
     };
     int tile = wave;
     go(tile, min(n_tiles, (min_vis - p0) / kKvTile), std::true_type{});
     go(tile, n_tiles, std::false_type{});
 
-    const float sum = sum_groups(R.l[0]), up = R.vref * (1.0f / 16384.0f);
+    __syncthreads();   // (the queries have been read)
+    const float sum = sum_groups(R.l), up = unit.up * (1.0f / 16384.0f);
     if (g == 0) {
-        S.m[wave][col] = R.mc[0];
+        S.m[wave][col] = R.mc;
         S.l[wave][col] = sum;
     }
 #pragma unroll
-    for (int n = 0; n < ND; n++) *(float4v *)&S.acc[wave][col][16 * n + 4 * g] = R.acc[0][n] * up;
+    for (int n = 0; n < ND; n++) *(float4v *)&S.acc[wave][col][16 * n + 4 * g] = R.acc[n] * up;
     __syncthreads();
 }
 
@@ -428,16 +475,16 @@ __device__ __forceinline__ void stream(const AttnQ8Args &a, Shared &S, const uin
 template <typename RowOf>
 __device__ __forceinline__ void finish(const AttnQ8Args &a, Shared &S, int part, RowOf row_of)
 {
-    for (int i = threadIdx.x; i < 16 * (W / 4); i += 64 * NW) {
+    for (int i = threadIdx.x; i < 16 * (W / 4); i += 256) {
         const int row = i / (W / 4), d = 4 * (i % (W / 4));
         const RowRef r = row_of(row);
         if (!r.valid || d >= a.hd) continue;
         float top = kNegInf, sum = 0.0f;
 #pragma unroll
-        for (int w = 0; w < NW; w++) top = fmaxf(top, S.m[w][row]);
+        for (int w = 0; w < 4; w++) top = fmaxf(top, S.m[w][row]);
         float4v o = {0, 0, 0, 0};
 #pragma unroll
-        for (int w = 0; w < NW; w++) {
+        for (int w = 0; w < 4; w++) {
             // a wave without a visible position has the sum 0 (and one that saw NaN a NaN)
             const float f = S.m[w][row] == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(S.m[w][row] - top);
             if (S.l[w][row] == 0.0f) continue;
@@ -462,105 +509,125 @@ __device__ __forceinline__ void finish(const AttnQ8Args &a, Shared &S, int part,
     }
 }
 
-// rows: the tiles as fp16 operands in LDS, in fragments of 1 KB, a lane's 16 bytes after another's: K by (t, n),
-// V by (n, kb).  A second buffer takes the next tile while this one is read, where there is room.
-constexpr int NB = W <= 128 ? 2 : 1;
+// A wave's share of a tile that the workgroup brings from memory to LDS: K of positions 16 wave .. and V of dims
+// 16 (wave + 4 j) .., requested one tile ahead.
+struct Share {
+    static constexpr int NV = (ND + 3) / 4;
+    uint4v ka[NC > 0 ? NC : 1], va[NV];
+    uint2v kb;
+    float scale;
+
+    __device__ __forceinline__ void load(const uint8_t *rec, int wave, int g, int col)
+    {
+        const uint8_t *k = rec + (16 * wave + col) * W, *v = rec + kKvTile * W + col * kKvTile + 16 * g;
+#pragma unroll
+        for (int n = 0; n < NC; n++) ka[n] = *(const uint4v *)(k + 64 * n + 16 * g);
+        if constexpr (TAIL) kb = *(const uint2v *)(k + 64 * NC + 8 * g);
+#pragma unroll
+        for (int j = 0; j < NV; j++)
+            if (wave + 4 * j < ND) va[j] = *(const uint4v *)(v + 16 * kKvTile * (wave + 4 * j));
+        if (threadIdx.x < 2 * kKvTile) scale = ((const float *)(rec + 2 * kKvTile * W))[threadIdx.x];
+    }
+
+    // The scales of a tile with `left` positions: K by wave 0, V, in `unit`, by wave 1.
+    __device__ __forceinline__ void put_scales(float (&to)[2][kKvTile], float2 &info, VUnit &unit, int wave, int lane, int left)
+    {
+        if (wave == 0) {
+            to[0][lane] = scale;
+        } else if (wave == 1) {
+            float v = lane < left ? scale : 0.0f;
+            const float down = unit.take(v);
+            to[1][lane] = v;
+            if (lane == 0) info = make_float2(unit.up, down);
+        }
+    }
+};
+
+// rows: fragments of 1 KB, a lane's 16 bytes after another's: K by (t, n), V by (n, kb).
+constexpr int NB = W <= 128 ? 2 : 1;   // a second buffer takes the next tile while this one is read, where there is room
 struct Tiles {
     half8 k[NB][4][NK][64], v[NB][ND][2][64];
     float scale[NB][2][kKvTile];
+    float2 unit[NB];   // the unit of the tile's V scales, and what sums are multiplied with
 };
 
-// Positions [p0, p1), all seen by every row; the workgroup's wave w has the rows row_of(0 .. 16 MT - 1).
-// Writes the rows' part.
-template <int MT, typename RowOf>
-__device__ __forceinline__ void rows(const AttnQ8Args &a, Tiles &S, const uint8_t *cache, int p0, int p1, int part, RowOf row_of)
+// Positions [p0, p1), all seen by every row; each of the four waves has its own rows row_of(0 .. 15).  Writes the
+// rows' part.
+template <typename RowOf>
+__device__ __forceinline__ void rows(const AttnQ8Args &a, Tiles &S, QRows *Q, const uint8_t *cache, int p0, int p1, int part,
+                                       RowOf row_of)
 {
     const int lane = threadIdx.x & 63, g = lane >> 4, col = lane & 15, wave = wave_id();
     const int n_tiles = (p1 - p0 + kKvTile - 1) / kKvTile;
     constexpr size_t REC = kv_tile_bytes(W);
-    constexpr int NV = (ND + 3) / 4;   // V groups that a wave brings in
-
-    half8 qh[MT][NK], ql[MT][NK];
-    Running<MT> R;
-    R.clear();
-    load_q<MT>(a, qh, ql, R.c, g, col, row_of);
-    const bool busy = __any(row_of(0).valid);
-
-    // this wave's share of a tile: K of positions 16 wave .., V of dims 16 (wave + 4 j) ..
-    uint4v ka[NC > 0 ? NC : 1], va[NV];
-    uint2v kb2;
-    float sc = 0.0f;
-    const auto load = [&](const uint8_t *rec) {
-        const uint8_t *k = rec + (16 * wave + col) * W, *v = rec + kKvTile * W + col * kKvTile + 16 * g;
-#pragma unroll
-        for (int n = 0; n < NC; n++) ka[n] = *(const uint4v *)(k + 64 * n + 16 * g);
-        if constexpr (TAIL) kb2 = *(const uint2v *)(k + 64 * NC + 8 * g);
-#pragma unroll
-        for (int j = 0; j < NV; j++)
-            if (wave + 4 * j < ND) va[j] = *(const uint4v *)(v + 16 * kKvTile * (wave + 4 * j));
-        if (threadIdx.x < 2 * kKvTile) sc = ((const float *)(rec + 2 * kKvTile * W))[threadIdx.x];
-    };
     const uint8_t *rec = cache + (size_t)(p0 / kKvTile) * REC;
-    load(rec);
+    Share in;
+    in.load(rec, wave, g, col);
+
+    half8 qh[NK], ql[NK];
+    Running R;
+    VUnit unit;        // of the wave that brings the V scales
+    float vup = kLeast;
+    bring_q(a, Q[wave], lane, 64, row_of);
+    __syncthreads();
+    take_q(a, Q[wave], qh, ql, R.c, g, col);
+    __syncthreads();
+    const int busy = __any(row_of(0).valid);   // (a wave without rows brings its share of the tiles)
+
     const auto go = [&](int &tile, int end, auto whole) {
         for (; tile < end; tile++) {
             const int b = NB == 2 ? tile & 1 : 0;
             if (NB == 1 && tile > 0) __syncthreads();   // the tile before has been read
 #pragma unroll
             for (int n = 0; n < NC; n++) {
-                S.k[b][wave][2 * n][lane] = halves(ka[n][0], ka[n][1]);
-                S.k[b][wave][2 * n + 1][lane] = halves(ka[n][2], ka[n][3]);
+                S.k[b][wave][2 * n][lane] = halves(in.ka[n][0], in.ka[n][1]);
+                S.k[b][wave][2 * n + 1][lane] = halves(in.ka[n][2], in.ka[n][3]);
             }
-            if constexpr (TAIL) S.k[b][wave][NK - 1][lane] = halves(kb2[0], kb2[1]);
+            if constexpr (TAIL) S.k[b][wave][NK - 1][lane] = halves(in.kb[0], in.kb[1]);
 #pragma unroll
-            for (int j = 0; j < NV; j++)
+            for (int j = 0; j < Share::NV; j++)
                 if (wave + 4 * j < ND) {
-                    S.v[b][wave + 4 * j][0][lane] = halves(va[j][0], va[j][1]);
-                    S.v[b][wave + 4 * j][1][lane] = halves(va[j][2], va[j][3]);
+                    S.v[b][wave + 4 * j][0][lane] = halves(in.va[j][0], in.va[j][1]);
+                    S.v[b][wave + 4 * j][1][lane] = halves(in.va[j][2], in.va[j][3]);
                 }
-            if (threadIdx.x < 2 * kKvTile) S.scale[b][threadIdx.x >> 6][threadIdx.x & 63] = sc;
+            in.put_scales(S.scale[b], S.unit[b], unit, wave, lane, p1 - p0 - tile * kKvTile);
             rec += REC;
-            if (tile + 1 < n_tiles) load(rec);
+            if (tile + 1 < n_tiles) in.load(rec, wave, g, col);
             __syncthreads();
-            if (!busy) continue;
-            float4v x[MT][4];
-            scores<MT>(x, qh, ql, [&](int t, int n) { return S.k[b][t][n][lane]; });
-            const int left = p1 - p0 - tile * kKvTile;
-            int seen[MT];
-#pragma unroll
-            for (int mt = 0; mt < MT; mt++) seen[mt] = left;
-            half8 ph[MT][2], pl[MT][2];
+            if (!asked(busy)) continue;
+            float4v x[4];
+            scores<true>(x, qh, ql, [&](int t, int n) { return S.k[b][t][n][lane]; });
+            vup = S.unit[b].x;
+            half8 ph[2], pl[2];
             R.template step<decltype(whole)::value>(
                 x, [&](int t) { return *(const float4v *)&S.scale[b][0][16 * t + 4 * g]; },
-                [&](int t) { return *(const float4v *)&S.scale[b][1][16 * t + 4 * g]; }, S.scale[b][1][lane], ph, pl, left, seen, lane);
-            weigh<MT>(R.acc, ph, pl, [&](int n, int kb) { return S.v[b][n][kb][lane]; });
+                [&](int t) { return *(const float4v *)&S.scale[b][1][16 * t + 4 * g]; }, S.unit[b].y, ph, pl,
+                p1 - p0 - tile * kKvTile, g);
+            weigh<true>(R.acc, ph, pl, [&](int n, int kb) { return S.v[b][n][kb][lane]; });
         }
     };
     int tile = 0;
     go(tile, (p1 - p0) / kKvTile, std::true_type{});
     go(tile, n_tiles, std::false_type{});
-    if (!busy) return;
+    const RowRef r = row_of(col);
+    const float sum = sum_groups(R.l), up = vup * (1.0f / 16384.0f);
+    if (!r.valid) return;
+    const int64_t id = (int64_t)part * a.n_rows + (int64_t)r.token * a.n_head + r.head;
+    if (g == 0) a.part_ml[id * 2] = R.mc, a.part_ml[id * 2 + 1] = sum;
+    float *dst = a.part_acc + id * a.hd + 4 * g;
 #pragma unroll
-    for (int mt = 0; mt < MT; mt++) {
-        const RowRef r = row_of(16 * mt + col);
-        const float sum = sum_groups(R.l[mt]), up = R.vref * (1.0f / 16384.0f);
-        if (!r.valid) continue;
-        const int64_t id = (int64_t)part * a.n_rows + (int64_t)r.token * a.n_head + r.head;
-        if (g == 0) a.part_ml[id * 2] = R.mc[mt], a.part_ml[id * 2 + 1] = sum;
-#pragma unroll
-        for (int n = 0; n < ND; n++)
-            if (16 * n + 4 * g < a.hd) *(float4v *)(a.part_acc + id * a.hd + 16 * n + 4 * g) = R.acc[mt][n] * up;
-    }
+    for (int n = 0; n < ND; n++)
+        if (16 * n + 4 * g < a.hd) *(float4v *)(dst + 16 * n) = R.acc[n] * up;
 }
 
-// PRE, MTP: how the prefix is gone through, and 16-row blocks per wave there; the sequences' own positions:
-// stream.
-template <AttnQ8Pre PRE, int MTP>
-__global__ __launch_bounds__(64 * NW, W <= 64 && MTP == 1 ? 3 : W <= 128 ? 2 : 1) void k_attn_q8(const AttnQ8Args a)
+// PRE: how the prefix is gone through; the sequences' own positions: stream.
+template <AttnQ8Pre PRE>
+__global__ __launch_bounds__(256, W <= 64 ? 3 : W <= 128 ? 2 : 1) void k_attn_q8(const AttnQ8Args a)
 {
     union Mem {
         Shared own;
         std::conditional_t<PRE == PRE_ROWS, Tiles, int> tiles;
+        QRows q[PRE == PRE_ROWS ? 4 : 1];
     };
     __shared__ __align__(16) char mem[sizeof(Mem)];
     Mem &S = *(Mem *)mem;
@@ -571,14 +638,15 @@ __global__ __launch_bounds__(64 * NW, W <= 64 && MTP == 1 ? 3 : W <= 128 ? 2 : 1
         const int pairs = a.n_kv * a.pre_splits, pair = b % pairs, rb = b / pairs;
         const int head = pair % a.n_kv, split = pair / a.n_kv;
         const int p0 = split * a.pre_chunk, p1 = min(a.prefix_len, p0 + a.pre_chunk);
-        const int row0 = PRE == PRE_ROWS ? (rb * 4 + wave_id()) * 16 * MTP : rb * 16, n_rows = a.n_seq * a.n_q * group;
+        const int row0 = PRE == PRE_ROWS ? (rb * 4 + wave_id()) * 16 : rb * 16, n_rows = a.n_seq * a.n_q * group;
         const auto row_of = [&](int r) {
             const int id = row0 + r;
-            return RowRef{id < n_rows, id / group, head * group + id % group};
+            const int t = by_group(id, a.inv_group);
+            return RowRef{id < n_rows, t, head * group + id - t * group};
         };
         const uint8_t *cache = a.cache + (size_t)(a.prefix_slot * (int64_t)a.n_kv + head) * a.head_bytes;
         if constexpr (PRE == PRE_ROWS) {
-            rows<MTP>(a, S.tiles, cache, p0, p1, split, row_of);
+            rows(a, S.tiles, S.q, cache, p0, p1, split, row_of);
         } else {
             stream(a, S.own, cache, p0, p1, a.prefix_len, row_of, [&](int) { return a.prefix_len; });
             finish(a, S.own, split, row_of);
@@ -596,29 +664,30 @@ __global__ __launch_bounds__(64 * NW, W <= 64 && MTP == 1 ? 3 : W <= 128 ? 2 : 1
     const int row0 = rb * 16, n_rows = a.n_q * group;
     const auto row_of = [&](int r) {
         const int id = row0 + r;
-        return RowRef{id < n_rows, seq * a.n_q + id / group, head * group + id % group};
+        const int t = by_group(id, a.inv_group);
+        return RowRef{id < n_rows, seq * a.n_q + t, head * group + id - t * group};
     };
     const int part = a.pre_splits + split;
-    if (p0 >= p1) {
-        // nothing here: zeros, or a part without weight
-        for (int i = threadIdx.x; i < 16 * W; i += 64 * NW) {
-            const int row = i / W, d = i % W;
-            const RowRef r = row_of(row);
-            if (!r.valid || d >= a.hd) continue;
-            const int64_t id = (int64_t)r.token * a.n_head + r.head;
-            if (a.direct) {
-                a.out[id * a.hd + d] = 0.0f;
-            } else if (d == 0) {
-                float *ml = a.part_ml + (part * a.n_rows + id) * 2;
-                ml[0] = kNegInf, ml[1] = 0.0f;
-            }
-        }
+    if (p0 < p1) {
+        // the first of the n_q tokens sees len - n_q + 1 positions, each further one sees one more
+        stream(a, S.own, a.cache + (size_t)(slot * (int64_t)a.n_kv + head) * a.head_bytes, p0, p1, len - a.n_q + 1,
+               row_of, [&](int r) { return len - a.n_q + 1 + by_group(row0 + r, a.inv_group); });
+        finish(a, S.own, part, row_of);
         return;
     }
-    // the first of the n_q tokens sees len - n_q + 1 positions, each further one sees one more
-    stream(a, S.own, a.cache + (size_t)(slot * (int64_t)a.n_kv + head) * a.head_bytes, p0, p1, len - a.n_q + 1, row_of,
-                [&](int r) { return len - a.n_q + 1 + (row0 + r) / group; });
-    finish(a, S.own, part, row_of);
+    // nothing here: zeros, or a part without weight
+    for (int i = threadIdx.x; i < 16 * W; i += 256) {
+        const int row = i / W, d = i % W;
+        const RowRef r = row_of(row);
+        if (!r.valid || d >= a.hd) continue;
+        const int64_t id = (int64_t)r.token * a.n_head + r.head;
+        if (a.direct) {
+            a.out[id * a.hd + d] = 0.0f;
+        } else if (d == 0) {
+            float *ml = a.part_ml + (part * a.n_rows + id) * 2;
+            ml[0] = kNegInf, ml[1] = 0.0f;
+        }
+    }
 }
 
 }  // namespace
@@ -628,11 +697,13 @@ __global__ __launch_bounds__(64 * NW, W <= 64 && MTP == 1 ? 3 : W <= 128 ? 2 : 1
 hipError_t SMX_LAUNCH_NAME(SMX_ATTN_W)(const AttnQ8Args &a, const AttnQ8Plan &p, hipStream_t s)
 {
     const unsigned blocks = (unsigned)p.blocks;
-    if (p.pre == PRE_NONE) k_attn_q8<PRE_NONE, 1><<<blocks, 64 * NW, 0, s>>>(a);
-    else if (p.pre == PRE_STREAM) k_attn_q8<PRE_STREAM, 1><<<blocks, 64 * NW, 0, s>>>(a);
-    else if (p.mt_pre == 1) k_attn_q8<PRE_ROWS, 1><<<blocks, 64 * NW, 0, s>>>(a);
-    else if constexpr (kAttnQ8Narrow<SMX_ATTN_W>) k_attn_q8<PRE_ROWS, 2><<<blocks, 64 * NW, 0, s>>>(a);
-    else return hipErrorInvalidValue;
+    if (p.pre == PRE_NONE) {
+        k_attn_q8<PRE_NONE><<<blocks, 256, 0, s>>>(a);
+    } else if (p.pre == PRE_STREAM) {
+        k_attn_q8<PRE_STREAM><<<blocks, 256, 0, s>>>(a);
+    } else {
+        k_attn_q8<PRE_ROWS><<<blocks, 256, 0, s>>>(a);
+    }
     return hipGetLastError();
 }
 

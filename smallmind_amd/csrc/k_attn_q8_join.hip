@@ -102,20 +102,16 @@ AttnQ8Plan attn_q8_plan(const KvView &c, int n_seq, int n_q, int n_head, int pre
 {
     AttnQ8Plan p{};
     const int64_t group = n_head / c.n_kv, own_rows = n_q * group, pre_rows = n_seq * own_rows;
-    const bool narrow = c.w <= 128 ? kAttnQ8Narrow<128> : kAttnQ8Narrow<256>;
     p.own_blocks = (int)((own_rows + 15) / 16);
-    p.mt_pre = 1;
     if (prefix_len > 0) {
-        // one block of rows: nothing to share; from there on the tiles are turned into fp16 once for all waves,
-        // and two blocks per wave share what it reads of them
+        // several blocks of rows: the tiles are turned into fp16 once for four of them
         p.pre = pre_rows > 16 ? PRE_ROWS : PRE_STREAM;
-        if (pre_rows > 64 && narrow) p.mt_pre = 2;
-        const int block = p.pre == PRE_ROWS ? 64 * p.mt_pre : 16;
+        const int block = p.pre == PRE_ROWS ? 64 : 16;
         p.pre_blocks = (int)((pre_rows + block - 1) / block);
     }
     const int64_t own_units = (int64_t)n_seq * c.n_kv * p.own_blocks, pre_units = (int64_t)c.n_kv * p.pre_blocks;
     cut(max_len, own_units, 512, &p.own_chunk, &p.own_splits);
-    if (prefix_len > 0) cut(prefix_len, pre_units, 256, &p.pre_chunk, &p.pre_splits);
+    if (prefix_len > 0) cut(prefix_len, pre_units, 512, &p.pre_chunk, &p.pre_splits);
     p.parts = p.own_splits + p.pre_splits;
     p.pre_wgs = pre_units * p.pre_splits;
     p.blocks = p.pre_wgs + own_units * p.own_splits;
@@ -139,6 +135,7 @@ hipError_t launch_attn_q8(const KvView &c, const AttnQ8Plan &p, const float *q, 
     a.part_acc = (float *)work;
     a.part_ml = work ? (float *)work + p.parts * a.n_rows * c.hd : nullptr;
     a.q_stride = q_stride;
+    a.inv_group = (double)c.n_kv / n_head;
     a.scale_log2e = (float)(1.4426950408889634 / sqrt((double)c.hd));
     a.q_vec = ((uintptr_t)q & 15) == 0 && q_stride % 4 == 0;
     a.out_vec = ((uintptr_t)out & 15) == 0;

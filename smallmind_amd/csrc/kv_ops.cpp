@@ -48,6 +48,7 @@ int check_attention(const smx_kv_cache *c, int n_seq, int n_q, int n_head, int p
 {
     const KvView &v = c->view;
     if (n_head <= 0 || n_head % v.n_kv) SMX_FAIL(SMX_EINVAL, "%s: n_head %d must be a multiple of the cache's %d KV heads", fn, n_head, v.n_kv);
+    if (n_head > 65535) SMX_FAIL(SMX_EUNSUPPORTED, "%s: more than 65535 heads", fn);
     if (n_seq <= 0 || n_q <= 0) SMX_FAIL(SMX_EINVAL, "%s: need n_seq and n_q of at least 1", fn);
     if (max_len < 0 || max_len > v.ctx || prefix_len < 0 || prefix_len > v.ctx)
         SMX_FAIL(SMX_EINVAL, "%s: max_len %d and prefix_len %d must be within 0 .. ctx %d", fn, max_len, prefix_len, v.ctx);

@@ -9,10 +9,6 @@
 
 namespace smx {
 
-// Rows of up to 128 leave registers for two 16-row blocks of a prefix's rows per wave, and for two waves per SIMD.
-template <int W>
-constexpr bool kAttnQ8Narrow = W <= 128;
-
 // How the rows go through the prefix (k_attn_q8.hip).
 enum AttnQ8Pre { PRE_NONE, PRE_STREAM, PRE_ROWS };
 
@@ -24,6 +20,7 @@ struct AttnQ8Args {
     const int32_t *slots, *lens;
     float *part_ml, *part_acc;  // [parts][n_rows][2], [parts][n_rows][hd]
     int64_t q_stride, n_rows;   // n_rows = n_seq * n_q * n_head
+    double inv_group;           // n_kv / n_head
     float scale_log2e;          // log2(e) / sqrt(hd)
     int q_vec, out_vec;         // q, out may be read and written as float4
     int n_slots, n_seq, n_q, n_head, n_kv, hd;
@@ -35,7 +32,6 @@ struct AttnQ8Args {
 
 // How a call is cut up.
 struct AttnQ8Plan {
-    int mt_pre;                 // 16-row blocks per wave (PRE_ROWS)
     AttnQ8Pre pre;
     int own_chunk, own_splits, own_blocks;
     int pre_chunk, pre_splits, pre_blocks;

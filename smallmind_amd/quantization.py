@@ -388,7 +388,7 @@ class GpuKvCache:
         return self._h
 
     def close(self):
-        if getattr(self, "_h", None) and self._h.value and _lib._lib is not None:
+        if getattr(self, "_h", None) and self._h.value and _lib is not None and _lib._lib is not None:
             _lib._lib.smx_kv_cache_destroy(self._h)
             self._h = ctypes.c_void_p()
 
