@@ -2,16 +2,19 @@
 //
 // A row x (head_dim values of one token's K or V in one KV head) is kept as Q8Tensor.Quantize keeps a
 // block (Q8Tensor.cs:72-128): scale = fl32(max |x_i| / 127), code_i = the integer nearest to
-// x_i / scale, ties to even, at most 127 in size.  The nearest integer is exact: a first guess n from
-// the rounded quotient is at most one off, r = x - n scale is exact in fp32 (n scale and x agree in their
-// leading bits, or n = 0), and 2 |r| against scale says which side of the border x lies on.  A row
+// x_i / scale, ties to even, at most 127 in size.  The nearest integer is exact.  x times the rounded
+// reciprocal is within 2^-16 of x / scale, so its nearest integer n is the code unless it comes within
+// 2^-15 of a half; lanes that hold such a value look again: r = x - n scale is exact in fp32 (n scale
+// and x agree in their leading bits, or n = 0), and 2 |r| against scale says which side of the border x lies on.
+// (Looking at every value that way took 18 instructions each, where memory leaves time for about ten.)  A row
 // with a NaN or an infinity gets the scale NaN and zero codes: it reads back as NaN, and attention
 // that sees it gives NaN.
 //
 // One workgroup handles 64 tokens of K or V of one KV head; 16 lanes share a row, so a row's maximum is four
 // DPP steps.  K rows go straight to the cache.  V lies transposed, a byte per position: rows pass
 // through LDS, and wherever four tokens follow one another from a position that is a multiple of 4
-// (prompts) their bytes move as one dword; the rest (one token of each of many sequences) as bytes.
+// (prompts) their bytes move as 4 x 4 blocks, a dword for each dim; the rest (one token of each of many
+// sequences) as bytes.
 #include "smx_device.h"
 #include "smx_internal.h"
 #include "smx_kvcache.h"
@@ -43,12 +46,23 @@ __device__ __forceinline__ float nearest_code(float x, float scale, float n)
     return fminf(127.0f, fmaxf(-127.0f, n));
 }
 
-// The places of a workgroup's 64 tokens, and how their V bytes move: row r stands for itself (one
-// byte per dim), leads four rows (a dword), or is one of those three that follow.
+// Columns of a 4 x 4 block of bytes from its rows, and back.
+__device__ __forceinline__ void transpose4(uint32_t (&w)[4])
+{
+    const uint32_t a = __builtin_amdgcn_perm(w[1], w[0], 0x05010400u), b = __builtin_amdgcn_perm(w[1], w[0], 0x07030602u);
+    const uint32_t c = __builtin_amdgcn_perm(w[3], w[2], 0x05010400u), d = __builtin_amdgcn_perm(w[3], w[2], 0x07030602u);
+    w[0] = __builtin_amdgcn_perm(c, a, 0x05040100u);
+    w[1] = __builtin_amdgcn_perm(c, a, 0x07060302u);
+    w[2] = __builtin_amdgcn_perm(d, b, 0x05040100u);
+    w[3] = __builtin_amdgcn_perm(d, b, 0x07060302u);
+}
+
+// The places of a workgroup's 64 tokens, and how their V bytes move: in fours, by the row that leads them,
+// or singly.
 struct Places {
     int slot[kRows], pos[kRows];   // slot < 0: no place
-    int jobs[kRows];               // rows that move bytes; bit 8: four of them
-    int n_jobs;
+    int four[kRows / 4], one[kRows];
+    int n_four, n_one;
 };
 
 __device__ __forceinline__ void find_places(Places &S, const KvView &c, const int32_t *slots, const int32_t *pos, int t0,
@@ -71,16 +85,34 @@ __device__ __forceinline__ void find_places(Places &S, const KvView &c, const in
             const int so = __shfl_down(s, k, 64), po = __shfl_down(p, k, 64);
             lead = lead && so == s && po == p + k;
         }
+        // two leaders are at least four rows apart, since both their positions are multiples of 4
         const uint64_t leads = __ballot(lead);
-        // a row is taken along by a leader among the three rows before it: two leaders are at least
-        // four rows apart, since both their positions are multiples of 4
-        const bool follows = ((leads << 1 | leads << 2 | leads << 3) >> tid & 1) != 0;
-        const bool job = s >= 0 && !follows;
-        const uint64_t all = __ballot(job);
-        if (job) S.jobs[__popcll(all & ((1ull << tid) - 1))] = tid | (lead ? 256 : 0);
-        if (tid == 0) S.n_jobs = __popcll(all);
+        const bool led = ((leads | leads << 1 | leads << 2 | leads << 3) >> tid & 1) != 0;
+        const uint64_t ones = __ballot(s >= 0 && !led);
+        const uint64_t before = (1ull << tid) - 1;
+        if (lead) S.four[__popcll(leads & before)] = tid;
+        if (s >= 0 && !led) S.one[__popcll(ones & before)] = tid;
+        if (tid == 0) S.n_four = __popcll(leads), S.n_one = __popcll(ones);
     }
     __syncthreads();
+}
+
+// f(four, 4-dim group) for all fours and f(one, dim) for all single rows, fours and rows fastest, so that
+// neighbouring lanes have neighbouring positions of one dim.
+template <int W, typename F4, typename F1>
+__device__ __forceinline__ void each_place(const Places &S, F4 four, F1 one)
+{
+    const int n4 = S.n_four, n1 = S.n_one;
+    // quotients of i < 2^14 by n <= 64
+    const uint32_t m4 = 0xFFFFFFFFu / (uint32_t)max(n4, 1) + 1u, m1 = 0xFFFFFFFFu / (uint32_t)max(n1, 1) + 1u;
+    for (int i = threadIdx.x; i < n4 * (W / 4); i += kT) {
+        const int q = n4 == 1 ? i : (int)__umulhi((uint32_t)i, m4);
+        four(S.four[i - q * n4], q);
+    }
+    for (int i = threadIdx.x; i < n1 * W; i += kT) {
+        const int d = n1 == 1 ? i : (int)__umulhi((uint32_t)i, m1);
+        one(S.one[i - d * n1], d);
+    }
 }
 
 // W: the cache's row width (head_dim rounded up); VEC: rows may be read as float4.
@@ -136,26 +168,47 @@ __global__ __launch_bounds__(kT) void k_kv_append(KvView c, const float *__restr
         // below 2^-100 the reciprocal could leave the range of fp32: divide
         const bool small = !(scale >= 7.8886090522101181e-31f);
         const float inv = small ? 0.0f : 1.0f / scale;
+        // x inv + 1.5 2^23 + 128 has its nearest integer, plus 128, in the low byte
+        constexpr float kMagic = 12582912.0f + kKvZero;
+        float far = 0.0f;
+        uint32_t w[Q];
+#pragma unroll
+        for (int q = 0; q < Q; q++) {
+            uint32_t u[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const float xe = x[j][q][e], f = __builtin_fmaf(xe, inv, kMagic);
+                far = fmaxf(far, fabsf(__builtin_fmaf(xe, inv, kMagic - f)));
+                u[e] = __float_as_uint(f);
+            }
+            w[q] = __builtin_amdgcn_perm(__builtin_amdgcn_perm(u[3], u[2], 0x0C0C0400u),
+                                         __builtin_amdgcn_perm(u[1], u[0], 0x0C0C0400u), 0x05040100u);
+        }
+        if (small || !(far < 0.5f - 3.0517578125e-5f)) {   // (NaN: not finite)
+#pragma unroll
+            for (int q = 0; q < Q; q++) {
+                w[q] = 0;
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const float xe = x[j][q][e];
+                    float code = 0.0f;
+                    if (!small) {
+                        code = nearest_code(xe, scale, __builtin_rintf(xe * inv));
+                    } else if (finite && scale > 0.0f) {
+                        // (a subnormal scale may be far below max |x| / 127: clamped before the division)
+                        const float xc = fminf(127.0f * scale, fmaxf(-127.0f * scale, xe));
+                        code = nearest_code(xc, scale, __builtin_rintf(xc / scale));
+                    }
+                    w[q] |= (uint32_t)((int)code + kKvZero) << (8 * e);
+                }
+            }
+        }
 #pragma unroll
         for (int q = 0; q < Q; q++) {
             const int d = 64 * q + 4 * lane16;
-            uint32_t w = 0;
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const float xe = x[j][q][e];
-                float code = 0.0f;
-                if (!small) {
-                    code = nearest_code(xe, scale, __builtin_rintf(xe * inv));
-                } else if (finite && scale > 0.0f) {
-                    // (a subnormal scale may be far below max |x| / 127: clamped before the division)
-                    const float xc = fminf(127.0f * scale, fmaxf(-127.0f * scale, xe));
-                    code = nearest_code(xc, scale, __builtin_rintf(xc / scale));
-                }
-                w |= (uint32_t)((int)code + kKvZero) << (8 * e);
-            }
             if (W % 64 == 0 || d < W) {
-                if (is_v) codes[r * (W / 4 + 1) + d / 4] = w;
-                else if (slot >= 0) *(uint32_t *)(rec + (size_t)(ps % kKvTile) * W + d) = w;
+                if (is_v) codes[r * (W / 4 + 1) + d / 4] = w[q];
+                else if (slot >= 0) *(uint32_t *)(rec + (size_t)(ps % kKvTile) * W + d) = w[q];
             }
         }
         if (slot >= 0 && lane16 == 0)
@@ -163,18 +216,23 @@ __global__ __launch_bounds__(kT) void k_kv_append(KvView c, const float *__restr
     }
     if (!is_v) return;
     __syncthreads();
-    const uint8_t *b = (const uint8_t *)codes;
-    constexpr int RB = W + 4;   // bytes of a row in LDS
-    const int jobs = S.n_jobs;
-    for (int i = tid; i < jobs * W; i += kT) {
-        const int d = i / jobs, jb = S.jobs[i - d * jobs], r = jb & 255;
+    constexpr int RD = W / 4 + 1;   // dwords of a row in LDS
+    const auto place = [&](int r) {
         const int ps = S.pos[r];
-        uint8_t *dst = c.base + c.tile_off(S.slot[r], head, ps / kKvTile) + (size_t)kKvTile * W + d * kKvTile +
-                       kv_v_byte(ps % kKvTile);
-        const uint8_t *s = b + r * RB + d;
-        if (jb & 256) *(uint32_t *)dst = (uint32_t)s[0] | (uint32_t)s[RB] << 8 | (uint32_t)s[2 * RB] << 16 | (uint32_t)s[3 * RB] << 24;
-        else *dst = s[0];
-    }
+        return c.base + c.tile_off(S.slot[r], head, ps / kKvTile) + (size_t)kKvTile * W + kv_v_byte(ps % kKvTile);
+    };
+    each_place<W>(
+        S,
+        [&](int r, int q) {
+            uint32_t w[4];
+#pragma unroll
+            for (int k = 0; k < 4; k++) w[k] = codes[(r + k) * RD + q];
+            transpose4(w);
+            uint8_t *dst = place(r) + 4 * q * kKvTile;
+#pragma unroll
+            for (int k = 0; k < 4; k++) *(uint32_t *)(dst + k * kKvTile) = w[k];
+        },
+        [&](int r, int d) { place(r)[d * kKvTile] = ((const uint8_t *)codes)[4 * r * RD + d]; });
 }
 
 // The values of one K or V row group of 64 tokens: rows of [n_tok][n_kv][hd]; tokens without a place give 0.
@@ -193,22 +251,23 @@ __global__ __launch_bounds__(kT) void k_kv_read(KvView c, const int32_t *__restr
     const int n = min(kRows, n_tok - t0);
     find_places(S, c, slots, pos, t0, n_tok);
     if (is_v) {
-        uint8_t *b = (uint8_t *)codes;
-        constexpr int RB = W + 4;
-        const int jobs = S.n_jobs;
-        for (int i = tid; i < jobs * W; i += kT) {
-            const int d = i / jobs, jb = S.jobs[i - d * jobs], r = jb & 255;
+        constexpr int RD = W / 4 + 1;
+        const auto place = [&](int r) {
             const int ps = S.pos[r];
-            const uint8_t *s = c.base + c.tile_off(S.slot[r], head, ps / kKvTile) + (size_t)kKvTile * W + d * kKvTile +
-                               kv_v_byte(ps % kKvTile);
-            uint8_t *o = b + r * RB + d;
-            if (jb & 256) {
-                const uint32_t w = *(const uint32_t *)s;
-                o[0] = (uint8_t)w, o[RB] = (uint8_t)(w >> 8), o[2 * RB] = (uint8_t)(w >> 16), o[3 * RB] = (uint8_t)(w >> 24);
-            } else {
-                o[0] = *s;
-            }
-        }
+            return c.base + c.tile_off(S.slot[r], head, ps / kKvTile) + (size_t)kKvTile * W + kv_v_byte(ps % kKvTile);
+        };
+        each_place<W>(
+            S,
+            [&](int r, int q) {
+                const uint8_t *src = place(r) + 4 * q * kKvTile;
+                uint32_t w[4];
+#pragma unroll
+                for (int k = 0; k < 4; k++) w[k] = *(const uint32_t *)(src + k * kKvTile);
+                transpose4(w);
+#pragma unroll
+                for (int k = 0; k < 4; k++) codes[(r + k) * RD + q] = w[k];
+            },
+            [&](int r, int d) { ((uint8_t *)codes)[4 * r * RD + d] = place(r)[d * kKvTile]; });
         __syncthreads();
     }
 #pragma unroll

@@ -11,7 +11,9 @@
 //
 // One workgroup of 1024 threads per sequence.  What has to be read is one row of p and one of q; a wave
 // sums a stretch of the vocabulary, the wave in whose stretch the threshold falls is found from the 16
-// sums, and that stretch is read again (from the cache) by all threads, a few values each.
+// sums, and that stretch is read again (from the cache) by all threads, a few values each.  What bounds it is
+// the chain of loads that wait for one another (length, drafts' probabilities, rows, stretch) and, for
+// the rows, how many a compute unit has in flight: kBatch values of each per thread.
 #include "smx_device.h"
 #include "smx_internal.h"
 
@@ -21,6 +23,7 @@ namespace {
 
 constexpr int kT = 1024;
 constexpr int kW = kT / 64;
+constexpr int kBatch = 16;
 
 struct VerifyArgs {
     const float *p, *q;
@@ -50,7 +53,7 @@ __device__ __forceinline__ double wave_scan_f64(double v, int lane)
 
 struct VerifyShared {
     double sum[kW], scan[kW];
-    int found, last;
+    int first[kW], last[kW];
 };
 
 // The token drawn with `u` from weights max(p - q, 0) (q: a row, or 1 at token `hot`, or nothing) over the
@@ -60,20 +63,31 @@ __device__ __forceinline__ int draw(VerifyShared &S, const float *__restrict__ p
                                     int vocab, double u)
 {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const auto weight = [&](int j) -> double {
-        double w = (double)p[j];
-        if constexpr (MODE == 1) w -= (double)q[j];
+    const auto weight = [&](int j, float pj, float qj) -> double {
+        double w = (double)pj;
+        if constexpr (MODE == 1) w -= (double)qj;
         if constexpr (MODE == 2) w -= j == hot ? 1.0 : 0.0;
-        return w > 0.0 ? w : 0.0;   // (a NaN weighs nothing)
+        return fmax(w, 0.0);   // (a NaN weighs nothing)
     };
     const int seg = ((vocab + kW - 1) / kW + 63) & ~63;
     const int a = min(vocab, wave * seg), e = min(vocab, a + seg);
     double c = 0.0;
-#pragma unroll 8
-    for (int j = a + lane; j < e; j += 64) c += weight(j);
+    int j0 = a + lane;
+    for (; j0 - lane + 64 * kBatch <= e; j0 += 64 * kBatch) {
+        const float *pj = p + j0, *qj = q + j0;
+        float pv[kBatch], qv[kBatch];
+#pragma unroll
+        for (int k = 0; k < kBatch; k++) {
+            pv[k] = pj[64 * k];
+            if constexpr (MODE == 1) qv[k] = qj[64 * k];
+        }
+#pragma unroll
+        for (int k = 0; k < kBatch; k++) c += weight(j0 + 64 * k, pv[k], MODE == 1 ? qv[k] : 0.0f);
+    }
+#pragma unroll 4
+    for (; j0 < e; j0 += 64) c += weight(j0, p[j0], MODE == 1 ? q[j0] : 0.0f);
     c = wave_sum_f64(c);
     if (lane == 0) S.sum[wave] = c;
-    if (tid == 0) S.found = vocab, S.last = -1;
     __syncthreads();
     double total = 0.0, before = 0.0;
 #pragma unroll
@@ -98,7 +112,7 @@ __device__ __forceinline__ int draw(VerifyShared &S, const float *__restrict__ p
     // each thread a few consecutive weights of that stretch, in order
     const int per = (seg + kT - 1) / kT, f = min(b1, b0 + tid * per), l = min(b1, f + per);
     double own = 0.0;
-    for (int j = f; j < l; j++) own += weight(j);
+    for (int j = f; j < l; j++) own += weight(j, p[j], MODE == 1 ? q[j] : 0.0f);
     const double upto = wave_scan_f64(own, lane);
     if (lane == 63) S.scan[wave] = upto;
     __syncthreads();
@@ -106,21 +120,26 @@ __device__ __forceinline__ int draw(VerifyShared &S, const float *__restrict__ p
 #pragma unroll
     for (int w = 0; w < kW; w++) r += w < wave ? S.scan[w] : 0.0;
     r += upto - own;
-    int last = -1;
+    int first = -1, last = -1;
     for (int j = f; j < l; j++) {
-        const double w = weight(j);
+        const double w = weight(j, p[j], MODE == 1 ? q[j] : 0.0f);
         r += w;
         if (w > 0.0) {
             last = j;
-            if (r > at) {
-                atomicMin(&S.found, j);
-                break;
-            }
+            if (first < 0 && r > at) first = j;
         }
     }
-    if (last >= 0) atomicMax(&S.last, last);
+    // the lowest of all; without one (rounding hides the threshold) the last token with weight
+    const uint64_t some = __ballot(first >= 0), any = __ballot(last >= 0);
+    if (lane == 0) {
+        S.first[wave] = some ? __builtin_amdgcn_readlane(first, __ffsll((unsigned long long)some) - 1) : vocab;
+        S.last[wave] = any ? __builtin_amdgcn_readlane(last, 63 - __clzll((unsigned long long)any)) : -1;
+    }
     __syncthreads();
-    return S.found < vocab ? S.found : S.last;
+    int lo = vocab, hi = -1;
+#pragma unroll
+    for (int w = 0; w < kW; w++) lo = min(lo, S.first[w]), hi = max(hi, S.last[w]);
+    return lo < vocab ? lo : hi;
 }
 
 __global__ __launch_bounds__(kT) void k_verify(const VerifyArgs a)
@@ -129,33 +148,34 @@ __global__ __launch_bounds__(kT) void k_verify(const VerifyArgs a)
     const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
     const int n = a.lens ? min(a.lens[b], a.n_draft) : a.n_draft;
     int32_t *out = a.tokens + (int64_t)b * (a.n_draft + 1);
+    const double u = (double)a.u_draw[b];
+    const int32_t *x = a.draft + (int64_t)b * a.n_draft;
+    const float *p = a.p + (int64_t)b * (a.n_draft + 1) * a.p_stride;
+    const float *q = a.q ? a.q + (int64_t)b * a.n_draft * a.q_stride : nullptr;
+    // drafts taken: every wave finds it for itself (all that can be is requested before n is known)
+    int taken = max(n, 0);
+    for (int i0 = 0; i0 < a.n_draft; i0 += 64) {
+        const int i = i0 + lane;
+        bool no = true;
+        if (i < a.n_draft) {
+            const int t = x[i];
+            const double ua = (double)a.u_accept[(int64_t)b * a.n_draft + i];
+            if ((unsigned)t < (unsigned)a.vocab) {
+                const double qt = q ? (double)q[i * a.q_stride + t] : 1.0;
+                no = !(ua * qt < (double)p[i * a.p_stride + t]);
+            }
+        }
+        const uint64_t refused = __ballot(no || i >= n);
+        if (refused) {
+            taken = max(0, min(n, i0 + __ffsll((unsigned long long)refused) - 1));
+            break;
+        }
+    }
     if (n < 0) {   // no sequence here
         for (int i = tid; i <= a.n_draft; i += kT) out[i] = -1;
         if (tid == 0) a.accepted[b] = 0;
         return;
     }
-    const int32_t *x = a.draft + (int64_t)b * a.n_draft;
-    const float *p = a.p + (int64_t)b * (a.n_draft + 1) * a.p_stride;
-    const float *q = a.q ? a.q + (int64_t)b * a.n_draft * a.q_stride : nullptr;
-    // drafts taken: every wave finds it for itself
-    int taken = n;
-    for (int i0 = 0; i0 < n; i0 += 64) {
-        bool no = false;
-        if (i0 + lane < n) {
-            const int i = i0 + lane, t = x[i];
-            no = true;
-            if ((unsigned)t < (unsigned)a.vocab) {
-                const double qt = q ? (double)q[i * a.q_stride + t] : 1.0;
-                no = !((double)a.u_accept[(int64_t)b * a.n_draft + i] * qt < (double)p[i * a.p_stride + t]);
-            }
-        }
-        const uint64_t refused = __ballot(no);
-        if (refused) {
-            taken = i0 + __ffsll((unsigned long long)refused) - 1;
-            break;
-        }
-    }
-    const double u = (double)a.u_draw[b];
     const float *row = p + taken * a.p_stride;
     int tok = -1;
     if (taken < n) {
