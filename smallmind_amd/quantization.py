@@ -50,9 +50,15 @@ def smq_pack(qtype: int, data, scales, rows: int, cols: int, block_size: int) ->
     return out
 
 
+_T = None
+
+
 def _torch():
-    import torch
-    return torch
+    global _T
+    if _T is None:
+        import torch
+        _T = torch
+    return _T
 
 
 def _ptr(t) -> ctypes.c_void_p:
@@ -287,16 +293,19 @@ def sample(logits, u: float, context=None, temperature: float = 1.0, top_k: int 
 
 
 # ---- serving operators: 8-bit KV cache, attention over it, drafted tokens ------------------------
-def _on_device(device, *tensors):
-    """Checks that the tensors are on `device` and makes it current (a context manager)."""
-    for t in tensors:
-        if t is not None and t.device != device:
-            raise ValueError(f"operands must be on {device}, not {t.device}")
+# These are called once per layer and token, with kernels of a few microseconds: the checks below ask each
+# tensor only what a wrong call would differ in, and sizes of work memory are kept per set of sizes.
+def _raw_stream(index: int) -> int:
     torch = _torch()
-    return _SAME_DEVICE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+    try:
+        return torch._C._cuda_getCurrentRawStream(index)
+    except AttributeError:
+        return torch.cuda.current_stream(index).cuda_stream
 
 
-class _SameDevice:
+class _Here:
+    """The current device, already the right one."""
+
     def __enter__(self):
         return self
 
@@ -304,27 +313,36 @@ class _SameDevice:
         return False
 
 
-_SAME_DEVICE = _SameDevice()
+_HERE = _Here()
+
+
+def _on_device(index: int, *tensors):
+    """Checks that the tensors are on cuda device `index` and makes it current (a context manager)."""
+    for t in tensors:
+        if t is not None and t.get_device() != index:
+            raise ValueError(f"operands must be on cuda:{index}, not {t.device}")
+    cuda = _torch().cuda
+    return _HERE if cuda.current_device() == index else cuda.device(index)
 
 
 def _int32(t, n: int, what: str):
-    if t.dtype != _torch().int32 or not t.is_contiguous() or t.numel() != n:
+    if t.dtype is not _torch().int32 or t.numel() != n or not t.is_contiguous():
         raise ValueError(f"{what} must be a contiguous int32 tensor of {n} elements")
-    return t
 
 
 def _rows(t, heads: int, head_dim: int, what: str) -> int:
     """The distance between the [heads][head_dim] rows of t [..., heads, head_dim], which may lie in the
     rows of a wider matrix (a fused projection)."""
-    if t.dtype != _torch().float32 or t.dim() < 3 or t.shape[-2:] != (heads, head_dim):
-        raise ValueError(f"{what} must be float32 [..., {heads}, {head_dim}], is {t.dtype} {tuple(t.shape)}")
+    shape = t.shape
+    if t.dtype is not _torch().float32 or len(shape) < 3 or shape[-2] != heads or shape[-1] != head_dim:
+        raise ValueError(f"{what} must be float32 [..., {heads}, {head_dim}], is {t.dtype} {tuple(shape)}")
     row = heads * head_dim
-    if t.numel() == 0:
+    if t.is_contiguous() or t.numel() == 0:
         return row
-    lead, strides = t.shape[:-2], t.stride()
+    strides = t.stride()
     ok = (strides[-1] == 1 or head_dim == 1) and (strides[-2] == head_dim or heads == 1)
     step, n = None, 1
-    for size, st in zip(reversed(lead), reversed(strides[:-2])):
+    for size, st in zip(reversed(shape[:-2]), reversed(strides[:-2])):
         if size == 1:
             continue
         if step is None:
@@ -345,6 +363,7 @@ class GpuKvCache:
 
     def __init__(self, n_slots: int, n_kv_head: int, head_dim: int, ctx: int, device=None):
         self._h = ctypes.c_void_p()
+        self._work = {}      # work memory of an attention call, by its sizes
         torch = _torch()
         with torch.cuda.device(device if device is not None else torch.cuda.current_device()):
             self.device = torch.device("cuda", torch.cuda.current_device())
@@ -354,38 +373,53 @@ class GpuKvCache:
     @property
     def nbytes(self) -> int:
         b = ctypes.c_int64()
-        call("smx_kv_cache_info", self._h, None, None, None, None, ctypes.byref(b))
+        call("smx_kv_cache_info", self._handle(), None, None, None, None, ctypes.byref(b))
         return b.value
 
     def append(self, k, v, slots, pos):
         """Writes token t's rows k[t], v[t] ([n_tok, n_kv_head, head_dim] float32, possibly slices of a fused
         projection) to position pos[t] of slot slots[t] (int32).  Places the cache does not have (-1) are
         skipped; a place named twice is left with undefined contents."""
-        n = slots.numel()
-        ks, vs = _rows(k, self.n_kv_head, self.head_dim, "k"), _rows(v, self.n_kv_head, self.head_dim, "v")
-        if k.numel() != v.numel() or k.numel() != n * self.n_kv_head * self.head_dim:
+        n, kv, hd, index = slots.numel(), self.n_kv_head, self.head_dim, self.device.index
+        ks, vs = _rows(k, kv, hd, "k"), _rows(v, kv, hd, "v")
+        if k.numel() != n * kv * hd or v.numel() != n * kv * hd:
             raise ValueError(f"k and v must hold one row per token ({n})")
-        with _on_device(self.device, k, v, _int32(slots, n, "slots"), _int32(pos, n, "pos")):
+        _int32(slots, n, "slots")
+        _int32(pos, n, "pos")
+        with _on_device(index, k, v, slots, pos):
             if n:
                 call("smx_kv_append", self._handle(), k.data_ptr(), ks, v.data_ptr(), vs, slots.data_ptr(),
-                     pos.data_ptr(), n, _stream())
+                     pos.data_ptr(), n, _raw_stream(index))
 
     def read(self, slots, pos):
         """(k, v), each [n_tok, n_kv_head, head_dim] float32: the values the cache holds at these places (zeros
         at places it does not have)."""
-        torch, n = _torch(), slots.numel()
-        with _on_device(self.device, _int32(slots, n, "slots"), _int32(pos, n, "pos")):
+        torch, n, index = _torch(), slots.numel(), self.device.index
+        _int32(slots, n, "slots")
+        _int32(pos, n, "pos")
+        with _on_device(index, slots, pos):
             k = torch.empty((n, self.n_kv_head, self.head_dim), dtype=torch.float32, device=self.device)
             v = torch.empty_like(k)
             if n:
                 call("smx_kv_read", self._handle(), slots.data_ptr(), pos.data_ptr(), n, k.data_ptr(), v.data_ptr(),
-                     _stream())
+                     _raw_stream(index))
         return k, v
 
     def _handle(self):
         if not self._h.value:
             raise ValueError("the cache is closed")
         return self._h
+
+    def _work_bytes(self, n_seq: int, n_q: int, n_head: int, prefix_len: int, max_len: int) -> int:
+        key = (n_seq, n_q, n_head, prefix_len, max_len)
+        need = self._work.get(key)
+        if need is None:
+            b = ctypes.c_int64()
+            call("smx_attention_work_bytes", self._handle(), *key, ctypes.byref(b))
+            if len(self._work) >= 4096:
+                self._work.clear()
+            need = self._work[key] = b.value
+        return need
 
     def close(self):
         if getattr(self, "_h", None) and self._h.value and _lib is not None and _lib._lib is not None:
@@ -397,19 +431,21 @@ class GpuKvCache:
 
 
 def _attention_q8(q, cache, prefix, slots, lens, max_len, name):
-    torch = _torch()
+    torch, h, index = _torch(), cache._handle(), cache.device.index
     if q.dim() != 4:
         raise ValueError("q must be [n_seq, n_q, n_head, head_dim]")
-    n_seq, n_q, n_head, hd = q.shape
+    n_seq, n_q, n_head, _ = q.shape
     stride = _rows(q, n_head, cache.head_dim, "q")
-    max_len = cache.ctx if max_len is None else max_len
-    with _on_device(cache.device, q, _int32(slots, n_seq, "slots"), _int32(lens, n_seq, "lens")):
-        out = torch.empty((n_seq, n_q, n_head, hd), dtype=torch.float32, device=cache.device)
-        h, need = cache._handle(), ctypes.c_int64()
-        call("smx_attention_work_bytes", h, n_seq, n_q, n_head, prefix[1] if prefix else 0, max_len, ctypes.byref(need))
-        work = torch.empty(need.value, dtype=torch.uint8, device=cache.device) if need.value else None
+    if max_len is None:
+        max_len = cache.ctx
+    _int32(slots, n_seq, "slots")
+    _int32(lens, n_seq, "lens")
+    with _on_device(index, q, slots, lens):
+        out = torch.empty(q.shape, dtype=torch.float32, device=cache.device)
+        need = cache._work_bytes(n_seq, n_q, n_head, prefix[1] if prefix else 0, max_len)
+        work = torch.empty(need, dtype=torch.uint8, device=cache.device) if need else None
         call(name, h, q.data_ptr(), stride, out.data_ptr(), n_seq, n_q, n_head, *prefix, slots.data_ptr(), lens.data_ptr(),
-             max_len, work.data_ptr() if need.value else None, need.value, _stream())
+             max_len, work.data_ptr() if need else None, need, _raw_stream(index))
     return out
 
 
@@ -437,27 +473,31 @@ def verify_draft(target, draft, tokens, u_accept, u_draw, lens=None):
     u_draw [n_seq]: uniform numbers in [0, 1); lens [n_seq] int32: drafted tokens per sequence (default:
     n_draft, negative: an empty place).  Returns (out [n_seq, n_draft + 1], accepted [n_seq]) int32: the
     accepted tokens, one drawn token, then -1."""
-    torch = _torch()
-    if target.dim() != 3 or target.shape[1] < 1:
+    torch, index = _torch(), target.get_device()
+    shape = target.shape
+    if len(shape) != 3 or shape[1] < 1:
         raise ValueError("target must be [n_seq, n_draft + 1, vocab]")
-    n_seq, n_draft, vocab = target.shape[0], target.shape[1] - 1, target.shape[2]
-    ts = _rows(target.unsqueeze(-2), 1, vocab, "target")
+    if index < 0:
+        raise ValueError("operands must be device (cuda) tensors")
+    n_seq, n_draft, vocab = shape[0], shape[1] - 1, shape[2]
+    ts = _rows(target.unsqueeze(2), 1, vocab, "target")
     ds = 0
     if draft is not None:
         if draft.shape != (n_seq, n_draft, vocab):
             raise ValueError(f"draft must be {(n_seq, n_draft, vocab)}, is {tuple(draft.shape)}")
-        ds = _rows(draft.unsqueeze(-2), 1, vocab, "draft")
-    for u, shape, what in ((u_accept, (n_seq, n_draft), "u_accept"), (u_draw, (n_seq,), "u_draw")):
-        if tuple(u.shape) != shape or u.dtype != torch.float32 or not u.is_contiguous():
-            raise ValueError(f"{what} must be contiguous float32 {shape}")
+        ds = _rows(draft.unsqueeze(2), 1, vocab, "draft")
+    for u, want, what in ((u_accept, (n_seq, n_draft), "u_accept"), (u_draw, (n_seq,), "u_draw")):
+        if u.shape != want or u.dtype is not torch.float32 or not u.is_contiguous():
+            raise ValueError(f"{what} must be contiguous float32 {want}")
+    _int32(tokens, n_seq * n_draft, "tokens")
     if lens is not None:
         _int32(lens, n_seq, "lens")
-    with _on_device(target.device, draft, _int32(tokens, n_seq * n_draft, "tokens"), u_accept, u_draw, lens):
+    with _on_device(index, draft, tokens, u_accept, u_draw, lens):
         out = torch.empty((n_seq, n_draft + 1), dtype=torch.int32, device=target.device)
         accepted = torch.empty(n_seq, dtype=torch.int32, device=target.device)
         call("smx_verify_draft", target.data_ptr(), ts, None if draft is None else draft.data_ptr(), ds,
              tokens.data_ptr(), None if lens is None else lens.data_ptr(), u_accept.data_ptr(), u_draw.data_ptr(), n_seq,
-             n_draft, vocab, out.data_ptr(), accepted.data_ptr(), _stream())
+             n_draft, vocab, out.data_ptr(), accepted.data_ptr(), _raw_stream(index))
     return out, accepted
 
 
