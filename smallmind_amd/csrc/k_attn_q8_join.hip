@@ -1,6 +1,8 @@
 // k_attn_q8_join.hip -- the plan of the attention over the 8-bit KV cache and the sum of its parts.
 #include <math.h>
 
+#include <algorithm>
+
 #include "smx_attn_q8.h"
 #include "smx_device.h"
 #include "smx_internal.h"
@@ -78,14 +80,20 @@ __global__ __launch_bounds__(256) void k_attn_q8_join(const AttnQ8Args a)
     }
 }
 
-// Chunks of a length that make about `want` workgroups of `units` rows of workgroups: whole multiples of
-// four tiles, one for each wave of a workgroup.
-void cut(int len, int64_t units, int64_t want, int *chunk, int *splits)
+// Cuts a length into chunks, given the workgroups `units` that every chunk makes.  Two workgroups per compute unit
+// (512) keep it busy; up to there chunks of at least four tiles, one for each wave, as a shorter one spends
+// its time on the queries (64 sequences over 2048 shared positions, 128 dims: 23.5 us in chunks of four, 31 of
+// two).  Where that leaves most of the chip idle, chunks of two tiles (1 x 1024, 128 dims: 9.4 for 9.7 us; 16 sequences
+// over 512 shared positions: 10.1 for 11.6).
+void cut(int len, int64_t units, int *chunk, int *splits)
 {
-    const int unit = 4 * kKvTile, most = (len + unit - 1) / unit;
-    int64_t n = (want + units - 1) / units;
-    n = n < 1 ? 1 : n > most ? most : n;
-    *chunk = n == 0 ? unit : (int)(((int64_t)len + n - 1) / n + unit - 1) / unit * unit;
+    const int64_t tiles = (len + kKvTile - 1) / kKvTile;
+    int64_t n = std::min((512 + units - 1) / units, (tiles + 3) / 4);
+    if (n * units < 128) n = std::max(n, std::min((128 + units - 1) / units, (tiles + 1) / 2));
+    n = std::max<int64_t>(n, 1);
+    int64_t c = (tiles + n - 1) / n;
+    if (c > 4) c = (c + 3) / 4 * 4;
+    *chunk = (int)std::max<int64_t>(c, 1) * kKvTile;
     *splits = (len + *chunk - 1) / *chunk;
 }
 
@@ -110,8 +118,15 @@ AttnQ8Plan attn_q8_plan(const KvView &c, int n_seq, int n_q, int n_head, int pre
         p.pre_blocks = (int)((pre_rows + block - 1) / block);
     }
     const int64_t own_units = (int64_t)n_seq * c.n_kv * p.own_blocks, pre_units = (int64_t)c.n_kv * p.pre_blocks;
-    cut(max_len, own_units, 512, &p.own_chunk, &p.own_splits);
-    if (prefix_len > 0) cut(prefix_len, pre_units, 512, &p.pre_chunk, &p.pre_splits);
+    cut(max_len, own_units, &p.own_chunk, &p.own_splits);
+    if (prefix_len > 0) {
+        cut(prefix_len, pre_units, &p.pre_chunk, &p.pre_splits);
+    } else if ((int64_t)(max_len + kKvTile - 1) / kKvTile * c.w <= 1024) {
+        // a single part, which needs no second launch: 512 positions of 64 dims 6.3 us for 7.8 in two parts, 1024 8.6
+        // for 7.9 and the launch saved, 512 of 128 dims 8.8 for 9.5, 512 of 256 dims 14 for 12
+        p.own_chunk = std::max(1, (max_len + kKvTile - 1) / kKvTile) * kKvTile;
+        p.own_splits = max_len > 0 ? 1 : 0;
+    }
     p.parts = p.own_splits + p.pre_splits;
     p.pre_wgs = pre_units * p.pre_splits;
     p.blocks = p.pre_wgs + own_units * p.own_splits;
