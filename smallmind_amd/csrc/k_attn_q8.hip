@@ -164,22 +164,31 @@ struct VTile {
     uint4v a[ND];
 };
 
+// NT: past the caches (what a call reads once and they would not hold until the next call).
+template <bool NT, typename T>
+__device__ __forceinline__ T fetch(const uint8_t *p)
+{
+    return NT ? __builtin_nontemporal_load((const T *)p) : *(const T *)p;
+}
+
+template <bool NT>
 __device__ __forceinline__ void load_k(KTile &k, const uint8_t *rec, int g, int col)
 {
 #pragma unroll
     for (int t = 0; t < 4; t++) {
         const uint8_t *p = rec + (16 * t + col) * W;
 #pragma unroll
-        for (int n = 0; n < NC; n++) k.a[t][n] = *(const uint4v *)(p + 64 * n + 16 * g);
-        if constexpr (TAIL) k.b[t] = *(const uint2v *)(p + 64 * NC + 8 * g);
+        for (int n = 0; n < NC; n++) k.a[t][n] = fetch<NT, uint4v>(p + 64 * n + 16 * g);
+        if constexpr (TAIL) k.b[t] = fetch<NT, uint2v>(p + 64 * NC + 8 * g);
     }
 }
 
+template <bool NT>
 __device__ __forceinline__ void load_v(VTile &v, const uint8_t *rec, int g, int col)
 {
     const uint8_t *p = rec + kKvTile * W + col * kKvTile + 16 * g;
 #pragma unroll
-    for (int n = 0; n < ND; n++) v.a[n] = *(const uint4v *)(p + 16 * kKvTile * n);
+    for (int n = 0; n < ND; n++) v.a[n] = fetch<NT, uint4v>(p + 16 * kKvTile * n);
 }
 
 struct RowRef {          // a row of the batch
@@ -395,7 +404,7 @@ struct Shared {
 
 // stream: the four waves take the tiles of positions [p0, p1) in turn; vis_of(row): positions that the row
 // sees, counted from the slot's first, min_vis at least.
-template <typename RowOf, typename VisOf>
+template <bool NT, typename RowOf, typename VisOf>
 __device__ __forceinline__ void stream(const AttnQ8Args &a, Shared &S, const uint8_t *cache, int p0, int p1, int min_vis,
                                        RowOf row_of, VisOf vis_of)
 {
@@ -414,8 +423,8 @@ __device__ __forceinline__ void stream(const AttnQ8Args &a, Shared &S, const uin
         kone = p[0], vone = p[kKvTile];
     };
     if (wave < n_tiles) {
-        load_k(kt, rec, g, col);
-        load_v(vt, rec, g, col);
+        load_k<NT>(kt, rec, g, col);
+        load_v<NT>(vt, rec, g, col);
         load_scales();
     }
     half8 qh[NK], ql[NK];
@@ -442,14 +451,14 @@ __device__ __forceinline__ void stream(const AttnQ8Args &a, Shared &S, const uin
                 if (TAIL && n == NK - 1) return halves(kt.b[t][0], kt.b[t][1]);
                 return halves(kt.a[t][n >> 1][2 * (n & 1)], kt.a[t][n >> 1][2 * (n & 1) + 1]);
             });
-            if (more) load_k(kt, rec, g, col);
+            if (more) load_k<NT>(kt, rec, g, col);
             half8 ph[2], pl[2];
             R.template step<decltype(whole)::value>(
                 x, [&](int t) { return *(const float4v *)&scale[0][16 * t + 4 * g]; },
                 [&](int t) { return *(const float4v *)&scale[1][16 * t + 4 * g]; }, vdown, ph, pl, vis - at, g);
             weigh<false>(R.acc, ph, pl, [&](int n, int kb) { return halves(vt.a[n][2 * kb], vt.a[n][2 * kb + 1]); });
             if (more) {
-                load_v(vt, rec, g, col);
+                load_v<NT>(vt, rec, g, col);
                 load_scales();
             }
             wave_fence();
@@ -620,8 +629,8 @@ __device__ __forceinline__ void rows(const AttnQ8Args &a, Tiles &S, QRows *Q, co
         if (16 * n + 4 * g < a.hd) *(float4v *)(dst + 16 * n) = R.acc[n] * up;
 }
 
-// PRE: how the prefix is gone through; the sequences' own positions: stream.
-template <AttnQ8Pre PRE>
+// PRE: how the prefix is gone through; the sequences' own positions: stream, NT or not.
+template <AttnQ8Pre PRE, bool NT>
 __global__ __launch_bounds__(256, W <= 64 ? 3 : W <= 128 ? 2 : 1) void k_attn_q8(const AttnQ8Args a)
 {
     union Mem {
@@ -648,7 +657,7 @@ __global__ __launch_bounds__(256, W <= 64 ? 3 : W <= 128 ? 2 : 1) void k_attn_q8
         if constexpr (PRE == PRE_ROWS) {
             rows(a, S.tiles, S.q, cache, p0, p1, split, row_of);
         } else {
-            stream(a, S.own, cache, p0, p1, a.prefix_len, row_of, [&](int) { return a.prefix_len; });
+            stream<false>(a, S.own, cache, p0, p1, a.prefix_len, row_of, [&](int) { return a.prefix_len; });
             finish(a, S.own, split, row_of);
         }
         return;
@@ -670,7 +679,7 @@ __global__ __launch_bounds__(256, W <= 64 ? 3 : W <= 128 ? 2 : 1) void k_attn_q8
     const int part = a.pre_splits + split;
     if (p0 < p1) {
         // the first of the n_q tokens sees len - n_q + 1 positions, each further one sees one more
-        stream(a, S.own, a.cache + (size_t)(slot * (int64_t)a.n_kv + head) * a.head_bytes, p0, p1, len - a.n_q + 1,
+        stream<NT>(a, S.own, a.cache + (size_t)(slot * (int64_t)a.n_kv + head) * a.head_bytes, p0, p1, len - a.n_q + 1,
                row_of, [&](int r) { return len - a.n_q + 1 + by_group(row0 + r, a.inv_group); });
         finish(a, S.own, part, row_of);
         return;
@@ -697,13 +706,10 @@ __global__ __launch_bounds__(256, W <= 64 ? 3 : W <= 128 ? 2 : 1) void k_attn_q8
 hipError_t SMX_LAUNCH_NAME(SMX_ATTN_W)(const AttnQ8Args &a, const AttnQ8Plan &p, hipStream_t s)
 {
     const unsigned blocks = (unsigned)p.blocks;
-    if (p.pre == PRE_NONE) {
-        k_attn_q8<PRE_NONE><<<blocks, 256, 0, s>>>(a);
-    } else if (p.pre == PRE_STREAM) {
-        k_attn_q8<PRE_STREAM><<<blocks, 256, 0, s>>>(a);
-    } else {
-        k_attn_q8<PRE_ROWS><<<blocks, 256, 0, s>>>(a);
-    }
+    if (p.pre == PRE_NONE && p.past_caches) k_attn_q8<PRE_NONE, true><<<blocks, 256, 0, s>>>(a);
+    else if (p.pre == PRE_NONE) k_attn_q8<PRE_NONE, false><<<blocks, 256, 0, s>>>(a);
+    else if (p.pre == PRE_STREAM) k_attn_q8<PRE_STREAM, false><<<blocks, 256, 0, s>>>(a);
+    else k_attn_q8<PRE_ROWS, false><<<blocks, 256, 0, s>>>(a);
     return hipGetLastError();
 }
 

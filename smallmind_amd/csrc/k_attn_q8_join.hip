@@ -127,6 +127,9 @@ AttnQ8Plan attn_q8_plan(const KvView &c, int n_seq, int n_q, int n_head, int pre
         p.own_chunk = std::max(1, (max_len + kKvTile - 1) / kKvTile) * kKvTile;
         p.own_splits = max_len > 0 ? 1 : 0;
     }
+    // read once, and more than the memory-side cache holds from call to call (256 MB): 64 x 8192 positions of 8 x 128 dims
+    // 139 -> 132 us; 32 x 2048 of them, which it holds, 24 -> 27
+    p.past_caches = p.own_blocks == 1 && (double)n_seq * c.n_kv * max_len * 2 * c.w > 256.0 * (1 << 20);
     p.parts = p.own_splits + p.pre_splits;
     p.pre_wgs = pre_units * p.pre_splits;
     p.blocks = p.pre_wgs + own_units * p.own_splits;

@@ -33,6 +33,7 @@ struct AttnQ8Args {
 // How a call is cut up.
 struct AttnQ8Plan {
     AttnQ8Pre pre;
+    bool past_caches;           // the sequences' positions are read past the caches (PRE_NONE)
     int own_chunk, own_splits, own_blocks;
     int pre_chunk, pre_splits, pre_blocks;
     int parts;

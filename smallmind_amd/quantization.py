@@ -330,6 +330,13 @@ def _int32(t, n: int, what: str):
         raise ValueError(f"{what} must be a contiguous int32 tensor of {n} elements")
 
 
+def _matrix_rows(t, width: int, what: str) -> int:
+    """The distance between the rows of t [..., width], evenly spaced."""
+    if t.is_contiguous() and t.dtype is _torch().float32:
+        return width
+    return _rows(t.unsqueeze(-2), 1, width, what)
+
+
 def _rows(t, heads: int, head_dim: int, what: str) -> int:
     """The distance between the [heads][head_dim] rows of t [..., heads, head_dim], which may lie in the
     rows of a wider matrix (a fused projection)."""
@@ -480,12 +487,12 @@ def verify_draft(target, draft, tokens, u_accept, u_draw, lens=None):
     if index < 0:
         raise ValueError("operands must be device (cuda) tensors")
     n_seq, n_draft, vocab = shape[0], shape[1] - 1, shape[2]
-    ts = _rows(target.unsqueeze(2), 1, vocab, "target")
+    ts = _matrix_rows(target, vocab, "target")
     ds = 0
     if draft is not None:
         if draft.shape != (n_seq, n_draft, vocab):
             raise ValueError(f"draft must be {(n_seq, n_draft, vocab)}, is {tuple(draft.shape)}")
-        ds = _rows(draft.unsqueeze(2), 1, vocab, "draft")
+        ds = _matrix_rows(draft, vocab, "draft")
     for u, want, what in ((u_accept, (n_seq, n_draft), "u_accept"), (u_draw, (n_seq,), "u_draw")):
         if u.shape != want or u.dtype is not torch.float32 or not u.is_contiguous():
             raise ValueError(f"{what} must be contiguous float32 {want}")
