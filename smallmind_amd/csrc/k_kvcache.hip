@@ -10,7 +10,7 @@
 // with a NaN or an infinity gets the scale NaN and zero codes: it reads back as NaN, and attention
 // that sees it gives NaN.
 //
-// One workgroup handles 64 tokens of K or V of one KV head; 16 lanes share a row, so a row's maximum is four
+// One workgroup handles 64 (or 16) tokens of K or V of one KV head; 16 lanes share a row, so a row's maximum is four
 // DPP steps.  K rows go straight to the cache.  V lies transposed, a byte per position: rows pass
 // through LDS, and wherever four tokens follow one another from a position that is a multiple of 4
 // (prompts) their bytes move as 4 x 4 blocks, a dword for each dim; the rest (one token of each of many
@@ -24,7 +24,9 @@ namespace smx {
 namespace {
 
 constexpr int kT = 256;
-constexpr int kRows = 64;   // tokens per workgroup
+constexpr int kRows = 64;   // tokens per workgroup, at most
+
+typedef float float4v __attribute__((ext_vector_type(4)));
 
 // Maximum of the 16 lanes of a row group.
 __device__ __forceinline__ uint32_t row16_umax(uint32_t v)
@@ -65,11 +67,12 @@ struct Places {
     int n_four, n_one;
 };
 
+template <int ROWS>
 __device__ __forceinline__ void find_places(Places &S, const KvView &c, const int32_t *slots, const int32_t *pos, int t0,
                                             int n_tok)
 {
     const int tid = threadIdx.x;
-    if (tid < kRows) {
+    if (tid < ROWS) {
         int s = -1, p = 0;
         if (t0 + tid < n_tok) {
             s = slots[t0 + tid];
@@ -79,7 +82,7 @@ __device__ __forceinline__ void find_places(Places &S, const KvView &c, const in
         if (s < 0) p = 0;
         S.slot[tid] = s;
         S.pos[tid] = p;
-        bool lead = s >= 0 && (p & 3) == 0 && tid + 3 < kRows;
+        bool lead = s >= 0 && (p & 3) == 0 && tid + 3 < ROWS;
 #pragma unroll
         for (int k = 1; k < 4; k++) {
             const int so = __shfl_down(s, k, 64), po = __shfl_down(p, k, 64);
@@ -115,8 +118,9 @@ __device__ __forceinline__ void each_place(const Places &S, F4 four, F1 one)
     }
 }
 
-// W: the cache's row width (head_dim rounded up); VEC: rows may be read as float4.
-template <int W, bool VEC>
+// W: the cache's row width (head_dim rounded up); VEC: rows may be read as float4; NT: past the caches; ROWS:
+// tokens per workgroup.
+template <int W, bool VEC, bool NT, int ROWS>
 __global__ __launch_bounds__(kT) void k_kv_append(KvView c, const float *__restrict__ k, int64_t k_stride,
                                                   const float *__restrict__ v, int64_t v_stride,
                                                   const int32_t *__restrict__ slots, const int32_t *__restrict__ pos,
@@ -124,36 +128,37 @@ __global__ __launch_bounds__(kT) void k_kv_append(KvView c, const float *__restr
 {
     constexpr int Q = (W + 63) / 64;   // groups of four values per lane
     __shared__ Places S;
-    __shared__ uint32_t codes[kRows * (W / 4 + 1)];
+    __shared__ uint32_t codes[ROWS * (W / 4 + 1)];
     const int tid = threadIdx.x, lane16 = tid & 15;
-    const int head = (blockIdx.x >> 1) % c.n_kv, t0 = (int)((blockIdx.x >> 1) / c.n_kv) * kRows;
+    const int head = (blockIdx.x >> 1) % c.n_kv, t0 = (int)((blockIdx.x >> 1) / c.n_kv) * ROWS;
     const bool is_v = blockIdx.x & 1;
     const float *src = is_v ? v : k;
     const int64_t stride = is_v ? v_stride : k_stride;
-    const int n = min(kRows, n_tok - t0);
+    const int n = min(ROWS, n_tok - t0);
 
-    float x[4][Q][4];
+    float x[ROWS / 16][Q][4];
 #pragma unroll
-    for (int j = 0; j < 4; j++) {
+    for (int j = 0; j < ROWS / 16; j++) {
         const int r = (tid >> 4) + 16 * j;
         const float *p = src + (int64_t)(t0 + r) * stride + (int64_t)head * c.hd;
 #pragma unroll
         for (int q = 0; q < Q; q++) {
             const int d = 64 * q + 4 * lane16;
             if constexpr (VEC) {
-                float4 f = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                if (r < n && d < c.hd) f = *(const float4 *)(p + d);
-                x[j][q][0] = f.x, x[j][q][1] = f.y, x[j][q][2] = f.z, x[j][q][3] = f.w;
+                float4v f = {0.0f, 0.0f, 0.0f, 0.0f};
+                if (r < n && d < c.hd) f = NT ? __builtin_nontemporal_load((const float4v *)(p + d)) : *(const float4v *)(p + d);
+#pragma unroll
+                for (int e = 0; e < 4; e++) x[j][q][e] = f[e];
             } else {
 #pragma unroll
                 for (int e = 0; e < 4; e++) x[j][q][e] = r < n && d + e < c.hd ? p[d + e] : 0.0f;
             }
         }
     }
-    find_places(S, c, slots, pos, t0, n_tok);
+    find_places<ROWS>(S, c, slots, pos, t0, n_tok);
 
 #pragma unroll
-    for (int j = 0; j < 4; j++) {
+    for (int j = 0; j < ROWS / 16; j++) {
         const int r = (tid >> 4) + 16 * j;
         uint32_t m = 0;
 #pragma unroll
@@ -235,21 +240,21 @@ __global__ __launch_bounds__(kT) void k_kv_append(KvView c, const float *__restr
         [&](int r, int d) { place(r)[d * kKvTile] = ((const uint8_t *)codes)[4 * r * RD + d]; });
 }
 
-// The values of one K or V row group of 64 tokens: rows of [n_tok][n_kv][hd]; tokens without a place give 0.
-template <int W, bool VEC>
+// The values of K or V of a workgroup's tokens: rows of [n_tok][n_kv][hd]; tokens without a place give 0.
+template <int W, bool VEC, bool NT, int ROWS>
 __global__ __launch_bounds__(kT) void k_kv_read(KvView c, const int32_t *__restrict__ slots,
                                                 const int32_t *__restrict__ pos, int n_tok, float *__restrict__ k,
                                                 float *__restrict__ v)
 {
     constexpr int Q = (W + 63) / 64;
     __shared__ Places S;
-    __shared__ uint32_t codes[kRows * (W / 4 + 1)];
+    __shared__ uint32_t codes[ROWS * (W / 4 + 1)];
     const int tid = threadIdx.x, lane16 = tid & 15;
-    const int head = (blockIdx.x >> 1) % c.n_kv, t0 = (int)((blockIdx.x >> 1) / c.n_kv) * kRows;
+    const int head = (blockIdx.x >> 1) % c.n_kv, t0 = (int)((blockIdx.x >> 1) / c.n_kv) * ROWS;
     const bool is_v = blockIdx.x & 1;
     float *dst = is_v ? v : k;
-    const int n = min(kRows, n_tok - t0);
-    find_places(S, c, slots, pos, t0, n_tok);
+    const int n = min(ROWS, n_tok - t0);
+    find_places<ROWS>(S, c, slots, pos, t0, n_tok);
     if (is_v) {
         constexpr int RD = W / 4 + 1;
         const auto place = [&](int r) {
@@ -271,7 +276,7 @@ __global__ __launch_bounds__(kT) void k_kv_read(KvView c, const int32_t *__restr
         __syncthreads();
     }
 #pragma unroll
-    for (int j = 0; j < 4; j++) {
+    for (int j = 0; j < ROWS / 16; j++) {
         const int r = (tid >> 4) + 16 * j;
         if (r >= n) continue;
         const int slot = S.slot[r], ps = S.pos[r];
@@ -284,11 +289,13 @@ __global__ __launch_bounds__(kT) void k_kv_read(KvView c, const int32_t *__restr
             if (d >= c.hd) continue;
             uint32_t w = 0x01010101u * kKvZero;
             if (slot >= 0) w = is_v ? codes[r * (W / 4 + 1) + d / 4] : *(const uint32_t *)(rec + (size_t)(ps % kKvTile) * W + d);
-            float f[4];
+            float4v f;
 #pragma unroll
             for (int e = 0; e < 4; e++) f[e] = (float)((int)(w >> (8 * e) & 255u) - kKvZero) * scale;
-            if constexpr (VEC) {
-                *(float4 *)(p + d) = make_float4(f[0], f[1], f[2], f[3]);
+            if constexpr (NT) {
+                __builtin_nontemporal_store(f, (float4v *)(p + d));
+            } else if constexpr (VEC) {
+                *(float4v *)(p + d) = f;
             } else {
 #pragma unroll
                 for (int e = 0; e < 4; e++) p[d + e] = f[e];
@@ -313,18 +320,32 @@ hipError_t by_width(int w, F f)
     return hipErrorInvalidValue;
 }
 
+// Tokens per workgroup: 64, or 16 where that would leave compute units without work (a token for each of 128
+// sequences, 8 heads of 128: writing 11.8 -> 6.9 us, reading 13.8 -> 5.9).
+bool few(const KvView &c, int n_tok) { return (int64_t)((n_tok + kRows - 1) / kRows) * c.n_kv * 2 < 512; }
+
+unsigned blocks_of(const KvView &c, int n_tok, int rows) { return (unsigned)((int64_t)((n_tok + rows - 1) / rows) * c.n_kv * 2); }
+
+// Bytes of K and V as floats.
+double float_bytes(const KvView &c, int n_tok) { return 8.0 * n_tok * c.n_kv * c.hd; }
+
 }  // namespace
 
 hipError_t launch_kv_append(const KvView &c, const float *k, int64_t k_stride, const float *v, int64_t v_stride,
                             const int32_t *slots, const int32_t *pos, int n_tok, hipStream_t s)
 {
-    const unsigned blocks = (unsigned)((int64_t)((n_tok + kRows - 1) / kRows) * c.n_kv * 2);
+    const unsigned n64 = blocks_of(c, n_tok, 64), n16 = blocks_of(c, n_tok, 16);
     // float4 reads need 16-byte aligned rows (head_dim is a multiple of 8)
     const bool vec = (((uintptr_t)k | (uintptr_t)v) & 15) == 0 && k_stride % 4 == 0 && v_stride % 4 == 0;
+    // rows that the caches (8 x 4 MB) could not keep anyway: 16 x 2047 tokens of 8 x 128 dims 73 -> 69 us; 4 x 2000 of 1 x 256
+    // (16 MB) 10.8 -> 11.1
+    const bool nt = float_bytes(c, n_tok) > 32.0 * (1 << 20);
     return by_width(c.w, [&](auto w) {
         constexpr int W = decltype(w)::value;
-        if (vec) k_kv_append<W, true><<<blocks, kT, 0, s>>>(c, k, k_stride, v, v_stride, slots, pos, n_tok);
-        else k_kv_append<W, false><<<blocks, kT, 0, s>>>(c, k, k_stride, v, v_stride, slots, pos, n_tok);
+        if (!vec) k_kv_append<W, false, false, 64><<<n64, kT, 0, s>>>(c, k, k_stride, v, v_stride, slots, pos, n_tok);
+        else if (few(c, n_tok)) k_kv_append<W, true, false, 16><<<n16, kT, 0, s>>>(c, k, k_stride, v, v_stride, slots, pos, n_tok);
+        else if (nt) k_kv_append<W, true, true, 64><<<n64, kT, 0, s>>>(c, k, k_stride, v, v_stride, slots, pos, n_tok);
+        else k_kv_append<W, true, false, 64><<<n64, kT, 0, s>>>(c, k, k_stride, v, v_stride, slots, pos, n_tok);
         return hipGetLastError();
     });
 }
@@ -332,12 +353,17 @@ hipError_t launch_kv_append(const KvView &c, const float *k, int64_t k_stride, c
 hipError_t launch_kv_read(const KvView &c, const int32_t *slots, const int32_t *pos, int n_tok, float *k, float *v,
                           hipStream_t s)
 {
-    const unsigned blocks = (unsigned)((int64_t)((n_tok + kRows - 1) / kRows) * c.n_kv * 2);
+    const unsigned n64 = blocks_of(c, n_tok, 64), n16 = blocks_of(c, n_tok, 16);
     const bool vec = (((uintptr_t)k | (uintptr_t)v) & 15) == 0;
+    // from a few MB on, values written past the caches do not push the codes out of them: 16 x 2047 tokens of 8 x 128 dims
+    // 86 -> 51 us, 4096 of 4 x 64 (8 MB) 6.2 -> 5.7; 16 of 4 x 64 4.5 -> 4.8
+    const bool nt = float_bytes(c, n_tok) > 4.0 * (1 << 20);
     return by_width(c.w, [&](auto w) {
         constexpr int W = decltype(w)::value;
-        if (vec) k_kv_read<W, true><<<blocks, kT, 0, s>>>(c, slots, pos, n_tok, k, v);
-        else k_kv_read<W, false><<<blocks, kT, 0, s>>>(c, slots, pos, n_tok, k, v);
+        if (!vec) k_kv_read<W, false, false, 64><<<n64, kT, 0, s>>>(c, slots, pos, n_tok, k, v);
+        else if (few(c, n_tok)) k_kv_read<W, true, false, 16><<<n16, kT, 0, s>>>(c, slots, pos, n_tok, k, v);
+        else if (nt) k_kv_read<W, true, true, 64><<<n64, kT, 0, s>>>(c, slots, pos, n_tok, k, v);
+        else k_kv_read<W, true, false, 64><<<n64, kT, 0, s>>>(c, slots, pos, n_tok, k, v);
         return hipGetLastError();
     });
 }

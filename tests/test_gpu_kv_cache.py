@@ -60,6 +60,41 @@ def test_rows_come_back_as_they_were_encoded(Q, hd, kind, n):
     c.close()
 
 
+@pytest.mark.parametrize("hd,kv", [(8, 2), (64, 2), (128, 3), (256, 3), (232, 2)])
+@pytest.mark.parametrize("kind", ["prompts", "mixed"])
+def test_many_rows(Q, hd, kv, kind):
+    """Enough rows for the kernels of many (and of more than the caches hold): runs of odd lengths at odd
+    positions, and runs among single tokens and places that do not exist."""
+    import torch
+    rng = np.random.default_rng(hd + kv)
+    slots, per, ctx = 9, 1001, 1100
+    n = slots * per
+    s, p = np.repeat(np.arange(slots), per), np.tile(np.arange(per) + 33, slots)
+    if kind == "mixed":
+        order = np.arange(n)
+        for a in range(0, n, 700):      # every few hundred tokens, 90 in another order
+            b = min(n, a + 90)
+            order[a:b] = rng.permutation(order[a:b])
+        s, p = s[order].copy(), p[order].copy()
+        s[::97], p[::89] = -1, ctx
+    k, v = (rng.normal(0, 1, (n, kv, hd)).astype(np.float32) for _ in range(2))
+    c = Q.GpuKvCache(slots, kv, hd, ctx)
+    c.append(dev(k), dev(v), i32(s), i32(p))
+    gk, gv = c.read(i32(s), i32(p))
+    ok = (s >= 0) & (p < ctx)
+    for g, x in ((gk, k), (gv, v)):
+        assert np.array_equal(g.cpu().numpy(), np.where(ok[:, None, None], R.held(x), np.float32(0)))
+    # nothing else was written
+    gk, gv = c.read(i32(np.repeat(np.arange(slots), ctx)), i32(np.tile(np.arange(ctx), slots)))
+    seen = np.zeros((slots, ctx), bool)
+    seen[s[ok], p[ok]] = True
+    for g in (gk, gv):
+        rows = (g.abs().amax((1, 2)) > 0).cpu().numpy().reshape(slots, ctx)
+        assert np.array_equal(rows, seen)
+    c.close()
+    torch.cuda.empty_cache()
+
+
 def test_places_that_the_cache_does_not_have(Q):
     rng = np.random.default_rng(3)
     c = Q.GpuKvCache(2, 2, 64, 70)
