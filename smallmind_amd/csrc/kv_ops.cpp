@@ -115,6 +115,7 @@ SMX_API int smx_kv_cache_create(int n_slots, int n_kv_head, int head_dim, int ct
     if (e != hipSuccess) {
         if (c->view.base) (void)hipFree(c->view.base);
         delete c;
+        (void)hipGetLastError();   // reported here; the check after the next launch is not to find it again
         SMX_HIP(e);
     }
     *out = c;

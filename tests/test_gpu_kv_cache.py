@@ -260,6 +260,17 @@ def test_attention_shared(Q, hd, group, n_q, n_seq, P):
     f.cache.close()
 
 
+def test_a_cache_that_does_not_fit_leaves_no_error_behind(Q):
+    from smallmind_amd._lib import SmxError
+    with pytest.raises(SmxError):      # 145 TB
+        Q.GpuKvCache(1 << 10, 64, 128, 1 << 23)
+    c = Q.GpuKvCache(1, 1, 64, 8)
+    x = np.ones((1, 1, 64), np.float32)
+    c.append(dev(x), dev(x), i32([0]), i32([0]))
+    assert np.array_equal(c.read(i32([0]), i32([0]))[0].cpu().numpy(), R.held(x))
+    c.close()
+
+
 def test_attention_over_a_prefix_alone_and_over_none(Q):
     f = Filled(Q, 4, 2, 64, 500, 9)
     rng = np.random.default_rng(1)
