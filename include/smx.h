@@ -227,9 +227,11 @@ SMX_API int smx_attention_work_bytes(const smx_kv_cache *c, int n_seq, int n_q, 
 /* Attention of the last n_q tokens of each of n_seq sequences over the cache (MultiHeadAttention.cs:676-844 with
  * the exponential itself in place of FastExp).  Sequence b's positions are the first lens_dev[b] of slot
  * slots_dev[b], its n_q tokens (already appended) among them; token i sees all up to itself, the first
- * lens_dev[b] - n_q + 1 + i.  One token each: decode; several: drafted tokens.  q: token i of sequence b at
- * q_dev + (b * n_q + i) * q_stride, [n_head][head_dim]; out_dev [n_seq][n_q][n_head][head_dim]; scores
- * are scaled by 1 / sqrt(head_dim); n_head a multiple of n_kv_head.  max_len: at least every length (a
+ * lens_dev[b] - n_q + 1 + i.  One token each: decode; several: drafted tokens.  n_seq and n_q
+ * are at least 1.  Keys and values are up to 2^96 in size, scaled scores below 2^126 (sums in fp32 hold
+ * no more).  q: token i of sequence b at q_dev + (b * n_q + i) * q_stride, [n_head][head_dim];
+ * out_dev [n_seq][n_q][n_head][head_dim]; scores are scaled by 1 / sqrt(head_dim); n_head a multiple of
+ * n_kv_head.  max_len: at least every length (a
  * greater one counts as max_len); a tight bound saves workgroups.  A row that sees nothing, and the rows
  * of a sequence whose slot the cache does not have, are zeros.  work_dev: smx_attention_work_bytes bytes,
  * 16-byte aligned, free for other use when the call's work is done; calls that may overlap, replays of captured graphs among

@@ -260,6 +260,29 @@ def test_attention_shared(Q, hd, group, n_q, n_seq, P):
     f.cache.close()
 
 
+@pytest.mark.parametrize("hd", [8, 96, 160, 192, 224])
+@pytest.mark.parametrize("group,n_q,n_seq,P", [(8, 4, 3, 129), (4, 1, 5, 600), (3, 2, 1, 64), (1, 7, 11, 200)])
+def test_attention_shared_at_other_widths(Q, hd, group, n_q, n_seq, P):
+    f = Filled(Q, n_seq + 1, 2, hd, 600, hd + P)
+    rng = np.random.default_rng(hd * group + P)
+    lens = np.array([9, 70, 0, 300, 64, 5, 1, 11, 2, 63, 65])[:n_seq]
+    slots = np.arange(n_seq)
+    q = rng.normal(0, 1.3, (n_seq, n_q, 2 * group, hd)).astype(np.float32)
+    close(Q.attention_shared(dev(q), f.cache, n_seq, P, i32(slots), i32(lens), 300), reference(f, q, slots, lens, (n_seq, P)))
+    f.cache.close()
+
+
+def test_more_new_tokens_than_positions_and_many_of_them(Q):
+    """A prompt's chunk of 150 tokens of several lengths: blocks of rows that see nothing, part of a chunk, all."""
+    f = Filled(Q, 5, 1, 64, 700, 13)
+    rng = np.random.default_rng(14)
+    q = rng.normal(0, 1, (5, 150, 3, 64)).astype(np.float32)
+    slots, lens = np.array([0, 1, 2, 3, 4]), np.array([700, 150, 20, 0, 151])
+    close(Q.attention_cached(dev(q), f.cache, i32(slots), i32(lens)), reference(f, q, slots, lens))
+    close(Q.attention_shared(dev(q), f.cache, 4, 77, i32(slots), i32(lens)), reference(f, q, slots, lens, (4, 77)))
+    f.cache.close()
+
+
 def test_a_cache_that_does_not_fit_leaves_no_error_behind(Q):
     from smallmind_amd._lib import SmxError
     with pytest.raises(SmxError):      # 145 TB
@@ -269,6 +292,85 @@ def test_a_cache_that_does_not_fit_leaves_no_error_behind(Q):
     c.append(dev(x), dev(x), i32([0]), i32([0]))
     assert np.array_equal(c.read(i32([0]), i32([0]))[0].cpu().numpy(), R.held(x))
     c.close()
+
+
+@pytest.mark.parametrize("hd", [64, 256])
+@pytest.mark.parametrize("k_up,q_up,v_up", [(96, -96, 96), (-90, 90, -80), (60, -50, 0)])
+def test_sizes_next_to_the_documented_limits(Q, hd, k_up, q_up, v_up):
+    rng = np.random.default_rng([hd, k_up + 128])
+    f = Filled(Q, 2, 2, hd, 200, hd)
+    unit = (rng.uniform(-1, 1, s).astype(np.float32) for s in ((2, 200, 2, hd), (2, 200, 2, hd), (2, 3, 6, hd)))
+    f.k, f.v, q = (x * np.float32(2.0 ** up) for x, up in zip(unit, (k_up, v_up, q_up)))
+    f.cache.append(dev(f.k.reshape(400, 2, hd)), dev(f.v.reshape(400, 2, hd)), i32(np.repeat([0, 1], 200)),
+                   i32(np.tile(np.arange(200), 2)))
+    f.hk, f.hv = R.held(f.k), R.held(f.v)
+    close(Q.attention_cached(dev(q), f.cache, i32([0, 1]), i32([200, 77])), reference(f, q, [0, 1], [200, 77]))
+    close(Q.attention_shared(dev(q), f.cache, 1, 130, i32([0, 1]), i32([200, 77])),
+          reference(f, q, [0, 1], [200, 77], (1, 130)))
+    f.cache.close()
+
+
+def test_one_slot_for_many_sequences(Q):
+    """600 sequences in three slots: the form for more than the caches hold, and equal rows give equal outputs."""
+    import torch
+    f = Filled(Q, 3, 2, 128, 1000, 21)
+    rng = np.random.default_rng(22)
+    q = rng.normal(0, 1, (3, 1, 4, 128)).astype(np.float32)
+    slots, lens = np.array([2, 0, 1]), np.array([1000, 517, 64])
+    got = Q.attention_cached(dev(np.tile(q, (200, 1, 1, 1))), f.cache, i32(np.tile(slots, 200)), i32(np.tile(lens, 200)))
+    got = got.reshape(200, 3, 1, 4, 128)
+    assert torch.equal(got, got[:1].expand_as(got))
+    close(got[0], reference(f, q, slots, lens))
+    f.cache.close()
+
+
+@pytest.mark.parametrize("P", [0, 130])
+@pytest.mark.parametrize("length", [40, 2000])
+def test_outputs_that_are_not_aligned(Q, P, length):
+    import torch
+
+    from smallmind_amd._lib import call
+    f = Filled(Q, 2, 1, 64, 2000, 23)
+    rng = np.random.default_rng(24)
+    q = rng.normal(0, 1, (1, 2, 4, 64)).astype(np.float32)
+    n = ctypes.c_int64()
+    call("smx_attention_work_bytes", f.cache._h, 1, 2, 4, P, length, ctypes.byref(n))
+    work = torch.empty(n.value + 16, dtype=torch.uint8, device="cuda")
+    buf = torch.full((1 + q.size + 8,), 7.0, device="cuda")
+    dq, slots, lens = dev(q), i32([0]), i32([length])
+    call("smx_attention_shared", f.cache._h, dq.data_ptr(), 256, buf[1:].data_ptr(), 1, 2, 4, 1, P, slots.data_ptr(),
+         lens.data_ptr(), length, work.data_ptr(), n.value, None)
+    torch.cuda.synchronize()
+    assert bool((buf[0] == 7.0) & (buf[1 + q.size:] == 7.0).all())
+    close(buf[1:1 + q.size].reshape(q.shape), reference(f, q, [0], [length], (1, P) if P else None))
+    f.cache.close()
+
+
+def test_calls_from_several_threads(Q):
+    import threading
+
+    import torch
+    f = Filled(Q, 5, 2, 64, 400, 15)
+    q = torch.randn(4, 2, 8, 64, device="cuda")
+    slots, lens = i32([0, 1, 2, 3]), i32([400, 7, 130, 64])
+    want = Q.attention_shared(q, f.cache, 4, 300, slots, lens)
+    torch.cuda.synchronize()
+    bad = []
+
+    def work():
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                got = Q.attention_shared(q, f.cache, 4, 300, slots, lens)
+                torch.cuda.current_stream().synchronize()
+                if not bool((got == want).all()):
+                    bad.append(1)
+    threads = [threading.Thread(target=work) for _ in range(3)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad
+    f.cache.close()
 
 
 def test_attention_over_a_prefix_alone_and_over_none(Q):
@@ -557,6 +659,29 @@ def test_verify_draft(Q, vocab, n_seq, n_draft):
     check_verify(Q, p, q, x, ua, ud)
     ud[:] = np.float32(1 - 2.0 ** -24)
     check_verify(Q, p, q, x, ua, ud)
+
+
+def test_verify_captured_and_replayed(Q):
+    import torch
+    rng = np.random.default_rng(77)
+    sets = [drafts(rng, 5, 4, 1003) for _ in range(4)]
+    now = [dev(a) for a in sets[0]]
+    run = lambda t: Q.verify_draft(*t)  # noqa: E731
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        run(now)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=s):
+        out = run(now)
+    for data in sets + sets[:1]:
+        for t, a in zip(now, data):
+            t.copy_(dev(a))
+        g.replay()
+        want = run([dev(a) for a in data])
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want))
 
 
 def test_verify_many_drafts_and_none(Q):
