@@ -31,7 +31,8 @@ struct smx_kv_cache {
 
 namespace {
 
-constexpr int64_t kMaxGrid = INT64_C(0x7FFFFFFF);
+constexpr int64_t kMaxOutputs = INT64_C(0x7FFFFFFF);
+constexpr int64_t kMaxBlocks = (1 << 24) - 1;   // of 256 threads: a launch has fewer than 2^32
 
 // The cache's memory is on its device, so the call's stream has to be too.
 int check_device(const smx_kv_cache *c, const char *fn)
@@ -52,10 +53,11 @@ int check_attention(const smx_kv_cache *c, int n_seq, int n_q, int n_head, int p
     if (n_seq <= 0 || n_q <= 0) SMX_FAIL(SMX_EINVAL, "%s: need n_seq and n_q of at least 1", fn);
     if (max_len < 0 || max_len > v.ctx || prefix_len < 0 || prefix_len > v.ctx)
         SMX_FAIL(SMX_EINVAL, "%s: max_len %d and prefix_len %d must be within 0 .. ctx %d", fn, max_len, prefix_len, v.ctx);
-    if ((double)n_seq * n_q * n_head * v.hd > (double)kMaxGrid)
+    if ((double)n_seq * n_q * n_head * v.hd > (double)kMaxOutputs)
         SMX_FAIL(SMX_EUNSUPPORTED, "%s: %d x %d tokens of %d heads are too many outputs", fn, n_seq, n_q, n_head);
     *plan = attn_q8_plan(v, n_seq, n_q, n_head, prefix_len, max_len);
-    if (plan->blocks > kMaxGrid) SMX_FAIL(SMX_EUNSUPPORTED, "%s: too many sequences for one launch", fn);
+    // (the join has fewer: at most 2^31 outputs, four per thread, and several threads for one only where rows are few)
+    if (plan->blocks > kMaxBlocks) SMX_FAIL(SMX_EUNSUPPORTED, "%s: too many sequences for one launch", fn);
     return SMX_OK;
 }
 
@@ -154,7 +156,7 @@ SMX_API int smx_kv_append(smx_kv_cache *c, const float *k_dev, int64_t k_stride,
         SMX_FAIL(SMX_EINVAL, "smx_kv_append: k_stride %lld and v_stride %lld must be at least n_kv_head * head_dim = %lld",
                  (long long)k_stride, (long long)v_stride, (long long)row);
     if (((uintptr_t)k_dev | (uintptr_t)v_dev) & 3) SMX_FAIL(SMX_EINVAL, "smx_kv_append: misaligned pointer");
-    if (n_tok < 0 || ((int64_t)n_tok + 63) / 64 * c->view.n_kv * 2 > kMaxGrid)
+    if (n_tok < 0 || ((int64_t)n_tok + 63) / 64 * c->view.n_kv * 2 > kMaxBlocks)
         SMX_FAIL(SMX_EINVAL, "smx_kv_append: n_tok %d out of range", n_tok);
     if (n_tok == 0) return SMX_OK;
     const int rc = check_device(c, "smx_kv_append");
@@ -168,7 +170,7 @@ SMX_API int smx_kv_read(const smx_kv_cache *c, const int32_t *slots_dev, const i
 {
     if (!c || !k_dev || !v_dev || !slots_dev || !pos_dev) SMX_FAIL(SMX_EINVAL, "smx_kv_read: null argument");
     if (((uintptr_t)k_dev | (uintptr_t)v_dev) & 3) SMX_FAIL(SMX_EINVAL, "smx_kv_read: misaligned pointer");
-    if (n_tok < 0 || ((int64_t)n_tok + 63) / 64 * c->view.n_kv * 2 > kMaxGrid)
+    if (n_tok < 0 || ((int64_t)n_tok + 63) / 64 * c->view.n_kv * 2 > kMaxBlocks)
         SMX_FAIL(SMX_EINVAL, "smx_kv_read: n_tok %d out of range", n_tok);
     if (n_tok == 0) return SMX_OK;
     const int rc = check_device(c, "smx_kv_read");
@@ -212,6 +214,7 @@ SMX_API int smx_verify_draft(const float *target_dev, int64_t target_stride, con
         SMX_FAIL(SMX_EINVAL, "smx_verify_draft: null argument");
     if (n_seq <= 0 || n_draft < 0 || n_draft > 65535 || vocab <= 0 || vocab > (1 << 24))
         SMX_FAIL(SMX_EINVAL, "smx_verify_draft: need n_seq >= 1, 0 <= n_draft <= 65535, 1 <= vocab <= 2^24");
+    if (n_seq > kMaxBlocks / 4) SMX_FAIL(SMX_EUNSUPPORTED, "smx_verify_draft: too many sequences for one launch");
     if (target_stride < vocab || (draft_dev && n_draft > 0 && draft_stride < vocab))
         SMX_FAIL(SMX_EINVAL, "smx_verify_draft: rows must be at least vocab apart");
     if (((uintptr_t)target_dev | (uintptr_t)draft_dev) & 3) SMX_FAIL(SMX_EINVAL, "smx_verify_draft: misaligned pointer");

@@ -294,6 +294,25 @@ def test_a_cache_that_does_not_fit_leaves_no_error_behind(Q):
     c.close()
 
 
+def test_more_than_a_launch_takes_is_refused(Q):
+    """Sizes whose grids pass 2^32 threads; nothing is launched."""
+    import torch
+
+    from smallmind_amd._lib import load
+    L, c = load(), Q.GpuKvCache(1, 1, 8, 4096)
+    t = torch.zeros(4096, device="cuda")
+    i = torch.zeros(64, dtype=torch.int32, device="cuda")
+    for n_tok in (2**31 - 1, 2**31 - 64, 2**30, 2**29):
+        assert L.smx_kv_append(c._h, t.data_ptr(), 8, t.data_ptr(), 8, i.data_ptr(), i.data_ptr(), n_tok, None) == -1
+        assert L.smx_kv_read(c._h, i.data_ptr(), i.data_ptr(), n_tok, t.data_ptr(), t.data_ptr(), None) == -1
+    n = ctypes.c_int64()
+    for n_seq, n_q, P, code in ((2**24, 1, 0, -5), (2**24 - 1, 1, 0, 0), (2**24 - 1, 1, 64, -5), (2**23, 8, 64, 0)):
+        assert L.smx_attention_work_bytes(c._h, n_seq, n_q, 1, P, 64, ctypes.byref(n)) == code, (n_seq, n_q, P)
+    assert L.smx_verify_draft(t.data_ptr(), 8, None, 8, i.data_ptr(), None, t.data_ptr(), t.data_ptr(), 2**22, 1, 8, i.data_ptr(),
+                              i.data_ptr(), None) == -5
+    c.close()
+
+
 @pytest.mark.parametrize("hd", [64, 256])
 @pytest.mark.parametrize("k_up,q_up,v_up", [(96, -96, 96), (-90, 90, -80), (60, -50, 0)])
 def test_sizes_next_to_the_documented_limits(Q, hd, k_up, q_up, v_up):
