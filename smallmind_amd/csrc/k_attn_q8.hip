@@ -9,10 +9,14 @@
 // one pass over the positions, in tiles of 64.  The scales stay out of the products, so these take the
 // codes themselves, which fp16 holds exactly.  The other operands, q and w_p = 2^(c (x_p - m)) b_p, go
 // in as two fp16 values each, high part and remainder, both rounded to nearest, after a power of two has
-// brought the largest of the row (of q) or of the scales (b) below 2^15: 22 bits of every value down to
-// 2^-28 of the largest, 2^-39 of it in absolute terms, against the 24 bits of fp32; sums are fp32.
-// (One fp16 part would leave 11 bits: errors of 1e-4 where the fp32 outputs should have 1e-6.  bf16 parts
-// need three, and half as much again of the matrix instructions.)
+// brought the row's largest below 2^15 (q) or to at most 2^14 (w: the largest that the row has seen, relative to its
+// running maximum).  That is 22 bits of every value down to 2^-17 of the largest and, below that, 2^-38 of the largest
+// in absolute terms, against the 24 bits of fp32; sums are fp32.  So a position's weight is off by no more than
+// 2^-38 of what the row's largest term has, whatever the sizes of the V that other rows see or that the softmax
+// ignores.  (The power of two of w by the scales b alone, which are at hand before the weights, would save the search for the
+// largest, 1 % of the time with a shared prefix; but a large b that a row does not see, or that has no weight, would leave
+// the others no bits.  One fp16 part would leave 11 bits: errors of 1e-4 where the fp32 outputs should have 1e-6.  bf16
+// parts need three, and half as much again of the matrix instructions.)
 //
 // Layout.  A wave computes S^T = K q^T on 16x16x32 matrix instructions: lane 16 g + c gets
 // row c's x at positions 16 t + 4 g + i, which is how the second product out^T = V^T w^T wants them, so the
@@ -59,7 +63,8 @@ constexpr bool TAIL = W % 64 != 0;       // and a 32-wide one: 8 bytes per lane
 constexpr int NK = W / 32;               // matrix instructions along a K row
 constexpr int ND = W / 16;               // 16-dim groups of the output
 constexpr float kNegInf = -__builtin_huge_valf();
-constexpr float kLeast = 7.8886090522101181e-31f;   // 2^-100: no power of two below it is used as a scale
+constexpr float kLeast = 7.8886090522101181e-31f;   // 2^-100: no power of two below it is used as a scale of q
+constexpr float kLeastW = 1.9259299443872359e-34f;  // 2^-112: nor one below this for w (2^-39 of it is less than fp32 holds)
 
 __device__ __forceinline__ half8 halves(uint32_t lo, uint32_t hi)
 {
@@ -81,13 +86,6 @@ __device__ __forceinline__ float pow2_above(float f)
     return __uint_as_float((__float_as_uint(f) + 0x7FFFFFu) & 0x7F800000u);
 }
 
-// Brings a tile's V scales, a position's per lane, below 2^14 by a power of two that grows with them; returns what
-// sums in the old power's units are multiplied with.  (NaN scales stay NaN and do not count.)
-struct VUnit {
-    float up = kLeast;   // the power of two, at least every scale so far
-    __device__ __forceinline__ float take(float &scale);
-};
-
 // Two values as fp16 parts: h the nearest, l what is left.
 __device__ __forceinline__ void split(float a, float b, half2v &h, half2v &l)
 {
@@ -107,15 +105,6 @@ __device__ __forceinline__ float max_groups(float v)   // over the four lanes of
     v = fmaxf(p.x, p.y);
     p = swap16(v, v);
     return fmaxf(p.x, p.y);
-}
-
-__device__ __forceinline__ float max_lanes(float v)   // over the wave
-{
-    v = fmaxf(v, dpp_mov<0xB1>(v));
-    v = fmaxf(v, dpp_mov<0x4E>(v));
-    v = fmaxf(v, dpp_mov<0x141>(v));
-    v = fmaxf(v, dpp_mov<0x140>(v));
-    return max_groups(v);
 }
 
 __device__ __forceinline__ float sum_groups(float v)
@@ -143,15 +132,6 @@ __device__ __forceinline__ void wave_fence()
 {
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
-}
-
-__device__ __forceinline__ float VUnit::take(float &scale)
-{
-    const float was = up;
-    up = fmaxf(up, pow2_above(max_lanes(fmaxf(scale, kLeast))));
-    const float down = __uint_as_float((254u << 23) - __float_as_uint(up));   // 1 / up
-    scale *= 16384.0f * down;
-    return was * down;
 }
 
 struct KTile {
@@ -326,6 +306,8 @@ __device__ __forceinline__ void weigh(float4v (&acc)[ND], const half8 (&ph)[2], 
 struct Running {
     // m: the largest x so far; mc: c m as rounded, the exponent that acc and l are relative to
     float m = kNegInf, mc = kNegInf, l = 0.0f, c;
+    // most: the largest w so far, relative to m; unit: the power of two above it, in whose 2^-14ths acc is
+    float most = 0.0f, unit = kLeastW;
     float4v acc[ND];
 
     __device__ __forceinline__ Running()
@@ -334,13 +316,11 @@ struct Running {
         for (int n = 0; n < ND; n++) acc[n] = float4v{0, 0, 0, 0};
     }
 
-    // One tile: x (K q^T) becomes the weights' parts, acc and l move to the new maximum.  ks(t), vs(t): the
-    // scales of this lane's positions, those of V as VUnit left them; vdown: what it returned.  With WHOLE every
-    // position counts for every row; otherwise the row sees the tile's first `vis`; what is not seen weighs
-    // nothing whatever its scales hold.
+    // One tile: x (K q^T) becomes the weights' parts, acc and l move to the new maximum and unit.  ks(t), vs(t): the
+    // scales of this lane's positions.  With WHOLE every position counts for every row; otherwise the row sees
+    // the tile's first `vis`; what is not seen weighs nothing, and sets no unit, whatever its scales hold.
     template <bool WHOLE, typename KsOf, typename VsOf>
-    __device__ __forceinline__ void step(float4v (&x)[4], KsOf ks, VsOf vs, float vdown, half8 (&ph)[2], half8 (&pl)[2], int vis,
-                                         int g)
+    __device__ __forceinline__ void step(float4v (&x)[4], KsOf ks, VsOf vs, half8 (&ph)[2], half8 (&pl)[2], int vis, int g)
     {
         float top = m;
 #pragma unroll
@@ -357,33 +337,40 @@ struct Running {
         const float now = top == kNegInf ? 0.0f : top * c;
         const float alpha = __builtin_amdgcn_exp2f(mc - now);
         if (top != kNegInf) m = top, mc = now;
-        const float down = alpha * vdown;
-        if (__any(down != 1.0f)) {
-#pragma unroll
-            for (int n = 0; n < ND; n++) acc[n] *= down;
-        }
-        float sum = 0.0f;
+        float sum = 0.0f, big = 0.0f;
 #pragma unroll
         for (int t = 0; t < 4; t++) {
             const float4v v = vs(t);
-            float w[4];
 #pragma unroll
             for (int i = 0; i < 4; i++) {
                 const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(x[t][i], c, -now));
                 sum += p;
-                w[i] = p * v[i];
-                if (!WHOLE && 16 * t + 4 * g + i >= vis) w[i] = 0.0f;
+                x[t][i] = p * v[i];
+                if (!WHOLE && 16 * t + 4 * g + i >= vis) x[t][i] = 0.0f;
+                big = fmaxf(big, x[t][i]);   // (a NaN sets no unit)
             }
+        }
+        l = l * alpha + sum;
+        most = fmaxf(most * alpha, max_groups(big));
+        const float was = alpha * unit;   // at most twice the new unit
+        unit = pow2_above(fmaxf(most, kLeastW));
+        const float down = was * __uint_as_float((254u << 23) - __float_as_uint(unit));   // was / unit
+        if (__any(down != 1.0f)) {
+#pragma unroll
+            for (int n = 0; n < ND; n++) acc[n] *= down;
+        }
+        const float mul = __uint_as_float((268u << 23) - __float_as_uint(unit));   // 2^14 / unit
+#pragma unroll
+        for (int t = 0; t < 4; t++) {
 #pragma unroll
             for (int i = 0; i < 4; i += 2) {
                 half2v h, r;
-                split(w[i], w[i + 1], h, r);
+                split(x[t][i] * mul, x[t][i + 1] * mul, h, r);
                 put(ph[t >> 1], 4 * (t & 1) + i, h);
                 put(pl[t >> 1], 4 * (t & 1) + i, r);
             }
             here();
         }
-        l = l * alpha + sum;
     }
 };
 
@@ -413,7 +400,6 @@ __device__ __forceinline__ void stream(const AttnQ8Args &a, Shared &S, const uin
     KTile kt;
     VTile vt;
     float kone = 0.0f, vone = 0.0f;
-    VUnit unit;
     float (*scale)[kKvTile] = S.scale[wave];
     const auto load_scales = [&]() {
         const float *p = (const float *)(rec + 2 * kKvTile * W) + lane;
@@ -436,8 +422,6 @@ __device__ __forceinline__ void stream(const AttnQ8Args &a, Shared &S, const uin
         for (; tile < end; tile += 4) {
             // a position's scales per lane, to be read by the lanes whose x belongs to it
             const int at = p0 + tile * kKvTile;
-            if (!decltype(whole)::value && lane >= p1 - at) vone = 0.0f;
-            const float vdown = unit.take(vone);
             scale[0][lane] = kone;
             scale[1][lane] = vone;
             wave_fence();
@@ -452,7 +436,7 @@ __device__ __forceinline__ void stream(const AttnQ8Args &a, Shared &S, const uin
             half8 ph[2], pl[2];
             R.template step<decltype(whole)::value>(
                 x, [&](int t) { return *(const float4v *)&scale[0][16 * t + 4 * g]; },
-                [&](int t) { return *(const float4v *)&scale[1][16 * t + 4 * g]; }, vdown, ph, pl, vis - at, g);
+                [&](int t) { return *(const float4v *)&scale[1][16 * t + 4 * g]; }, ph, pl, vis - at, g);
             weigh<false>(R.acc, ph, pl, [&](int n, int kb) { return halves(vt.a[n][2 * kb], vt.a[n][2 * kb + 1]); });
             if (more) {
                 load_v<NT>(vt, rec, g, col);
@@ -466,7 +450,7 @@ __device__ __forceinline__ void stream(const AttnQ8Args &a, Shared &S, const uin
     go(tile, n_tiles, std::false_type{});
 
     __syncthreads();   // (the queries have been read)
-    const float sum = sum_groups(R.l), up = unit.up * (1.0f / 16384.0f);
+    const float sum = sum_groups(R.l), up = R.unit * (1.0f / 16384.0f);
     if (g == 0) {
         S.m[wave][col] = R.mc;
         S.l[wave][col] = sum;
@@ -535,17 +519,9 @@ struct Share {
         if (threadIdx.x < 2 * kKvTile) scale = ((const float *)(rec + 2 * kKvTile * W))[threadIdx.x];
     }
 
-    // The scales of a tile with `left` positions: K by wave 0, V, in `unit`, by wave 1.
-    __device__ __forceinline__ void put_scales(float (&to)[2][kKvTile], float2 &info, VUnit &unit, int wave, int lane, int left)
+    __device__ __forceinline__ void put_scales(float (&to)[2][kKvTile]) const
     {
-        if (wave == 0) {
-            to[0][lane] = scale;
-        } else if (wave == 1) {
-            float v = lane < left ? scale : 0.0f;
-            const float down = unit.take(v);
-            to[1][lane] = v;
-            if (lane == 0) info = make_float2(unit.up, down);
-        }
+        if (threadIdx.x < 2 * kKvTile) to[threadIdx.x / kKvTile][threadIdx.x % kKvTile] = scale;
     }
 };
 
@@ -554,7 +530,6 @@ constexpr int NB = W <= 128 ? 2 : 1;   // a second buffer takes the next tile wh
 struct Tiles {
     half8 k[NB][4][NK][64], v[NB][ND][2][64];
     float scale[NB][2][kKvTile];
-    float2 unit[NB];   // the unit of the tile's V scales, and what sums are multiplied with
 };
 
 // Positions [p0, p1), all seen by every row; each of the four waves has its own rows row_of(0 .. 15).  Writes the
@@ -572,8 +547,6 @@ __device__ __forceinline__ void rows(const AttnQ8Args &a, Tiles &S, QRows *Q, co
 
     half8 qh[NK], ql[NK];
     Running R;
-    VUnit unit;        // of the wave that brings the V scales
-    float vup = kLeast;
     bring_q(a, Q[wave], lane, 64, row_of);
     __syncthreads();
     take_q(a, Q[wave], qh, ql, R.c, g, col);
@@ -596,19 +569,17 @@ __device__ __forceinline__ void rows(const AttnQ8Args &a, Tiles &S, QRows *Q, co
                     S.v[b][wave + 4 * j][0][lane] = halves(in.va[j][0], in.va[j][1]);
                     S.v[b][wave + 4 * j][1][lane] = halves(in.va[j][2], in.va[j][3]);
                 }
-            in.put_scales(S.scale[b], S.unit[b], unit, wave, lane, p1 - p0 - tile * kKvTile);
+            in.put_scales(S.scale[b]);
             rec += REC;
             if (tile + 1 < n_tiles) in.load(rec, wave, g, col);
             __syncthreads();
             if (!asked(busy)) continue;
             float4v x[4];
             scores<true>(x, qh, ql, [&](int t, int n) { return S.k[b][t][n][lane]; });
-            vup = S.unit[b].x;
             half8 ph[2], pl[2];
             R.template step<decltype(whole)::value>(
                 x, [&](int t) { return *(const float4v *)&S.scale[b][0][16 * t + 4 * g]; },
-                [&](int t) { return *(const float4v *)&S.scale[b][1][16 * t + 4 * g]; }, S.unit[b].y, ph, pl,
-                p1 - p0 - tile * kKvTile, g);
+                [&](int t) { return *(const float4v *)&S.scale[b][1][16 * t + 4 * g]; }, ph, pl, p1 - p0 - tile * kKvTile, g);
             weigh<true>(R.acc, ph, pl, [&](int n, int kb) { return S.v[b][n][kb][lane]; });
         }
     };
@@ -616,7 +587,7 @@ __device__ __forceinline__ void rows(const AttnQ8Args &a, Tiles &S, QRows *Q, co
     go(tile, (p1 - p0) / kKvTile, std::true_type{});
     go(tile, n_tiles, std::false_type{});
     const RowRef r = row_of(col);
-    const float sum = sum_groups(R.l), up = vup * (1.0f / 16384.0f);
+    const float sum = sum_groups(R.l), up = R.unit * (1.0f / 16384.0f);
     if (!r.valid) return;
     const int64_t id = (int64_t)part * a.n_rows + (int64_t)r.token * a.n_head + r.head;
     if (g == 0) a.part_ml[id * 2] = R.mc, a.part_ml[id * 2 + 1] = sum;

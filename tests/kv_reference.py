@@ -94,3 +94,37 @@ def verify(target, draft, tokens, u_accept, u_draw, lens, vocab):
                 break
         acc[b] = i
     return out, acc
+
+
+def attention_by_terms(q, k, v, visible):
+    """attention() with a bound for every element that goes by the row's own weighted terms p_j v_j, not by the
+    largest v: (out, bound), each [rows][hd], in 64 bits.
+
+    With p_j the weights relative to the largest (p <= 1), A = sum p |v| per element and S = sum p:
+      scores    q in two fp16 parts is off by 2^-22 of each element and 2^-38 of the row's largest; the 2 hd products
+                are added in fp32 (a rounding of 2^-24 of the sum of sizes for each, 2^-24 each for the scale of K and for
+                K's held value); the exponent's difference and product are 3 roundings of |score| and of the largest
+                one.  Weight j moves by that e_j relative to itself, and by 2^-22 for the exponential and the rounding
+                of p times V's scale; numerator and S both move.
+      weights   two fp16 parts: 2^-22 of each, and 2^-38 of the largest p_j max|v_j|, for each position.
+      sums      the two parts' products (2 n), S (n) and the joins of waves and parts, 2^-24 of A or S each."""
+    q, k, v = (np.asarray(a, np.float64) for a in (q, k, v))
+    rows, hd = q.shape
+    out, bound = np.zeros((rows, v.shape[1])), np.zeros((rows, v.shape[1]))
+    for r in range(rows):
+        vis = visible[r]
+        n = int(vis.sum())
+        if not n:
+            continue
+        kk, vv = k[vis], v[vis]
+        s = kk @ q[r] / math.sqrt(hd)
+        p = np.exp(s - s.max())
+        S, A = p.sum(), p @ np.abs(vv)
+        out[r] = p @ vv / S
+        mass = (np.abs(kk) @ np.abs(q[r])) / math.sqrt(hd)
+        reach = np.abs(kk).sum(1) * np.abs(q[r]).max() / math.sqrt(hd)
+        e = mass * (2.0 ** -22 + (2 * hd + 2) * 2.0 ** -24) + reach * 2.0 ** -38 + 3 * (np.abs(s) + abs(s.max())) * 2.0 ** -24
+        e += 2.0 ** -22
+        most = (p * np.abs(vv).max(1)).max()
+        bound[r] = ((p * e) @ np.abs(vv) + A * ((p @ e) / S + 2.0 ** -22 + (3 * n + 16) * 2.0 ** -24) + n * 2.0 ** -38 * most) / S
+    return out, bound

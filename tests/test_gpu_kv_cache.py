@@ -1,6 +1,7 @@
 """The 8-bit KV cache, the attention over it and the verification of drafted tokens on the GPU, against
 plain 64-bit forms."""
 import ctypes
+import math
 
 import numpy as np
 import pytest
@@ -637,6 +638,114 @@ def test_captured_steps_replay(Q):
             sl = np.arange(n) + gi * n
             f.hk[sl, start[gi] + step], f.hv[sl, start[gi] + step] = R.held(xk[gi, step]), R.held(xv[gi, step])
             close(st["out"], reference(f, xq[gi, step], sl, start[gi] + step + 1, (2 * n, 300)))
+    f.cache.close()
+
+
+def by_terms(f, q, slots, lens, prefix=None):
+    """reference() with the bound that goes by each row's own weighted terms, for every element."""
+    n_seq, n_q, H, hd = q.shape
+    kv, P = f.hk.shape[2], prefix[1] if prefix else 0
+    G = H // kv
+    out, bound = np.zeros(q.shape), np.zeros(q.shape)
+    for b in range(n_seq):
+        n = max(0, min(int(lens[b]), f.hk.shape[1]))
+        for h in range(kv):
+            k, v = f.hk[slots[b], :n, h], f.hv[slots[b], :n, h]
+            if P:
+                k, v = np.concatenate([f.hk[prefix[0], :P, h], k]), np.concatenate([f.hv[prefix[0], :P, h], v])
+            at = slice(h * G, (h + 1) * G)
+            for i in range(n_q):
+                vis = np.zeros((G, P + n), bool)
+                vis[:, :P + max(0, n - n_q + 1 + i)] = True
+                out[b, i, at], bound[b, i, at] = R.attention_by_terms(q[b, i, at], k, v, vis)
+    return out, bound
+
+
+def close_by_terms(got, want):
+    ref, bound = want
+    err = np.abs(got.cpu().numpy().astype(np.float64) - ref)
+    assert (err <= bound).all(), (float((err / np.maximum(bound, 1e-300)).max()), np.argwhere(~(err <= bound))[:4])
+
+
+class Held:
+    """A cache holding the rows k, v [slots][ctx][kv][hd]."""
+
+    def __init__(self, Q, k, v):
+        slots, ctx, kv, hd = k.shape
+        n = slots * ctx
+        self.cache = Q.GpuKvCache(slots, kv, hd, ctx)
+        self.cache.append(dev(k.reshape(n, kv, hd)), dev(v.reshape(n, kv, hd)), i32(np.repeat(np.arange(slots), ctx)),
+                          i32(np.tile(np.arange(ctx), slots)))
+        self.hk, self.hv = R.held(k), R.held(v)
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("group", [1, 6])
+@pytest.mark.parametrize("up", [20, 30, 60, 90])
+def test_large_values_that_only_later_tokens_see(Q, hd, group, up):
+    """Drafted tokens whose V is far above the rest: the tokens before them do not see it, and keep all their bits."""
+    rng = np.random.default_rng([hd, group, up])
+    n_q, lens, P = 4, np.array([40, 64, 67, 300]), 90
+    k, v = (rng.normal(0, 1, (5, 300, 2, hd)).astype(np.float32) for _ in range(2))
+    for b, n in enumerate(lens):
+        v[b, n - 3:n] *= np.exp2(np.float32(up) * np.array([1, 0.5, 1], np.float32))[:, None, None]
+    f = Held(Q, k, v)
+    q = rng.normal(0, 1, (4, n_q, 2 * group, hd)).astype(np.float32)
+    slots = np.arange(4)
+    close_by_terms(Q.attention_cached(dev(q), f.cache, i32(slots), i32(lens)), by_terms(f, q, slots, lens))
+    close_by_terms(Q.attention_shared(dev(q), f.cache, 4, P, i32(slots), i32(lens)), by_terms(f, q, slots, lens, (4, P)))
+    f.cache.close()
+
+
+@pytest.mark.parametrize("hd", [32, 64, 128, 256])
+@pytest.mark.parametrize("up", [25, 40, 80])
+def test_large_values_that_the_softmax_ignores(Q, hd, up):
+    """Positions with a weight of e^-100 and a V far above the rest (early, late, in other waves' tiles, in a prefix), and one
+    with nearly all the weight and a V of zeros: the others keep their bits."""
+    rng = np.random.default_rng([hd, up])
+    n, lens, P = 500, np.array([500, 333, 64, 20]), 200
+    slots = np.arange(4)
+    q = rng.choice([-1.0, 1.0], (4, 1, 2, hd)).astype(np.float32)
+    k, v = (rng.normal(0, 1, (5, n, 1, hd)).astype(np.float32) for _ in range(2))
+    # scores against every query: 0 +- a few; with `away` added to them by the first element
+    q[..., 0] = 8.0
+    k[..., 0] = 0.0
+    away = math.sqrt(hd) / 8.0
+    for s in range(5):
+        hidden = rng.choice(n, 40, replace=False)
+        if s < 4:
+            hidden = hidden[hidden < lens[s] - 4]
+        hidden = np.union1d(hidden, [0, 5])
+        k[s, hidden], v[s, hidden] = 0.0, v[s, hidden] * np.float32(2.0 ** up)
+        k[s, hidden, :, 0] = -100 * away
+    k[3, 7], v[3, 7], v[0, 130] = 0.0, 0.0, 0.0
+    k[3, 7, :, 0] = 25 * away
+    f = Held(Q, k, v)
+    close_by_terms(Q.attention_cached(dev(q), f.cache, i32(slots), i32(lens)), by_terms(f, q, slots, lens))
+    for seqs in (4, 1):      # (both ways through a prefix)
+        t = slice(0, seqs)
+        qs = np.tile(q[t], (1, 1, 10, 1)) if seqs == 4 else q[t]
+        close_by_terms(Q.attention_shared(dev(qs), f.cache, 4, P, i32(slots[t]), i32(lens[t])), by_terms(f, qs, slots[t], lens[t], (4, P)))
+    f.cache.close()
+
+
+@pytest.mark.parametrize("hd", [8, 64, 128, 256])
+def test_operands_keep_both_parts(Q, hd):
+    """Two positions, and values that one fp16 part would round all in one direction: for q by more than the bound, and
+    for V's scales likewise."""
+    up = np.float32(1 + 0.97 * 2.0 ** -11)
+    q = np.full((1, 1, 1, hd), up, np.float32)
+    k = np.zeros((1, 2, 1, hd), np.float32)
+    k[0, 0] = 2.0 / math.sqrt(hd)            # a score of 2 beside one of 0
+    v = np.zeros((1, 2, 1, hd), np.float32)
+    v[0, 0], v[0, 1] = 127 * up, -127 * up
+    f = Held(Q, k, v)
+    want = by_terms(f, q, [0], [2])
+    for wrong in (R.attention_by_terms(np.float16(q[0, 0]).astype(np.float64), f.hk[0, :, 0], f.hv[0, :, 0], np.ones((1, 2), bool))[0],
+                  want[0][0, 0] / up):
+        assert (np.abs(wrong - want[0][0, 0]) > want[1][0, 0]).all()
+    close_by_terms(Q.attention_cached(dev(q), f.cache, i32([0]), i32([2])), want)
+    close_by_terms(Q.attention_shared(dev(q), f.cache, 0, 2, i32([0]), i32([0])), by_terms(f, q, [0], [0], (0, 2)))
     f.cache.close()
 
 
