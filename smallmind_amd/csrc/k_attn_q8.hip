@@ -205,20 +205,21 @@ __device__ __forceinline__ void bring_q(const AttnQ8Args &a, QRows &S, int first
     }
 }
 
-// The power of two that a row of q is brought to the range of fp16 with, and c in the units of the products.
+// The power of two that a row of q is brought to the range of fp16 with, and the units of the products, as AttnQ8Args has
+// scores.
 struct QScale {
-    float mul, c;
+    float mul, unit;
 };
 // amax: the largest finite element; bad: the row holds a NaN or an infinity, and becomes NaN.
 __device__ __forceinline__ QScale q_scale(const AttnQ8Args &a, float amax, bool bad)
 {
     const float unit = amax > kLeast ? __uint_as_float(__float_as_uint(amax) & 0x7F800000u) : kLeast;   // 2^e
     const float mul = __uint_as_float((268u << 23) - __float_as_uint(unit));                            // 2^14 / unit
-    return QScale{bad ? __uint_as_float(0x7FC00000u) : mul, a.scale_log2e * (unit * (1.0f / 16384.0f))};
+    return QScale{bad ? __uint_as_float(0x7FC00000u) : mul, unit * (1.0f / 262144.0f)};
 }
 
-// The operands of the rows in S, and c.
-__device__ __forceinline__ void take_q(const AttnQ8Args &a, const QRows &S, half8 (&qh)[NK], half8 (&ql)[NK], float &c, int g, int col)
+// The operands of the rows in S, and the units of their products.
+__device__ __forceinline__ void take_q(const AttnQ8Args &a, const QRows &S, half8 (&qh)[NK], half8 (&ql)[NK], float &xu, int g, int col)
 {
     float4v f[NK][2];
     uint32_t top = 0;
@@ -234,7 +235,7 @@ __device__ __forceinline__ void take_q(const AttnQ8Args &a, const QRows &S, half
         }
     }
     const QScale q = q_scale(a, max_groups(__uint_as_float(min(top, 0x7F7FFFFFu))), max_groups(top > 0x7F7FFFFFu ? 1.0f : 0.0f) > 0.0f);
-    c = q.c;
+    xu = q.unit;
 #pragma unroll
     for (int n = 0; n < NK; n++)
 #pragma unroll
@@ -304,8 +305,8 @@ __device__ __forceinline__ void weigh(float4v (&acc)[ND], const half8 (&ph)[2], 
 
 // The running softmax of a block of rows, a row per column of 16 lanes.
 struct Running {
-    // m: the largest x so far; mc: c m as rounded, the exponent that acc and l are relative to
-    float m = kNegInf, mc = kNegInf, l = 0.0f, c;
+    // m: the largest x so far, that acc and l are relative to; xu: the units of x
+    float m = kNegInf, l = 0.0f, xu;
     // most: the largest w so far, relative to m; unit: the power of two above it, in whose 2^-14ths acc is
     float most = 0.0f, unit = kLeastW;
     float4v acc[ND];
@@ -319,8 +320,10 @@ struct Running {
     // One tile: x (K q^T) becomes the weights' parts, acc and l move to the new maximum and unit.  ks(t), vs(t): the
     // scales of this lane's positions.  With WHOLE every position counts for every row; otherwise the row sees
     // the tile's first `vis`; what is not seen weighs nothing, and sets no unit, whatever its scales hold.
+    // Exponents are (x - m) c, not x c - (m c), which saves an instruction: m c rounded is off by up to 2^-24 of it, and a
+    // weight that is 2^off too large leaves fp16 when scores pass 2^26.
     template <bool WHOLE, typename KsOf, typename VsOf>
-    __device__ __forceinline__ void step(float4v (&x)[4], KsOf ks, VsOf vs, half8 (&ph)[2], half8 (&pl)[2], int vis, int g)
+    __device__ __forceinline__ void step(float4v (&x)[4], float c, KsOf ks, VsOf vs, half8 (&ph)[2], half8 (&pl)[2], int vis, int g)
     {
         float top = m;
 #pragma unroll
@@ -334,16 +337,16 @@ struct Running {
         }
         top = max_groups(top);
         // (a row that has seen nothing yet: x = -inf against 0)
-        const float now = top == kNegInf ? 0.0f : top * c;
-        const float alpha = __builtin_amdgcn_exp2f(mc - now);
-        if (top != kNegInf) m = top, mc = now;
+        const float base = top == kNegInf ? 0.0f : top;
+        const float alpha = __builtin_amdgcn_exp2f((m - base) * c);
+        m = top;
         float sum = 0.0f, big = 0.0f;
 #pragma unroll
         for (int t = 0; t < 4; t++) {
             const float4v v = vs(t);
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(x[t][i], c, -now));
+                const float p = __builtin_amdgcn_exp2f((x[t][i] - base) * c);
                 sum += p;
                 x[t][i] = p * v[i];
                 if (!WHOLE && 16 * t + 4 * g + i >= vis) x[t][i] = 0.0f;
@@ -414,7 +417,8 @@ __device__ __forceinline__ void stream(const AttnQ8Args &a, Shared &S, const uin
     Running R;
     bring_q(a, S.q, threadIdx.x, 256, row_of);
     __syncthreads();
-    take_q(a, S.q, qh, ql, R.c, g, col);
+    take_q(a, S.q, qh, ql, R.xu, g, col);
+    const float c = a.scale_log2e * R.xu;
     const int vis = row_of(col).valid ? vis_of(col) : 0;
 
     // tiles that every row sees all of, then the rest: the same code with and without the bounds
@@ -435,7 +439,7 @@ __device__ __forceinline__ void stream(const AttnQ8Args &a, Shared &S, const uin
             if (more) load_k<NT>(kt, rec, g, col);
             half8 ph[2], pl[2];
             R.template step<decltype(whole)::value>(
-                x, [&](int t) { return *(const float4v *)&scale[0][16 * t + 4 * g]; },
+                x, c, [&](int t) { return *(const float4v *)&scale[0][16 * t + 4 * g]; },
                 [&](int t) { return *(const float4v *)&scale[1][16 * t + 4 * g]; }, ph, pl, vis - at, g);
             weigh<false>(R.acc, ph, pl, [&](int n, int kb) { return halves(vt.a[n][2 * kb], vt.a[n][2 * kb + 1]); });
             if (more) {
@@ -452,7 +456,7 @@ __device__ __forceinline__ void stream(const AttnQ8Args &a, Shared &S, const uin
     __syncthreads();   // (the queries have been read)
     const float sum = sum_groups(R.l), up = R.unit * (1.0f / 16384.0f);
     if (g == 0) {
-        S.m[wave][col] = R.mc;
+        S.m[wave][col] = R.m * R.xu;
         S.l[wave][col] = sum;
     }
 #pragma unroll
@@ -461,7 +465,7 @@ __device__ __forceinline__ void stream(const AttnQ8Args &a, Shared &S, const uin
 }
 
 // Joins the waves' sums and writes the rows: the outputs, or with more parts to come the part's
-// maximum (in powers of two), sum and weighted sums.
+// maximum, sum and weighted sums.
 template <typename RowOf>
 __device__ __forceinline__ void finish(const AttnQ8Args &a, Shared &S, int part, RowOf row_of)
 {
@@ -476,7 +480,7 @@ __device__ __forceinline__ void finish(const AttnQ8Args &a, Shared &S, int part,
 #pragma unroll
         for (int w = 0; w < 4; w++) {
             // a wave without a visible position has the sum 0 (and one that saw NaN a NaN)
-            const float f = S.m[w][row] == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(S.m[w][row] - top);
+            const float f = S.m[w][row] == kNegInf ? 0.0f : __builtin_amdgcn_exp2f((S.m[w][row] - top) * a.scale_log2e);
             if (S.l[w][row] == 0.0f) continue;
             sum += S.l[w][row] * f;
             o += *(const float4v *)&S.acc[w][row][d] * f;
@@ -549,7 +553,8 @@ __device__ __forceinline__ void rows(const AttnQ8Args &a, Tiles &S, QRows *Q, co
     Running R;
     bring_q(a, Q[wave], lane, 64, row_of);
     __syncthreads();
-    take_q(a, Q[wave], qh, ql, R.c, g, col);
+    take_q(a, Q[wave], qh, ql, R.xu, g, col);
+    const float c = a.scale_log2e * R.xu;
     __syncthreads();
     const int busy = __any(row_of(0).valid);   // (a wave without rows brings its share of the tiles)
 
@@ -578,7 +583,7 @@ __device__ __forceinline__ void rows(const AttnQ8Args &a, Tiles &S, QRows *Q, co
             scores<true>(x, qh, ql, [&](int t, int n) { return S.k[b][t][n][lane]; });
             half8 ph[2], pl[2];
             R.template step<decltype(whole)::value>(
-                x, [&](int t) { return *(const float4v *)&S.scale[b][0][16 * t + 4 * g]; },
+                x, c, [&](int t) { return *(const float4v *)&S.scale[b][0][16 * t + 4 * g]; },
                 [&](int t) { return *(const float4v *)&S.scale[b][1][16 * t + 4 * g]; }, ph, pl, p1 - p0 - tile * kKvTile, g);
             weigh<true>(R.acc, ph, pl, [&](int n, int kb) { return S.v[b][n][kb][lane]; });
         }
@@ -590,7 +595,7 @@ __device__ __forceinline__ void rows(const AttnQ8Args &a, Tiles &S, QRows *Q, co
     const float sum = sum_groups(R.l), up = R.unit * (1.0f / 16384.0f);
     if (!r.valid) return;
     const int64_t id = (int64_t)part * a.n_rows + (int64_t)r.token * a.n_head + r.head;
-    if (g == 0) a.part_ml[id * 2] = R.mc, a.part_ml[id * 2 + 1] = sum;
+    if (g == 0) a.part_ml[id * 2] = R.m * R.xu, a.part_ml[id * 2 + 1] = sum;
     float *dst = a.part_acc + id * a.hd + 4 * g;
 #pragma unroll
     for (int n = 0; n < ND; n++)

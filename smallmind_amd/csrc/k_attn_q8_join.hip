@@ -11,7 +11,7 @@ namespace smx {
 
 namespace {
 
-// out = sum_s 2^(m_s - M) acc_s / sum_s 2^(m_s - M) l_s over the parts s that have weight, M their largest m.
+// out = sum_s 2^(c (m_s - M)) acc_s / sum_s 2^(c (m_s - M)) l_s over the parts s that have weight, M their largest m.
 // What bounds it is the latency of the parts' loads, so a thread takes four dims of every PP-th part of a row,
 // requested four at a time, and PP threads join theirs through LDS in a fixed order.  Rows of a sequence
 // without a slot are 0.
@@ -20,12 +20,12 @@ struct Joined {
     float l, top;
 };
 
-__device__ __forceinline__ void join(Joined &a, float4 v, float l, float m)
+__device__ __forceinline__ void join(Joined &a, float4 v, float l, float m, float c)
 {
     if (l == 0.0f) return;   // a part without weight may hold anything in v
     const float up = fmaxf(a.top, m);
     // (-inf - -inf where nothing but NaN has been seen: the sum is NaN already)
-    const float f = __builtin_amdgcn_exp2f(m - up), g = a.l == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(a.top - up);
+    const float f = __builtin_amdgcn_exp2f((m - up) * c), g = a.l == 0.0f ? 0.0f : __builtin_amdgcn_exp2f((a.top - up) * c);
     a.top = up;
     a.l = a.l * g + l * f;
     a.o.x = a.o.x * g + v.x * f, a.o.y = a.o.y * g + v.y * f;
@@ -55,7 +55,7 @@ __global__ __launch_bounds__(256) void k_attn_q8_join(const AttnQ8Args a)
         }
 #pragma unroll
         for (int k = 0; k < 4; k++)
-            if (s0 + k * PP < a.parts) join(J, v[k], ml[k].y, ml[k].x);
+            if (s0 + k * PP < a.parts) join(J, v[k], ml[k].y, ml[k].x, a.scale_log2e);
     }
     if constexpr (PP > 1) {
         if (pp > 0) S[pp - 1][lane] = J;
@@ -64,7 +64,7 @@ __global__ __launch_bounds__(256) void k_attn_q8_join(const AttnQ8Args a)
 #pragma unroll
         for (int k = 0; k < PP - 1; k++) {
             const Joined &T = S[k][lane];
-            join(J, T.o, T.l, T.top);
+            join(J, T.o, T.l, T.top, a.scale_log2e);
         }
     }
     if (!in) return;
@@ -154,7 +154,7 @@ hipError_t launch_attn_q8(const KvView &c, const AttnQ8Plan &p, const float *q, 
     a.part_ml = work ? (float *)work + p.parts * a.n_rows * c.hd : nullptr;
     a.q_stride = q_stride;
     a.inv_group = (double)c.n_kv / n_head;
-    a.scale_log2e = (float)(1.4426950408889634 / sqrt((double)c.hd));
+    a.scale_log2e = (float)(1.4426950408889634 * 16.0 / sqrt((double)c.hd));
     a.q_vec = ((uintptr_t)q & 15) == 0 && q_stride % 4 == 0;
     a.out_vec = ((uintptr_t)out & 15) == 0;
     a.n_slots = c.n_slots;

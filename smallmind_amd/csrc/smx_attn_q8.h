@@ -21,7 +21,9 @@ struct AttnQ8Args {
     float *part_ml, *part_acc;  // [parts][n_rows][2], [parts][n_rows][hd]
     int64_t q_stride, n_rows;   // n_rows = n_seq * n_q * n_head
     double inv_group;           // n_kv / n_head
-    float scale_log2e;          // log2(e) / sqrt(hd)
+    // Scores are held as q . k / 16, no larger than what they stand for (hd <= 256), which spares them fp32's end;
+    // log2(e) 16 / sqrt(hd) makes them exponents.
+    float scale_log2e;
     int q_vec, out_vec;         // q, out may be read and written as float4
     int n_slots, n_seq, n_q, n_head, n_kv, hd;
     int max_len, own_chunk, own_splits, own_blocks;

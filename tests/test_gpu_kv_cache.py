@@ -749,6 +749,87 @@ def test_operands_keep_both_parts(Q, hd):
     f.cache.close()
 
 
+@pytest.mark.parametrize("hd", [16, 64, 256])
+@pytest.mark.parametrize("k_up,q_up", [(0, 12), (0, 24), (10, 16), (10, 19), (30, 30), (80, 30), (-60, 100), (89, -89), (89, 24)])
+def test_scores_of_every_size(Q, hd, k_up, q_up):
+    """K rows of whole multiples of 2^k_up and queries of 2^q_up: scores, up to 2^126, are exact in fp32, and so is which of them
+    are the largest.  With a step of 2^10 or more between scores these alone have weight, and the output is the mean of their V."""
+    rng = np.random.default_rng([hd, k_up + 100])
+    n, P, kv, n_q = 700, 300, 2, 3
+    codes = rng.integers(-100, 1, (3, n, kv))
+    codes[0] = np.sort(codes[0], 0)                     # the maximum moves with every few positions
+    codes[1] = np.sort(codes[1], 0)[::-1]
+    codes[2] -= 20                                      # all scores far below 0
+    k = np.zeros((3, n, kv, hd), np.float64)
+    k[..., 0] = 127                                     # the scale is 2^k_up; no query asks for this element
+    k[..., 1:9] = codes[..., None]
+    f = Held(Q, (k * 2.0 ** k_up).astype(np.float32), rng.normal(0, 1, (3, n, kv, hd)).astype(np.float32))
+    assert np.array_equal(f.hk, k * 2.0 ** k_up)
+    q = np.zeros((3, n_q, 2 * kv, hd), np.float32)
+    q[..., 1:9] = 2.0 ** q_up
+    # a step between scores: 8 q k / sqrt(hd); one of 2^10 in fp32 makes a weight of exp2(-2^10) = 0
+    step = 8 * 2.0 ** (k_up + q_up) / math.sqrt(hd)
+    assert step >= 2.0 ** 10 or (k_up, q_up) == (89, -89)
+    slots, lens = np.array([2, 0, 1]), np.array([700, 611, 66])
+    for prefix in (None, (2, P)):
+        for b, (slot, length) in enumerate(zip(slots, lens)):
+            if prefix is None:
+                got = Q.attention_cached(dev(q[b:b + 1]), f.cache, i32([slot]), i32([length]))
+            else:
+                got = Q.attention_shared(dev(q[b:b + 1]), f.cache, *prefix, i32([slot]), i32([length]))
+            ref, bound = by_terms(f, q[b:b + 1], [slot], [length], prefix)
+            if step >= 2.0 ** 10:
+                # equal scores have equal weights, whatever their size: what is left of the bound is sums and V's parts
+                bound = bound * 0
+                for i in range(n_q):
+                    for h in range(2 * kv):
+                        c, v = codes[slot, :length - n_q + 1 + i, h // 2], f.hv[slot, :length - n_q + 1 + i, h // 2]
+                        if prefix:
+                            c, v = np.concatenate([codes[2, :P, h // 2], c]), np.concatenate([f.hv[2, :P, h // 2], v])
+                        v = v[c == c.max()].astype(np.float64)
+                        assert np.allclose(ref[0, i, h], v.mean(0), rtol=1e-12, atol=1e-12)
+                        bound[0, i, h] = np.abs(v).mean(0) * (2.0 ** -21 + (3 * len(v) + 16) * 2.0 ** -24) + len(v) * 2.0 ** -38 * np.abs(v).max()
+            close_by_terms(got, (ref, bound))
+    # all three at once, through the other way of the prefix
+    qq = np.tile(q, (1, 2, 2, 1))
+    a = Q.attention_shared(dev(qq), f.cache, 2, P, i32(slots), i32(lens)).cpu().numpy()
+    if step >= 2.0 ** 10:
+        assert np.isfinite(a).all() and (np.abs(a) <= np.abs(f.hv).max() * 1.001).all()
+        i, h = 5, 0
+        c, v = np.concatenate([codes[2, :P, 0], codes[2, :700, 0]]), np.concatenate([f.hv[2, :P, 0], f.hv[2, :700, 0]])
+        v = v[c == c.max()].astype(np.float64)
+        tol = np.abs(v).mean(0) * (2.0 ** -21 + (3 * len(v) + 16) * 2.0 ** -24) + len(v) * 2.0 ** -38 * np.abs(v).max()
+        assert (np.abs(a[0, i, h] - v.mean(0)) <= tol).all()
+    f.cache.close()
+
+
+def test_small_differences_of_large_scores(Q):
+    """Scores of some 2^24 that differ by whole numbers: exact in fp32, so the weights are those of the differences, in one tile, over the
+    tiles of several waves and over parts."""
+    rng = np.random.default_rng(5)
+    hd, n = 64, 1500
+    less = rng.integers(0, 12, n)
+    less[rng.integers(0, n, 9)] = 0
+    k = np.zeros((1, n, 1, hd), np.float32)
+    k[..., 0], k[..., 1] = 127, 127 - less[None, :, None]
+    # (2^13 127 127 + 8 (127 - less)) / 8: whole numbers below 2^24
+    q = np.zeros((1, 1, 1, hd), np.float32)
+    q[..., 0], q[..., 1] = 2.0 ** 13 * 127, 8.0
+    f = Held(Q, k, rng.normal(0, 1, (1, n, 1, hd)).astype(np.float32))
+    p = np.exp(-less * 1.0)[:, None]
+    for length in (50, 300, 1500):
+        w, v = p[:length], f.hv[0, :length, 0].astype(np.float64)
+        ref, A = (w * v).sum(0) / w.sum(), (w * np.abs(v)).sum(0) / w.sum()
+        # exponents, differences of up to 11, within 3 roundings; the exponential 2^-22; the weights' parts; the sums
+        tol = A * (2 * (11 * 3 * 2.0 ** -24 + 2.0 ** -22) + 2.0 ** -22 + (3 * length + 16) * 2.0 ** -24)
+        for got in (Q.attention_cached(dev(q), f.cache, i32([0]), i32([length])),
+                    Q.attention_shared(dev(q), f.cache, 0, length, i32([0]), i32([0])),
+                    Q.attention_shared(dev(np.tile(q, (1, 1, 20, 1))), f.cache, 0, length, i32([0]), i32([0]))):
+            g = got.cpu().numpy()[0, 0].astype(np.float64)
+            assert (np.abs(g - ref) <= tol).all(), (length, float((np.abs(g - ref) / tol).max()))
+    f.cache.close()
+
+
 # ---- verification of drafted tokens ---------------------------------------------------------------
 def drafts(rng, n_seq, n_draft, vocab, zeros=False):
     lg = rng.normal(0, 2.5, (n_seq, n_draft + 1, vocab))
