@@ -255,7 +255,8 @@ SMX_API int smx_attention_shared(const smx_kv_cache *c, const float *q_dev, int6
  * which the running sum exceeds u_draw_dev[b] times the whole.  Uniform numbers in [0, 1).  out_dev
  * [n_seq][n_draft + 1]: the accepted tokens, the drawn one (-1 if every weight is 0), then -1;
  * accepted_dev [n_seq]: how many were accepted.  A negative length marks an empty place: -1 throughout,
- * none accepted.  A NaN probability counts as 0, a token outside the vocabulary is refused. */
+ * none accepted.  A token outside the vocabulary is refused.  A NaN in a target row counts as 0.  A NaN in a draft
+ * row says nothing to accept by: its token is refused when drafted and weighs nothing in max(p_i - q_i, 0). */
 SMX_API int smx_verify_draft(const float *target_dev, int64_t target_stride, const float *draft_dev, int64_t draft_stride,
                              const int32_t *tokens_dev, const int32_t *lens_dev, const float *u_accept_dev,
                              const float *u_draw_dev, int n_seq, int n_draft, int vocab, int32_t *out_dev,

@@ -7,7 +7,7 @@
 // is drawn: from max(p_i - q_i, 0), normalised, at the draft i that was refused, or from p_n when
 // none was, so that every token is distributed as the target's.  Weights and their running sums C are
 // held in 64 bits and the product u_i q_i is exact there; the token is the lowest j of positive weight with
-// C_j > u C_last.
+// C_j > u C_last.  Where p or q is NaN, the comparison is false and the weight 0.
 //
 // One workgroup of 1024 threads per sequence.  What has to be read is one row of p and one of q; a wave
 // sums a stretch of the vocabulary, the wave in whose stretch the threshold falls is found from the 16

@@ -479,7 +479,8 @@ def verify_draft(target, draft, tokens, u_accept, u_draw, lens=None):
     None: tokens chosen without a distribution); tokens [n_seq, n_draft] int32; u_accept [n_seq, n_draft] and
     u_draw [n_seq]: uniform numbers in [0, 1); lens [n_seq] int32: drafted tokens per sequence (default:
     n_draft, negative: an empty place).  Returns (out [n_seq, n_draft + 1], accepted [n_seq]) int32: the
-    accepted tokens, one drawn token, then -1."""
+    accepted tokens, one drawn token, then -1.  A token whose draft probability is NaN is refused, and not drawn in
+    its place."""
     torch, index = _torch(), target.get_device()
     shape = target.shape
     if len(shape) != 3 or shape[1] < 1:

@@ -922,6 +922,25 @@ def test_verify_of_odd_probabilities(Q):
     check_verify(Q, p, None, x, ua, ud)
 
 
+def test_verify_where_a_row_holds_nan(Q):
+    """By what is documented, value by value: a NaN in the target's row is a 0; one in the draft's refuses its token,
+    which then weighs nothing beside max(p - q, 0) of the others, and may come again only from p alone."""
+    nan = np.nan
+    p = np.array([[[0.5, 0.25, 0.25, 0.0], [1, 0, 0, 0]]] * 6, np.float32)
+    q = np.array([[[0.25, 0.5, 0.25, 0.0]]] * 6, np.float32)
+    x, ua, ud = np.zeros((6, 1), np.int32), np.zeros((6, 1), np.float32), np.zeros(6, np.float32)
+    q[1, 0, 0] = nan                                  # the token's own: refused, though p = 0.5 > 0; nothing left: from p
+    q[2, 0], p[2, 0] = [nan, 0.1, 0.25, 0.0], [0.5, 0.25, 0.25, 0.0]     # only token 1 has a difference
+    p[3, 0, 0] = nan                                  # counts as 0: refused, drawn from the rest
+    p[3, 0, 2] = 0.5
+    x[4, 0], q[4, 0], p[4, 0] = 1, [0.25, 0.5, nan, 0.0], [0.5, 0.0, 0.5, 0.0]     # refused; 2 does not count
+    ud[4] = 0.999
+    x[5, 0], q[5, 0] = 1, [nan, 0.125, 0.25, 0.0]     # accepted: its own probabilities are numbers
+    out, acc = Q.verify_draft(dev(p), dev(q), dev(x), dev(ua), dev(ud))
+    assert acc.tolist() == [1, 0, 0, 0, 0, 1]
+    assert out.tolist() == [[0, 0], [0, -1], [1, -1], [2, -1], [0, -1], [1, 0]]
+
+
 def test_verify_rows_of_wider_matrices_and_unaligned(Q):
     rng = np.random.default_rng(6)
     p, q, x, ua, ud = drafts(rng, 3, 3, 777)
