@@ -325,6 +325,12 @@ def _on_device(index: int, *tensors):
     return _HERE if cuda.current_device() == index else cuda.device(index)
 
 
+def _c_int(n: int, what: str):
+    """Refuses what a C int would take for another number."""
+    if not -0x80000000 <= n <= 0x7FFFFFFF:
+        raise ValueError(f"{what} {n} is out of range")
+
+
 def _int32(t, n: int, what: str):
     if t.dtype is not _torch().int32 or t.numel() != n or not t.is_contiguous():
         raise ValueError(f"{what} must be a contiguous int32 tensor of {n} elements")
@@ -371,6 +377,8 @@ class GpuKvCache:
     def __init__(self, n_slots: int, n_kv_head: int, head_dim: int, ctx: int, device=None):
         self._h = ctypes.c_void_p()
         self._work = {}      # work memory of an attention call, by its sizes
+        for n, what in ((n_slots, "n_slots"), (n_kv_head, "n_kv_head"), (head_dim, "head_dim"), (ctx, "ctx")):
+            _c_int(n, what)
         torch = _torch()
         with torch.cuda.device(device if device is not None else torch.cuda.current_device()):
             self.device = torch.device("cuda", torch.cuda.current_device())
@@ -393,6 +401,7 @@ class GpuKvCache:
             raise ValueError(f"k and v must hold one row per token ({n})")
         _int32(slots, n, "slots")
         _int32(pos, n, "pos")
+        _c_int(n, "the number of tokens")
         with _on_device(index, k, v, slots, pos):
             if n:
                 call("smx_kv_append", self._handle(), k.data_ptr(), ks, v.data_ptr(), vs, slots.data_ptr(),
@@ -404,6 +413,7 @@ class GpuKvCache:
         torch, n, index = _torch(), slots.numel(), self.device.index
         _int32(slots, n, "slots")
         _int32(pos, n, "pos")
+        _c_int(n, "the number of tokens")
         with _on_device(index, slots, pos):
             k = torch.empty((n, self.n_kv_head, self.head_dim), dtype=torch.float32, device=self.device)
             v = torch.empty_like(k)
@@ -445,6 +455,10 @@ def _attention_q8(q, cache, prefix, slots, lens, max_len, name):
     stride = _rows(q, n_head, cache.head_dim, "q")
     if max_len is None:
         max_len = cache.ctx
+    _c_int(max_len, "max_len")
+    for n in prefix:
+        _c_int(n, "prefix_slot or prefix_len")
+    _c_int(n_seq * n_q * n_head, "n_seq * n_q * n_head")
     _int32(slots, n_seq, "slots")
     _int32(lens, n_seq, "lens")
     with _on_device(index, q, slots, lens):
@@ -488,6 +502,8 @@ def verify_draft(target, draft, tokens, u_accept, u_draw, lens=None):
     if index < 0:
         raise ValueError("operands must be device (cuda) tensors")
     n_seq, n_draft, vocab = shape[0], shape[1] - 1, shape[2]
+    for n, what in ((n_seq, "n_seq"), (n_draft, "n_draft"), (vocab, "vocab")):
+        _c_int(n, what)
     ts = _matrix_rows(target, vocab, "target")
     ds = 0
     if draft is not None:

@@ -79,3 +79,43 @@ def test_plain_verification_keeps_the_target_distribution():
                                     np.array([ud]), None, 3)
                     count[o[0, 0]] += 1
     assert np.allclose(count / count.sum(), p, atol=0.01)
+
+
+BIG = (1 << 32) + 1    # a C int takes it for 1
+
+
+@pytest.mark.parametrize("at", range(4))
+def test_cache_sizes_past_32_bits_are_refused(at):
+    from smallmind_amd.quantization import GpuKvCache
+    sizes = [1, 1, 64, 64]
+    sizes[at] += BIG - 1
+    with pytest.raises(ValueError, match="out of range"):
+        GpuKvCache(*sizes)
+
+
+@pytest.mark.parametrize("prefix,max_len", [((BIG, 10), 64), ((0, BIG), 64), ((0, -BIG), 64), ((0, 10), BIG), ((), BIG), ((), 1 << 31)])
+def test_lengths_past_32_bits_are_refused(prefix, max_len):
+    import types
+
+    import torch
+
+    from smallmind_amd import quantization as Q
+    cache = types.SimpleNamespace(device=torch.device("cuda", 0), head_dim=64, ctx=64, _handle=lambda: None)
+    q, i = torch.zeros(1, 1, 1, 64), torch.zeros(1, dtype=torch.int32)
+    with pytest.raises(ValueError, match="out of range"):
+        if prefix:
+            Q.attention_shared(q, cache, *prefix, i, i, max_len)
+        else:
+            Q.attention_cached(q, cache, i, i, max_len)
+
+
+def test_verify_sizes_past_32_bits_are_refused(monkeypatch):
+    import torch
+
+    from smallmind_amd import quantization as Q
+    for shape in ((1, 1, BIG), (BIG, 1, 1), (1, BIG + 1, 1)):
+        t = torch.empty(1).expand(shape)
+        monkeypatch.setattr(torch.Tensor, "get_device", lambda self: 0)
+        with pytest.raises(ValueError, match="out of range"):
+            Q.verify_draft(t, None, None, None, None)
+        monkeypatch.undo()
