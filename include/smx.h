@@ -204,7 +204,9 @@ SMX_API int smx_sample(const float *logits_dev, int n, const int32_t *context_de
  * scale = max |x| / 127 (fp32), codes = the integers nearest to x / scale, ties to even.  A row that holds a
  * NaN or an infinity reads back as NaN in every element.  head_dim: a multiple of 8 up to 256.  The
  * memory's layout is the library's own.  Calls on one cache are ordered by their streams as accesses to
- * one buffer are; the library holds no other state for them, and every call can be captured into a graph. */
+ * one buffer are; the library holds no other state for them.  Writing, reading, attention and verification can be
+ * captured into a graph; creating and destroying a cache cannot (they allocate, free and wait for the device), and a
+ * cache has to outlive the graphs that use it. */
 typedef struct smx_kv_cache smx_kv_cache;
 SMX_API int smx_kv_cache_create(int n_slots, int n_kv_head, int head_dim, int ctx, smx_kv_cache **out);
 /* Any of the pointers may be NULL; bytes: device memory of the cache. */
