@@ -830,6 +830,70 @@ def test_small_differences_of_large_scores(Q):
     f.cache.close()
 
 
+class Long(Held):
+    """Positions whose scores and values go up and down from tile to tile, so that a part lost, doubled or joined by the wrong
+    maximum moves the output by far more than sums of this length may be off."""
+
+    def __init__(self, Q, slots, n, kv, hd, seed):
+        rng = np.random.default_rng(seed)
+        tiles = -(-n // 64)
+        k, v = (rng.normal(0, 0.5, (slots, n, kv, hd)).astype(np.float32) for _ in range(2))
+        up = lambda x: np.repeat(x, 64, 1)[:, :n].astype(np.float32)  # noqa: E731
+        k[..., 0] += up(rng.normal(0, 2, (slots, tiles, kv)))
+        v += up(rng.uniform(0, 6, (slots, tiles, kv, 1)))
+        super().__init__(Q, k, v)
+
+
+@pytest.mark.parametrize("hd", [40, 64, 128, 256])
+def test_more_than_sixteen_parts(Q, hd):
+    """One long sequence alone: its positions and a prefix in dozens of parts, of which some are empty."""
+    import torch
+    n, kv, H = 8131, 2, 4
+    f = Long(Q, 3, n, kv, hd, hd)
+    rng = np.random.default_rng(hd + 1)
+    q = rng.normal(0, 0.4, (2, 2, H, hd)).astype(np.float32)
+    q[..., 0] = math.sqrt(hd) / 2
+    work = ctypes.c_int64()
+
+    def parts(n_seq, n_q, P, longest):
+        from smallmind_amd._lib import call
+        call("smx_attention_work_bytes", f.cache._h, n_seq, n_q, H, P, longest, ctypes.byref(work))
+        return work.value // (n_seq * n_q * H * (hd + 2) * 4)
+
+    assert parts(1, 2, 0, n) > 16 and parts(2, 2, 8000, 100) > 16
+    for slot, length in ((0, n), (2, 4500), (1, 65)):      # (the shorter ones: parts without positions behind them)
+        got = [Q.attention_cached(dev(q[:1]), f.cache, i32([slot]), i32([length])) for _ in range(3)]
+        assert torch.equal(got[0], got[1]) and torch.equal(got[0], got[2])
+        close_by_terms(got[0], by_terms(f, q[:1], [slot], [length]))
+    for slots, lens, P in (([0], [n], 8000), ([1], [0], n), ([0, -1], [77, 100], 8000), ([0, 1], [0, 100], 7937)):
+        b = len(slots)
+        got = [Q.attention_shared(dev(q[:b]), f.cache, 2, P, i32(slots), i32(lens), max(lens)) for _ in range(3)]
+        assert torch.equal(got[0], got[1]) and torch.equal(got[0], got[2])
+        for i in range(b):
+            if slots[i] < 0:
+                assert not got[0][i].any()
+            else:
+                close_by_terms(got[0][i:i + 1], by_terms(f, q[i:i + 1], slots[i:i + 1], lens[i:i + 1], (2, P)))
+    # 2 x 8 x 4 rows of a KV head, more than 16: the other way through the prefix, in as many parts
+    qq = np.tile(q, (1, 4, 2, 1))
+    got = Q.attention_shared(dev(qq), f.cache, 2, 8000, i32([0, 1]), i32([0, 100]), 100)
+    close_by_terms(got, by_terms(f, qq, [0, 1], [0, 100], (2, 8000)))
+    f.cache.close()
+    torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("hd,group,n_q", [(64, 5, 8), (128, 4, 33), (80, 2, 1)])
+def test_lengths_far_below_max_len(Q, hd, group, n_q):
+    """What a captured step has: max_len is the context's limit, the lengths are anything."""
+    f = Long(Q, 4, 5003, 2, hd, hd)
+    rng = np.random.default_rng(hd)
+    q = rng.normal(0, 0.5, (4, n_q, 2 * group, hd)).astype(np.float32)
+    slots, lens = np.array([3, 0, 1, 2]), np.array([900, 40, 5003, 0])
+    close_by_terms(Q.attention_cached(dev(q), f.cache, i32(slots), i32(lens)), by_terms(f, q, slots, lens))
+    close_by_terms(Q.attention_shared(dev(q), f.cache, 2, 700, i32(slots), i32(lens)), by_terms(f, q, slots, lens, (2, 700)))
+    f.cache.close()
+
+
 # ---- verification of drafted tokens ---------------------------------------------------------------
 def drafts(rng, n_seq, n_draft, vocab, zeros=False):
     lg = rng.normal(0, 2.5, (n_seq, n_draft + 1, vocab))
