@@ -231,7 +231,8 @@ SMX_API int smx_attention_work_bytes(const smx_kv_cache *c, int n_seq, int n_q, 
  * slots_dev[b], its n_q tokens (already appended) among them; token i sees all up to itself, the first
  * lens_dev[b] - n_q + 1 + i.  One token each: decode; several: drafted tokens.  n_seq and n_q
  * are at least 1.  Keys and values are up to 2^96 in size, scaled scores below 2^126 (sums in fp32 hold
- * no more).  q: token i of sequence b at q_dev + (b * n_q + i) * q_stride, [n_head][head_dim];
+ * no more).  Elements of q are held to 22 bits, or to 2^-38 of the largest of their row (one head of one token) where that is
+ * more, and so are weights times V's scales, to 2^-38 of the largest that the row sees; sums are fp32.  q: token i of sequence b at q_dev + (b * n_q + i) * q_stride, [n_head][head_dim];
  * out_dev [n_seq][n_q][n_head][head_dim]; scores are scaled by 1 / sqrt(head_dim); n_head a multiple of
  * n_kv_head.  max_len: at least every length (a
  * greater one counts as max_len); a tight bound saves workgroups.  A row that sees nothing, and the rows

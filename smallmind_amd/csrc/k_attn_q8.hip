@@ -34,9 +34,9 @@
 //           into fp16 once and keeps in LDS in the order of the matrix instructions' lanes.
 //
 // What bounds it.  64 sequences of up to 8192 positions, 8 x 128 dims: 126 us, 5.5 TB/s of codes, against the 6.4 of a
-// plain read.  16 of up to 1024, 32 x 64: 12.7 us, of which the memory takes 7.  128 sequences over 8192 shared positions,
-// 8 x 128 dims: 60 us; per 16 rows and 64 positions 260 vector instructions (softmax, splitting, the share of turning
-// codes into fp16) beside 64 matrix instructions of 16 clocks, 2320 clocks where issue alone would take 1640.
+// plain read.  16 of up to 1024, 32 x 64: 13.4 us, of which the memory takes 7.  128 sequences over 8192 shared positions,
+// 8 x 128 dims: 62 us; per 16 rows and 64 positions 280 vector instructions (softmax, splitting, the share of turning
+// codes into fp16) beside 64 matrix instructions of 16 clocks, 2280 clocks where issue alone would take about 1710.
 #include <type_traits>
 
 #include "smx_attn_q8.h"
