@@ -52,6 +52,7 @@ enum smx_type {
     SMX_TYPE_Q4_K = 12,
     SMX_TYPE_Q5_K = 13,
     SMX_TYPE_Q6_K = 14,
+    SMX_TYPE_BF16 = 30,     /* bfloat16 values: an element type of the paged cache's operators, not of weights */
     /* SmallMind's own SMQ blocks (Q8Tensor / Q4Tensor, src/SmallMind.Quantization/Tensors/Q8Tensor.cs,
      * Q4Tensor.cs): 1000 + the SMQ QuantScheme id (QuantScheme.cs: Q8_0 = 10, Q4_0 = 11).  As
      * upload bytes they are laid out in 32-element blocks, each the fp32 scale of the SMQ block
@@ -264,6 +265,121 @@ SMX_API int smx_verify_draft(const float *target_dev, int64_t target_stride, con
                              const int32_t *tokens_dev, const int32_t *lens_dev, const float *u_accept_dev,
                              const float *u_draw_dev, int n_seq, int n_draft, int vocab, int32_t *out_dev,
                              int32_t *accepted_dev, void *stream);
+
+/* ---- serving operators over a paged KV cache ------------------------------------------------------------------
+ * For hosts that keep their own forward pass and batch prompt chunks with single tokens.  The reference has no
+ * counterpart (one contiguous fp32 cache per session, TransformerModel.cs:476-506).
+ *
+ * A paged cache is a pool of n_pages pages of page_size positions (a power of two from 16 to 1024) on the current
+ * device.  Position p of a sequence lies in page table[p / page_size] at place p % page_size; tables are the host's, a page may be
+ * in several (a shared prefix).  K and V are kept as SMX_TYPE_F16 or SMX_TYPE_BF16.  head_dim: a multiple of 8
+ * up to 256.  A position whose K or V in a KV head holds a NaN or an infinity after rounding reads back as NaN in both
+ * rows of that head, and makes NaN of every output that sees it (of no other).  Positions never written are zeros.  The
+ * memory's layout is the library's own.  Calls on one cache are ordered by their streams as accesses to
+ * one buffer are; the library holds no other state for them.  All calls but create and destroy can be captured into a
+ * graph; a cache has to outlive the graphs that use it.
+ *
+ * Element types of rows: SMX_TYPE_F32, SMX_TYPE_F16, SMX_TYPE_BF16. */
+typedef struct smx_paged_cache smx_paged_cache;
+SMX_API int smx_paged_cache_create(int type, int n_pages, int n_kv_head, int head_dim, int page_size,
+                                   smx_paged_cache **out);
+/* Any of the pointers may be NULL; bytes: device memory of the cache. */
+SMX_API int smx_paged_cache_info(const smx_paged_cache *c, int *type, int *n_pages, int *n_kv_head, int *head_dim,
+                                 int *page_size, int64_t *bytes);
+SMX_API int smx_paged_cache_destroy(smx_paged_cache *c);
+/* Rotation of queries and keys by position.  Pair j of n_rot / 2 turns by the angle whose cosine and sine are at row
+ * pos, column j of the tables ([n_pos][n_rot / 2] floats, device; smx_rope_tables writes such), with pos the token's position on
+ * the pair's axis: the first sections[0] pairs turn by axis 0, the next sections[1] by axis 1, and so on (time,
+ * height, width of images and video); n_axes from 1 to 4, sections add up to n_rot / 2 (with one axis they are not read).
+ * halves 0: pair j is channels 2 j and 2 j + 1 (RotaryEmbedding.cs:85-121); 1: channels j and j + n_rot / 2.  n_rot is even and at most
+ * head_dim; channels from n_rot on are not turned.  A position that the tables do not have makes NaN of its channels. */
+typedef struct smx_rotation {
+    const float *cos_dev;
+    const float *sin_dev;
+    int32_t n_pos;
+    int32_t n_rot;
+    int32_t halves;
+    int32_t n_axes;
+    int32_t sections[4];
+} smx_rotation;
+/* Norms of queries and keys for each head and the rotation in one pass: x / sqrt(mean(x^2) + eps) * gamma over each head's
+ * head_dim values (RMSNormOps.cs:28-219 per head; not where gamma is NULL), then the rotation (not where rot is NULL), in fp32, rounded
+ * once to out_type.  Token t's rows: q_dev + t * q_stride [n_head][head_dim] and k_dev + t * k_stride [n_kv_head][head_dim], of
+ * in_type, strides in elements (both may lie in the rows of a fused projection).  gammas [head_dim] floats; pos_dev
+ * [n_axes][n_tok].  q_out_dev [n_tok][n_head][head_dim], k_out_dev [n_tok][n_kv_head][head_dim], not the inputs' memory.  q_dev or
+ * k_dev may be NULL. */
+SMX_API int smx_qk_norm_rope(int in_type, const void *q_dev, int64_t q_stride, int n_head, const void *k_dev,
+                             int64_t k_stride, int n_kv_head, int head_dim, const float *q_gamma_dev,
+                             const float *k_gamma_dev, float eps, const smx_rotation *rot, const int32_t *pos_dev, int n_tok,
+                             int out_type, void *q_out_dev, void *k_out_dev, void *stream);
+/* The same with the keys, and the values as they are, written to the cache: token t's to place places_dev[t] = page *
+ * page_size + place within the page.  A place that the cache does not have (-1, say, in a padded batch) is not
+ * written; a place named twice in one call is left with undefined contents.  q_dev may be NULL (q_out_dev then is not used). */
+SMX_API int smx_paged_append(smx_paged_cache *c, int in_type, const void *q_dev, int64_t q_stride, int n_head,
+                             const void *k_dev, int64_t k_stride, const void *v_dev, int64_t v_stride,
+                             const float *q_gamma_dev, const float *k_gamma_dev, float eps, const smx_rotation *rot,
+                             const int32_t *pos_dev, const int32_t *places_dev, int n_tok, int out_type, void *q_out_dev,
+                             void *stream);
+/* Reads rows back: k_dev, v_dev [n_tok][n_kv_head][head_dim] of the cache's type, 16-byte aligned.  Places that the cache does not
+ * have give zeros. */
+SMX_API int smx_paged_read(const smx_paged_cache *c, const int32_t *places_dev, int n_tok, void *k_dev, void *v_dev,
+                           void *stream);
+/* What a score is and who sees whom.  With s = scale * q . k (scale 0: 1 / sqrt(head_dim)) of a token at position t and a
+ * position p: cap > 0: s becomes cap * tanh(s / cap); slopes_dev ([n_head], or NULL): slopes[h] * |t - p| is taken off.  The token
+ * sees p if p is one of its sequence's first prefix_dev[b] positions ([n_seq], NULL: none; these are seen by
+ * tokens before them too), or if p <= t and, with window > 0, p > t - window. */
+typedef struct smx_attention_rules {
+    float scale;
+    float cap;
+    const float *slopes_dev;
+    const int32_t *prefix_dev;
+    int32_t window;
+    int32_t reserved;     /* must be zero */
+} smx_attention_rules;
+/* Bytes of work memory that an attention call, and a call for received weights, of these sizes needs (rules may be
+ * NULL; only window and whether there are prefixes count). */
+SMX_API int smx_attention_paged_work_bytes(const smx_paged_cache *c, int type, int n_tok, int n_head, int n_seq, int max_q,
+                                           int max_len, const smx_attention_rules *rules, int64_t *bytes);
+SMX_API int smx_attention_mass_work_bytes(const smx_paged_cache *c, int n_head, int n_seq, int max_q, int max_len,
+                                          int64_t *bytes);
+/* Attention of new tokens of n_seq sequences over the cache (MultiHeadAttention.cs:676-844 with the exponential itself in place of
+ * FastExp).  Sequence b's new tokens are rows starts_dev[b] .. starts_dev[b + 1] - 1 of the batch (starts do not
+ * decrease; at most max_q each, or what lies beyond is undefined; none: nothing to do), and the last of its lens_dev[b]
+ * positions (already appended, at most max_len; more count as max_len).  One token each: decode; several: chunks of
+ * prompts, drafted tokens; a batch may hold both.  Row b of tables_dev (table_stride pages apart, table_stride * page_size >=
+ * max_len) names the pages of its positions; a page that the cache does not have is not seen.
+ * q: token t at q_dev + t * q_stride, [n_head][head_dim] (n_head a multiple of n_kv_head); out_dev [n_tok][n_head][head_dim];
+ * lse_dev [n_tok][n_head] or NULL: the logarithm of the sum of the exponentials of the scores seen.  Rows of no sequence are left
+ * as they were; a row that sees nothing is zeros, and its lse -inf.  type: of q and out, the cache's or
+ * SMX_TYPE_F32.  With fp32, queries and weights count to 22 bits over an F16 cache (the query's elements to 2^-38 of the largest
+ * of their row, weights to 2^-31 of the largest where that is more) and to 24 over a BF16 one; with the cache's type weights are rounded to that.
+ * Sums are fp32; scores below 2^126.  rules may be NULL.  work_dev: smx_attention_paged_work_bytes bytes, 16-byte aligned,
+ * free for other use when the call's work is done; calls that may overlap, replays of captured graphs among them, need one each. */
+SMX_API int smx_attention_paged(const smx_paged_cache *c, int type, const void *q_dev, int64_t q_stride, void *out_dev,
+                                float *lse_dev, int n_tok, int n_head, int n_seq, const int32_t *starts_dev,
+                                const int32_t *lens_dev, const int32_t *tables_dev, int table_stride, int max_q, int max_len,
+                                const smx_attention_rules *rules, void *work_dev, int64_t work_bytes, void *stream);
+/* The attention weight that positions receive from the same rows: for every sequence, KV head and position
+ * mass_out[b][h][p] = mass[b][h][p] + the sum over b's new tokens and h's query heads of exp(score - lse), with lse_dev as
+ * smx_attention_paged gives it.  mass_dev: rows [n_seq * n_kv_head], mass_stride apart, of mass_width
+ * floats (what lies beyond counts as 0), or NULL; mass_out_dev [n_seq][n_kv_head][max_len], 0 from lens_dev[b] on, may be mass_dev
+ * itself where mass_stride is max_len.  Each sum's order is fixed.  work_dev: smx_attention_mass_work_bytes bytes, as above. */
+SMX_API int smx_attention_mass(const smx_paged_cache *c, int type, const void *q_dev, int64_t q_stride,
+                               const float *lse_dev, const float *mass_dev, int64_t mass_stride, int mass_width,
+                               float *mass_out_dev, int n_tok, int n_head, int n_seq, const int32_t *starts_dev,
+                               const int32_t *lens_dev, const int32_t *tables_dev, int table_stride, int max_q, int max_len,
+                               const smx_attention_rules *rules, void *work_dev, int64_t work_bytes, void *stream);
+/* Eviction: of every sequence's lens_dev[b] positions (more count as max_len) each KV head keeps n_keep, the last
+ * n_recent (at most n_keep) and those others with the most weight in mass_dev (rows [n_seq * n_kv_head] of max_len floats, mass_stride apart; the
+ * first of equals; NaN counts as less than any number), all where there are no more.  Their rows are copied in
+ * order to positions 0 .. of the pages that new_tables_dev names (new_stride * page_size >= n_keep; pages that no sequence of tables_dev reads, no
+ * page twice), kept_dev [n_seq][n_kv_head][n_keep] receives which they were (-1 beyond), new_lens_dev [n_seq] how
+ * many, new_mass_dev as kept_dev their weights (0 beyond).  The old pages are left as they are.  Positions then
+ * no longer say how far apart tokens are: a window or slopes count in what was kept. */
+SMX_API int smx_paged_evict(smx_paged_cache *c, const float *mass_dev, int64_t mass_stride, const int32_t *lens_dev,
+                            int n_seq, int max_len, int n_keep, int n_recent, const int32_t *tables_dev, int table_stride,
+                            const int32_t *new_tables_dev, int new_stride, int32_t *kept_dev, int32_t *new_lens_dev,
+                            float *new_mass_dev, void *stream);
 
 /* ---- model / session level --------------------------------------------------------------- */
 typedef struct smx_context smx_context;

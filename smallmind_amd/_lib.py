@@ -13,6 +13,7 @@ LIB_PATH = os.path.join(HERE, "libsmx.so")
 
 # GGUF tensor type ids (GgufTensorType.cs:6-52)
 F32, F16, Q4_0, Q8_0, Q4_K, Q5_K, Q6_K = 0, 1, 2, 8, 12, 13, 14
+BF16 = 30    # an element type of the paged cache's operators, not of weights
 ARCH_LLAMA, ARCH_GPT2 = 0, 1
 
 STATUS = {0: "SMX_OK", -1: "SMX_EINVAL", -2: "SMX_ENOMEM", -3: "SMX_EDEVICE", -4: "SMX_EBUSY",
@@ -37,7 +38,9 @@ EXPORTS = [
     "smx_session_generate_sampled", "smx_batcher_create", "smx_batcher_add", "smx_batcher_add_sampled", "smx_batcher_remove",
     "smx_batcher_count", "smx_batcher_step", "smx_batcher_destroy",
     "smx_kv_cache_create", "smx_kv_cache_info", "smx_kv_cache_destroy", "smx_kv_append", "smx_kv_read",
-    "smx_attention_work_bytes", "smx_attention_cached", "smx_attention_shared", "smx_verify_draft",
+    "smx_attention_work_bytes", "smx_attention_cached", "smx_attention_shared", "smx_paged_cache_create", "smx_paged_cache_info", "smx_paged_cache_destroy", "smx_qk_norm_rope", "smx_paged_append",
+    "smx_paged_read", "smx_attention_paged_work_bytes", "smx_attention_mass_work_bytes", "smx_attention_paged",
+    "smx_attention_mass", "smx_paged_evict", "smx_verify_draft",
 ]
 
 
@@ -73,6 +76,16 @@ class SamplingC(ctypes.Structure):
                 ("min_p", ctypes.c_float), ("repetition_penalty", ctypes.c_float),
                 ("presence_penalty", ctypes.c_float), ("frequency_penalty", ctypes.c_float),
                 ("repetition_window", ctypes.c_int32)]
+
+
+class RotationC(ctypes.Structure):
+    _fields_ = [("cos_dev", ctypes.c_void_p), ("sin_dev", ctypes.c_void_p), ("n_pos", ctypes.c_int32), ("n_rot", ctypes.c_int32),
+                ("halves", ctypes.c_int32), ("n_axes", ctypes.c_int32), ("sections", ctypes.c_int32 * 4)]
+
+
+class AttentionRulesC(ctypes.Structure):
+    _fields_ = [("scale", ctypes.c_float), ("cap", ctypes.c_float), ("slopes_dev", ctypes.c_void_p), ("prefix_dev", ctypes.c_void_p),
+                ("window", ctypes.c_int32), ("reserved", ctypes.c_int32)]
 
 
 class GenStatsC(ctypes.Structure):
@@ -140,6 +153,18 @@ def load() -> ctypes.CDLL:
         "smx_attention_cached": (i32, [vp, vp, i64, vp, i32, i32, i32, vp, vp, i32, vp, i64, vp]),
         "smx_attention_shared": (i32, [vp, vp, i64, vp, i32, i32, i32, i32, i32, vp, vp, i32, vp, i64, vp]),
         "smx_verify_draft": (i32, [vp, i64, vp, i64, vp, vp, vp, vp, i32, i32, i32, vp, vp, vp]),
+        "smx_paged_cache_create": (i32, [i32, i32, i32, i32, i32, pp]),
+        "smx_paged_cache_info": (i32, [vp, vp, vp, vp, vp, vp, vp]),
+        "smx_paged_cache_destroy": (i32, [vp]),
+        "smx_qk_norm_rope": (i32, [i32, vp, i64, i32, vp, i64, i32, i32, vp, vp, f32, vp, vp, i32, i32, vp, vp, vp]),
+        "smx_paged_append": (i32, [vp, i32, vp, i64, i32, vp, i64, vp, i64, vp, vp, f32, vp, vp, vp, i32, i32, vp, vp]),
+        "smx_paged_read": (i32, [vp, vp, i32, vp, vp, vp]),
+        "smx_attention_paged_work_bytes": (i32, [vp, i32, i32, i32, i32, i32, i32, vp, ctypes.POINTER(i64)]),
+        "smx_attention_mass_work_bytes": (i32, [vp, i32, i32, i32, i32, ctypes.POINTER(i64)]),
+        "smx_attention_paged": (i32, [vp, i32, vp, i64, vp, vp, i32, i32, i32, vp, vp, vp, i32, i32, i32, vp, vp, i64, vp]),
+        "smx_attention_mass": (i32, [vp, i32, vp, i64, vp, vp, i64, i32, vp, i32, i32, i32, vp, vp, vp, i32, i32, i32, vp, vp,
+                                     i64, vp]),
+        "smx_paged_evict": (i32, [vp, vp, i64, vp, i32, i32, i32, i32, vp, i32, vp, i32, vp, vp, vp, vp]),
         "smx_context_create": (i32, [i32, pp]),
         "smx_context_destroy": (i32, [vp]),
         "smx_model_create": (i32, [vp, ctypes.POINTER(ModelConfigC), pp]),

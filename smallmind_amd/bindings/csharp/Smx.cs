@@ -24,6 +24,7 @@ namespace SmallMind.Backends.Rocm
         public const int OK = 0, EINVAL = -1, ENOMEM = -2, EDEVICE = -3, EBUSY = -4,
                          EUNSUPPORTED = -5, ESTATE = -6, ERANGE = -7, ECANCELED = -8, ETIMEDOUT = -9;
         public const int F32 = 0, F16 = 1, Q4_0 = 2, Q8_0 = 8, Q4_K = 12, Q5_K = 13, Q6_K = 14;
+        public const int BF16 = 30;   // an element type of the paged cache's operators, not of weights
         // SMQ Q8Tensor / Q4Tensor blocks in their upload layout (smx_smq_pack)
         public const int SMQ_Q8 = 1010, SMQ_Q4 = 1011;
 
@@ -37,6 +38,23 @@ namespace SmallMind.Backends.Rocm
 
         [StructLayout(LayoutKind.Sequential)]
         public struct GenStats { public double PrefillMs, DecodeMs; public int NPrefill, NDecode; }
+
+        [StructLayout(LayoutKind.Sequential)]
+        public struct Rotation           // smx_rotation
+        {
+            public void* CosDev, SinDev;
+            public int NPos, NRot, Halves, NAxes;
+            public fixed int Sections[4];
+        }
+
+        [StructLayout(LayoutKind.Sequential)]
+        public struct AttentionRules     // smx_attention_rules
+        {
+            public float Scale, Cap;     // 0: 1 / sqrt(head_dim), not capped
+            public float* SlopesDev;
+            public int* PrefixDev;
+            public int Window, Reserved;
+        }
 
         [StructLayout(LayoutKind.Sequential)]
         public struct Sampling               // smx_sampling; ProductionInferenceOptions.cs:19-87
@@ -109,6 +127,34 @@ namespace SmallMind.Backends.Rocm
         [DllImport(Lib)] public static extern int smx_attention_shared(IntPtr cache, float* qDev, long qStride,
             float* outDev, int nSeq, int nQ, int nHead, int prefixSlot, int prefixLen, int* slotsDev, int* lensDev,
             int maxLen, void* workDev, long workBytes, IntPtr stream);
+        [DllImport(Lib)] public static extern int smx_paged_cache_create(int type, int nPages, int nKvHead, int headDim,
+            int pageSize, out IntPtr cache);
+        [DllImport(Lib)] public static extern int smx_paged_cache_info(IntPtr cache, int* type, int* nPages, int* nKvHead,
+            int* headDim, int* pageSize, long* bytes);
+        [DllImport(Lib)] public static extern int smx_paged_cache_destroy(IntPtr cache);
+        // rot: a Rotation, rules: an AttentionRules (their addresses, or zero)
+        [DllImport(Lib)] public static extern int smx_qk_norm_rope(int inType, void* qDev, long qStride, int nHead, void* kDev,
+            long kStride, int nKvHead, int headDim, float* qGammaDev, float* kGammaDev, float eps, IntPtr rot, int* posDev,
+            int nTok, int outType, void* qOutDev, void* kOutDev, IntPtr stream);
+        [DllImport(Lib)] public static extern int smx_paged_append(IntPtr cache, int inType, void* qDev, long qStride, int nHead,
+            void* kDev, long kStride, void* vDev, long vStride, float* qGammaDev, float* kGammaDev, float eps, IntPtr rot,
+            int* posDev, int* placesDev, int nTok, int outType, void* qOutDev, IntPtr stream);
+        [DllImport(Lib)] public static extern int smx_paged_read(IntPtr cache, int* placesDev, int nTok, void* kDev, void* vDev,
+            IntPtr stream);
+        [DllImport(Lib)] public static extern int smx_attention_paged_work_bytes(IntPtr cache, int type, int nTok, int nHead,
+            int nSeq, int maxQ, int maxLen, IntPtr rules, out long bytes);
+        [DllImport(Lib)] public static extern int smx_attention_mass_work_bytes(IntPtr cache, int nHead, int nSeq, int maxQ,
+            int maxLen, out long bytes);
+        [DllImport(Lib)] public static extern int smx_attention_paged(IntPtr cache, int type, void* qDev, long qStride,
+            void* outDev, float* lseDev, int nTok, int nHead, int nSeq, int* startsDev, int* lensDev, int* tablesDev,
+            int tableStride, int maxQ, int maxLen, IntPtr rules, void* workDev, long workBytes, IntPtr stream);
+        [DllImport(Lib)] public static extern int smx_attention_mass(IntPtr cache, int type, void* qDev, long qStride,
+            float* lseDev, float* massDev, long massStride, int massWidth, float* massOutDev, int nTok, int nHead, int nSeq,
+            int* startsDev, int* lensDev, int* tablesDev, int tableStride, int maxQ, int maxLen, IntPtr rules, void* workDev,
+            long workBytes, IntPtr stream);
+        [DllImport(Lib)] public static extern int smx_paged_evict(IntPtr cache, float* massDev, long massStride, int* lensDev,
+            int nSeq, int maxLen, int nKeep, int nRecent, int* tablesDev, int tableStride, int* newTablesDev, int newStride,
+            int* keptDev, int* newLensDev, float* newMassDev, IntPtr stream);
         [DllImport(Lib)] public static extern int smx_verify_draft(float* targetDev, long targetStride, float* draftDev,
             long draftStride, int* tokensDev, int* lensDev, float* uAcceptDev, float* uDrawDev, int nSeq, int nDraft,
             int vocab, int* outDev, int* acceptedDev, IntPtr stream);

@@ -1,0 +1,191 @@
+// k_attn_paged_join.hip -- how the attention over the paged KV cache and the sum of received weights are cut up, their
+// dispatch by row width and element type, and the sums of their parts.
+#include <math.h>
+
+#include <algorithm>
+
+#include "smx_attn_paged.h"
+#include "smx_device.h"
+#include "smx_internal.h"
+
+namespace smx {
+
+namespace {
+
+// out = sum_s 2^(e_s - E) acc_s / sum_s 2^(e_s - E) l_s over the parts s that have weight, E their largest exponent e.
+struct Joined {
+    float4 o;
+    float l, top;
+};
+
+__device__ __forceinline__ void join(Joined &a, float4 v, float l, float e)
+{
+    if (e == -__builtin_huge_valf()) return;   // a part without weight may hold anything in v
+    const float up = fmaxf(a.top, e);
+    const float f = __builtin_amdgcn_exp2f(e - up), g = a.top == -__builtin_huge_valf() ? 0.0f : __builtin_amdgcn_exp2f(a.top - up);
+    a.top = up;
+    a.l = a.l * g + l * f;
+    a.o.x = a.o.x * g + v.x * f, a.o.y = a.o.y * g + v.y * f;
+    a.o.z = a.o.z * g + v.z * f, a.o.w = a.o.w * g + v.w * f;
+}
+
+// What bounds it is the latency of the parts' loads: a thread takes four dims of every PP-th part of a row, requested
+// four at a time, and PP threads join theirs through LDS in a fixed order.  Rows outside the sequences stay as they are.
+template <int PP>
+__global__ __launch_bounds__(256) void k_attn_paged_join(const AttnPgArgs a)
+{
+    constexpr int R = 256 / PP;   // threads of a block that each have other outputs
+    __shared__ Joined S[PP > 1 ? PP - 1 : 1][PP > 1 ? R : 1];
+    const int lane = threadIdx.x % R, pp = threadIdx.x / R;
+    const int64_t i = (int64_t)blockIdx.x * R + lane, n_rows = (int64_t)a.n_tok * a.n_head;
+    const int per = a.c.hd / 4;
+    bool in = i < n_rows * per;
+    const int64_t row = in ? i / per : 0;
+    const int d = in ? 4 * (int)(i - row * per) : 0, token = (int)(row / a.n_head);
+    in = in && token >= ld_uniform(a.starts) && token < ld_uniform(a.starts + a.n_seq);
+    Joined J{make_float4(0.0f, 0.0f, 0.0f, 0.0f), 0.0f, -__builtin_huge_valf()};
+    for (int s0 = pp; s0 < a.parts; s0 += 4 * PP) {
+        float2 ml[4];
+        float4 v[4];
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const int s = min(s0 + k * PP, a.parts - 1);
+            ml[k] = *(const float2 *)(a.part_ml + (s * n_rows + row) * 2);
+            v[k] = *(const float4 *)(a.part_acc + (s * n_rows + row) * a.c.hd + d);
+        }
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+            if (s0 + k * PP < a.parts) join(J, v[k], ml[k].y, ml[k].x);
+    }
+    if constexpr (PP > 1) {
+        if (pp > 0) S[pp - 1][lane] = J;
+        __syncthreads();
+        if (pp > 0) return;
+#pragma unroll
+        for (int k = 0; k < PP - 1; k++) {
+            const Joined &T = S[k][lane];
+            join(J, T.o, T.l, T.top);
+        }
+    }
+    if (!in) return;
+    const bool none = J.top == -__builtin_huge_valf();
+    const float inv = none ? 0.0f : 1.0f / J.l;
+    if (a.lse && d == 0) a.lse[row] = none ? J.top : (__builtin_amdgcn_logf(J.l) + J.top) * 0.69314718055994531f;
+    const float o[4] = {J.o.x * inv, J.o.y * inv, J.o.z * inv, J.o.w * inv};
+    const int64_t at = row * a.c.hd + d;
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        if (a.io == PG_F32) ((float *)a.out)[at + e] = o[e];
+        else if (a.io == PG_F16) ((_Float16 *)a.out)[at + e] = (_Float16)o[e];
+        else ((__bf16 *)a.out)[at + e] = (__bf16)o[e];
+    }
+}
+
+// The parts of received weights, and what there was before.
+__global__ __launch_bounds__(256) void k_attn_mass_join(const AttnPgArgs a)
+{
+    const int64_t n = (int64_t)a.n_seq * a.c.n_kv * a.max_len, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= n) return;
+    const int64_t pair = i / a.max_len;
+    const int p = (int)(i - pair * a.max_len);
+    float sum = 0.0f;
+    for (int k = 0; k < a.mass_parts; k++) sum += a.mass_part[k * n + i];
+    const float was = a.mass && p < a.mass_width ? a.mass[pair * a.mass_stride + p] : 0.0f;
+    a.mass_out[i] = p < a.lens[pair / a.c.n_kv] ? was + sum : 0.0f;
+}
+
+}  // namespace
+
+#define SMX_ALL(X) X(32, 0) X(64, 0) X(96, 0) X(128, 0) X(192, 0) X(256, 0) X(32, 1) X(64, 1) X(96, 1) X(128, 1) X(192, 1) X(256, 1)
+#define SMX_DECL(w, b)                                                                                      \
+    hipError_t launch_attn_paged_w##w##_b##b(const AttnPgArgs &a, const AttnPgPlan &p, hipStream_t s);      \
+    hipError_t launch_attn_mass_w##w##_b##b(const AttnPgArgs &a, const MassPgPlan &p, hipStream_t s);       \
+    int attn_paged_waves_w##w##_b##b(int io);
+SMX_ALL(SMX_DECL)
+#undef SMX_DECL
+
+AttnPgPlan attn_paged_plan(const PgView &c, int io, int n_tok, int n_head, int n_seq, int max_q, int max_len, int window, bool prefix)
+{
+    AttnPgPlan p{};
+    const int64_t group = n_head / c.n_kv, rows = max_q * group;
+    const int64_t tiles = std::max(1, (max_len + kPgTile - 1) / kPgTile);
+    int waves = 4;
+#define SMX_CASE(w_, b) if (c.w == w_ && c.bf16 == b) waves = attn_paged_waves_w##w_##_b##b(io);
+    SMX_ALL(SMX_CASE)
+#undef SMX_CASE
+    p.kind = rows <= kPgRows ? 0 : waves == 8 && rows > 128 ? 2 : 1;
+    const int block = p.kind == 2 ? 256 : 128;
+    // what a block goes through at most, where the window says so, and how many blocks that is done by
+    const int64_t span = window > 0 ? std::min<int64_t>(tiles, (window + (p.kind ? block / group + 1 : (int64_t)max_q)) / kPgTile + 2) : tiles;
+    int64_t units = (int64_t)n_seq * c.n_kv;
+    if (p.kind) {
+        p.tile_blocks = (int)(n_tok * group / block + n_seq);
+        units = std::max<int64_t>(1, (n_tok * group + block - 1) / block) * c.n_kv;
+    }
+    int64_t n = 1;
+    if (p.kind == 0) {
+        n = std::min((512 + units - 1) / units, (span + 3) / 4);
+        if (n * units < 128) n = std::max(n, std::min((128 + units - 1) / units, (span + 1) / 2));
+    } else if (units < 256) {
+        n = std::min((256 + units - 1) / units, (span + 7) / 8);
+    }
+    n = std::max<int64_t>(n, 1);
+    p.chunk = (int)((span + n - 1) / n);
+    const int64_t all = window > 0 && !prefix ? span : tiles;
+    p.parts = n == 1 ? 1 : (int)((all + p.chunk - 1) / p.chunk);
+    p.tile_wgs = p.kind ? (int64_t)p.tile_blocks * c.n_kv * p.parts : 0;
+    // short sequences of a batch with longer ones go their own way
+    p.blocks = p.tile_wgs + (p.kind == 0 || n_seq > 1 ? (int64_t)n_seq * c.n_kv * p.parts : 0);
+    p.work_bytes = p.parts > 1 ? (int64_t)p.parts * n_tok * n_head * (c.hd + 2) * 4 : 0;
+    return p;
+}
+
+hipError_t launch_attn_paged(AttnPgArgs a, const AttnPgPlan &p, void *work, hipStream_t s)
+{
+    a.tile_wgs = (int)p.tile_wgs;
+    a.tile_blocks = p.tile_blocks;
+    a.short_rows = p.kind && a.n_seq > 1 ? kPgRows : 0;
+    a.chunk = p.chunk;
+    a.parts = p.parts;
+    const int64_t rows = (int64_t)a.n_tok * a.n_head;
+    a.part_acc = (float *)work;
+    a.part_ml = work ? (float *)work + p.parts * rows * a.c.hd : nullptr;
+    hipError_t e = hipErrorInvalidValue;
+#define SMX_CASE(w_, b) if (a.c.w == w_ && a.c.bf16 == b) e = launch_attn_paged_w##w_##_b##b(a, p, s);
+    SMX_ALL(SMX_CASE)
+#undef SMX_CASE
+    if (e != hipSuccess || p.parts == 1) return e;
+    // about four parts per thread
+    const int64_t n = rows * (a.c.hd / 4);
+    if (p.parts <= 4) k_attn_paged_join<1><<<(unsigned)((n + 255) / 256), 256, 0, s>>>(a);
+    else if (p.parts <= 16) k_attn_paged_join<4><<<(unsigned)((n + 63) / 64), 256, 0, s>>>(a);
+    else k_attn_paged_join<16><<<(unsigned)((n + 15) / 16), 256, 0, s>>>(a);
+    return hipGetLastError();
+}
+
+MassPgPlan attn_mass_plan(const PgView &c, int n_head, int n_seq, int max_q, int max_len)
+{
+    MassPgPlan p{};
+    const int64_t rows = (int64_t)max_q * (n_head / c.n_kv);
+    const int64_t units = (int64_t)n_seq * c.n_kv * ((max_len + 127) / 128);
+    p.parts = (int)std::max<int64_t>(1, std::min((1024 + units - 1) / units, rows / 512));
+    p.blocks = units * p.parts;
+    p.work_bytes = p.parts > 1 ? (int64_t)p.parts * n_seq * c.n_kv * max_len * 4 : 0;
+    return p;
+}
+
+hipError_t launch_attn_mass(AttnPgArgs a, const MassPgPlan &p, void *work, hipStream_t s)
+{
+    a.mass_parts = p.parts;
+    a.mass_part = (float *)work;
+    hipError_t e = hipErrorInvalidValue;
+#define SMX_CASE(w_, b) if (a.c.w == w_ && a.c.bf16 == b) e = launch_attn_mass_w##w_##_b##b(a, p, s);
+    SMX_ALL(SMX_CASE)
+#undef SMX_CASE
+    if (e != hipSuccess || p.parts == 1) return e;
+    const int64_t n = (int64_t)a.n_seq * a.c.n_kv * a.max_len;
+    k_attn_mass_join<<<(unsigned)((n + 255) / 256), 256, 0, s>>>(a);
+    return hipGetLastError();
+}
+
+}  // namespace smx

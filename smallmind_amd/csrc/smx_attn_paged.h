@@ -1,0 +1,60 @@
+// smx_attn_paged.h -- arguments of the attention over the paged KV cache and of the weights that positions receive.
+// The kernels are built once per row width and element type (k_attn_paged.hip); the plan, the dispatch and the joining
+// of parts are in k_attn_paged_join.hip.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "smx_paged.h"
+
+namespace smx {
+
+constexpr int kPgTile = 64;      // positions that are gone through at once
+constexpr int kPgRows = 32;      // rows (a query head of a token) of a wave
+
+struct AttnPgArgs {
+    PgView c;
+    const void *q;               // token t, head h at t * q_stride + h * hd (elements)
+    void *out;                   // [n_tok][n_head][hd]
+    float *lse;                  // [n_tok][n_head] or null
+    const int32_t *starts;       // [n_seq + 1]
+    const int32_t *lens;         // [n_seq]
+    const int32_t *tables;       // [n_seq][table_stride]
+    const float *slopes;         // [n_head] or null
+    const int32_t *prefix;       // [n_seq] or null
+    float *part_ml, *part_acc;   // [parts][n_tok * n_head][2], [..][hd]
+    // weights received: mass [n_seq * n_kv] rows of mass_width floats, mass_stride apart (or null), mass_out rows of max_len;
+    // lse_in [n_tok][n_head]; with mass_parts > 1 part p goes to mass_part + p * n_seq * n_kv * max_len
+    const float *mass, *lse_in;
+    float *mass_out, *mass_part;
+    int64_t mass_stride;
+    int mass_width, mass_parts;
+    int64_t q_stride;
+    double inv_group;            // n_kv / n_head
+    float scale_log2e;           // of plain scores, as exponents of 2
+    float cap_in, cap_out;       // scores * cap_in -> tanh -> * cap_out is an exponent of 2; cap_in 0: not capped
+    int window;                  // 0: none
+    int q_vec, out_vec;          // q, out may be read and written 16 bytes at a time
+    int page_shift, table_stride;
+    int n_tok, n_head, group, n_seq, max_q, max_len;
+    int io;                      // PgType of q and out
+    int tile_wgs, tile_blocks;   // workgroups (blocks of rows) of the many-row path; the rest take short sequences
+    int short_rows;              // sequences of up to this many rows go the short way (0: none do)
+    int chunk, parts;            // tiles of a part; parts (1: the outputs are written at once)
+};
+
+// How a call is cut up.
+struct AttnPgPlan {
+    int kind;                    // 0: every sequence is short; 1: blocks of 128 rows; 2: blocks of 256
+    int chunk, parts, tile_blocks;
+    int64_t tile_wgs, blocks;
+    int64_t work_bytes;
+};
+
+struct MassPgPlan {
+    int parts;
+    int64_t blocks, work_bytes;
+};
+
+}  // namespace smx

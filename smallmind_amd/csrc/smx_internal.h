@@ -9,6 +9,7 @@
 #include <string>
 
 #include "../../include/smx.h"
+#include "smx_attn_paged.h"
 #include "smx_attn_q8.h"
 #include "smx_kvcache.h"
 
@@ -368,6 +369,18 @@ hipError_t launch_attn_q8(const KvView &c, const AttnQ8Plan &plan, const float *
 hipError_t launch_verify(const float *p, int64_t p_stride, const float *q, int64_t q_stride, const int32_t *draft,
                          const int32_t *lens, const float *u_accept, const float *u_draw, int n_seq, int n_draft,
                          int vocab, int32_t *tokens, int32_t *accepted, hipStream_t s);
+
+// ---- paged KV cache (smx_paged.h), attention over it, received weights, eviction ---------------
+hipError_t launch_paged_write(PgWriteArgs a, int in_type, hipStream_t s);
+// k, v: [n_tok][n_kv][hd] of the cache's type
+hipError_t launch_paged_read(const PgView &c, const int32_t *places, int n_tok, void *k, void *v, hipStream_t s);
+// How a call is cut up (the same for every content of device memory), and the call with work of plan.work_bytes bytes.
+AttnPgPlan attn_paged_plan(const PgView &c, int io, int n_tok, int n_head, int n_seq, int max_q, int max_len, int window,
+                           bool prefix);
+hipError_t launch_attn_paged(AttnPgArgs a, const AttnPgPlan &p, void *work, hipStream_t s);
+MassPgPlan attn_mass_plan(const PgView &c, int n_head, int n_seq, int max_q, int max_len);
+hipError_t launch_attn_mass(AttnPgArgs a, const MassPgPlan &p, void *work, hipStream_t s);
+hipError_t launch_paged_evict(const PgEvictArgs &a, int n_seq, hipStream_t s);
 
 // ---- errors and block geometry (host_common.cpp) ------------------------------------------
 void set_error(const std::string &msg);

@@ -525,7 +525,341 @@ def verify_draft(target, draft, tokens, u_accept, u_draw, lens=None):
     return out, accepted
 
 
+# ---- serving operators over a paged KV cache ------------------------------------------------------
+_ELEM = None
+
+
+def _elem_type(dtype, what: str) -> int:
+    """The smx_type of rows of this torch type."""
+    global _ELEM
+    if _ELEM is None:
+        torch = _torch()
+        _ELEM = {torch.float32: _lib.F32, torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
+    t = _ELEM.get(dtype)
+    if t is None:
+        raise ValueError(f"{what} must be float32, float16 or bfloat16, is {dtype}")
+    return t
+
+
+def _token_rows(t, n_head, head_dim: int, what: str) -> int:
+    """The distance between the [heads][head_dim] rows of t [n_tok, heads, head_dim], which may lie in the rows of a wider
+    matrix (a fused projection)."""
+    shape = t.shape
+    if len(shape) != 3 or shape[2] != head_dim or (n_head is not None and shape[1] != n_head):
+        raise ValueError(f"{what} must be [n_tok, {n_head or 'heads'}, {head_dim}], is {tuple(shape)}")
+    row = shape[1] * head_dim
+    if t.is_contiguous() or t.numel() == 0:
+        return row
+    s = t.stride()
+    step = s[0] if shape[0] > 1 else row
+    if (s[2] != 1 and head_dim > 1) or (s[1] != head_dim and shape[1] > 1) or step < row:
+        raise ValueError(f"{what}: tokens must be rows of contiguous heads")
+    return step
+
+
+def _floats(t, n: int, what: str):
+    if t.dtype is not _torch().float32 or t.numel() != n or not t.is_contiguous():
+        raise ValueError(f"{what} must be a contiguous float32 tensor of {n} elements")
+
+
+def _opt(t):
+    return None if t is None else t.data_ptr()
+
+
+class Rotation:
+    """The rotation of queries and keys by position (smx_rotation).  cos and sin [n_pos, n_rot / 2] float32 on the device
+    (rope_tables gives such); sections: how many pairs turn by each axis, in order (default: all by one); halves: pair j
+    is channels j and j + n_rot / 2, otherwise 2 j and 2 j + 1."""
+
+    def __init__(self, cos, sin, sections=None, halves: bool = False):
+        if cos.dim() != 2 or cos.shape != sin.shape or cos.shape[0] < 1 or cos.shape[1] < 1:
+            raise ValueError("cos and sin must be [n_pos, n_rot / 2]")
+        n_pos, half = cos.shape
+        _c_int(n_pos, "n_pos")
+        _c_int(2 * half, "n_rot")
+        _floats(cos, n_pos * half, "cos")
+        _floats(sin, n_pos * half, "sin")
+        sections = [half] if sections is None else [int(n) for n in sections]
+        if not 1 <= len(sections) <= 4 or min(sections) < 0 or sum(sections) != half:
+            raise ValueError(f"sections must be 1 to 4 numbers that add up to {half}, are {sections}")
+        self.cos, self.sin, self.n_axes = cos, sin, len(sections)
+        self._c = _lib.RotationC(cos.data_ptr(), sin.data_ptr(), n_pos, 2 * half, int(bool(halves)), len(sections),
+                                 (ctypes.c_int32 * 4)(*sections))
+
+
+def _turning(rotation, pos, n: int):
+    """(tables and positions to check, what the call takes for them)."""
+    if rotation is None:
+        return (), None, None
+    if pos is None:
+        raise ValueError("the rotation needs positions")
+    _int32(pos, n * rotation.n_axes, "pos")
+    return (rotation.cos, rotation.sin, pos), ctypes.byref(rotation._c), pos.data_ptr()
+
+
+def _eps(eps: float) -> float:
+    if not 0.0 <= eps < float("inf"):
+        raise ValueError(f"eps {eps} must be finite and not negative")
+    return eps
+
+
+def qk_norm_rope(q, k, q_gamma=None, k_gamma=None, eps: float = 1e-6, rotation: Rotation | None = None, pos=None, dtype=None):
+    """Norms of queries and keys for each head and the rotation by position in one pass (smx_qk_norm_rope).  q [n_tok, n_head,
+    head_dim] and k [n_tok, n_kv_head, head_dim] float32, float16 or bfloat16 (tokens may be rows of a fused projection);
+    gammas [head_dim] float32 (None: no norm); pos [n_tok], or [n_axes, n_tok], int32.  Returns (q, k) of `dtype` (default:
+    as they come), rounded once."""
+    torch, index = _torch(), q.get_device()
+    if index < 0:
+        raise ValueError("operands must be device (cuda) tensors")
+    if q.dim() != 3 or k.dtype is not q.dtype or k.dim() != 3 or q.shape[0] != k.shape[0]:
+        raise ValueError("q and k must be [n_tok, heads, head_dim] of one type")
+    n, n_head, hd = q.shape
+    qs, ks = _token_rows(q, n_head, hd, "q"), _token_rows(k, None, hd, "k")
+    dtype = q.dtype if dtype is None else dtype
+    tin, tout = _elem_type(q.dtype, "q"), _elem_type(dtype, "dtype")
+    for g, what in ((q_gamma, "q_gamma"), (k_gamma, "k_gamma")):
+        if g is not None:
+            _floats(g, hd, what)
+    for x, what in ((n, "n_tok"), (n_head, "n_head"), (k.shape[1], "n_kv_head"), (hd, "head_dim")):
+        _c_int(x, what)
+    turn, rot, at = _turning(rotation, pos, n)
+    with _on_device(index, k, q_gamma, k_gamma, *turn):
+        qo = torch.empty(q.shape, dtype=dtype, device=q.device)
+        ko = torch.empty(k.shape, dtype=dtype, device=q.device)
+        if n and n_head + k.shape[1]:
+            call("smx_qk_norm_rope", tin, q.data_ptr(), qs, n_head, k.data_ptr(), ks, k.shape[1], hd, _opt(q_gamma), _opt(k_gamma),
+                 _eps(eps), rot, at, n, tout, qo.data_ptr(), ko.data_ptr(), _raw_stream(index))
+    return qo, ko
+
+
+class GpuPagedCache:
+    """A KV cache in pages of page_size positions (a power of two from 16 to 1024), float16 or bfloat16 (smx_paged_cache_*).  Position
+    p of a sequence lies in page table[p // page_size], at place page * page_size + p % page_size of the cache; tables are
+    the caller's.  head_dim: a multiple of 8 up to 256.  Lives on `device` (default: the current one)."""
+
+    def __init__(self, dtype, n_pages: int, n_kv_head: int, head_dim: int, page_size: int = 64, device=None):
+        self._h = ctypes.c_void_p()
+        self._work = {}      # work memory of a call, by its sizes
+        torch = _torch()
+        if dtype not in (torch.float16, torch.bfloat16):
+            raise ValueError(f"a paged cache is float16 or bfloat16, not {dtype}")
+        for n, what in ((n_pages, "n_pages"), (n_kv_head, "n_kv_head"), (head_dim, "head_dim"), (page_size, "page_size")):
+            _c_int(n, what)
+        with torch.cuda.device(device if device is not None else torch.cuda.current_device()):
+            self.device = torch.device("cuda", torch.cuda.current_device())
+            call("smx_paged_cache_create", _elem_type(dtype, "dtype"), n_pages, n_kv_head, head_dim, page_size, ctypes.byref(self._h))
+        self.dtype, self.n_pages, self.n_kv_head, self.head_dim, self.page_size = dtype, n_pages, n_kv_head, head_dim, page_size
+
+    @property
+    def nbytes(self) -> int:
+        b = ctypes.c_int64()
+        call("smx_paged_cache_info", self._handle(), None, None, None, None, None, ctypes.byref(b))
+        return b.value
+
+    def append(self, k, v, places, q=None, q_gamma=None, k_gamma=None, eps: float = 1e-6, rotation: Rotation | None = None, pos=None,
+               dtype=None):
+        """Writes token t's rows k[t], v[t] ([n_tok, n_kv_head, head_dim] float32, float16 or bfloat16, possibly slices of a fused
+        projection) to place places[t] (int32; -1, or any that the cache does not have: skipped; one named twice is left
+        with undefined contents).  With k_gamma or a rotation the keys are normed and turned as they are by qk_norm_rope; with q
+        ([n_tok, n_head, head_dim] of k's type) so are the queries, and they are returned, of `dtype` (default: as they
+        come)."""
+        torch, n, kv, hd, index = _torch(), places.numel(), self.n_kv_head, self.head_dim, self.device.index
+        ks, vs = _token_rows(k, kv, hd, "k"), _token_rows(v, kv, hd, "v")
+        if k.shape[0] != n or v.shape[0] != n or v.dtype is not k.dtype:
+            raise ValueError(f"k and v must hold one row per token ({n}), of one type")
+        tin = tout = _elem_type(k.dtype, "k")
+        _int32(places, n, "places")
+        _c_int(n, "the number of tokens")
+        n_head = qs = 0
+        if q is not None:
+            if q.dtype is not k.dtype or q.dim() != 3 or q.shape[0] != n or q.shape[1] < 1:
+                raise ValueError(f"q must be [{n}, n_head, {hd}] of k's type")
+            n_head, qs = q.shape[1], _token_rows(q, q.shape[1], hd, "q")
+            _c_int(n_head, "n_head")
+            dtype = q.dtype if dtype is None else dtype
+            tout = _elem_type(dtype, "dtype")
+        for g, what in ((q_gamma, "q_gamma"), (k_gamma, "k_gamma")):
+            if g is not None:
+                _floats(g, hd, what)
+        turn, rot, at = _turning(rotation, pos, n)
+        with _on_device(index, k, v, places, q, q_gamma, k_gamma, *turn):
+            out = None if q is None else torch.empty(q.shape, dtype=dtype, device=self.device)
+            if n:
+                call("smx_paged_append", self._handle(), tin, _opt(q), qs, n_head, k.data_ptr(), ks, v.data_ptr(), vs, _opt(q_gamma),
+                     _opt(k_gamma), _eps(eps), rot, at, places.data_ptr(), n, tout, _opt(out), _raw_stream(index))
+        return out
+
+    def read(self, places):
+        """(k, v), each [n_tok, n_kv_head, head_dim] of the cache's type: the rows at these places (zeros at places it does not
+        have)."""
+        torch, n, index = _torch(), places.numel(), self.device.index
+        _int32(places, n, "places")
+        _c_int(n, "the number of tokens")
+        with _on_device(index, places):
+            k = torch.empty((n, self.n_kv_head, self.head_dim), dtype=self.dtype, device=self.device)
+            v = torch.empty_like(k)
+            if n:
+                call("smx_paged_read", self._handle(), places.data_ptr(), n, k.data_ptr(), v.data_ptr(), _raw_stream(index))
+        return k, v
+
+    def evict(self, mass, lens, n_keep: int, n_recent: int, tables, new_tables):
+        """Keeps n_keep positions of every sequence and KV head: the last n_recent and those others with the most weight in
+        mass [n_seq, n_kv_head, max_len] float32 (the first of equals); all where there are no more.  lens [n_seq], tables
+        [n_seq, pages] and new_tables [n_seq, pages] int32: the kept rows are copied in order to positions 0 .. of the new
+        pages, which must be others than any sequence's old ones (smx_paged_evict).  Returns (kept [n_seq, n_kv_head, n_keep]
+        int32, -1 beyond; new lens [n_seq] int32; their weights [n_seq, n_kv_head, n_keep] float32)."""
+        torch, index = _torch(), self.device.index
+        if mass.dim() != 3 or mass.shape[1] != self.n_kv_head or mass.shape[0] < 1:
+            raise ValueError(f"mass must be [n_seq, {self.n_kv_head}, max_len]")
+        n_seq, kv, max_len = mass.shape
+        stride = _mass_rows(mass)
+        _int32(lens, n_seq, "lens")
+        for n, what in ((n_seq, "n_seq"), (max_len, "max_len"), (n_keep, "n_keep"), (n_recent, "n_recent")):
+            _c_int(n, what)
+        for t, what in ((tables, "tables"), (new_tables, "new_tables")):
+            _table(t, n_seq, what)
+        with _on_device(index, mass, lens, tables, new_tables):
+            kept = torch.empty((n_seq, kv, max(n_keep, 0)), dtype=torch.int32, device=self.device)
+            new_lens = torch.empty(n_seq, dtype=torch.int32, device=self.device)
+            new_mass = torch.empty(kept.shape, dtype=torch.float32, device=self.device)
+            call("smx_paged_evict", self._handle(), mass.data_ptr(), stride, lens.data_ptr(), n_seq, max_len, n_keep, n_recent,
+                 tables.data_ptr(), tables.shape[1], new_tables.data_ptr(), new_tables.shape[1], kept.data_ptr(),
+                 new_lens.data_ptr(), new_mass.data_ptr(), _raw_stream(index))
+        return kept, new_lens, new_mass
+
+    def _handle(self):
+        if not self._h.value:
+            raise ValueError("the cache is closed")
+        return self._h
+
+    def _work_bytes(self, name: str, key, rules=()) -> int:
+        need = self._work.get((name, key, rules))
+        if need is None:
+            b = ctypes.c_int64()
+            extra = ()
+            if name == "smx_attention_paged_work_bytes":
+                c = _lib.AttentionRulesC(0.0, 0.0, None, 16 if rules[1] else None, rules[0], 0)   # (asked whether there are prefixes)
+                extra = (ctypes.byref(c),)
+            call(name, self._handle(), *key, *extra, ctypes.byref(b))
+            if len(self._work) >= 4096:
+                self._work.clear()
+            need = self._work[(name, key, rules)] = b.value
+        return need
+
+    def close(self):
+        if getattr(self, "_h", None) and self._h.value and _lib is not None and _lib._lib is not None:
+            _lib._lib.smx_paged_cache_destroy(self._h)
+            self._h = ctypes.c_void_p()
+
+    def __del__(self):
+        self.close()
+
+
+def _table(t, n_seq: int, what: str):
+    if t.dtype is not _torch().int32 or t.dim() != 2 or t.shape[0] != n_seq or not t.is_contiguous():
+        raise ValueError(f"{what} must be a contiguous int32 [{n_seq}, pages] tensor")
+    _c_int(t.shape[1], "pages")
+
+
+def _mass_rows(mass) -> int:
+    """The distance between the rows of mass [n_seq, n_kv_head, width], evenly spaced."""
+    return _matrix_rows(mass, mass.shape[2], "mass")
+
+
+def _rules(n_seq, n_head, scale, cap, slopes, window, prefix):
+    if slopes is not None:
+        _floats(slopes, n_head, "slopes")
+    if prefix is not None:
+        _int32(prefix, n_seq, "prefix")
+    _c_int(window, "window")
+    for x, what in ((0.0 if scale is None else scale, "scale"), (cap, "cap")):
+        if not 0.0 <= x < 3.4e38:
+            raise ValueError(f"{what} {x} must be finite and not negative")
+    if scale is not None and not scale > 0.0:
+        raise ValueError("scale must be positive")
+    return _lib.AttentionRulesC(0.0 if scale is None else scale, cap, _opt(slopes), _opt(prefix), window, 0)
+
+
+def _paged_batch(q, cache, starts, lens, tables, max_q, max_len):
+    """Checks what the calls over a batch have in common: (n_tok, n_head, n_seq, q's stride, q's type, max_len)."""
+    if q.dim() != 3:
+        raise ValueError("q must be [n_tok, n_head, head_dim]")
+    n_tok, n_head, _ = q.shape
+    stride = _token_rows(q, n_head, cache.head_dim, "q")
+    t = _elem_type(q.dtype, "q")
+    if t != _lib.F32 and q.dtype is not cache.dtype:
+        raise ValueError(f"q must be float32 or the cache's {cache.dtype}, is {q.dtype}")
+    n_seq = lens.numel()
+    _int32(lens, n_seq, "lens")
+    _int32(starts, n_seq + 1, "starts")
+    _table(tables, n_seq, "tables")
+    if max_len is None:
+        max_len = min(tables.shape[1] * cache.page_size, 1 << 24)
+    _c_int(max_q, "max_q")
+    _c_int(max_len, "max_len")
+    _c_int(n_tok * n_head, "n_tok * n_head")
+    return n_tok, n_head, n_seq, stride, t, max_len
+
+
+def attention_paged(q, cache: GpuPagedCache, starts, lens, tables, max_q: int, max_len: int | None = None, scale: float | None = None,
+                    cap: float = 0.0, slopes=None, window: int = 0, prefix=None, lse: bool = False, out=None):
+    """Attention of a ragged batch of new tokens over a paged cache (smx_attention_paged).  q [n_tok, n_head, head_dim] float32 or of the
+    cache's type (tokens may be rows of a fused projection).  Sequence b's new tokens are rows starts[b] .. starts[b + 1] - 1
+    ([n_seq + 1]; at most max_q each) and the last of its lens[b] positions (already appended), which lie in the pages
+    tables[b] ([n_seq, pages]); all int32 on the device.  max_len: an upper bound of lens (default: what the tables
+    hold); a tight one is faster.  A token at position t sees positions p <= t; with window > 0, those with p > t - window; and the
+    first prefix[b] ([n_seq] int32) whatever its own.  scale (default 1 / sqrt(head_dim)) times q . k, capped to cap *
+    tanh(score / cap) where cap > 0, less slopes[h] * |t - p| ([n_head] float32).
+    Returns [n_tok, n_head, head_dim] of q's type, or that and, with lse, the logarithms of the sums of exponentials
+    [n_tok, n_head] float32.  Rows that see nothing are zeros (lse -inf).  Rows of no sequence are left as they are in
+    `out`, undefined where that is not given."""
+    torch, h, index = _torch(), cache._handle(), cache.device.index
+    n_tok, n_head, n_seq, stride, t, max_len = _paged_batch(q, cache, starts, lens, tables, max_q, max_len)
+    rules = _rules(n_seq, n_head, scale, cap, slopes, window, prefix)
+    if out is not None and (out.shape != q.shape or out.dtype is not q.dtype or not out.is_contiguous()):
+        raise ValueError(f"out must be contiguous {q.dtype} {tuple(q.shape)}")
+    with _on_device(index, q, starts, lens, tables, slopes, prefix, out):
+        if out is None:
+            out = torch.empty(q.shape, dtype=q.dtype, device=cache.device)
+        sums = torch.empty((n_tok, n_head), dtype=torch.float32, device=cache.device) if lse else None
+        need = cache._work_bytes("smx_attention_paged_work_bytes", (t, n_tok, n_head, n_seq, max_q, max_len), (window, prefix is not None))
+        work = torch.empty(need, dtype=torch.uint8, device=cache.device) if need else None
+        call("smx_attention_paged", h, t, q.data_ptr(), stride, out.data_ptr(), _opt(sums), n_tok, n_head, n_seq, starts.data_ptr(),
+             lens.data_ptr(), tables.data_ptr(), tables.shape[1], max_q, max_len, ctypes.byref(rules), _opt(work), need,
+             _raw_stream(index))
+    return (out, sums) if lse else out
+
+
+def attention_mass(q, lse, cache: GpuPagedCache, starts, lens, tables, max_q: int, max_len: int | None = None, mass=None,
+                   scale: float | None = None, cap: float = 0.0, slopes=None, window: int = 0, prefix=None):
+    """The attention weight that every position has received (smx_attention_mass): mass [n_seq, n_kv_head, width] float32 (None, or
+    beyond width: 0) plus the sum over each sequence's new tokens and each KV head's query heads of exp(score - lse).  lse
+    [n_tok, n_head] as attention_paged gives it for the same q, lengths and rules.  Returns [n_seq, n_kv_head, max_len]
+    float32, 0 from lens[b] on: what evict decides by."""
+    torch, h, index = _torch(), cache._handle(), cache.device.index
+    n_tok, n_head, n_seq, stride, t, max_len = _paged_batch(q, cache, starts, lens, tables, max_q, max_len)
+    rules = _rules(n_seq, n_head, scale, cap, slopes, window, prefix)
+    _floats(lse, n_tok * n_head, "lse")
+    width = mass_stride = 0
+    if mass is not None:
+        if mass.dim() != 3 or mass.shape[:2] != (n_seq, cache.n_kv_head):
+            raise ValueError(f"mass must be [{n_seq}, {cache.n_kv_head}, width]")
+        width, mass_stride = mass.shape[2], _mass_rows(mass)
+        _c_int(width, "width")
+    with _on_device(index, q, lse, starts, lens, tables, mass, slopes, prefix):
+        out = torch.empty((n_seq, cache.n_kv_head, max(max_len, 0)), dtype=torch.float32, device=cache.device)
+        if out.numel() == 0 and max_len == 0:
+            return out
+        need = cache._work_bytes("smx_attention_mass_work_bytes", (n_head, n_seq, max_q, max_len))
+        work = torch.empty(need, dtype=torch.uint8, device=cache.device) if need else None
+        call("smx_attention_mass", h, t, q.data_ptr(), stride, lse.data_ptr(), _opt(mass), mass_stride, width, out.data_ptr(), n_tok,
+             n_head, n_seq, starts.data_ptr(), lens.data_ptr(), tables.data_ptr(), tables.shape[1], max_q, max_len,
+             ctypes.byref(rules), _opt(work), need, _raw_stream(index))
+    return out
+
+
 __all__ = ["GgufTensorType", "GpuWeightTensor", "SmxError", "dequantize", "quantize", "fill_normal",
            "rmsnorm", "layernorm", "rope_tables", "rope_", "scale_mask_softmax_", "attention_decode",
            "silu_mul", "gelu", "argmax", "sample", "row_bytes", "BLOCK_ELEMS", "BLOCK_BYTES", "GpuKvCache",
-           "attention_cached", "attention_shared", "verify_draft"]
+           "attention_cached", "attention_shared", "verify_draft", "Rotation", "qk_norm_rope", "GpuPagedCache",
+           "attention_paged", "attention_mass"]

@@ -1,0 +1,147 @@
+"""Refusals of the operators over a paged KV cache that need no device, and the plain forms' own closed cases."""
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+from tests import paged_reference as R
+
+P = ctypes.c_void_p(256)   # never followed: the call is refused first
+F32, F16, BF16 = 0, 1, 30
+
+
+@pytest.fixture(scope="module")
+def lib():
+    from smallmind_amd import _lib
+    return _lib.load()
+
+
+@pytest.mark.parametrize("args,code", [((F32, 8, 4, 64, 64), -5), ((8, 8, 4, 64, 64), -5), ((F16, 0, 4, 64, 64), -1), ((F16, 8, 0, 64, 64), -1),
+                                       ((F16, -1, 4, 64, 64), -1), ((F16, 8, 4, 0, 64), -5), ((F16, 8, 4, 60, 64), -5),
+                                       ((F16, 8, 4, 264, 64), -5), ((F16, 8, 4, 64, 0), -5), ((F16, 8, 4, 64, 8), -5), ((F16, 8, 4, 64, 48), -5),
+                                       ((F16, 8, 4, 64, 2048), -5), ((F16, 8, 4, 64, -64), -5), ((F16, 1 << 30, 1, 64, 64), -5),
+                                       ((F16, 8, 65536, 64, 64), -5), ((BF16, (1 << 21) - 1, 65535, 256, 1024), -2)])
+def test_cache_create_refuses(lib, args, code):
+    h = ctypes.c_void_p(77)
+    assert lib.smx_paged_cache_create(*args, ctypes.byref(h)) == code
+    assert h.value is None
+    assert b"smx_paged_cache_create" in lib.smx_last_error()
+
+
+def test_null_caches_are_refused(lib):
+    n = ctypes.c_int64()
+    assert lib.smx_paged_cache_create(F16, 8, 4, 64, 64, None) == -1
+    assert lib.smx_paged_cache_info(None, None, None, None, None, None, None) == -1
+    assert lib.smx_paged_cache_destroy(None) == 0
+    assert lib.smx_paged_append(None, F32, None, 0, 0, P, 64, P, 64, None, None, 0.0, None, None, P, 1, F32, None, None) == -1
+    assert lib.smx_paged_read(None, P, 1, P, P, None) == -1
+    assert lib.smx_attention_paged_work_bytes(None, F32, 1, 1, 1, 1, 64, None, ctypes.byref(n)) == -1
+    assert lib.smx_attention_mass_work_bytes(None, 1, 1, 1, 64, ctypes.byref(n)) == -1
+    assert lib.smx_attention_paged(None, F32, P, 64, P, None, 1, 1, 1, P, P, P, 1, 1, 64, None, P, 1 << 20, None) == -1
+    assert lib.smx_attention_mass(None, F32, P, 64, P, None, 0, 0, P, 1, 1, 1, P, P, P, 1, 1, 64, None, P, 1 << 20, None) == -1
+    assert lib.smx_paged_evict(None, P, 64, P, 1, 64, 32, 8, P, 1, P, 1, P, P, P, None) == -1
+
+
+def rotation(**k):
+    from smallmind_amd._lib import RotationC
+    d = dict(cos=256, sin=256, n_pos=8, n_rot=64, halves=0, n_axes=1, sections=(0, 0, 0, 0))
+    d.update(k)
+    return RotationC(d["cos"], d["sin"], d["n_pos"], d["n_rot"], d["halves"], d["n_axes"], (ctypes.c_int32 * 4)(*d["sections"]))
+
+
+def test_qk_norm_rope_refuses(lib):
+    def run(tin=F32, q=P, qs=128, nh=2, k=P, ks=64, kv=1, hd=64, gq=None, gk=None, eps=1e-6, rot=None, pos=P, n=3, tout=F32, qo=P, ko=P):
+        return lib.smx_qk_norm_rope(tin, q, qs, nh, k, ks, kv, hd, gq, gk, eps, None if rot is None else ctypes.byref(rot), pos, n, tout, qo,
+                                    ko, None)
+    assert run(n=0) == 0        # nothing to do
+    odd = ctypes.c_void_p(258)
+    for bad in (dict(q=None, k=None), dict(qo=None), dict(ko=None), dict(n=-1), dict(nh=0), dict(nh=65536, qs=1 << 30), dict(kv=0),
+                dict(qs=127), dict(ks=63), dict(q=odd), dict(k=odd), dict(qo=odd), dict(ko=odd), dict(tin=F16, q=ctypes.c_void_p(257)),
+                dict(gq=P, eps=-1.0), dict(gk=P, eps=float("nan")), dict(gq=P, eps=float("inf")), dict(gq=ctypes.c_void_p(257)),
+                dict(rot=rotation(cos=None)), dict(rot=rotation(sin=None)), dict(rot=rotation(), pos=None), dict(rot=rotation(cos=257)),
+                dict(rot=rotation(n_pos=0)), dict(rot=rotation(n_rot=0)), dict(rot=rotation(n_rot=63)), dict(rot=rotation(n_rot=66)),
+                dict(rot=rotation(halves=2)), dict(rot=rotation(n_axes=0)), dict(rot=rotation(n_axes=5)),
+                dict(rot=rotation(n_axes=2, sections=(16, 15, 0, 0))), dict(rot=rotation(n_axes=2, sections=(33, -1, 0, 0))),
+                dict(rot=rotation(n_axes=3, sections=(2**31 - 1, 2**31 - 1, 34, 0)))):
+        assert run(**bad) == -1, bad
+        assert b"smx_qk_norm_rope" in lib.smx_last_error()
+    for bad in (dict(tin=2), dict(tout=8), dict(hd=60), dict(hd=264, qs=1024, ks=512), dict(hd=0), dict(n=2**31 - 1)):
+        assert run(**bad) == -5, bad
+
+
+def test_python_refuses_before_any_call():
+    import types
+
+    from smallmind_amd import quantization as Q
+    cos = torch.zeros(4, 8)
+    for bad in (dict(cos=torch.zeros(4)), dict(sin=torch.zeros(4, 7)), dict(cos=torch.zeros(4, 8, dtype=torch.float64)), dict(sections=[4, 5]),
+                dict(sections=[9, -1]), dict(sections=[]), dict(sections=[2, 2, 2, 1, 1]), dict(cos=torch.zeros(8, 4).t())):
+        with pytest.raises(ValueError):
+            Q.Rotation(**{**dict(cos=cos, sin=cos), **bad})
+    with pytest.raises(ValueError, match="float16 or bfloat16"):
+        Q.GpuPagedCache(torch.float32, 4, 1, 64)
+    big = (1 << 32) + 1
+    for at in range(4):
+        sizes = [4, 1, 64, 64]
+        sizes[at] += big - 1
+        with pytest.raises(ValueError, match="out of range"):
+            Q.GpuPagedCache(torch.float16, *sizes)
+    cache = types.SimpleNamespace(device=torch.device("cuda", 0), head_dim=64, page_size=16, n_kv_head=1, dtype=torch.float16,
+                                  _handle=lambda: None)
+    q, one, two, tab = torch.zeros(1, 1, 64), torch.zeros(1, dtype=torch.int32), torch.zeros(2, dtype=torch.int32), torch.zeros(1, 4, dtype=torch.int32)
+    lse = torch.zeros(1, 1)
+    for bad in (dict(q=torch.zeros(1, 64)), dict(q=torch.zeros(1, 1, 32)), dict(q=q.double()), dict(q=q.bfloat16()), dict(starts=one),
+                dict(starts=two.long()), dict(lens=two), dict(tables=torch.zeros(4, dtype=torch.int32)), dict(tables=torch.zeros(2, 4, dtype=torch.int32)),
+                dict(tables=tab.long()), dict(max_q=big), dict(max_len=big), dict(max_len=1 << 31), dict(window=big), dict(cap=-1.0),
+                dict(cap=float("nan")), dict(scale=0.0), dict(scale=float("inf")), dict(slopes=torch.zeros(2)), dict(slopes=torch.zeros(1).double()),
+                dict(prefix=two), dict(prefix=torch.zeros(1))):
+        a = {**dict(q=q, starts=two, lens=one, tables=tab, max_q=1, max_len=64), **bad}
+        with pytest.raises(ValueError):
+            Q.attention_paged(a.pop("q"), cache, a.pop("starts"), a.pop("lens"), a.pop("tables"), a.pop("max_q"), a.pop("max_len"), **a)
+        a = {**dict(q=q, starts=two, lens=one, tables=tab, max_q=1, max_len=64), **bad}
+        with pytest.raises(ValueError):
+            Q.attention_mass(a.pop("q"), lse, cache, a.pop("starts"), a.pop("lens"), a.pop("tables"), a.pop("max_q"), a.pop("max_len"), **a)
+    for bad in (torch.zeros(1, 64), torch.zeros(2, 1, 64), torch.zeros(1, 2, 64), torch.zeros(1, 1, 64).double()):
+        with pytest.raises(ValueError):
+            Q.attention_mass(q, lse, cache, two, one, tab, 1, 64, mass=bad)
+    with pytest.raises(ValueError):
+        Q.attention_mass(q, torch.zeros(2, 1), cache, two, one, tab, 1, 64)
+    with pytest.raises(ValueError, match="out must"):
+        Q.attention_paged(q, cache, two, one, tab, 1, 64, out=torch.zeros(1, 1, 64).half())
+
+
+def test_plain_rotation_keeps_lengths_and_turns_by_axes():
+    rng = np.random.default_rng(0)
+    x = rng.normal(0, 1, (5, 2, 16))
+    a = rng.uniform(0, 6, (9, 6))
+    pos = rng.integers(0, 9, (2, 5))
+    for halves in (False, True):
+        y, _ = R.turned(x, None, 0.0, np.cos(a), np.sin(a), pos, [2, 4], halves)
+        assert np.allclose((y ** 2).sum(-1), (x ** 2).sum(-1)) and np.array_equal(y[..., 12:], x[..., 12:])
+        z = (x[..., :6] + 1j * x[..., 6:12]) if halves else x[..., 0:12:2] + 1j * x[..., 1:12:2]
+        ang = np.concatenate([a[pos[0], :2], a[pos[1], 2:]], 1)[:, None]
+        w = z * np.exp(1j * ang)
+        got = (y[..., :6] + 1j * y[..., 6:12]) if halves else y[..., 0:12:2] + 1j * y[..., 1:12:2]
+        assert np.allclose(got, w)
+
+
+def test_plain_attention_and_received_weights_agree():
+    rng = np.random.default_rng(1)
+    q, k, v = rng.normal(0, 1, (6, 8)), rng.normal(0, 1, (10, 8)), rng.normal(0, 1, (10, 8))
+    see = R.visible(4, 6, 10, prefix=2, window=3)
+    assert see[0].tolist() == [True, True, True, True, True] + [False] * 5
+    assert R.visible(-2, 3, 4).sum() == 1 and not R.visible(-2, 3, 4)[:2].any()
+    S = R.Scores(q, k, np.arange(4, 10), torch.float32, torch.float16, cap=5.0, slope=0.1)
+    out, bound, lse, _ = R.attention(S, v, see, torch.float32, torch.float16)
+    w, _ = R.received(S, lse, see)
+    assert np.isclose(w.sum(), 6) and (bound < 1e-3).all()
+    assert np.allclose(out[0], np.exp(S.s[0, :5] - lse[0]) @ v[:5])
+
+
+def test_plain_eviction():
+    m = np.array([1.0, 3.0, 3.0, np.nan, 0.5, 3.0, 9.0, 9.0])
+    assert R.evict(m, 8, 4, 2) == [1, 2, 6, 7]
+    assert R.evict(m, 6, 8, 0) == [0, 1, 2, 3, 4, 5]
+    assert R.evict(m, 6, 5, 0) == [0, 1, 2, 4, 5]
+    assert R.evict(m, 8, 3, 3) == [5, 6, 7] and R.evict(m, 0, 3, 3) == []
