@@ -337,7 +337,7 @@ typedef struct smx_attention_rules {
     int32_t reserved;     /* must be zero */
 } smx_attention_rules;
 /* Bytes of work memory that an attention call, and a call for received weights, of these sizes needs (rules may be
- * NULL; only window and whether there are prefixes count). */
+ * NULL; only the window counts). */
 SMX_API int smx_attention_paged_work_bytes(const smx_paged_cache *c, int type, int n_tok, int n_head, int n_seq, int max_q,
                                            int max_len, const smx_attention_rules *rules, int64_t *bytes);
 SMX_API int smx_attention_mass_work_bytes(const smx_paged_cache *c, int n_head, int n_seq, int max_q, int max_len,

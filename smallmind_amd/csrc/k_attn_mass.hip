@@ -48,7 +48,8 @@ __global__ __launch_bounds__(kWaves * 64) void k_attn_mass(const AttnPgArgs a)
 #pragma unroll
     for (int i = 0; i < 16; i++) sum[i] = 0.0f;
     if (s0 < s1) {
-        const Rows16 r0 = rows16(a, s, head, at / kPgGroup), r1 = rows16(a, s, head, at / kPgGroup + 1);
+        const Pages P(a, s, head, at / kPgGroup);
+        const Rows16 r0 = P.rows(a, at / kPgGroup), r1 = P.rows(a, at / kPgGroup + 1);
         const uint8_t *p = (lane & 16 ? r1.p : r0.p) + (lane & 15) * ROW;
         elem8 k[NK];
 #pragma unroll
@@ -83,8 +84,8 @@ __global__ __launch_bounds__(kWaves * 64) void k_attn_mass(const AttnPgArgs a)
                 for (int n = 0; n < NK; n++)
 #pragma unroll
                     for (int q = 0; q < kParts<F32>; q++) x = mfma(k[n], M.q[j][q][n][lane], x);
-                if (S.shaped) shape(a, S, x, r, at, h);
-                if (!r0.there || !r1.there || !B.whole(s.pre, at, 32)) mask(x, r, s.pre, at, h, r0.there, r1.there);
+                if (S.shaped) shape<true>(a, S, x, r, at, h);   // (the sums are fp32 whatever the queries)
+                if (!r0.there || !r1.there || !B.whole(s.pre, at, 32)) mask(x, seen(a, s, r, at, h, r0.there, r1.there));
                 const float l = M.lse[j][lane];
                 // (past the last row the columns repeat it: they count for nothing)
 #pragma unroll

@@ -43,9 +43,9 @@ struct Running {
             for (int i = 0; i < 16; i++) acc[n][i] = 0.0f;
     }
 
-    // x of KT * 32 positions become weights' parts: w[part][16 positions].
-    template <int KT, int NP>
-    __device__ __forceinline__ void step(float16v (&x)[KT], float c, elem8 (&w)[NP][2 * KT])
+    // Moves the reference to what x of KT * 32 positions holds, where that calls for it; returns e: their weights are 2^(x c + e).
+    template <int KT>
+    __device__ __forceinline__ float refer(float16v (&x)[KT], float c)
     {
         float top = x[0][0];
 #pragma unroll
@@ -79,20 +79,23 @@ struct Running {
                 e = kOff;
             }
         }
-        float sum = 0.0f;
+        return e;
+    }
+
+    // x of 32 positions becomes weights' parts: w[part][16 positions].
+    template <int NP>
+    __device__ __forceinline__ void weigh(const float16v &x, float c, float e, elem8 (&w)[NP][2])
+    {
 #pragma unroll
-        for (int t = 0; t < KT; t++) {
+        for (int i = 0; i < 16; i += 2) {
+            const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i], c, e)), q = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i + 1], c, e));
+            l += p;
+            l += q;
+            elem2 s[NP];
+            split(p, q, s);
 #pragma unroll
-            for (int i = 0; i < 16; i++) {
-                const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(x[t][i], c, e));
-                sum += p;
-                elem s[NP];
-                split(p, s);
-#pragma unroll
-                for (int k = 0; k < NP; k++) w[k][2 * t + (i >> 3)][i & 7] = s[k];
-            }
+            for (int k = 0; k < NP; k++) w[k][i >> 3][i & 7] = s[k][0], w[k][i >> 3][(i & 7) + 1] = s[k][1];
         }
-        l += sum;
     }
 };
 
@@ -156,129 +159,252 @@ __device__ __forceinline__ void finish_empty(const AttnPgArgs &a, const Row &r, 
     a.part_ml[2 * at] = kNegInf, a.part_ml[2 * at + 1] = 0.0f;
 }
 
-// ---- many rows -------------------------------------------------------------------------------------
-struct Tile {
-    uint8_t k[kPgTile * ROW], v[kPgTile * ROW];
+// What N waves hand to as many others, a value per lane.
+template <int N> struct Handed {
+    float m[N][64], b[N][64], l[N][64];
+    float acc[N][ND * 16][64];
+
+    __device__ __forceinline__ void put(int i, int lane, const Running &R)
+    {
+        m[i][lane] = R.m, b[i][lane] = R.b, l[i][lane] = R.l;
+#pragma unroll
+        for (int d = 0; d < ND; d++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) acc[i][d * 16 + e][lane] = R.acc[d][e];
+    }
+    // added to R
+    __device__ __forceinline__ void join(int i, int lane, Running &R) const
+    {
+        // the higher of the two references; one without weight brings nothing
+        const float om = m[i][lane], ob = b[i][lane], ol = l[i][lane];
+        const bool none = om == kNegInf && ol == 0.0f, up = !none && (R.m == kNegInf || ob < R.b);
+        const float nb = up ? ob : R.b;
+        const float f = R.m == kNegInf && R.l == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(nb - R.b), g = none ? 0.0f : __builtin_amdgcn_exp2f(nb - ob);
+        R.l = R.l * f + ol * g;
+#pragma unroll
+        for (int n = 0; n < ND; n++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) {
+                const float o = acc[i][n * 16 + e][lane];
+                R.acc[n][e] = R.acc[n][e] * f + (none ? 0.0f : o * g);
+            }
+        if (up) R.m = om;
+        R.b = nb;
+    }
 };
 
-// A tile of positions on its way to LDS: each of NW waves brings a share of its kilobytes.
-template <int NW>
-__device__ __forceinline__ void bring(const AttnPgArgs &a, const Seq &s, int head, int tile, Tile &T, int wave, int lane)
-{
-    constexpr int PER = W / 32;   // kilobytes of 16 rows
+// ---- many rows -------------------------------------------------------------------------------------
+// A wave's share (of four) of the kilobytes of a tile's K, and as much of its V: where they are, and the way to LDS.
+struct Share {
+    static constexpr int PER = W / 32, N = PER;   // kilobytes of 16 rows; of a wave
+    const uint8_t *src[N];
+
+    __device__ __forceinline__ void find(const AttnPgArgs &a, const Pages &P, int tile, int wave)
+    {
 #pragma unroll
-    for (int i0 = 0; i0 < 4 * PER; i0 += NW) {
-        const int i = i0 + wave;
-        if (4 * PER % NW != 0 && i >= 4 * PER) break;
-        const int b = i / PER, off = b * 16 * ROW + (i - b * PER) * 1024;
-        const uint8_t *src = rows16(a, s, head, 4 * tile + b).p + (i - b * PER) * 1024 + lane * 16;
-        to_lds(src, T.k + off);
-        to_lds(src + a.c.v_off(), T.v + off);
+        for (int j = 0; j < N; j++) {
+            const int i = j * 4 + wave, b = i / PER;
+            src[j] = P.rows(a, 4 * tile + b).p + (i - b * PER) * 1024;
+        }
+    }
+    __device__ __forceinline__ void bring(uint8_t *to, size_t off, int wave, int lane) const
+    {
+#pragma unroll
+        for (int j = 0; j < N; j++) {
+            to_lds(src[j] + off, lane * 16, to + (j * 4 + wave) * 1024);
+        }
+    }
+};
+
+// Two tiles' K and V.
+struct Tiles {
+    uint8_t k[2][kPgTile * ROW], v[2][kPgTile * ROW];
+};
+// Those of NG groups of four waves, then what they hand over at the end.
+template <int NG> union Many {
+    Tiles t[NG];
+    Handed<NG == 2 ? 4 : 1> j;
+};
+
+// Tells the compiler how to order a block: its N matrix instructions, NP for every READS reads from LDS, with each the ordinary
+// and transcendental vector instructions that share the block; two operands are read before them all.
+template <int N, int NP, int READS, int VALU, int TRANS>
+__device__ __forceinline__ void interleave()
+{
+    __builtin_amdgcn_sched_group_barrier(0x100, 2 * READS, 0);
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        if (i % NP == 0) __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);
+        if (VALU) __builtin_amdgcn_sched_group_barrier(0x002, VALU, 0);
+        if (TRANS) __builtin_amdgcn_sched_group_barrier(0x400, TRANS, 0);
     }
 }
 
-template <bool F32, int NW>
-__device__ __forceinline__ void many(const AttnPgArgs &a, Tile (&T)[2], const Seq &s, int head, int row0, int part)
+// A block of 128 rows, gone through by NG groups of four waves that take tiles in turn.
+template <bool F32, int NG>
+__device__ __forceinline__ void many(const AttnPgArgs &a, Many<NG> &M, const Seq &s, int head, int row0, int part)
 {
-    const int lane = threadIdx.x & 63, h = lane >> 5, wave = wave_id();
+    constexpr int NP = kParts<F32>;
+    // 32-position halves of a tile at once: two where registers suffice, and then the next tile's scores while this one's weigh
+    constexpr int KT = W * NP > 512 ? 1 : 2;
+    constexpr bool AHEAD = KT == 2;
+    const int lane = threadIdx.x & 63, h = lane >> 5, wave = wave_id() & 3, group = wave_id() >> 2;
     const int mine = row0 + wave * kPgRows;
-    const int t0 = row_of(a, s, head, row0).t, t1 = row_of(a, s, head, row0 + NW * kPgRows - 1).t;
+    Tiles &T = M.t[group];
+    const int t0 = row_of(a, s, head, row0).t, t1 = row_of(a, s, head, row0 + 4 * kPgRows - 1).t;
     const Range rg = range_of(a, s, __builtin_amdgcn_readfirstlane(t0), __builtin_amdgcn_readfirstlane(t1));
-    const int i0 = part * a.chunk, i1 = a.parts > 1 ? min(rg.count, i0 + a.chunk) : rg.count;
+    // an even share of what there is to go through, but no less than chunk
+    const int per = max((rg.count + a.parts - 1) / a.parts, a.chunk), i0 = part * per, i1 = min(rg.count, i0 + per);
     const Row r = row_of(a, s, head, mine + (lane & 31));
     const bool busy = mine < s.rows;   // (a wave without rows brings its share of the tiles)
     if (i0 >= i1) {
-        if (a.parts > 1) { if (busy) finish_empty(a, r, h, part); return; }
+        if (!busy || group) return;
+        if (a.parts > 1) { finish_empty(a, r, h, part); return; }
         Running R;
-        if (busy) finish<F32>(a, R, r, h, part);
+        finish<F32>(a, R, r, h, part);
         return;
     }
-    bring<NW>(a, s, head, rg.tile(i0), T[0], wave, lane);
+    const int mine0 = i0 + group;   // this group's first tile
+    Pages P(a, s, head, 4 * rg.tile(min(mine0, i1 - 1)));
+    Share kv;
+    uint32_t there = 0;   // whether the cache has the pages of the tiles on their way, four bits each, the first one's lowest
+    const auto bring_k = [&](int i, int to, int bits) {
+        const int tile = rg.tile(i);
+        P.go(a, s, 4 * tile);
+        there |= (uint32_t)(P.ok >> (4 * tile & 63) & 15) << bits;
+        kv.find(a, P, tile, wave);
+        kv.bring(T.k[to], 0, wave, lane);
+    };
+    const auto bring_v = [&](int to) { kv.bring(T.v[to], a.c.v_off(), wave, lane); };   // of the K brought last
+    if (mine0 < i1) {
+        bring_k(mine0, 0, 0);
+        bring_v(0);
+    }
+    if (AHEAD && mine0 + NG < i1) bring_k(mine0 + NG, 1, 4);
     Query<F32> Q;
     load_q<F32>(a, r, h, Q);
     const Shape S(a, r, Q.unit);
     const Bounds B = bounds_of(a, s, mine, kPgRows);
     const LaneAt L(lane);
-    constexpr int KT = W * kParts<F32> > 512 ? 1 : 2;   // 32-position halves of a tile at once: two where registers suffice
     Running R;
-    for (int i = i0; i < i1; i++) {
-        const int tile = rg.tile(i), at = tile * kPgTile;
-        wait_all();
-        __syncthreads();   // this tile is there, the one before has been read
-        if (i + 1 < i1) bring<NW>(a, s, head, rg.tile(i + 1), T[(i + 1 - i0) & 1], wave, lane);
-        if (!busy || B.none(s.pre, at, kPgTile)) continue;
-        const Tile &C = T[(i - i0) & 1];
-        bool there[4], all = true;
+    const auto scores = [&](float16v (&x)[KT], const uint8_t *k, int t0) {
 #pragma unroll
-        for (int b = 0; b < 4; b++) there[b] = rows16(a, s, head, 4 * tile + b).there, all = all && there[b];
-        const bool cut = !all || !B.whole(s.pre, at, kPgTile);
+        for (int n = 0; n < NK; n++)
 #pragma unroll
-        for (int t0 = 0; t0 < 2; t0 += KT) {
-            float16v x[KT];
+            for (int t = 0; t < KT; t++) {
+                const elem8 kk = L.key(k + (t0 + t) * 32 * ROW, n);
 #pragma unroll
-            for (int t = 0; t < KT; t++)
-#pragma unroll
-                for (int e = 0; e < 16; e++) x[t][e] = 0.0f;
-#pragma unroll
-            for (int n = 0; n < NK; n++)
-#pragma unroll
-                for (int t = 0; t < KT; t++) {
-                    const elem8 k = L.key(C.k + (t0 + t) * 32 * ROW, n);
-#pragma unroll
-                    for (int p = 0; p < kParts<F32>; p++) x[t] = mfma(k, Q.q[p][n], x[t]);
-                }
-            if (S.shaped) {
-#pragma unroll
-                for (int t = 0; t < KT; t++) shape(a, S, x[t], r, at + 32 * (t0 + t), h);
+                for (int p = 0; p < NP; p++) x[t] = mfma(kk, Q.q[p][n], n || p ? x[t] : float16v(0.0f));
             }
-            if (cut) {
+    };
+    const auto sees = [&](int i) { return busy && i < i1 && !B.none(s.pre, rg.tile(i) * kPgTile, kPgTile); };
+    const auto add_v = [&](const elem8 (&w)[NP][2], const uint8_t *v) {   // of 32 positions
 #pragma unroll
-                for (int t = 0; t < KT; t++) mask(x[t], r, s.pre, at + 32 * (t0 + t), h, there[2 * (t0 + t)], there[2 * (t0 + t) + 1]);
+        for (int b = 0; b < 2; b++)
+#pragma unroll
+            for (int d = 0; d < ND; d++) {
+                const elem8 vv = L.val(v + b * 16 * ROW, d);
+#pragma unroll
+                for (int p = 0; p < NP; p++) R.acc[d] = mfma(vv, w[p][b], R.acc[d]);
             }
-            elem8 w[kParts<F32>][2 * KT];
-            R.step<KT, kParts<F32>>(x, S.c, w);
-#pragma unroll
-            for (int b = 0; b < 2 * KT; b++)
-#pragma unroll
-                for (int d = 0; d < ND; d++) {
-                    const elem8 v = L.val(C.v + (2 * t0 + b) * 16 * ROW, d);
-#pragma unroll
-                    for (int p = 0; p < kParts<F32>; p++) R.acc[d] = mfma(v, w[p][b], R.acc[d]);
-                }
+    };
+    bool on = sees(mine0);
+    // tile i, its scores in x (AHEAD) and its buffers `at`; the next one's scores go to y
+    const auto go = [&](int i, float16v (&x)[KT], float16v (&y)[KT], int at) {
+        const int pos = rg.tile(i) * kPgTile;   // (past the last tile: not used)
+        wait_loads<0>();
+        __syncthreads();   // K of the next tile (without AHEAD this one's) and V of this are there, those before have been read
+        const uint32_t th = there & 15;
+        there >>= 4;
+        if (AHEAD) {
+            if (i + NG < i1) bring_v(at ^ 1);
+            if (i + 2 * NG < i1) bring_k(i + 2 * NG, at, 4);
+        } else if (i + NG < i1) {
+            bring_k(i + NG, at ^ 1, 0);
+            bring_v(at ^ 1);
         }
+        const bool cut = th != 15 || !B.whole(s.pre, pos, kPgTile), more = AHEAD && sees(i + NG);
+        if (!more) {   // (what y holds is not used: this says so)
+#pragma unroll
+            for (int t = 0; t < KT; t++) y[t] = float16v(0.0f);
+        }
+        if (on) {
+#pragma unroll
+            for (int t0 = 0; t0 < 2; t0 += KT) {
+                if (!AHEAD) scores(x, T.k[at], t0);
+                if (S.shaped) {
+#pragma unroll
+                    for (int t = 0; t < KT; t++) shape<F32>(a, S, x[t], r, pos + 32 * (t0 + t), h);
+                }
+                if (cut) {
+#pragma unroll
+                    for (int t = 0; t < KT; t++)
+                        mask(x[t], seen(a, s, r, pos + 32 * (t0 + t), h, th >> 2 * (t0 + t) & 1, th >> (2 * (t0 + t) + 1) & 1));
+                }
+                const float e = R.template refer<KT>(x, S.c);
+                // vector instructions of the softmax beside the matrix instructions: the first half's beside the next tile's scores,
+                // the second half's beside the first half's sums
+                constexpr int VALU = 16 * (NP == 1 ? 5 : NP == 2 ? 8 : 16) / 2;   // of 16 elements
+                constexpr int MK = 2 * NK * NP, MV = 2 * ND * NP;                   // matrix instructions
+                const uint8_t *v = T.v[at] + t0 * 32 * ROW;
+                elem8 w[KT][NP][2];
+                // (16-bit weights are so few instructions that the whole softmax goes beside the scores: 2048 tokens over 32768
+                // positions, 128 dims, 1060 us for 1090)
+                constexpr bool BOTH = KT == 2 && NP == 1;
+                if (more) {
+                    scores(y, T.k[at ^ 1], 0);
+                    R.template weigh<NP>(x[0], S.c, e, w[0]);
+                    if constexpr (BOTH) R.template weigh<NP>(x[1], S.c, e, w[1]);
+                    interleave<MK, NP, 1, ((1 + BOTH) * VALU + MK - 1) / MK, ((1 + BOTH) * 16 + MK - 1) / MK>();
+                } else {
+                    R.template weigh<NP>(x[0], S.c, e, w[0]);
+                    if constexpr (BOTH) R.template weigh<NP>(x[1], S.c, e, w[1]);
+                }
+                if constexpr (BOTH) {
+                    add_v(w[0], v);
+                } else if constexpr (KT == 2) {
+                    __builtin_amdgcn_sched_barrier(0);
+                    add_v(w[0], v);
+                    R.template weigh<NP>(x[1], S.c, e, w[1]);
+                    interleave<MV, NP, 2, (VALU + MV - 1) / MV, (16 + MV - 1) / MV>();
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                add_v(w[KT - 1], v + (KT - 1) * 32 * ROW);
+                interleave<(1 + BOTH) * MV, NP, 2, 0, 0>();
+            }
+        } else if (more) {
+            scores(y, T.k[at ^ 1], 0);
+        }
+        on = AHEAD ? more : sees(i + NG);
+    };
+    float16v x[KT], y[KT];
+    if (AHEAD) {
+        wait_loads<0>();
+        __syncthreads();
+        if (on) scores(x, T.k[0], 0);
     }
-    if (busy) finish<F32>(a, R, r, h, part);
+    for (int i = i0; i < i1; i += 2 * NG) {   // (every wave meets the same barriers)
+        go(i + group, x, y, 0);
+        if (i + NG < i1) go(i + NG + group, y, x, 1);
+    }
+    if constexpr (NG == 2) {
+        __syncthreads();
+        if (group) M.j.put(wave, lane, R);
+        __syncthreads();
+        if (group) return;
+        M.j.join(wave, lane, R);
+    }
+    // (the row found anew: its numbers need not be kept while the tiles go by)
+    if (busy) finish<F32>(a, R, row_of(a, s, head, mine + (opaque_tid() & 31)), opaque_tid() >> 5 & 1, part);
 }
 
 // ---- few rows --------------------------------------------------------------------------------------
 // Memory of NW waves: V of 32 positions twice for each, then the joining of their sums.
 template <int NW> union Few {
     uint8_t v[NW][2][32 * ROW];
-    struct {
-        float m[NW / 2][64], b[NW / 2][64], l[NW / 2][64];
-        float acc[NW / 2][ND * 16][64];
-    } j;
+    Handed<NW / 2> j;
 };
-
-// `of` added to R.
-__device__ __forceinline__ void join(Running &R, float m, float b, float l, const float (*acc)[64], int lane)
-{
-    // the higher of the two references; one without weight brings nothing
-    const bool none = m == kNegInf && l == 0.0f;
-    const bool up = !none && (R.m == kNegInf || b < R.b);
-    const float nb = up ? b : R.b;
-    const float f = R.m == kNegInf && R.l == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(nb - R.b), g = none ? 0.0f : __builtin_amdgcn_exp2f(nb - b);
-    R.l = R.l * f + l * g;
-#pragma unroll
-    for (int n = 0; n < ND; n++)
-#pragma unroll
-        for (int i = 0; i < 16; i++) {
-            const float o = acc[n * 16 + i][lane];
-            R.acc[n][i] = R.acc[n][i] * f + (none ? 0.0f : o * g);
-        }
-    if (up) R.m = m;
-    R.b = nb;
-}
 
 template <bool F32, int NW>
 __device__ __forceinline__ void few(const AttnPgArgs &a, Few<NW> &F, const Seq &s, int head, int part)
@@ -288,7 +414,7 @@ __device__ __forceinline__ void few(const AttnPgArgs &a, Few<NW> &F, const Seq &
     const Row last = row_of(a, s, head, s.rows - 1);
     const Range rg = range_of(a, s, s.first, __builtin_amdgcn_readfirstlane(last.t));
     // halves of tiles
-    const int i0 = 2 * part * a.chunk, i1 = a.parts > 1 ? min(2 * rg.count, i0 + 2 * a.chunk) : 2 * rg.count;
+    const int per = 2 * max((rg.count + a.parts - 1) / a.parts, a.chunk), i0 = part * per, i1 = min(2 * rg.count, i0 + per);
     if (i0 >= i1) {
         if (wave) return;
         if (a.parts > 1) { finish_empty(a, r, h, part); return; }
@@ -299,10 +425,12 @@ __device__ __forceinline__ void few(const AttnPgArgs &a, Few<NW> &F, const Seq &
     const auto pos_of = [&](int i) { return rg.tile(i >> 1) * kPgTile + 32 * (i & 1); };
     const uint32_t row_at = (lane & 15) * ROW;
     elem8 k[NK];
+    Pages P(a, s, head, pos_of(min(i0 + wave, i1 - 1)) / kPgGroup);
     Rows16 r0{}, r1{};
     const auto find = [&](int i) {
         const int blk = pos_of(i) / kPgGroup;
-        r0 = rows16(a, s, head, blk), r1 = rows16(a, s, head, blk + 1);
+        P.go(a, s, blk);
+        r0 = P.rows(a, blk), r1 = P.rows(a, blk + 1);
     };
     const auto fetch_k = [&]() {
         const uint8_t *p = (lane & 16 ? r1.p : r0.p) + row_at;
@@ -312,8 +440,8 @@ __device__ __forceinline__ void few(const AttnPgArgs &a, Few<NW> &F, const Seq &
     const auto fetch_v = [&](uint8_t *v) {
 #pragma unroll
         for (int j = 0; j < W / 32; j++) {
-            to_lds(r0.p + a.c.v_off() + 1024 * j + lane * 16, v + 1024 * j);
-            to_lds(r1.p + a.c.v_off() + 1024 * j + lane * 16, v + 16 * ROW + 1024 * j);
+            to_lds(r0.p + a.c.v_off() + 1024 * j, lane * 16, v + 1024 * j);
+            to_lds(r1.p + a.c.v_off() + 1024 * j, lane * 16, v + 16 * ROW + 1024 * j);
         }
     };
     if (i0 + wave < i1) {
@@ -332,24 +460,23 @@ __device__ __forceinline__ void few(const AttnPgArgs &a, Few<NW> &F, const Seq &
         const uint8_t *v = F.v[wave][buf];
         const int at = pos_of(i);
         const bool th0 = r0.there, th1 = r1.there, cut = !th0 || !th1 || !B.whole(s.pre, at, 32), more = i + NW < i1;
-        wait_all();
+        wait_loads<0>();
         if (more) {
             find(i + NW);
             fetch_v(F.v[wave][buf ^ 1]);
         }
         float16v x[1];
 #pragma unroll
-        for (int e = 0; e < 16; e++) x[0][e] = 0.0f;
-#pragma unroll
         for (int n = 0; n < NK; n++)
 #pragma unroll
-            for (int p = 0; p < kParts<F32>; p++) x[0] = mfma(k[n], Q.q[p][n], x[0]);
+            for (int p = 0; p < kParts<F32>; p++) x[0] = mfma(k[n], Q.q[p][n], n || p ? x[0] : float16v(0.0f));
         if (more) fetch_k();
         if (B.none(s.pre, at, 32)) continue;
-        if (S.shaped) shape(a, S, x[0], r, at, h);
-        if (cut) mask(x[0], r, s.pre, at, h, th0, th1);
+        if (S.shaped) shape<F32>(a, S, x[0], r, at, h);
+        if (cut) mask(x[0], seen(a, s, r, at, h, th0, th1));
         elem8 w[kParts<F32>][2];
-        R.step<1, kParts<F32>>(x, S.c, w);
+        const float e = R.refer<1>(x, S.c);
+        R.weigh<kParts<F32>>(x[0], S.c, e, w);
 #pragma unroll
         for (int b = 0; b < 2; b++)
 #pragma unroll
@@ -363,31 +490,28 @@ __device__ __forceinline__ void few(const AttnPgArgs &a, Few<NW> &F, const Seq &
 #pragma unroll
     for (int n = NW / 2; n >= 1; n /= 2) {
         __syncthreads();
-        if (wave >= n && wave < 2 * n) {
-            F.j.m[wave - n][lane] = R.m, F.j.b[wave - n][lane] = R.b, F.j.l[wave - n][lane] = R.l;
-#pragma unroll
-            for (int d = 0; d < ND; d++)
-#pragma unroll
-                for (int i = 0; i < 16; i++) F.j.acc[wave - n][d * 16 + i][lane] = R.acc[d][i];
-        }
+        if (wave >= n && wave < 2 * n) F.j.put(wave - n, lane, R);
         __syncthreads();
-        if (wave < n) join(R, F.j.m[wave][lane], F.j.b[wave][lane], F.j.l[wave][lane], F.j.acc[wave], lane);
+        if (wave < n) F.j.join(wave, lane, R);
     }
     if (wave == 0) finish<F32>(a, R, r, h, part);
 }
 
-// Finds the block's sequence.  Block x belongs to the last sequence whose first block floor(start * group / rows) + b is
+// Finds the block's sequence.  Block x belongs to the last sequence whose first block floor(start * group / 128) + b is
 // not above x: no sequence has more blocks than lie between its own first and the next one's.
-template <bool F32, int NW>
-__device__ __forceinline__ void many_rows(const AttnPgArgs &a, Tile (&T)[2])
+template <bool F32, int NG>
+__device__ __forceinline__ void many_rows(const AttnPgArgs &a, Many<NG> &M)
 {
-    const int pairs = a.c.n_kv * a.parts;
-    const int block = a.tile_blocks - 1 - (int)blockIdx.x / pairs, pair = (int)blockIdx.x % pairs;
+    constexpr int ROWS = 4 * kPgRows;
+    // KV head and part fastest; of equal shares of the blocks, one for each sequence, the last ones first: late tokens see most
+    const int pairs = a.c.n_kv * a.parts, x = (int)blockIdx.x / pairs, pair = (int)blockIdx.x % pairs;
+    const int share = (a.tile_blocks + a.n_seq - 1) / a.n_seq, block = (x % a.n_seq) * share + share - 1 - x / a.n_seq;
+    if (block >= a.tile_blocks) return;
     const int lane = threadIdx.x & 63;
     int b = -1;
     for (int b0 = 0; b0 < a.n_seq; b0 += 64) {
         const int i = min(b0 + lane, a.n_seq - 1);
-        const int64_t first = (int64_t)min(max(a.starts[i], 0), a.n_tok) * a.group / (NW * kPgRows) + i;
+        const int64_t first = (int64_t)min(max(a.starts[i], 0), a.n_tok) * a.group / ROWS + i;
         const int n = __popcll(__ballot(b0 + lane < a.n_seq && first <= block));
         b += n;
         if (n < 64) break;
@@ -395,26 +519,26 @@ __device__ __forceinline__ void many_rows(const AttnPgArgs &a, Tile (&T)[2])
     b = __builtin_amdgcn_readfirstlane(b);
     if (b < 0) return;
     const Seq s = seq_of(a, b);
-    const int64_t first = (int64_t)s.start * a.group / (NW * kPgRows) + b;
-    const int64_t row0 = (block - first) * (NW * kPgRows);
+    const int64_t row0 = (block - ((int64_t)s.start * a.group / ROWS + b)) * ROWS;
     if (row0 >= s.rows || s.rows <= a.short_rows) return;
-    many<F32, NW>(a, T, s, pair % a.c.n_kv, (int)row0, pair / a.c.n_kv);
+    many<F32, NG>(a, M, s, pair % a.c.n_kv, (int)row0, pair / a.c.n_kv);
 }
 
-// Workgroups [0, tile_wgs): blocks of NW * 32 rows (KV head and part fastest, the last blocks, which see most, first); the others: a
-// short sequence each.  MANY: there are any of the former.
-template <bool F32, bool MANY, int NW>
-__global__ __launch_bounds__(NW * 64, !MANY && W <= 128 && W * kParts<F32> <= 256 ? 2 : 1) void k_attn_paged(const AttnPgArgs a)
+// Workgroups [0, tile_wgs): blocks of 128 rows, NG groups of four waves each; the others: a short sequence each.  NG = 0: there are
+// only these.
+template <bool F32, int NG>
+__global__ __launch_bounds__(NG == 2 ? 512 : 256, NG == 0 && W <= 128 && W * kParts<F32> <= 256 ? 2 : 1) void k_attn_paged(const AttnPgArgs a)
 {
+    constexpr int NW = NG == 2 ? 8 : 4;
     union Mem {
-        Tile tiles[MANY ? 2 : 1];
+        Many<NG == 2 ? 2 : 1> many;
         Few<NW> few;
     };
-    __shared__ __align__(1024) char mem[MANY ? sizeof(Mem) : sizeof(Few<NW>)];
+    __shared__ __align__(1024) char mem[NG ? sizeof(Mem) : sizeof(Few<NW>)];
     Mem &M = *(Mem *)mem;
-    if constexpr (MANY) {
+    if constexpr (NG > 0) {
         if ((int)blockIdx.x < a.tile_wgs) {
-            many_rows<F32, NW>(a, M.tiles);
+            many_rows<F32, NG>(a, M.many);
             return;
         }
     }
@@ -424,16 +548,16 @@ __global__ __launch_bounds__(NW * 64, !MANY && W <= 128 && W * kParts<F32> <= 25
     few<F32, NW>(a, M.few, s, unit % a.c.n_kv, i / units);
 }
 
-// Waves of the blocks of many rows: eight where their registers suffice (256 a lane), else four (512).
-template <bool F32> constexpr int kManyWaves = W * (1 + kParts<F32>) <= 256 ? 8 : 4;
+// Whether two groups of four waves find registers: 256 a lane.
+template <bool F32> constexpr bool kTwoGroups = W <= 128 && W * (1 + kParts<F32>) <= (kParts<F32> == 1 ? 256 : 192);
 
 template <bool F32>
 hipError_t launch(const AttnPgArgs &a, const AttnPgPlan &p, hipStream_t s)
 {
     const unsigned n = (unsigned)p.blocks;
-    if (p.kind == 0) k_attn_paged<F32, false, 4><<<n, 256, 0, s>>>(a);
-    else if (p.kind == 1) k_attn_paged<F32, true, 4><<<n, 256, 0, s>>>(a);
-    else if constexpr (kManyWaves<F32> == 8) k_attn_paged<F32, true, 8><<<n, 512, 0, s>>>(a);
+    if (p.groups == 0) k_attn_paged<F32, 0><<<n, 256, 0, s>>>(a);
+    else if (p.groups == 1) k_attn_paged<F32, 1><<<n, 256, 0, s>>>(a);
+    else if constexpr (kTwoGroups<F32>) k_attn_paged<F32, 2><<<n, 512, 0, s>>>(a);
     else return hipErrorInvalidValue;
     return hipGetLastError();
 }
@@ -446,6 +570,6 @@ hipError_t SMX_PG_NAME(launch_attn_paged, SMX_PG_W, SMX_PG_BF16)(const AttnPgArg
 {
     return a.io == PG_F32 ? launch<true>(a, p, s) : launch<false>(a, p, s);
 }
-int SMX_PG_NAME(attn_paged_waves, SMX_PG_W, SMX_PG_BF16)(int io) { return io == PG_F32 ? kManyWaves<true> : kManyWaves<false>; }
+bool SMX_PG_NAME(attn_paged_two, SMX_PG_W, SMX_PG_BF16)(int io) { return io == PG_F32 ? kTwoGroups<true> : kTwoGroups<false>; }
 
 }  // namespace smx

@@ -48,10 +48,12 @@ __global__ __launch_bounds__(256) void k_attn_paged_join(const AttnPgArgs a)
         float2 ml[4];
         float4 v[4];
 #pragma unroll
+        for (int k = 0; k < 4; k++) ml[k] = *(const float2 *)(a.part_ml + (min(s0 + k * PP, a.parts - 1) * n_rows + row) * 2);
+#pragma unroll
         for (int k = 0; k < 4; k++) {
             const int s = min(s0 + k * PP, a.parts - 1);
-            ml[k] = *(const float2 *)(a.part_ml + (s * n_rows + row) * 2);
-            v[k] = *(const float4 *)(a.part_acc + (s * n_rows + row) * a.c.hd + d);
+            v[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (ml[k].x != -__builtin_huge_valf()) v[k] = *(const float4 *)(a.part_acc + (s * n_rows + row) * a.c.hd + d);
         }
 #pragma unroll
         for (int k = 0; k < 4; k++)
@@ -100,42 +102,48 @@ __global__ __launch_bounds__(256) void k_attn_mass_join(const AttnPgArgs a)
 #define SMX_DECL(w, b)                                                                                      \
     hipError_t launch_attn_paged_w##w##_b##b(const AttnPgArgs &a, const AttnPgPlan &p, hipStream_t s);      \
     hipError_t launch_attn_mass_w##w##_b##b(const AttnPgArgs &a, const MassPgPlan &p, hipStream_t s);       \
-    int attn_paged_waves_w##w##_b##b(int io);
+    bool attn_paged_two_w##w##_b##b(int io);
 SMX_ALL(SMX_DECL)
 #undef SMX_DECL
 
-AttnPgPlan attn_paged_plan(const PgView &c, int io, int n_tok, int n_head, int n_seq, int max_q, int max_len, int window, bool prefix)
+AttnPgPlan attn_paged_plan(const PgView &c, int io, int n_tok, int n_head, int n_seq, int max_q, int max_len, int window)
 {
     AttnPgPlan p{};
     const int64_t group = n_head / c.n_kv, rows = max_q * group;
     const int64_t tiles = std::max(1, (max_len + kPgTile - 1) / kPgTile);
-    int waves = 4;
-#define SMX_CASE(w_, b) if (c.w == w_ && c.bf16 == b) waves = attn_paged_waves_w##w_##_b##b(io);
+    bool two = false;
+#define SMX_CASE(w_, b) if (c.w == w_ && c.bf16 == b) two = attn_paged_two_w##w_##_b##b(io);
     SMX_ALL(SMX_CASE)
 #undef SMX_CASE
-    p.kind = rows <= kPgRows ? 0 : waves == 8 && rows > 128 ? 2 : 1;
-    const int block = p.kind == 2 ? 256 : 128;
+    constexpr int block = 4 * kPgRows;
+    p.groups = rows <= kPgRows ? 0 : 1;
     // what a block goes through at most, where the window says so, and how many blocks that is done by
-    const int64_t span = window > 0 ? std::min<int64_t>(tiles, (window + (p.kind ? block / group + 1 : (int64_t)max_q)) / kPgTile + 2) : tiles;
-    int64_t units = (int64_t)n_seq * c.n_kv;
-    if (p.kind) {
+    const int64_t span = window > 0 ? std::min<int64_t>(tiles, (window + (p.groups ? block / group + 1 : (int64_t)max_q)) / kPgTile + 2) : tiles;
+    int64_t units = (int64_t)n_seq * c.n_kv, n = 1;
+    p.chunk = p.groups ? 1 : 4;
+    if (p.groups == 0) {
+        n = std::min((512 + units - 1) / units, (span + 3) / 4);
+        if (n * units < 128) n = std::max(n, std::min((128 + units - 1) / units, (span + 1) / 2)), p.chunk = 2;
+    } else {
         p.tile_blocks = (int)(n_tok * group / block + n_seq);
         units = std::max<int64_t>(1, (n_tok * group + block - 1) / block) * c.n_kv;
+        // Two groups of four waves on a block until there are 512 blocks, two for every compute unit (1024 tokens over 1024
+        // positions, 32 x 128 dims, 256 blocks: 27.8 us for 31.8 with one group; 4096 over 4096, 1024 blocks: 176 for 153).
+        if (two && units < 512) p.groups = 2;
+        // Parts up to one workgroup for every compute unit, of no fewer than four tiles.  n parts save 1 - 1 / n of the tiles'
+        // time, about a microsecond each at 128 dims, and cost a launch, 4 us, and their sums' way to memory and back, 8 bytes
+        // each at 5 TB/s: the best n is where these are equal, if that gains anything (64 tokens over 32768 positions, 16
+        // blocks: 504 us in one part, 55 in 16; 512 over 4096, 128 blocks of fp32, 64 dims: 73 and 52 in two; two chunks of 512
+        // with a window of 1024, 128 blocks of 128 dims: 40 and 58 in two).
+        const double save = (double)span * c.w / 128, part = (double)n_tok * n_head * c.hd * 8 / 5e6;
+        n = std::min({(int64_t)sqrt(save / part), 256 / units, (span + 3) / 4});
+        if (n > 1 && save * (1 - 1.0 / n) < 4 + part * n) n = 1;
     }
-    int64_t n = 1;
-    if (p.kind == 0) {
-        n = std::min((512 + units - 1) / units, (span + 3) / 4);
-        if (n * units < 128) n = std::max(n, std::min((128 + units - 1) / units, (span + 1) / 2));
-    } else if (units < 256) {
-        n = std::min((256 + units - 1) / units, (span + 7) / 8);
-    }
-    n = std::max<int64_t>(n, 1);
-    p.chunk = (int)((span + n - 1) / n);
-    const int64_t all = window > 0 && !prefix ? span : tiles;
-    p.parts = n == 1 ? 1 : (int)((all + p.chunk - 1) / p.chunk);
-    p.tile_wgs = p.kind ? (int64_t)p.tile_blocks * c.n_kv * p.parts : 0;
+    p.parts = (int)std::max<int64_t>(n, 1);
+    const int64_t shares = p.groups ? (p.tile_blocks + n_seq - 1) / n_seq * (int64_t)n_seq : 0;   // (blocks in equal shares)
+    p.tile_wgs = shares * c.n_kv * p.parts;
     // short sequences of a batch with longer ones go their own way
-    p.blocks = p.tile_wgs + (p.kind == 0 || n_seq > 1 ? (int64_t)n_seq * c.n_kv * p.parts : 0);
+    p.blocks = p.tile_wgs + (p.groups == 0 || n_seq > 1 ? (int64_t)n_seq * c.n_kv * p.parts : 0);
     p.work_bytes = p.parts > 1 ? (int64_t)p.parts * n_tok * n_head * (c.hd + 2) * 4 : 0;
     return p;
 }
@@ -144,7 +152,7 @@ hipError_t launch_attn_paged(AttnPgArgs a, const AttnPgPlan &p, void *work, hipS
 {
     a.tile_wgs = (int)p.tile_wgs;
     a.tile_blocks = p.tile_blocks;
-    a.short_rows = p.kind && a.n_seq > 1 ? kPgRows : 0;
+    a.short_rows = p.groups && a.n_seq > 1 ? kPgRows : 0;
     a.chunk = p.chunk;
     a.parts = p.parts;
     const int64_t rows = (int64_t)a.n_tok * a.n_head;

@@ -200,8 +200,8 @@ int check_work(const void *work, int64_t have, int64_t need, const char *fn)
 int plan_attention(const smx_paged_cache *c, int type, int n_tok, int n_head, int n_seq, int max_q, int max_len,
                    const smx_attention_rules *r, const char *fn, AttnPgPlan *p)
 {
-    *p = attn_paged_plan(c->view, elem_type(type), n_tok, n_head, n_seq, max_q < n_tok ? max_q : n_tok, max_len, window_of(r, max_len),
-                         r && r->prefix_dev);
+    *p = attn_paged_plan(c->view, elem_type(type), n_tok, n_head, n_seq, max_q < n_tok ? max_q : n_tok, max_len,
+                         window_of(r, max_len));
     if (p->blocks > kMaxBlocks) SMX_FAIL(SMX_EUNSUPPORTED, "%s: too many workgroups for one launch", fn);
     return SMX_OK;
 }

@@ -41,12 +41,12 @@ struct AttnPgArgs {
     int io;                      // PgType of q and out
     int tile_wgs, tile_blocks;   // workgroups (blocks of rows) of the many-row path; the rest take short sequences
     int short_rows;              // sequences of up to this many rows go the short way (0: none do)
-    int chunk, parts;            // tiles of a part; parts (1: the outputs are written at once)
+    int chunk, parts;            // tiles that a part has at least; parts (1: the outputs are written at once)
 };
 
 // How a call is cut up.
 struct AttnPgPlan {
-    int kind;                    // 0: every sequence is short; 1: blocks of 128 rows; 2: blocks of 256
+    int groups;                  // of four waves that share a block of 128 rows; 0: every sequence is short
     int chunk, parts, tile_blocks;
     int64_t tile_wgs, blocks;
     int64_t work_bytes;

@@ -49,17 +49,19 @@ __device__ __forceinline__ float sum_halves(float v)
 
 __device__ __forceinline__ int by_group(int id, double inv_group) { return (int)(((double)id + 0.5) * inv_group); }
 
-// 16 bytes per lane from g to LDS at l + 16 * lane
-__device__ __forceinline__ void to_lds(const void *g, void *l)
+// 16 bytes per lane from g + off (g the same in every lane) to LDS at l + 16 * lane
+__device__ __forceinline__ void to_lds(const uint8_t *g, uint32_t off, void *l)
 {
     const uint32_t la = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void *)l;
-    asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(g), "{m0}"(la) : "memory");
+    asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(g), "{m0}"(la) : "memory");
 }
-// The wave's loads have landed, its LDS reads are done.
-__device__ __forceinline__ void wait_all()
+// All but the wave's last N loads have landed, its LDS reads are done.
+template <int N>
+__device__ __forceinline__ void wait_loads()
 {
+    static_assert(N >= 0 && N < 64, "vmcnt has 6 bits");
     asm volatile("" ::: "memory");
-    __builtin_amdgcn_s_waitcnt(7 << 4);
+    __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | (7 << 4));
     asm volatile("" ::: "memory");
 }
 
@@ -100,11 +102,12 @@ __device__ __forceinline__ Range range_of(const AttnPgArgs &a, const Seq &s, int
     return r;
 }
 
-// A lane's row: what it sees are positions below pre, and those from lo to below hi.
+// A lane's row: a token at position t.  What it sees are positions below the sequence's pre, and those from lo to below hi.
 struct Row {
-    int token, head;
-    int t, lo, hi;
+    int token, head, t;
     bool valid;
+    __device__ __forceinline__ int lo(const AttnPgArgs &a) const { return a.window > 0 ? max(0, t - a.window + 1) : 0; }
+    __device__ __forceinline__ int hi(const Seq &s) const { return min(max(t + 1, 0), s.len); }
 };
 __device__ __forceinline__ Row row_of(const AttnPgArgs &a, const Seq &s, int kv_head, int id)
 {
@@ -114,41 +117,80 @@ __device__ __forceinline__ Row row_of(const AttnPgArgs &a, const Seq &s, int kv_
     r.token = s.start + tok;
     r.head = kv_head * a.group + i - tok * a.group;
     r.t = s.first + tok;
-    r.lo = a.window > 0 ? max(0, r.t - a.window + 1) : 0;
-    r.hi = min(max(r.t + 1, 0), s.len);
     return r;
 }
 
-// Rows of 16 positions, block `blk` of a sequence, in KV head h: the address, and whether the cache has the page.
+// Rows of 16 positions of a sequence in one KV head: the address, and whether the cache has the page.
 struct Rows16 {
     const uint8_t *p;
     bool there;
 };
-__device__ __forceinline__ Rows16 rows16(const AttnPgArgs &a, const Seq &s, int head, int blk)
-{
-    // (beyond the last position: its block again, which no table lacks)
-    const int j = max(min(blk, (s.len + kPgGroup - 1) / kPgGroup - 1), 0) * kPgGroup;
-    const int pg = ld_uniform(s.table + (j >> a.page_shift));
-    Rows16 r;
-    r.there = (unsigned)pg < (unsigned)a.c.n_pages;
-    r.p = a.c.k_row(r.there ? pg : 0, head, j & (a.c.page - 1));
-    return r;
-}
+
+// A wave's view of a sequence's page table: lane l has the page of the 16 positions 64 * win + l, and of those 64 further on, so
+// that a tile's pages are at hand when its rows are asked for.
+struct Pages {
+    int win, id, next;
+    uint64_t ok;           // which of them the cache has
+    int last;              // (beyond the last position: its page again, which no table lacks)
+    const uint8_t *base;   // of the KV head in page 0
+    uint32_t kb;           // from page to page
+
+    __device__ __forceinline__ int at(const AttnPgArgs &a, const Seq &s, int w) const
+    {
+        return s.table[(max(min(64 * w + (int)(threadIdx.x & 63), last), 0) * kPgGroup) >> a.page_shift];
+    }
+    __device__ __forceinline__ void check(const AttnPgArgs &a) { ok = __ballot((unsigned)id < (unsigned)a.c.n_pages); }
+    __device__ __forceinline__ Pages(const AttnPgArgs &a, const Seq &s, int head, int blk)
+    {
+        base = a.c.base + head * a.c.head_bytes();
+        kb = (uint32_t)(a.c.n_kv * (a.c.head_bytes() >> 10));
+        last = (s.len + kPgGroup - 1) / kPgGroup - 1;
+        win = blk >> 6;
+        id = at(a, s, win), next = at(a, s, win + 1);
+        check(a);
+    }
+    // block blk's window
+    __device__ __forceinline__ void go(const AttnPgArgs &a, const Seq &s, int blk)
+    {
+        const int w = blk >> 6;
+        if (w == win) return;
+        id = w == win + 1 ? next : at(a, s, w);
+        next = at(a, s, w + 1);
+        win = w;
+        check(a);
+    }
+    __device__ __forceinline__ Rows16 rows(const AttnPgArgs &a, int blk) const
+    {
+        Rows16 r;
+        r.there = ok >> (blk & 63) & 1;
+        const uint32_t pg = r.there ? __builtin_amdgcn_readlane(id, blk & 63) : 0;
+        r.p = base + (((uint64_t)pg * kb << 10) + (uint32_t)(((min(blk, last) * kPgGroup) & (a.c.page - 1)) * ROW));
+        return r;
+    }
+};
 
 // ---- operands --------------------------------------------------------------------------------------
 // Parts of a row of queries and of weights: 16-bit queries one, fp32 ones two of fp16 or three of bf16.
 template <bool F32> constexpr int kParts = F32 ? (BF16 ? 3 : 2) : 1;
 
+// Two values' parts, each the nearest to what the ones before leave.
 template <int NP>
-__device__ __forceinline__ void split(float f, elem (&p)[NP])
+__device__ __forceinline__ void split(float f, float g, elem2 (&p)[NP])
 {
-    p[0] = (elem)f;
-    if constexpr (NP > 1) {
-        const float r = f - (float)p[0];
-        p[1] = (elem)r;
-        if constexpr (NP > 2) p[2] = (elem)(r - (float)p[1]);
+    p[0] = elem2{(elem)f, (elem)g};
+    if constexpr (NP == 2) {
+        // what is left, exactly, the half read as fp16 by the same instruction (written as such, the compiler converts it first)
+        float a, b;
+        asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(a) : "v"(p[0]), "v"(f));
+        asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(b) : "v"(p[0]), "v"(g));
+        p[1] = elem2{(elem)a, (elem)b};
+    } else if constexpr (NP == 3) {
+        float a = f - (float)p[0][0], b = g - (float)p[0][1];
+        p[1] = elem2{(elem)a, (elem)b};
+        p[2] = elem2{(elem)(a - (float)p[1][0]), (elem)(b - (float)p[1][1])};
     }
 }
+static_assert(BF16 || kParts<true> == 2, "two parts are fp16");
 
 template <bool F32> struct Query {
     elem8 q[kParts<F32>][NK];
@@ -215,38 +257,31 @@ __device__ __forceinline__ void load_q(const AttnPgArgs &a, const Row &r, int h,
 #pragma unroll
         for (int n = 0; n < NK; n++)
 #pragma unroll
-            for (int e = 0; e < 8; e++) {
-                elem p[kParts<F32>];
-                split(f[n][e] * mul, p);
+            for (int e = 0; e < 8; e += 2) {
+                elem2 p[kParts<F32>];
+                split(f[n][e] * mul, f[n][e + 1] * mul, p);
 #pragma unroll
-                for (int k = 0; k < kParts<F32>; k++) Q.q[k][n][e] = p[k];
+                for (int k = 0; k < kParts<F32>; k++) Q.q[k][n][e] = p[k][0], Q.q[k][n][e + 1] = p[k][1];
             }
     }
 }
 
 // Where a lane finds its operands among rows in LDS.  K: row r = lane % 32 of 32, unit 2 n + h.  V^T: for dims
 // 32 d + lane % 32 the positions 4 h + .. and 8 + 4 h + .. of 16, each from an 8-byte piece that sixteen lanes transpose
-// between them.
-constexpr int KO = W % 64 == 0 ? 4 : 2;   // places after which pg_unit's turn of the units repeats
+// between them.  pg_unit's turn and a row's start leave the rest of a unit's number to be put in by one exclusive or.
 struct LaneAt {
-    uint32_t k[KO], v[2][2];
+    uint32_t k0, v0;
     __device__ __forceinline__ LaneAt(int lane)
     {
-        const int r = lane & 31, h = lane >> 5;
-#pragma unroll
-        for (int j = 0; j < KO; j++) k[j] = r * ROW + 16 * pg_unit(W, 2 * j + h, r);
-#pragma unroll
-        for (int p = 0; p < 2; p++)
-#pragma unroll
-            for (int j = 0; j < 2; j++) {
-                const int key = 8 * p + 4 * h + ((lane & 15) >> 2), u = 4 * j + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
-                v[p][j] = key * ROW + 16 * pg_unit(W, u, key) + 8 * (lane & 1);
-            }
+        const int r = lane & 31, h = lane >> 5, key = 4 * h + ((lane & 15) >> 2), u = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+        k0 = r * ROW + 16 * pg_unit(W, h, r);
+        v0 = key * ROW + 16 * pg_unit(W, u, key) + 8 * (lane & 1);
     }
     // of the 32 rows at `rows`, operand n
     __device__ __forceinline__ elem8 key(const uint8_t *rows, int n) const
     {
-        return *(const elem8 *)(rows + k[n % KO] + 32 * KO * (n / KO));
+        if constexpr (W % 64 == 0) return *(const elem8 *)(rows + (k0 ^ (32 * (n % 4))) + 128 * (n / 4));
+        else return *(const elem8 *)(rows + (k0 ^ (32 * (n % 2))) + 64 * (n / 2));
     }
     // of the 16 rows at `rows`, dims 32 d ..
     __device__ __forceinline__ elem8 val(const uint8_t *rows, int d) const
@@ -254,8 +289,11 @@ struct LaneAt {
         typedef short4v __attribute__((address_space(3))) *at;
         union { short4v s[2]; elem8 e; } r;
 #pragma unroll
-        for (int p = 0; p < 2; p++)
-            r.s[p] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((at)(rows + v[p][d % 2] + 128 * (d / 2)));
+        for (int p = 0; p < 2; p++) {
+            // (eight rows further on the turn is the same, or unit 2's)
+            const uint32_t o = W % 64 == 0 ? (v0 ^ (64 * (d % 2))) + 128 * (d / 2) : (v0 ^ (32 * p)) + 64 * d;
+            r.s[p] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((at)(rows + o + 8 * ROW * p));
+        }
         return r.e;
     }
 };
@@ -295,32 +333,52 @@ struct Shape {
 // Position (of 32) of a lane's element i.
 __device__ __forceinline__ int pos32(int i, int h) { return 8 * (i >> 2) + 4 * h + (i & 3); }
 
-// x of 32 positions from `at` on.
+// x of 32 positions from `at` on.  With 16-bit outputs tanh is 1 - 2 / (1 + e^2y), off by up to 2^-21 where the series keeps
+// small values to 2^-24 of themselves: 2^-21 of the cap in a score, which a weight's 8 or 11 bits do not notice, for 5
+// instructions in place of 19.
+template <bool F32>
 __device__ __forceinline__ void shape(const AttnPgArgs &a, const Shape &S, float16v &x, const Row &r, int at, int h)
 {
-    if (a.cap_in != 0.0f) {
+    const float away = (float)(r.t - at - 4 * h);   // (exact: positions are below 2^24)
+    if (!F32 && a.cap_in != 0.0f) {
+        const float in = S.in * 2.8853900817779268f;
 #pragma unroll
-        for (int i = 0; i < 16; i++) x[i] = tanh_of(x[i] * S.in) * a.cap_out;
+        for (int i = 0; i < 16; i++)
+            x[i] = __builtin_fmaf(__builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x[i] * in)), -2.0f * a.cap_out, a.cap_out);
+        if (a.slopes) {
+#pragma unroll
+            for (int i = 0; i < 16; i++) x[i] = __builtin_fmaf(-S.slope, fabsf(away - (float)pos32(i, 0)), x[i]);
+        }
+    } else if (F32 && a.cap_in != 0.0f) {
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+            x[i] = tanh_of(x[i] * S.in) * a.cap_out;
+            if ((i & 3) == 3) __builtin_amdgcn_sched_barrier(0);   // (four at a time: all at once take too many registers)
+        }
+        if (a.slopes) {
+#pragma unroll
+            for (int i = 0; i < 16; i++) x[i] = __builtin_fmaf(-S.slope, fabsf(away - (float)pos32(i, 0)), x[i]);
+        }
     } else {
 #pragma unroll
-        for (int i = 0; i < 16; i++) x[i] *= S.in;
-    }
-    if (a.slopes) {
-        const int away = r.t - at - 4 * h;
-#pragma unroll
-        for (int i = 0; i < 16; i++) x[i] = __builtin_fmaf(-S.slope, fabsf((float)(away - pos32(i, 0))), x[i]);
+        for (int i = 0; i < 16; i++) x[i] = __builtin_fmaf(x[i], S.in, -S.slope * fabsf(away - (float)pos32(i, 0)));
     }
 }
 
-// -inf where the row does not see: there[b]: the cache has the page of positions 16 b ..
-__device__ __forceinline__ void mask(float16v &x, const Row &r, int pre, int at, int h, bool there0, bool there1)
+// Of 32 positions from `at` on the row sees those whose bit is set, as a lane has them (its 16 in every second four).
+__device__ __forceinline__ uint32_t below(int n) { return n >= 32 ? 0xFFFFFFFFu : n <= 0 ? 0u : (1u << n) - 1u; }
+__device__ __forceinline__ uint32_t seen(const AttnPgArgs &a, const Seq &s, const Row &r, int at, int h, bool there0, bool there1)
 {
-    const int p0 = at + 4 * h;
+    const uint32_t m = below(s.pre - at) | (below(r.hi(s) - at) & ~below(r.lo(a) - at));
+    return (m & ((there0 ? 0xFFFFu : 0u) | (there1 ? 0xFFFF0000u : 0u))) >> (4 * h);
+}
+// -inf where it does not.
+__device__ __forceinline__ void mask(float16v &x, uint32_t m)
+{
 #pragma unroll
     for (int i = 0; i < 16; i++) {
-        const int p = p0 + pos32(i, 0);
-        const bool see = (p < pre || (p >= r.lo && p < r.hi)) && (i < 8 ? there0 : there1);
-        x[i] = see ? x[i] : kNegInf;
+        const uint32_t on = (uint32_t)__builtin_amdgcn_sbfe((int)m, pos32(i, 0), 1);   // all ones or none
+        x[i] = __uint_as_float((__float_as_uint(x[i]) & on) | (0xFF800000u & ~on));
     }
 }
 
@@ -336,8 +394,8 @@ __device__ __forceinline__ Bounds bounds_of(const AttnPgArgs &a, const Seq &s, i
     // (a later token's bounds are no lower)
     const Row first = row_of(a, s, 0, row0), last = row_of(a, s, 0, row0 + n - 1);
     Bounds b;
-    b.lo0 = __builtin_amdgcn_readfirstlane(first.lo), b.lo1 = __builtin_amdgcn_readfirstlane(last.lo);
-    b.hi0 = __builtin_amdgcn_readfirstlane(first.hi), b.hi1 = __builtin_amdgcn_readfirstlane(last.hi);
+    b.lo0 = __builtin_amdgcn_readfirstlane(first.lo(a)), b.lo1 = __builtin_amdgcn_readfirstlane(last.lo(a));
+    b.hi0 = __builtin_amdgcn_readfirstlane(first.hi(s)), b.hi1 = __builtin_amdgcn_readfirstlane(last.hi(s));
     return b;
 }
 

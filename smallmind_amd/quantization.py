@@ -738,7 +738,7 @@ class GpuPagedCache:
             b = ctypes.c_int64()
             extra = ()
             if name == "smx_attention_paged_work_bytes":
-                c = _lib.AttentionRulesC(0.0, 0.0, None, 16 if rules[1] else None, rules[0], 0)   # (asked whether there are prefixes)
+                c = _lib.AttentionRulesC(0.0, 0.0, None, None, rules[0], 0)
                 extra = (ctypes.byref(c),)
             call(name, self._handle(), *key, *extra, ctypes.byref(b))
             if len(self._work) >= 4096:
@@ -822,7 +822,7 @@ def attention_paged(q, cache: GpuPagedCache, starts, lens, tables, max_q: int, m
         if out is None:
             out = torch.empty(q.shape, dtype=q.dtype, device=cache.device)
         sums = torch.empty((n_tok, n_head), dtype=torch.float32, device=cache.device) if lse else None
-        need = cache._work_bytes("smx_attention_paged_work_bytes", (t, n_tok, n_head, n_seq, max_q, max_len), (window, prefix is not None))
+        need = cache._work_bytes("smx_attention_paged_work_bytes", (t, n_tok, n_head, n_seq, max_q, max_len), (window,))
         work = torch.empty(need, dtype=torch.uint8, device=cache.device) if need else None
         call("smx_attention_paged", h, t, q.data_ptr(), stride, out.data_ptr(), _opt(sums), n_tok, n_head, n_seq, starts.data_ptr(),
              lens.data_ptr(), tables.data_ptr(), tables.shape[1], max_q, max_len, ctypes.byref(rules), _opt(work), need,

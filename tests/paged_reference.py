@@ -68,8 +68,10 @@ class Scores:
     parts: an operand of fp32 queries is off by 2^-22 (F16 cache: two parts) or 2^-24 (BF16: three) of itself and, over F16,
     by 2^-38 of the row's largest; cache-typed ones are exact.  hd products per part are added in fp32, each sum within 2^-23 of
     what has been added (the matrix unit may truncate).  Three roundings turn a product into an exponent; a cap adds 2^-20
-    of the score (the exponential branch of tanh: its argument, the exponential, 1 - e next to 0.4, the reciprocal), a bias 4 roundings
-    of the larger of the two."""
+    of the score (the exponential branch of tanh: its argument, the exponential, 1 - e next to 0.4, the reciprocal) or, with
+    cache-typed outputs, 2^-21 of the cap (1 - 2 / (1 + f): f is off by 2^-23 and by |2 y| 2^-24 of itself, the
+    derivative 2 f / (1 + f)^2 is at most 1/2 and falls faster than |y| grows; the sum, the reciprocal (2^-23 of at most 1, twice) and the last
+    sum), a bias 4 roundings of the larger of the two."""
 
     def __init__(self, q, k, t, io, cache, scale=None, cap=0.0, slope=0.0):
         q, k = np.asarray(q, np.float64), np.asarray(k, np.float64)
@@ -87,7 +89,7 @@ class Scores:
             if cap:
                 cap = float(np.float32(cap))
                 s = cap * np.tanh(s / cap)
-                e = e + np.abs(s) * 2.0 ** -20
+                e = e + (cap * 2.0 ** -21 if parts == 1 else np.abs(s) * 2.0 ** -20)
             if slope:
                 bias = float(np.float32(slope)) * np.abs(t[:, None] - np.arange(k.shape[0]))
                 e = e + 4 * 2.0 ** -24 * (np.abs(s) + bias)
