@@ -285,7 +285,7 @@ __device__ __forceinline__ void many(const AttnPgArgs &a, Many<NG> &M, const Seq
     Query<F32> Q;
     load_q<F32>(a, r, h, Q);
     const Shape S(a, r, Q.unit);
-    const Bounds B = bounds_of(a, s, mine, kPgRows);
+    const Bounds B = bounds_of(a, s, row_of(a, s, 0, mine).t, row_of(a, s, 0, mine + kPgRows - 1).t);
     const LaneAt L(lane);
     Running R;
     const auto scores = [&](float16v (&x)[KT], const uint8_t *k, int t0) {
@@ -335,12 +335,12 @@ __device__ __forceinline__ void many(const AttnPgArgs &a, Many<NG> &M, const Seq
                 if (!AHEAD) scores(x, T.k[at], t0);
                 if (S.shaped) {
 #pragma unroll
-                    for (int t = 0; t < KT; t++) shape<F32>(a, S, x[t], r, pos + 32 * (t0 + t), h);
+                    for (int t = 0; t < KT; t++) shape<F32>(a, S, x[t], r.t, pos + 32 * (t0 + t), h);
                 }
                 if (cut) {
 #pragma unroll
                     for (int t = 0; t < KT; t++)
-                        mask(x[t], seen(a, s, r, pos + 32 * (t0 + t), h, th >> 2 * (t0 + t) & 1, th >> (2 * (t0 + t) + 1) & 1));
+                        mask(x[t], seen(a, s, r.t, pos + 32 * (t0 + t), h, th >> 2 * (t0 + t) & 1, th >> (2 * (t0 + t) + 1) & 1));
                 }
                 const float e = R.template refer<KT>(x, S.c);
                 // vector instructions of the softmax beside the matrix instructions: the first half's beside the next tile's scores,
@@ -452,7 +452,7 @@ __device__ __forceinline__ void few(const AttnPgArgs &a, Few<NW> &F, const Seq &
     Query<F32> Q;
     load_q<F32>(a, r, h, Q);
     const Shape S(a, r, Q.unit);
-    const Bounds B = bounds_of(a, s, 0, kPgRows);
+    const Bounds B = bounds_of(a, s, s.first, last.t);
     const LaneAt L(lane);
     Running R;
     int buf = 0;
@@ -472,8 +472,8 @@ __device__ __forceinline__ void few(const AttnPgArgs &a, Few<NW> &F, const Seq &
             for (int p = 0; p < kParts<F32>; p++) x[0] = mfma(k[n], Q.q[p][n], n || p ? x[0] : float16v(0.0f));
         if (more) fetch_k();
         if (B.none(s.pre, at, 32)) continue;
-        if (S.shaped) shape<F32>(a, S, x[0], r, at, h);
-        if (cut) mask(x[0], seen(a, s, r, at, h, th0, th1));
+        if (S.shaped) shape<F32>(a, S, x[0], r.t, at, h);
+        if (cut) mask(x[0], seen(a, s, r.t, at, h, th0, th1));
         elem8 w[kParts<F32>][2];
         const float e = R.refer<1>(x, S.c);
         R.weigh<kParts<F32>>(x[0], S.c, e, w);

@@ -174,11 +174,18 @@ hipError_t launch_attn_paged(AttnPgArgs a, const AttnPgPlan &p, void *work, hipS
 MassPgPlan attn_mass_plan(const PgView &c, int n_head, int n_seq, int max_q, int max_len)
 {
     MassPgPlan p{};
-    const int64_t rows = (int64_t)max_q * (n_head / c.n_kv);
-    const int64_t units = (int64_t)n_seq * c.n_kv * ((max_len + 127) / 128);
-    p.parts = (int)std::max<int64_t>(1, std::min((1024 + units - 1) / units, rows / 512));
+    const int64_t rows = (int64_t)max_q * (n_head / c.n_kv), pairs = (int64_t)n_seq * c.n_kv;
+    p.parts = 1;
+    p.few = rows <= kPgRows;
+    if (p.few) {
+        // positions of a pair over enough workgroups for four of each compute unit, 128 at a time
+        p.blocks = pairs * std::max<int64_t>(1, std::min<int64_t>((1024 + pairs - 1) / pairs, (max_len + 127) / 128));
+        return p;
+    }
+    const int64_t keys = c.w <= 128 ? 256 : 128, units = pairs * ((max_len + keys - 1) / keys);
+    p.parts = (int)std::max<int64_t>(1, std::min((2048 + units - 1) / units, rows / 512));
     p.blocks = units * p.parts;
-    p.work_bytes = p.parts > 1 ? (int64_t)p.parts * n_seq * c.n_kv * max_len * 4 : 0;
+    p.work_bytes = p.parts > 1 ? (int64_t)p.parts * pairs * max_len * 4 : 0;
     return p;
 }
 

@@ -4,10 +4,13 @@
 // Mathematics.  x' = x / sqrt(mean x^2 + eps) * gamma per head, then each pair (a, b) of channels becomes
 // (a cos - b sin, a sin + b cos) with the angle of the pair's axis, all in fp32, rounded once.  V is rounded and kept.
 //
-// Layout.  A lane holds 8 channels of a row; a row's lanes (a power of two of them) sum its squares by lane exchanges.  Where
-// pairs lie half a row apart, a lane reads its partners' channels itself (from the L1 they have just come to), which leaves
-// head_dim and the rotated width free of any rule on lanes.  A work item is one query row, or one K row with its V row:
-// whether V is finite decides what K holds.
+// Layout.  A lane holds 8 channels of a row; a row's lanes (a power of two of them) sum its squares by lane exchanges.  A wave
+// stays with one token, whose cosines and sines and the weights of the norms its lanes load once, and takes its rows in turn, the next
+// ones on their way from memory.  Where pairs lie half a row apart, a lane reads its partners' channels itself (from the
+// L1 they have just come to), which leaves head_dim and the rotated width free of any rule on lanes.  A work item is one
+// query row, or one K row with its V row: whether V is finite decides what K holds.
+#include <algorithm>
+
 #include "smx_device.h"
 #include "smx_internal.h"
 
@@ -19,22 +22,21 @@ template <int TYPE> struct Elem { typedef float type; };
 template <> struct Elem<PG_F16> { typedef _Float16 type; };
 template <> struct Elem<PG_BF16> { typedef __bf16 type; };
 
-// Eight consecutive values from element `at` on.
+template <int TYPE> using Elem8 = typename Elem<TYPE>::type __attribute__((ext_vector_type(8)));
+
+// Eight consecutive values from element `at` on, as they are.
 template <int TYPE>
-__device__ __forceinline__ void load8(float (&x)[8], const void *p, int64_t at, bool vec)
+__device__ __forceinline__ Elem8<TYPE> load8(const void *p, int64_t at, bool vec)
 {
-    typedef typename Elem<TYPE>::type E;
-    const E *e = (const E *)p + at;
+    const typename Elem<TYPE>::type *e = (const typename Elem<TYPE>::type *)p + at;
+    Elem8<TYPE> v;
     if (vec) {
-        typedef E E8 __attribute__((ext_vector_type(8)));
-        E8 v;
         __builtin_memcpy(&v, __builtin_assume_aligned(e, 16), sizeof(v));
-#pragma unroll
-        for (int i = 0; i < 8; i++) x[i] = (float)v[i];
     } else {
 #pragma unroll
-        for (int i = 0; i < 8; i++) x[i] = (float)e[i];
+        for (int i = 0; i < 8; i++) v[i] = e[i];
     }
+    return v;
 }
 
 template <typename E>
@@ -113,104 +115,184 @@ __device__ __forceinline__ void angles(const PgRotation &r, int n_tok, int t, in
     }
 }
 
-// This lane's channels d0 .. d0 + 7 of the row at `at` of p, normed and turned.  `on`: the lane has channels.
-template <int TYPE>
-__device__ __forceinline__ void turned(const PgWriteArgs &a, float (&y)[8], const void *p, int64_t at, int d0, int t,
-                                       const float *gamma, bool on)
+// The sum over a row's lanes, 1 << shift of them (they run together, whatever the wave's other rows do).
+__device__ __forceinline__ float row_sum(float v, int shift)
 {
-    float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-    if (on) load8<TYPE>(x, p, at + d0, a.vec);
-    float r = 1.0f;
-    if (gamma) {
-        float sq = 0.0f;
-#pragma unroll
-        for (int i = 0; i < 8; i++) sq = __builtin_fmaf(x[i], x[i], sq);
-        for (int o = (1 << a.group_shift) >> 1; o > 0; o >>= 1) sq += __shfl_xor(sq, o, 64);
-        r = 1.0f / sqrtf(sq / (float)a.hd + a.eps);
-    }
-#pragma unroll
-    for (int i = 0; i < 8; i++) y[i] = gamma && on ? x[i] * r * gamma[d0 + i] : x[i];
+    if (shift > 0) v += dpp_mov<0xB1>(v);
+    if (shift > 1) v += dpp_mov<0x4E>(v);
+    if (shift > 2) v += dpp_mov<0x141>(v);
+    if (shift > 3) v += dpp_mov<0x140>(v);
+    if (shift > 4) v += swap16_other(v);
+    return v;
+}
+
+// What a lane turns its channels with: y[i] c[i] + partner[i] s[i], the sign in s.
+struct Turn {
+    float c[8], s[8];
+    int on;      // how many of the eight are turned
+    int e0;      // first channel of the eight partners (halves, where these lie together)
+};
+
+__device__ __forceinline__ Turn turn_of(const PgWriteArgs &a, int d0)   // (the angles follow)
+{
+    Turn r;
+    r.on = min(max(2 * a.rot.half - d0, 0), 8);
+    r.e0 = d0 < a.rot.half ? d0 + a.rot.half : d0 - a.rot.half;
+    return r;
+}
+
+__device__ __forceinline__ void angles_of(const PgWriteArgs &a, Turn &r, int t, int d0)
+{
     const int half = a.rot.half;
-    if (!on || d0 >= 2 * half) return;
+    if (r.on == 0) return;
     if (!a.rot.halves) {
         float c[4], s[4];
         angles<4>(a.rot, a.n_tok, t, d0 >> 1, c, s);
 #pragma unroll
-        for (int i = 0; i < 8; i += 2) {
-            if (d0 + i >= 2 * half) break;
-            const float u = y[i], v = y[i + 1];
-            y[i] = u * c[i >> 1] - v * s[i >> 1];
-            y[i + 1] = u * s[i >> 1] + v * c[i >> 1];
-        }
-        return;
-    }
-    if ((half & 7) == 0) {   // the eight partners lie together
-        const bool low = d0 < half;
-        const int e0 = low ? d0 + half : d0 - half;
-        float z[8], c[8], s[8];
-        load8<TYPE>(z, p, at + e0, a.vec);
-        angles<8>(a.rot, a.n_tok, t, low ? d0 : e0, c, s);
+        for (int i = 0; i < 8; i++) r.c[i] = c[i >> 1], r.s[i] = i & 1 ? s[i >> 1] : -s[i >> 1];
+    } else if ((half & 7) == 0) {
+        float s[8];
+        angles<8>(a.rot, a.n_tok, t, min(d0, r.e0), r.c, s);
+#pragma unroll
+        for (int i = 0; i < 8; i++) r.s[i] = d0 < half ? -s[i] : s[i];
+    } else {
 #pragma unroll
         for (int i = 0; i < 8; i++) {
-            const float w = gamma ? z[i] * r * gamma[e0 + i] : z[i];
-            y[i] = low ? y[i] * c[i] - w * s[i] : w * s[i] + y[i] * c[i];
+            const int d = d0 + i;
+            float c[1], s[1];
+            angles<1>(a.rot, a.n_tok, t, d < half ? d : d - half, c, s);
+            r.c[i] = c[0], r.s[i] = d < half ? -s[0] : s[0];
+        }
+    }
+}
+
+// A row on its way: this lane's channels and their partners.
+template <int TYPE> struct Raw {
+    Elem8<TYPE> x, z;
+};
+
+template <int TYPE>
+__device__ __forceinline__ void fetch(const PgWriteArgs &a, const Turn &T, Raw<TYPE> &r, const void *p, int64_t at, int d0)
+{
+    r.x = load8<TYPE>(p, at + d0, a.vec);
+    if (T.on == 0 || !a.rot.halves) return;
+    if ((a.rot.half & 7) == 0) {
+        r.z = load8<TYPE>(p, at + T.e0, a.vec);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const int d = min(d0 + i, 2 * a.rot.half - 1);
+            r.z[i] = ((const typename Elem<TYPE>::type *)p)[at + (d < a.rot.half ? d + a.rot.half : d - a.rot.half)];
+        }
+    }
+}
+
+// The row normed and turned.  gamma: the norm's weights in LDS, head_dim of them and more.
+template <int TYPE>
+__device__ __forceinline__ void finish(const PgWriteArgs &a, const Turn &T, const float *gamma, const Raw<TYPE> &r, bool norm, int d0, float (&y)[8])
+{
+    float f = 1.0f;
+    if (norm) {
+        float sq = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; i++) sq = __builtin_fmaf((float)r.x[i], (float)r.x[i], sq);
+        sq = row_sum(sq, a.group_shift);
+        f = 1.0f / sqrtf(sq / (float)a.hd + a.eps);
+    }
+    float x[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) x[i] = norm ? (float)r.x[i] * f * gamma[d0 + i] : (float)r.x[i];
+    if (a.rot.halves && norm && (a.rot.half & 7) == 0) {
+        const int e0 = T.on ? T.e0 : 0;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const float w = (float)r.z[i] * f * gamma[e0 + i];
+            y[i] = i < T.on ? x[i] * T.c[i] + w * T.s[i] : x[i];
         }
         return;
     }
 #pragma unroll
     for (int i = 0; i < 8; i++) {
-        const int d = d0 + i;
-        if (d >= 2 * half) break;
-        const bool low = d < half;
-        const int e = low ? d + half : d - half;
-        float c[1], s[1];
-        angles<1>(a.rot, a.n_tok, t, low ? d : e, c, s);
-        const float z = (float)((const typename Elem<TYPE>::type *)p)[at + e];
-        const float w = gamma ? z * r * gamma[e] : z;
-        y[i] = low ? y[i] * c[0] - w * s[0] : w * s[0] + y[i] * c[0];
+        float w = x[i ^ 1];
+        if (a.rot.halves) {
+            const int d = min(d0 + i, 2 * a.rot.half - 1);
+            w = norm ? (float)r.z[i] * f * gamma[d < a.rot.half ? d + a.rot.half : d - a.rot.half] : (float)r.z[i];
+        }
+        y[i] = i < T.on ? x[i] * T.c[i] + w * T.s[i] : x[i];
     }
 }
 
-// An item is 1 << group_shift lanes; a.groups items per token: the query heads, then the KV heads.
+// A wave takes rows `part`, `part + splits` .. (64 >> group_shift at a time) of one token: the query heads, then the KV heads.
 template <int TYPE>
 __global__ __launch_bounds__(256) void k_paged_write(const PgWriteArgs a)
 {
-    const int lane = threadIdx.x & ((1 << a.group_shift) - 1);
-    const int64_t item = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> a.group_shift;
-    const int64_t tt = item / a.groups;
-    if (tt >= a.n_tok) return;           // (whole items: the lanes that exchange stay together)
-    const int t = (int)tt, g = (int)(item - tt * a.groups), d0 = lane * 8;
+    __shared__ __align__(16) float gamma[2][kPgMaxHead];
+    if ((int)threadIdx.x < a.hd) {
+        gamma[0][threadIdx.x] = a.q_gamma ? a.q_gamma[threadIdx.x] : 1.0f;
+        gamma[1][threadIdx.x] = a.k_gamma ? a.k_gamma[threadIdx.x] : 1.0f;
+    }
+    __syncthreads();
+    const int wave = __builtin_amdgcn_readfirstlane((int)(blockIdx.x * 4 + (threadIdx.x >> 6)));
+    const int t = wave / a.splits, part = wave - t * a.splits;
+    if (t >= a.n_tok) return;
+    const int rows = 64 >> a.group_shift, lane = threadIdx.x & ((1 << a.group_shift) - 1), sub = (threadIdx.x & 63) >> a.group_shift;
+    const int d0 = lane * 8, nq = a.q ? a.n_head : 0, items = nq + (a.k ? a.n_kv : 0);
     const bool on = d0 < a.hd;
-    const int nq = a.q ? a.n_head : 0;
-    float y[8];
-    if (g < nq) {
-        turned<TYPE>(a, y, a.q, t * a.q_stride + (int64_t)g * a.hd, d0, t, a.q_gamma, on);
-        if (on) store8(a.out_type, a.q_out, ((int64_t)t * a.n_head + g) * a.hd + d0, y, a.vec);
-        return;
+    const int place = a.c.base ? a.places[t] : 0;
+    const bool there = !a.c.base || (place >= 0 && place < a.c.n_pages * a.c.page);
+    Turn T = turn_of(a, on ? d0 : a.hd);
+
+    // two turns ahead
+    struct Row {
+        Raw<TYPE> r;
+        Elem8<TYPE> v;
+    } ahead[2] = {};
+    const auto load = [&](Row &w, int g) {
+        if (!on || g >= items) return;
+        if (g < nq) {
+            fetch<TYPE>(a, T, w.r, a.q, t * a.q_stride + (int64_t)g * a.hd, d0);
+        } else {
+            const int64_t h = (int64_t)(g - nq) * a.hd;
+            fetch<TYPE>(a, T, w.r, a.k, t * a.k_stride + h, d0);
+            if (a.c.base) w.v = load8<TYPE>(a.v, t * a.v_stride + h + d0, a.vec);
+        }
+    };
+    const int step = a.splits * rows, g0 = part * rows + sub;
+    load(ahead[0], g0);
+    load(ahead[1], g0 + step);
+    angles_of(a, T, t, d0);
+    for (int g = g0; g < items; g += step) {
+        const Raw<TYPE> cur = ahead[0].r;
+        const Elem8<TYPE> cv = ahead[0].v;
+        ahead[0] = ahead[1];
+        load(ahead[1], g + 2 * step);
+        float y[8];
+        if (g < nq) {
+            finish<TYPE>(a, T, gamma[0], cur, a.q_gamma, d0, y);
+            if (on) store8(a.out_type, a.q_out, ((int64_t)t * a.n_head + g) * a.hd + d0, y, a.vec);
+            continue;
+        }
+        const int head = g - nq;
+        finish<TYPE>(a, T, gamma[1], cur, a.k_gamma, d0, y);
+        if (!a.c.base) {
+            if (on) store8(a.out_type, a.k_out, ((int64_t)t * a.n_kv + head) * a.hd + d0, y, a.vec);
+            continue;
+        }
+        float w[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) w[i] = (float)cv[i];
+        Unit ku = rounded(a.c.bf16, y), vu = rounded(a.c.bf16, w);
+        const uint64_t bad = __ballot(on && (ku.bad || vu.bad)) >> (sub << a.group_shift);   // this row's lanes lowest
+        if (!on || !there) continue;
+        if (bad & ((UINT64_C(1) << (1 << a.group_shift)) - 1)) {
+            ku.u = make_uint4(0x7FFF7FFFu, 0x7FFF7FFFu, 0x7FFF7FFFu, 0x7FFF7FFFu);
+            vu.u = make_uint4(0, 0, 0, 0);
+        }
+        const int p = place & (a.c.page - 1);
+        uint8_t *row = a.c.k_row(place / a.c.page, head, p) + 16 * pg_unit(a.c.w, lane, p);
+        *(uint4 *)row = ku.u;
+        *(uint4 *)(row + a.c.v_off()) = vu.u;
     }
-    const int head = g - nq;
-    if (!a.c.base) {
-        turned<TYPE>(a, y, a.k, t * a.k_stride + (int64_t)head * a.hd, d0, t, a.k_gamma, on);
-        if (on) store8(a.out_type, a.k_out, ((int64_t)t * a.n_kv + head) * a.hd + d0, y, a.vec);
-        return;
-    }
-    const int place = a.places[t];
-    if (place < 0 || place >= a.c.n_pages * a.c.page) return;
-    float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-    if (on) load8<TYPE>(v, a.v, t * a.v_stride + (int64_t)head * a.hd + d0, a.vec);
-    turned<TYPE>(a, y, a.k, t * a.k_stride + (int64_t)head * a.hd, d0, t, a.k_gamma, on);
-    Unit ku = rounded(a.c.bf16, y), vu = rounded(a.c.bf16, v);
-    int bad = on && (ku.bad || vu.bad);
-    for (int o = (1 << a.group_shift) >> 1; o > 0; o >>= 1) bad |= __shfl_xor(bad, o, 64);
-    if (!on) return;
-    if (bad) {
-        ku.u = make_uint4(0x7FFF7FFFu, 0x7FFF7FFFu, 0x7FFF7FFFu, 0x7FFF7FFFu);
-        vu.u = make_uint4(0, 0, 0, 0);
-    }
-    const int r = place & (a.c.page - 1);
-    uint8_t *row = a.c.k_row(place / a.c.page, head, r) + 16 * pg_unit(a.c.w, lane, r);
-    *(uint4 *)row = ku.u;
-    *(uint4 *)(row + a.c.v_off()) = vu.u;
 }
 
 // Reads rows back: [n_tok][n_kv][hd] in the cache's type; zeros for places that it does not have, NaN for a position
@@ -242,8 +324,10 @@ hipError_t launch_paged_write(PgWriteArgs a, int in_type, hipStream_t s)
 {
     a.group_shift = 0;
     while ((8 << a.group_shift) < a.hd) a.group_shift++;
-    a.groups = (a.q ? a.n_head : 0) + (a.k ? a.n_kv : 0);
-    const unsigned blocks = (unsigned)((((int64_t)a.n_tok * a.groups << a.group_shift) + 255) / 256);
+    // a token's rows over several waves where tokens are fewer than what keeps the chip busy (16 waves a compute unit)
+    const int items = (a.q ? a.n_head : 0) + (a.k ? a.n_kv : 0), rows = 64 >> a.group_shift, turns = (items + rows - 1) / rows;
+    a.splits = std::max(1, std::min(turns, 4096 / a.n_tok));
+    const unsigned blocks = (unsigned)(((int64_t)a.n_tok * a.splits + 3) / 4);
     if (in_type == PG_F32) k_paged_write<PG_F32><<<blocks, 256, 0, s>>>(a);
     else if (in_type == PG_F16) k_paged_write<PG_F16><<<blocks, 256, 0, s>>>(a);
     else k_paged_write<PG_BF16><<<blocks, 256, 0, s>>>(a);

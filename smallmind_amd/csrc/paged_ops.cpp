@@ -102,8 +102,7 @@ int check_rows(int in_type, const void *q, int64_t q_stride, int n_head, const v
         (k_out && misaligned(k_out, out)) || misaligned(q_gamma, 4) || misaligned(k_gamma, 4))
         SMX_FAIL(SMX_EINVAL, "%s: misaligned pointer", fn);
     if (((q && q_gamma) || (k && k_gamma)) && !(eps >= 0.0f && eps < INFINITY)) SMX_FAIL(SMX_EINVAL, "%s: eps must be finite and not negative", fn);
-    const int64_t items = ((int64_t)(q ? n_head : 0) + (k ? n_kv : 0)) * n_tok;
-    if (items > kMaxBlocks * 8) SMX_FAIL(SMX_EUNSUPPORTED, "%s: %d tokens are too many for one launch", fn, n_tok);
+    if (n_tok > kMaxBlocks * 4) SMX_FAIL(SMX_EUNSUPPORTED, "%s: %d tokens are too many for one launch", fn, n_tok);
     a->q = q, a->k = k, a->v = v;
     a->q_stride = q_stride, a->k_stride = k_stride, a->v_stride = v_stride;
     a->q_gamma = q_gamma, a->k_gamma = k_gamma, a->eps = eps;

@@ -53,6 +53,7 @@ struct AttnPgPlan {
 };
 
 struct MassPgPlan {
+    bool few;                    // every sequence has up to 32 rows per KV head
     int parts;
     int64_t blocks, work_bytes;
 };

@@ -102,13 +102,14 @@ __device__ __forceinline__ Range range_of(const AttnPgArgs &a, const Seq &s, int
     return r;
 }
 
-// A lane's row: a token at position t.  What it sees are positions below the sequence's pre, and those from lo to below hi.
+// A lane's row: a token at position t.  What it sees are positions below the sequence's
+// pre, and those from lo_of to below hi_of.
 struct Row {
     int token, head, t;
     bool valid;
-    __device__ __forceinline__ int lo(const AttnPgArgs &a) const { return a.window > 0 ? max(0, t - a.window + 1) : 0; }
-    __device__ __forceinline__ int hi(const Seq &s) const { return min(max(t + 1, 0), s.len); }
 };
+__device__ __forceinline__ int lo_of(const AttnPgArgs &a, int t) { return a.window > 0 ? max(0, t - a.window + 1) : 0; }
+__device__ __forceinline__ int hi_of(const Seq &s, int t) { return min(max(t + 1, 0), s.len); }
 __device__ __forceinline__ Row row_of(const AttnPgArgs &a, const Seq &s, int kv_head, int id)
 {
     Row r;
@@ -321,6 +322,7 @@ struct Shape {
     float in;            // products to scores (shaped)
     float slope;
     bool shaped;
+    Shape() = default;
     __device__ __forceinline__ Shape(const AttnPgArgs &a, const Row &r, float unit)
     {
         shaped = a.cap_in != 0.0f || a.slopes;
@@ -337,9 +339,9 @@ __device__ __forceinline__ int pos32(int i, int h) { return 8 * (i >> 2) + 4 * h
 // small values to 2^-24 of themselves: 2^-21 of the cap in a score, which a weight's 8 or 11 bits do not notice, for 5
 // instructions in place of 19.
 template <bool F32>
-__device__ __forceinline__ void shape(const AttnPgArgs &a, const Shape &S, float16v &x, const Row &r, int at, int h)
+__device__ __forceinline__ void shape(const AttnPgArgs &a, const Shape &S, float16v &x, int t, int at, int h)
 {
-    const float away = (float)(r.t - at - 4 * h);   // (exact: positions are below 2^24)
+    const float away = (float)(t - at - 4 * h);   // (exact: positions are below 2^24)
     if (!F32 && a.cap_in != 0.0f) {
         const float in = S.in * 2.8853900817779268f;
 #pragma unroll
@@ -365,11 +367,11 @@ __device__ __forceinline__ void shape(const AttnPgArgs &a, const Shape &S, float
     }
 }
 
-// Of 32 positions from `at` on the row sees those whose bit is set, as a lane has them (its 16 in every second four).
+// Of 32 positions from `at` on the row at t sees those whose bit is set, as a lane has them (its 16 in every second four).
 __device__ __forceinline__ uint32_t below(int n) { return n >= 32 ? 0xFFFFFFFFu : n <= 0 ? 0u : (1u << n) - 1u; }
-__device__ __forceinline__ uint32_t seen(const AttnPgArgs &a, const Seq &s, const Row &r, int at, int h, bool there0, bool there1)
+__device__ __forceinline__ uint32_t seen(const AttnPgArgs &a, const Seq &s, int t, int at, int h, bool there0, bool there1)
 {
-    const uint32_t m = below(s.pre - at) | (below(r.hi(s) - at) & ~below(r.lo(a) - at));
+    const uint32_t m = below(s.pre - at) | (below(hi_of(s, t) - at) & ~below(lo_of(a, t) - at));
     return (m & ((there0 ? 0xFFFFu : 0u) | (there1 ? 0xFFFF0000u : 0u))) >> (4 * h);
 }
 // -inf where it does not.
@@ -389,14 +391,10 @@ struct Bounds {
     __device__ __forceinline__ bool whole(int pre, int at, int n) const { return at + n <= pre || (at >= lo1 && at + n <= hi0); }
     __device__ __forceinline__ bool none(int pre, int at, int n) const { return at >= pre && (at >= hi1 || at + n <= lo0); }
 };
-__device__ __forceinline__ Bounds bounds_of(const AttnPgArgs &a, const Seq &s, int row0, int n)
+__device__ __forceinline__ Bounds bounds_of(const AttnPgArgs &a, const Seq &s, int t0, int t1)   // the first row's t, the last one's
 {
-    // (a later token's bounds are no lower)
-    const Row first = row_of(a, s, 0, row0), last = row_of(a, s, 0, row0 + n - 1);
-    Bounds b;
-    b.lo0 = __builtin_amdgcn_readfirstlane(first.lo(a)), b.lo1 = __builtin_amdgcn_readfirstlane(last.lo(a));
-    b.hi0 = __builtin_amdgcn_readfirstlane(first.hi(s)), b.hi1 = __builtin_amdgcn_readfirstlane(last.hi(s));
-    return b;
+    t0 = __builtin_amdgcn_readfirstlane(t0), t1 = __builtin_amdgcn_readfirstlane(t1);
+    return Bounds{lo_of(a, t0), lo_of(a, t1), hi_of(s, t0), hi_of(s, t1)};   // (a later token's are no lower)
 }
 
 }  // namespace

@@ -68,7 +68,7 @@ struct PgWriteArgs {
     int n_tok, n_head, n_kv, hd;
     int out_type;                 // of q_out and k_out
     int vec;                      // rows can be read and written 16 bytes at a time
-    int groups, group_shift;      // work items of a token; log2 of the lanes of a row
+    int splits, group_shift;      // waves that share a token's rows; log2 of the lanes of a row
 };
 
 // Arguments of the eviction (k_paged_evict.hip).
