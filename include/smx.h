@@ -340,8 +340,8 @@ typedef struct smx_attention_rules {
  * NULL; only the window counts). */
 SMX_API int smx_attention_paged_work_bytes(const smx_paged_cache *c, int type, int n_tok, int n_head, int n_seq, int max_q,
                                            int max_len, const smx_attention_rules *rules, int64_t *bytes);
-SMX_API int smx_attention_mass_work_bytes(const smx_paged_cache *c, int n_head, int n_seq, int max_q, int max_len,
-                                          int64_t *bytes);
+SMX_API int smx_attention_mass_work_bytes(const smx_paged_cache *c, int type, int n_head, int n_seq, int max_q,
+                                          int max_len, int64_t *bytes);
 /* Attention of new tokens of n_seq sequences over the cache (MultiHeadAttention.cs:676-844 with the exponential itself in place of
  * FastExp).  Sequence b's new tokens are rows starts_dev[b] .. starts_dev[b + 1] - 1 of the batch (starts do not
  * decrease; at most max_q each, or what lies beyond is undefined; none: nothing to do), and the last of its lens_dev[b]

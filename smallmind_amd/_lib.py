@@ -160,7 +160,7 @@ def load() -> ctypes.CDLL:
         "smx_paged_append": (i32, [vp, i32, vp, i64, i32, vp, i64, vp, i64, vp, vp, f32, vp, vp, vp, i32, i32, vp, vp]),
         "smx_paged_read": (i32, [vp, vp, i32, vp, vp, vp]),
         "smx_attention_paged_work_bytes": (i32, [vp, i32, i32, i32, i32, i32, i32, vp, ctypes.POINTER(i64)]),
-        "smx_attention_mass_work_bytes": (i32, [vp, i32, i32, i32, i32, ctypes.POINTER(i64)]),
+        "smx_attention_mass_work_bytes": (i32, [vp, i32, i32, i32, i32, i32, ctypes.POINTER(i64)]),
         "smx_attention_paged": (i32, [vp, i32, vp, i64, vp, vp, i32, i32, i32, vp, vp, vp, i32, i32, i32, vp, vp, i64, vp]),
         "smx_attention_mass": (i32, [vp, i32, vp, i64, vp, vp, i64, i32, vp, i32, i32, i32, vp, vp, vp, i32, i32, i32, vp, vp,
                                      i64, vp]),

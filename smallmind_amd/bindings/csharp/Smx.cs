@@ -143,7 +143,7 @@ namespace SmallMind.Backends.Rocm
             IntPtr stream);
         [DllImport(Lib)] public static extern int smx_attention_paged_work_bytes(IntPtr cache, int type, int nTok, int nHead,
             int nSeq, int maxQ, int maxLen, IntPtr rules, out long bytes);
-        [DllImport(Lib)] public static extern int smx_attention_mass_work_bytes(IntPtr cache, int nHead, int nSeq, int maxQ,
+        [DllImport(Lib)] public static extern int smx_attention_mass_work_bytes(IntPtr cache, int type, int nHead, int nSeq, int maxQ,
             int maxLen, out long bytes);
         [DllImport(Lib)] public static extern int smx_attention_paged(IntPtr cache, int type, void* qDev, long qStride,
             void* outDev, float* lseDev, int nTok, int nHead, int nSeq, int* startsDev, int* lensDev, int* tablesDev,

@@ -20,33 +20,46 @@ constexpr int kWaves = 4;
 constexpr int KT = W <= 128 ? 2 : 1;      // 32-position groups of a wave (many rows)
 constexpr int kKeys = 32 * KT * kWaves;   // positions of a workgroup
 
-// The sum over a row of lanes' first n columns (at least; the others hold 0).
-__device__ __forceinline__ float sum_columns(float v, int n)
+// The sums over a wave's 32 columns, element i's in lanes 32 h + i and 32 h + 16 + i: every exchange halves the elements that a lane
+// still adds up, keeping those whose number has the lane's bit (48 instructions; sixteen sums one by one, 112).
+__device__ __forceinline__ float pick(uint32_t m, float a, float b)   // m all ones: a, 0: b
 {
-    if (n > 1) v += dpp_mov<0xB1>(v);
-    if (n > 2) v += dpp_mov<0x4E>(v);
-    if (n > 4) v += dpp_mov<0x141>(v);
-    if (n > 8) v += dpp_mov<0x140>(v);
-    if (n > 16) v += swap16_other(v);
-    return v;
+    return __uint_as_float((__float_as_uint(a) & m) | (__float_as_uint(b) & ~m));
+}
+__device__ __forceinline__ float sum_columns(const float16v &x, int lane)
+{
+    const uint32_t m8 = -(uint32_t)(lane >> 3 & 1), m4 = -(uint32_t)(lane >> 2 & 1), m2 = -(uint32_t)(lane >> 1 & 1), m1 = -(uint32_t)(lane & 1);
+    float v[8], w[4], z[2];
+#pragma unroll
+    for (int i = 0; i < 8; i++) v[i] = pick(m8, x[i + 8], x[i]) + dpp_mov<0x128>(pick(m8, x[i], x[i + 8]));   // from lane ^ 8
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const int lo = i + (i & 2);   // 0 1 4 5
+        w[i] = pick(m2, v[lo + 2], v[lo]) + dpp_mov<0x4E>(pick(m2, v[lo], v[lo + 2]));                        // lane ^ 2
+    }
+#pragma unroll
+    for (int i = 0; i < 2; i++) z[i] = pick(m1, w[2 * i + 1], w[2 * i]) + dpp_mov<0xB1>(pick(m1, w[2 * i], w[2 * i + 1]));   // lane ^ 1
+    const float r = pick(m4, z[1], z[0]) + __shfl_xor(pick(m4, z[0], z[1]), 4, 64);
+    return r + swap16_other(r);
 }
 
-// What the positions of 32 from `at` on have received, in the first lane of each half.
-__device__ __forceinline__ void give(const AttnPgArgs &a, const Seq &s, int pair, int part, int at, int h, const float16v &sum)
-{
-    const int64_t row = (int64_t)pair * a.max_len, pairs = (int64_t)a.n_seq * a.c.n_kv;
-#pragma unroll
-    for (int i = 0; i < 16; i++) {
-        const int p = at + pos32(i, h);
-        if (p >= a.max_len) continue;
-        if (a.mass_parts > 1) {
-            a.mass_part[part * pairs * a.max_len + row + p] = sum[i];
-            continue;
-        }
-        const float was = a.mass && p < a.mass_width ? a.mass[pair * a.mass_stride + p] : 0.0f;
-        a.mass_out[row + p] = p < s.len ? was + sum[i] : 0.0f;
+// What the positions of 32 from `at` on have received, as sum_columns leaves it.
+struct Giving {
+    int p;
+    float was;
+    __device__ __forceinline__ Giving(const AttnPgArgs &a, int pair, int at, int lane)   // (asked early: what there was is on its way)
+    {
+        p = lane & 16 ? a.max_len : at + pos32(lane & 15, lane >> 5);
+        was = a.mass_parts == 1 && a.mass && p < a.mass_width && p < a.max_len ? a.mass[pair * a.mass_stride + p] : 0.0f;
     }
-}
+    __device__ __forceinline__ void give(const AttnPgArgs &a, const Seq &s, int pair, int part, float v) const
+    {
+        if (p >= a.max_len) return;
+        const int64_t at = (int64_t)pair * a.max_len + p;
+        if (a.mass_parts > 1) a.mass_part[(int64_t)part * a.n_seq * a.c.n_kv * a.max_len + at] = v;
+        else a.mass_out[at] = p < s.len ? was + v : 0.0f;
+    }
+};
 
 // K of 32 positions from `at` on as operands.
 __device__ __forceinline__ void load_k(const AttnPgArgs &a, const Seq &s, Pages &P, int at, int lane, elem8 (&k)[NK], bool &there0, bool &there1)
@@ -59,10 +72,9 @@ __device__ __forceinline__ void load_k(const AttnPgArgs &a, const Seq &s, Pages 
     there0 = r0.there, there1 = r1.there;
 }
 
-// What a row's products become a weight with: the shape of its scores, and lse as an exponent of 2.
-__device__ __forceinline__ float lse_of(const AttnPgArgs &a, const Row &r)
+// lse of a row as an exponent of 2: l is what the table has.
+__device__ __forceinline__ float lse_of(const Row &r, float l)
 {
-    const float l = a.lse_in[(int64_t)r.token * a.n_head + r.head];
     // (a row that sees nothing has -inf; one past the last repeats that one and counts for nothing)
     return !r.valid ? __builtin_huge_valf() : l == -__builtin_huge_valf() ? 0.0f : l * 1.4426950408889634f;
 }
@@ -85,17 +97,19 @@ __global__ __launch_bounds__(kWaves * 64) void k_attn_mass_few(const AttnPgArgs 
         Pages P(a, s, head, at / kPgGroup);
         load_k(a, s, P, at, lane, k[0], there[0][0], there[0][1]);
         const Row r = row_of(a, s, head, lane & 31);
-        const float lse = lse_of(a, r);
+        const float lse = lse_of(r, a.lse_in[(int64_t)r.token * a.n_head + r.head]);
         Query<F32> Q;
-        load_q<F32>(a, r, h, Q);
-        const Shape S(a, r, Q.unit);
+        load_q<F32, false>(a, r, h, Q);   // (a row that is not finite has an lse of NaN)
+        const Shape S(a, a.slopes ? a.slopes[r.head] : 0.0f, Q.unit);
         const Bounds B = bounds_of(a, s, s.first, row_of(a, s, head, s.rows - 1).t);
         const auto go = [&](const elem8 (&kk)[NK], bool th0, bool th1, elem8 (&next)[NK], bool (&th)[2]) {
+            const Giving G(a, pair, at, lane);
             if (at + step < s.len) load_k(a, s, P, at + step, lane, next, th[0], th[1]);
-            float16v x;
+            float sum;
             if (B.none(s.pre, at, 32)) {
-                x = float16v(0.0f);
+                sum = 0.0f;
             } else {
+                float16v x;
 #pragma unroll
                 for (int n = 0; n < NK; n++)
 #pragma unroll
@@ -103,9 +117,10 @@ __global__ __launch_bounds__(kWaves * 64) void k_attn_mass_few(const AttnPgArgs 
                 if (S.shaped) shape<true>(a, S, x, r.t, at, h);   // (the sums are fp32 whatever the queries)
                 if (!th0 || !th1 || !B.whole(s.pre, at, 32)) mask(x, seen(a, s, r.t, at, h, th0, th1));
 #pragma unroll
-                for (int i = 0; i < 16; i++) x[i] = sum_columns(__builtin_amdgcn_exp2f(__builtin_fmaf(x[i], S.c, -lse)), s.rows);
+                for (int i = 0; i < 16; i++) x[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i], S.c, -lse));
+                sum = sum_columns(x, lane);
             }
-            if ((lane & 31) == 0) give(a, s, pair, 0, at, h, x);
+            G.give(a, s, pair, 0, sum);
             at += step;
         };
         while (at < s.len) {
@@ -114,8 +129,7 @@ __global__ __launch_bounds__(kWaves * 64) void k_attn_mass_few(const AttnPgArgs 
         }
     }
     // positions that nobody sees: what they had, 0 beyond the sequence
-    for (; at < a.max_len; at += step)
-        if ((lane & 31) == 0) give(a, s, pair, 0, at, h, float16v(0.0f));
+    for (; at < a.max_len; at += step) Giving(a, pair, at, lane).give(a, s, pair, 0, 0.0f);
 }
 
 // ---- many rows ---------------------------------------------------------------------------------------
@@ -132,6 +146,8 @@ template <bool F32>
 __global__ __launch_bounds__(kWaves * 64) void k_attn_mass(const AttnPgArgs a)
 {
     constexpr int NB = kBlocks<F32>, NP = kParts<F32>;
+    constexpr bool FAST = NB == 4;   // (with fewer, registers are short)
+    const bool shaped = a.cap_in != 0.0f || a.slopes;
     __shared__ Stage<F32> M;
     const int lane = threadIdx.x & 63, h = lane >> 5, wave = wave_id();
     const int pairs = a.n_seq * a.c.n_kv, pair = blockIdx.x % pairs, rest = blockIdx.x / pairs;
@@ -145,8 +161,8 @@ __global__ __launch_bounds__(kWaves * 64) void k_attn_mass(const AttnPgArgs a)
         t_lo = max(0, k0 - s.first);
         if (a.window > 0) t_hi = (int)min((int64_t)t_hi, max((int64_t)0, (int64_t)k0 + kKeys - 1 + a.window - s.first));
     }
-    const int first = t_lo * a.group, blocks = k0 < s.len ? max(0, (t_hi * a.group - first + 32 * NB - 1) / (32 * NB)) : 0;
-    const int per = (blocks + a.mass_parts - 1) / a.mass_parts, s0 = part * per, s1 = min(blocks, s0 + per);
+    const int first = t_lo * a.group, blocks = k0 < s.len ? max(0, (t_hi * a.group - first + 32 * NB - 1) / (32 * NB)) : 0;   // of NB * 32 rows
+    const int s0 = part * a.mass_per, s1 = min(blocks, s0 + a.mass_per);
     float16v sum[KT];
 #pragma unroll
     for (int t = 0; t < KT; t++) sum[t] = float16v(0.0f);
@@ -160,14 +176,17 @@ __global__ __launch_bounds__(kWaves * 64) void k_attn_mass(const AttnPgArgs a)
             all = all && there[t][0] && there[t][1];
         }
         Query<F32> Q;
-        float lse = 0.0f;
+        float lse = 0.0f, slope = 0.0f;   // as loaded: nothing here is to wait for what has just been asked for
         Row r{};
         const auto fetch = [&](int st) {
             r = row_of(a, s, head, first + (st * NB + wave) * 32 + (lane & 31));
-            load_q<F32>(a, r, h, Q);
-            lse = lse_of(a, r);
+            load_q<F32, false>(a, r, h, Q);   // (a row that is not finite has an lse of NaN)
+            lse = a.lse_in[(int64_t)r.token * a.n_head + r.head];
+            if (a.slopes) slope = a.slopes[r.head];
         };
         if (wave < NB) fetch(s0);
+        // K has landed: otherwise the compiler, which does not know, has every turn wait for the rows just asked for
+        wait_loads<0>();
         for (int st = s0; st < s1; st++) {
             __syncthreads();   // the rows before have been read
             if (wave < NB) {
@@ -176,23 +195,15 @@ __global__ __launch_bounds__(kWaves * 64) void k_attn_mass(const AttnPgArgs a)
 #pragma unroll
                     for (int n = 0; n < NK; n++) M.q[wave][q][n][lane] = Q.q[q][n];
                 if (h == 0) {
-                    const Shape S(a, r, Q.unit);
-                    M.in[wave][lane] = S.in, M.slope[wave][lane] = S.slope, M.lse[wave][lane] = lse, M.t[wave][lane] = r.t;
+                    const Shape S(a, slope, Q.unit);
+                    M.in[wave][lane] = S.in, M.slope[wave][lane] = S.slope, M.lse[wave][lane] = lse_of(r, lse), M.t[wave][lane] = r.t;
                 }
             }
             __syncthreads();
             if (wave < NB && st + 1 < s1) fetch(st + 1);
-            const int row0 = first + st * 32 * NB;
-            for (int j = 0; j < NB; j++) {
-                if (row0 + 32 * j >= s.rows) break;
-                const int c = lane & 31, t = M.t[j][c];
-                const Bounds B = bounds_of(a, s, t, __builtin_amdgcn_readlane(t, 31));
-                if (at >= s.len || B.none(s.pre, at, 32 * KT)) continue;
-                Shape S;
-                S.shaped = a.cap_in != 0.0f || a.slopes;
-                S.in = M.in[j][c], S.slope = M.slope[j][c], S.c = S.shaped ? 1.0f : S.in;
-                const float l = M.lse[j][c];
-                float16v x[KT];
+            const int row0 = first + st * 32 * NB, c = lane & 31;
+            if (at >= s.len) continue;
+            const auto scores = [&](float16v (&x)[KT], int j) {
 #pragma unroll
                 for (int n = 0; n < NK; n++)
 #pragma unroll
@@ -201,7 +212,48 @@ __global__ __launch_bounds__(kWaves * 64) void k_attn_mass(const AttnPgArgs a)
 #pragma unroll
                         for (int u = 0; u < KT; u++) x[u] = mfma(k[u][n], qq, n || q ? x[u] : float16v(0.0f));
                     }
-                if (S.shaped) {
+            };
+            const auto add = [&](const float16v (&x)[KT], float by, float l) {
+#pragma unroll
+                for (int u = 0; u < KT; u++)
+#pragma unroll
+                    for (int i = 0; i < 16; i++) sum[u][i] += __builtin_amdgcn_exp2f(__builtin_fmaf(x[u][i], by, -l));
+            };
+            if constexpr (FAST) {
+                // every row sees all of the wave's positions: no bounds to look at, and the next rows' scores beside these ones' weights
+                const Bounds B = bounds_of(a, s, M.t[0][0], M.t[NB - 1][31]);
+                if (!shaped && all && row0 + 32 * NB <= s.rows && B.whole(s.pre, at, 32 * KT)) {
+                    float16v x[2][KT];
+                    scores(x[0], 0);
+#pragma unroll
+                    for (int j = 0; j < NB; j++) {
+                        __builtin_amdgcn_sched_barrier(0);
+                        if (j + 1 < NB) scores(x[(j + 1) & 1], j + 1);
+                        add(x[j & 1], M.in[j][c], M.lse[j][c]);
+                        constexpr int MK = NK * NP * KT, E = 16 * KT;   // matrix instructions, elements
+                        __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+#pragma unroll
+                        for (int i = 0; i < MK; i++) {
+                            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                            if (i % KT == 0) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+                            __builtin_amdgcn_sched_group_barrier(0x002, (2 * E + MK - 1) / MK, 0);
+                            __builtin_amdgcn_sched_group_barrier(0x400, (E + MK - 1) / MK, 0);
+                        }
+                    }
+                    continue;
+                }
+            }
+            for (int j = 0; j < NB; j++) {
+                if (row0 + 32 * j >= s.rows) break;
+                const int t = M.t[j][c];
+                const Bounds B = bounds_of(a, s, t, __builtin_amdgcn_readlane(t, 31));
+                if (B.none(s.pre, at, 32 * KT)) continue;
+                Shape S;
+                S.shaped = shaped;
+                S.in = M.in[j][c], S.slope = M.slope[j][c], S.c = shaped ? 1.0f : S.in;
+                float16v x[KT];
+                scores(x, j);
+                if (shaped) {
 #pragma unroll
                     for (int u = 0; u < KT; u++) shape<true>(a, S, x[u], t, at + 32 * u, h);   // (the sums are fp32 whatever the queries)
                 }
@@ -209,19 +261,12 @@ __global__ __launch_bounds__(kWaves * 64) void k_attn_mass(const AttnPgArgs a)
 #pragma unroll
                     for (int u = 0; u < KT; u++) mask(x[u], seen(a, s, t, at + 32 * u, h, there[u][0], there[u][1]));
                 }
-#pragma unroll
-                for (int u = 0; u < KT; u++)
-#pragma unroll
-                    for (int i = 0; i < 16; i++) sum[u][i] += __builtin_amdgcn_exp2f(__builtin_fmaf(x[u][i], S.c, -l));
+                add(x, S.c, M.lse[j][c]);
             }
         }
     }
 #pragma unroll
-    for (int u = 0; u < KT; u++) {
-#pragma unroll
-        for (int i = 0; i < 16; i++) sum[u][i] = sum_columns(sum[u][i], 32);
-        if ((lane & 31) == 0) give(a, s, pair, part, at + 32 * u, h, sum[u]);
-    }
+    for (int u = 0; u < KT; u++) Giving(a, pair, at + 32 * u, lane).give(a, s, pair, part, sum_columns(sum[u], lane));
 }
 
 }  // namespace

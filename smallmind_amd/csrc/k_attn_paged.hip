@@ -284,7 +284,7 @@ __device__ __forceinline__ void many(const AttnPgArgs &a, Many<NG> &M, const Seq
     if (AHEAD && mine0 + NG < i1) bring_k(mine0 + NG, 1, 4);
     Query<F32> Q;
     load_q<F32>(a, r, h, Q);
-    const Shape S(a, r, Q.unit);
+    const Shape S(a, a.slopes ? a.slopes[r.head] : 0.0f, Q.unit);
     const Bounds B = bounds_of(a, s, row_of(a, s, 0, mine).t, row_of(a, s, 0, mine + kPgRows - 1).t);
     const LaneAt L(lane);
     Running R;
@@ -451,7 +451,7 @@ __device__ __forceinline__ void few(const AttnPgArgs &a, Few<NW> &F, const Seq &
     }
     Query<F32> Q;
     load_q<F32>(a, r, h, Q);
-    const Shape S(a, r, Q.unit);
+    const Shape S(a, a.slopes ? a.slopes[r.head] : 0.0f, Q.unit);
     const Bounds B = bounds_of(a, s, s.first, last.t);
     const LaneAt L(lane);
     Running R;

@@ -171,7 +171,14 @@ hipError_t launch_attn_paged(AttnPgArgs a, const AttnPgPlan &p, void *work, hipS
     return hipGetLastError();
 }
 
-MassPgPlan attn_mass_plan(const PgView &c, int n_head, int n_seq, int max_q, int max_len)
+// Row blocks that k_attn_mass lays out at a time.
+static int attn_mass_blocks(const PgView &c, int io)
+{
+    const int parts = io != PG_F32 ? 1 : c.bf16 ? 3 : 2;
+    return parts * c.w <= 256 ? 4 : parts * c.w <= 512 ? 2 : 1;
+}
+
+MassPgPlan attn_mass_plan(const PgView &c, int io, int n_head, int n_seq, int max_q, int max_len)
 {
     MassPgPlan p{};
     const int64_t rows = (int64_t)max_q * (n_head / c.n_kv), pairs = (int64_t)n_seq * c.n_kv;
@@ -179,11 +186,16 @@ MassPgPlan attn_mass_plan(const PgView &c, int n_head, int n_seq, int max_q, int
     p.few = rows <= kPgRows;
     if (p.few) {
         // positions of a pair over enough workgroups for four of each compute unit, 128 at a time
-        p.blocks = pairs * std::max<int64_t>(1, std::min<int64_t>((1024 + pairs - 1) / pairs, (max_len + 127) / 128));
+        p.blocks = pairs * std::max<int64_t>(1, std::min<int64_t>((512 + pairs - 1) / pairs, (max_len + 127) / 128));
         return p;
     }
     const int64_t keys = c.w <= 128 ? 256 : 128, units = pairs * ((max_len + keys - 1) / keys);
-    p.parts = (int)std::max<int64_t>(1, std::min((2048 + units - 1) / units, rows / 512));
+    // parts of 1024 rows: equal work, however many rows a position is seen by (4095 tokens, 32 heads of 128: 121 us, as with
+    // 768 and 1536; 2048 and more leave the chip to the longest)
+    const int nb = attn_mass_blocks(c, io);
+    const int64_t blocks = (rows + 32 * nb - 1) / (32 * nb);
+    p.per = 32 / nb;
+    p.parts = (int)((blocks + p.per - 1) / p.per);
     p.blocks = units * p.parts;
     p.work_bytes = p.parts > 1 ? (int64_t)p.parts * pairs * max_len * 4 : 0;
     return p;
@@ -192,6 +204,7 @@ MassPgPlan attn_mass_plan(const PgView &c, int n_head, int n_seq, int max_q, int
 hipError_t launch_attn_mass(AttnPgArgs a, const MassPgPlan &p, void *work, hipStream_t s)
 {
     a.mass_parts = p.parts;
+    a.mass_per = p.per;
     a.mass_part = (float *)work;
     hipError_t e = hipErrorInvalidValue;
 #define SMX_CASE(w_, b) if (a.c.w == w_ && a.c.bf16 == b) e = launch_attn_mass_w##w_##_b##b(a, p, s);

@@ -69,18 +69,15 @@ struct Unit {
 };
 __device__ __forceinline__ Unit rounded(int bf16, const float (&x)[8])
 {
-    uint16_t h[8];
-    bool bad = false;
-    const uint32_t top = bf16 ? 0x7F80u : 0x7C00u;
+    uint32_t w[4], over = 0;
+    const uint32_t top = bf16 ? 0x7F807F80u : 0x7C007C00u, least = bf16 ? 0x00800080u : 0x04000400u;
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-        h[i] = bf16 ? __builtin_bit_cast(uint16_t, (__bf16)x[i]) : __builtin_bit_cast(uint16_t, (_Float16)x[i]);
-        bad |= (h[i] & top) == top;
+    for (int i = 0; i < 4; i++) {
+        typedef _Float16 half2v __attribute__((ext_vector_type(2)));
+        w[i] = bf16 ? bf16_pair(x[2 * i], x[2 * i + 1]) : __builtin_bit_cast(uint32_t, half2v{(_Float16)x[2 * i], (_Float16)x[2 * i + 1]});
+        over |= (w[i] & top) + least;   // an exponent of all ones carries into the sign's place
     }
-    Unit r;
-    r.bad = bad;
-    __builtin_memcpy(&r.u, h, 16);
-    return r;
+    return Unit{make_uint4(w[0], w[1], w[2], w[3]), (over & 0x80008000u) != 0};
 }
 
 // Cosines and sines of the pairs of this lane's channels: N of them from pair j0 on.
@@ -166,64 +163,82 @@ __device__ __forceinline__ void angles_of(const PgWriteArgs &a, Turn &r, int t, 
     }
 }
 
-// A row on its way: this lane's channels and their partners.
-template <int TYPE> struct Raw {
-    Elem8<TYPE> x, z;
+// What the lanes of a wave share about its token.
+struct Token {
+    Turn turn;
+    int t, d0, first, step;   // this lane's channels; its first row, and how far to the next one
+    bool on;                  // the lane has channels
 };
 
-template <int TYPE>
-__device__ __forceinline__ void fetch(const PgWriteArgs &a, const Turn &T, Raw<TYPE> &r, const void *p, int64_t at, int d0)
+// One kind of rows of a token: queries, or keys with their values (KV).  put(row, y, v): the row normed and turned, its V row.
+// f (x A + z B) with A = gamma c and B = gamma' s: the norm's factor f last.
+template <int TYPE, bool VEC, bool KV, typename Put>
+__device__ __forceinline__ void each_row(const PgWriteArgs &a, const Token &k, const void *src, const void *vsrc, int rows, const float *gamma,
+                                         bool norm, Put put)
 {
-    r.x = load8<TYPE>(p, at + d0, a.vec);
-    if (T.on == 0 || !a.rot.halves) return;
-    if ((a.rot.half & 7) == 0) {
-        r.z = load8<TYPE>(p, at + T.e0, a.vec);
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const int d = min(d0 + i, 2 * a.rot.half - 1);
-            r.z[i] = ((const typename Elem<TYPE>::type *)p)[at + (d < a.rot.half ? d + a.rot.half : d - a.rot.half)];
-        }
-    }
-}
-
-// The row normed and turned.  gamma: the norm's weights in LDS, head_dim of them and more.
-template <int TYPE>
-__device__ __forceinline__ void finish(const PgWriteArgs &a, const Turn &T, const float *gamma, const Raw<TYPE> &r, bool norm, int d0, float (&y)[8])
-{
-    float f = 1.0f;
-    if (norm) {
-        float sq = 0.0f;
-#pragma unroll
-        for (int i = 0; i < 8; i++) sq = __builtin_fmaf((float)r.x[i], (float)r.x[i], sq);
-        sq = row_sum(sq, a.group_shift);
-        f = 1.0f / sqrtf(sq / (float)a.hd + a.eps);
-    }
-    float x[8];
-#pragma unroll
-    for (int i = 0; i < 8; i++) x[i] = norm ? (float)r.x[i] * f * gamma[d0 + i] : (float)r.x[i];
-    if (a.rot.halves && norm && (a.rot.half & 7) == 0) {
-        const int e0 = T.on ? T.e0 : 0;
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const float w = (float)r.z[i] * f * gamma[e0 + i];
-            y[i] = i < T.on ? x[i] * T.c[i] + w * T.s[i] : x[i];
-        }
-        return;
-    }
+    typedef typename Elem<TYPE>::type E;
+    const Turn &T = k.turn;
+    const int half = a.rot.half, d0 = k.d0;
+    const bool halves = a.rot.halves, apart = halves && (half & 7) != 0, partial = 2 * half < a.hd;
+    float A[8], B[8];
 #pragma unroll
     for (int i = 0; i < 8; i++) {
-        float w = x[i ^ 1];
-        if (a.rot.halves) {
-            const int d = min(d0 + i, 2 * a.rot.half - 1);
-            w = norm ? (float)r.z[i] * f * gamma[d < a.rot.half ? d + a.rot.half : d - a.rot.half] : (float)r.z[i];
+        const int d = min(d0 + i, max(2 * half - 1, 0)), e = halves ? (d < half ? d + half : d - half) : d ^ 1;
+        A[i] = (norm ? gamma[d0 + i] : 1.0f) * (i < T.on ? T.c[i] : 1.0f);
+        B[i] = i < T.on ? (norm ? gamma[e] : 1.0f) * T.s[i] : 0.0f;
+    }
+    struct Raw {
+        Elem8<TYPE> x, z, v;
+    };
+    const E *x = (const E *)src + (int64_t)k.first * a.hd, *v = KV ? (const E *)vsrc + (int64_t)k.first * a.hd : nullptr;
+    const int64_t stride = (int64_t)k.step * a.hd;
+    const auto load = [&](Raw &r, int g) {
+        if (k.on && g < rows) {
+            r.x = load8<TYPE>(x, d0, VEC);
+            if (apart) {
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const int d = min(d0 + i, 2 * half - 1);
+                    r.z[i] = x[d < half ? d + half : d - half];
+                }
+            } else if (halves && T.on) {
+                r.z = load8<TYPE>(x, T.e0, VEC);
+            }
+            if (KV) r.v = load8<TYPE>(v, d0, VEC);
         }
-        y[i] = i < T.on ? x[i] * T.c[i] + w * T.s[i] : x[i];
+        x += stride;
+        if (KV) v += stride;
+    };
+    Raw ahead[2] = {};   // two turns ahead
+    load(ahead[0], k.first);
+    load(ahead[1], k.first + k.step);
+    for (int g = k.first; g < rows; g += k.step) {
+        const Raw r = ahead[0];
+        ahead[0] = ahead[1];
+        load(ahead[1], g + 2 * k.step);
+        float y[8], f = 1.0f;
+        if (norm) {
+            float sq = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 8; i++) sq = __builtin_fmaf((float)r.x[i], (float)r.x[i], sq);
+            const float m = row_sum(sq, a.group_shift) * a.inv_hd + a.eps;
+            f = __builtin_amdgcn_rsqf(m);
+            if (__any(m < 1.17549435e-38f)) f = 1.0f / sqrtf(m);   // (which takes no denormal numbers)
+        }
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            float z = halves ? (float)r.z[i] : (float)r.x[i ^ 1];
+            if (partial) z = i < T.on ? z : 0.0f;
+            y[i] = __builtin_fmaf(z, B[i], (float)r.x[i] * A[i]);
+            if (norm) y[i] *= f;
+        }
+        put(g, y, r.v);
     }
 }
 
-// A wave takes rows `part`, `part + splits` .. (64 >> group_shift at a time) of one token: the query heads, then the KV heads.
-template <int TYPE>
+// A wave takes rows `part`, `part + splits` .. (64 >> group_shift at a time) of one token, queries, then keys and values; with
+// q_parts > 0 only queries, or (from part q_parts on) only keys and values.
+template <int TYPE, bool VEC>
 __global__ __launch_bounds__(256) void k_paged_write(const PgWriteArgs a)
 {
     __shared__ __align__(16) float gamma[2][kPgMaxHead];
@@ -236,63 +251,46 @@ __global__ __launch_bounds__(256) void k_paged_write(const PgWriteArgs a)
     const int t = wave / a.splits, part = wave - t * a.splits;
     if (t >= a.n_tok) return;
     const int rows = 64 >> a.group_shift, lane = threadIdx.x & ((1 << a.group_shift) - 1), sub = (threadIdx.x & 63) >> a.group_shift;
-    const int d0 = lane * 8, nq = a.q ? a.n_head : 0, items = nq + (a.k ? a.n_kv : 0);
-    const bool on = d0 < a.hd;
-    const int place = a.c.base ? a.places[t] : 0;
-    const bool there = !a.c.base || (place >= 0 && place < a.c.n_pages * a.c.page);
-    Turn T = turn_of(a, on ? d0 : a.hd);
-
-    // two turns ahead
-    struct Row {
-        Raw<TYPE> r;
-        Elem8<TYPE> v;
-    } ahead[2] = {};
-    const auto load = [&](Row &w, int g) {
-        if (!on || g >= items) return;
-        if (g < nq) {
-            fetch<TYPE>(a, T, w.r, a.q, t * a.q_stride + (int64_t)g * a.hd, d0);
-        } else {
-            const int64_t h = (int64_t)(g - nq) * a.hd;
-            fetch<TYPE>(a, T, w.r, a.k, t * a.k_stride + h, d0);
-            if (a.c.base) w.v = load8<TYPE>(a.v, t * a.v_stride + h + d0, a.vec);
-        }
-    };
-    const int step = a.splits * rows, g0 = part * rows + sub;
-    load(ahead[0], g0);
-    load(ahead[1], g0 + step);
-    angles_of(a, T, t, d0);
-    for (int g = g0; g < items; g += step) {
-        const Raw<TYPE> cur = ahead[0].r;
-        const Elem8<TYPE> cv = ahead[0].v;
-        ahead[0] = ahead[1];
-        load(ahead[1], g + 2 * step);
-        float y[8];
-        if (g < nq) {
-            finish<TYPE>(a, T, gamma[0], cur, a.q_gamma, d0, y);
-            if (on) store8(a.out_type, a.q_out, ((int64_t)t * a.n_head + g) * a.hd + d0, y, a.vec);
-            continue;
-        }
-        const int head = g - nq;
-        finish<TYPE>(a, T, gamma[1], cur, a.k_gamma, d0, y);
-        if (!a.c.base) {
-            if (on) store8(a.out_type, a.k_out, ((int64_t)t * a.n_kv + head) * a.hd + d0, y, a.vec);
-            continue;
-        }
+    Token k;
+    k.t = t, k.d0 = lane * 8, k.on = k.d0 < a.hd;
+    const bool only_q = part < a.q_parts, only_kv = a.q_parts > 0 && !only_q;
+    const int own = only_kv ? part - a.q_parts : part, of = only_q ? a.q_parts : a.splits - a.q_parts;
+    k.first = own * rows + sub, k.step = of * rows;
+    k.turn = turn_of(a, k.on ? k.d0 : a.hd);
+    angles_of(a, k.turn, t, k.d0);
+    if (!k.on) k.d0 = 0;   // (never more than is there)
+    typedef typename Elem<TYPE>::type E;
+    if (a.q && !only_kv)
+        each_row<TYPE, VEC, false>(a, k, (const E *)a.q + t * a.q_stride, nullptr, a.n_head, gamma[0], a.q_gamma, [&](int g, const float (&y)[8], auto) {
+            if (k.on) store8(a.out_type, a.q_out, ((int64_t)t * a.n_head + g) * a.hd + k.d0, y, VEC);
+        });
+    if (!a.k || only_q) return;
+    const E *src = (const E *)a.k + t * a.k_stride;
+    if (!a.c.base) {
+        each_row<TYPE, VEC, false>(a, k, src, nullptr, a.n_kv, gamma[1], a.k_gamma, [&](int g, const float (&y)[8], auto) {
+            if (k.on) store8(a.out_type, a.k_out, ((int64_t)t * a.n_kv + g) * a.hd + k.d0, y, VEC);
+        });
+        return;
+    }
+    const int place = a.places[t];
+    if (place < 0 || place >= a.c.n_pages * a.c.page) return;
+    const int p = place & (a.c.page - 1);
+    uint8_t *to = a.c.k_row(place / a.c.page, 0, p) + 16 * pg_unit(a.c.w, lane, p);
+    each_row<TYPE, VEC, true>(a, k, src, (const E *)a.v + t * a.v_stride, a.n_kv, gamma[1], a.k_gamma, [&](int g, const float (&y)[8], Elem8<TYPE> v) {
         float w[8];
 #pragma unroll
-        for (int i = 0; i < 8; i++) w[i] = (float)cv[i];
+        for (int i = 0; i < 8; i++) w[i] = (float)v[i];
         Unit ku = rounded(a.c.bf16, y), vu = rounded(a.c.bf16, w);
-        const uint64_t bad = __ballot(on && (ku.bad || vu.bad)) >> (sub << a.group_shift);   // this row's lanes lowest
-        if (!on || !there) continue;
+        const uint64_t bad = __ballot(k.on && (ku.bad || vu.bad)) >> (sub << a.group_shift);   // this row's lanes lowest
+        if (!k.on) return;
         if (bad & ((UINT64_C(1) << (1 << a.group_shift)) - 1)) {
             ku.u = make_uint4(0x7FFF7FFFu, 0x7FFF7FFFu, 0x7FFF7FFFu, 0x7FFF7FFFu);
             vu.u = make_uint4(0, 0, 0, 0);
         }
-        const int p = place & (a.c.page - 1);
-        uint8_t *row = a.c.k_row(place / a.c.page, head, p) + 16 * pg_unit(a.c.w, lane, p);
+        uint8_t *row = to + g * a.c.head_bytes();
         *(uint4 *)row = ku.u;
         *(uint4 *)(row + a.c.v_off()) = vu.u;
-    }
+    });
 }
 
 // Reads rows back: [n_tok][n_kv][hd] in the cache's type; zeros for places that it does not have, NaN for a position
@@ -325,12 +323,20 @@ hipError_t launch_paged_write(PgWriteArgs a, int in_type, hipStream_t s)
     a.group_shift = 0;
     while ((8 << a.group_shift) < a.hd) a.group_shift++;
     // a token's rows over several waves where tokens are fewer than what keeps the chip busy (16 waves a compute unit)
-    const int items = (a.q ? a.n_head : 0) + (a.k ? a.n_kv : 0), rows = 64 >> a.group_shift, turns = (items + rows - 1) / rows;
-    a.splits = std::max(1, std::min(turns, 4096 / a.n_tok));
+    // and each kind of them over waves of its own where that still leaves every row its turn at once (16 tokens of 32 + 4 heads of
+    // 64: 5.4 us for 7.3)
+    const int rows = 64 >> a.group_shift, tq = ((a.q ? a.n_head : 0) + rows - 1) / rows, tk = ((a.k ? a.n_kv : 0) + rows - 1) / rows;
+    const bool apart = tq > 0 && tk > 0 && (int64_t)a.n_tok * (tq + tk) <= 4096;
+    a.q_parts = apart ? tq : 0;
+    a.splits = apart ? tq + tk : std::max(1, std::min(std::max(tq, tk), 4096 / a.n_tok));
     const unsigned blocks = (unsigned)(((int64_t)a.n_tok * a.splits + 3) / 4);
-    if (in_type == PG_F32) k_paged_write<PG_F32><<<blocks, 256, 0, s>>>(a);
-    else if (in_type == PG_F16) k_paged_write<PG_F16><<<blocks, 256, 0, s>>>(a);
-    else k_paged_write<PG_BF16><<<blocks, 256, 0, s>>>(a);
+    a.inv_hd = 1.0f / (float)a.hd;
+    if (in_type == PG_F32 && a.vec) k_paged_write<PG_F32, true><<<blocks, 256, 0, s>>>(a);
+    else if (in_type == PG_F32) k_paged_write<PG_F32, false><<<blocks, 256, 0, s>>>(a);
+    else if (in_type == PG_F16 && a.vec) k_paged_write<PG_F16, true><<<blocks, 256, 0, s>>>(a);
+    else if (in_type == PG_F16) k_paged_write<PG_F16, false><<<blocks, 256, 0, s>>>(a);
+    else if (a.vec) k_paged_write<PG_BF16, true><<<blocks, 256, 0, s>>>(a);
+    else k_paged_write<PG_BF16, false><<<blocks, 256, 0, s>>>(a);
     return hipGetLastError();
 }
 

@@ -205,9 +205,9 @@ int plan_attention(const smx_paged_cache *c, int type, int n_tok, int n_head, in
     return SMX_OK;
 }
 
-int plan_mass(const smx_paged_cache *c, int n_head, int n_seq, int max_q, int max_len, const char *fn, MassPgPlan *p)
+int plan_mass(const smx_paged_cache *c, int type, int n_head, int n_seq, int max_q, int max_len, const char *fn, MassPgPlan *p)
 {
-    *p = attn_mass_plan(c->view, n_head, n_seq, max_q, max_len);
+    *p = attn_mass_plan(c->view, elem_type(type), n_head, n_seq, max_q, max_len);
     if (p->blocks > kMaxBlocks || (double)n_seq * c->view.n_kv * max_len > (double)kMaxOutputs)
         SMX_FAIL(SMX_EUNSUPPORTED, "%s: %d sequences of %d positions are too many outputs", fn, n_seq, max_len);
     return SMX_OK;
@@ -346,16 +346,16 @@ SMX_API int smx_attention_paged_work_bytes(const smx_paged_cache *c, int type, i
     return rc;
 }
 
-SMX_API int smx_attention_mass_work_bytes(const smx_paged_cache *c, int n_head, int n_seq, int max_q, int max_len, int64_t *bytes)
+SMX_API int smx_attention_mass_work_bytes(const smx_paged_cache *c, int type, int n_head, int n_seq, int max_q, int max_len, int64_t *bytes)
 {
     const char *fn = "smx_attention_mass_work_bytes";
     if (!c || !bytes) SMX_FAIL(SMX_EINVAL, "%s: null argument", fn);
-    int rc = check_batch(c, SMX_TYPE_F32, 0, n_head, n_seq, max_q, max_len, fn);
+    int rc = check_batch(c, type, 0, n_head, n_seq, max_q, max_len, fn);
     if (rc != SMX_OK) return rc;
     *bytes = 0;
     if (max_len == 0) return SMX_OK;
     MassPgPlan p;
-    rc = plan_mass(c, n_head, n_seq, max_q, max_len, fn, &p);
+    rc = plan_mass(c, type, n_head, n_seq, max_q, max_len, fn, &p);
     if (rc == SMX_OK) *bytes = p.work_bytes;
     return rc;
 }
@@ -401,7 +401,7 @@ SMX_API int smx_attention_mass(const smx_paged_cache *c, int type, const void *q
     if (misaligned(lse_dev, 4) || misaligned(mass_dev, 4) || misaligned(mass_out_dev, 4)) SMX_FAIL(SMX_EINVAL, "%s: misaligned pointer", fn);
     if (max_len == 0) return SMX_OK;
     MassPgPlan p;
-    if ((rc = plan_mass(c, n_head, n_seq, max_q, max_len, fn, &p)) != SMX_OK) return rc;
+    if ((rc = plan_mass(c, type, n_head, n_seq, max_q, max_len, fn, &p)) != SMX_OK) return rc;
     if ((rc = check_work(work_dev, work_bytes, p.work_bytes, fn)) != SMX_OK) return rc;
     if ((rc = check_device(c, fn)) != SMX_OK) return rc;
     AttnPgArgs a = batch_args(c, type, q_dev, q_stride, n_tok, n_head, n_seq, starts_dev, lens_dev, tables_dev, table_stride, max_q,

@@ -29,7 +29,7 @@ struct AttnPgArgs {
     const float *mass, *lse_in;
     float *mass_out, *mass_part;
     int64_t mass_stride;
-    int mass_width, mass_parts;
+    int mass_width, mass_parts, mass_per;   // mass_per: rows' blocks of a part
     int64_t q_stride;
     double inv_group;            // n_kv / n_head
     float scale_log2e;           // of plain scores, as exponents of 2
@@ -54,7 +54,7 @@ struct AttnPgPlan {
 
 struct MassPgPlan {
     bool few;                    // every sequence has up to 32 rows per KV head
-    int parts;
+    int parts, per;
     int64_t blocks, work_bytes;
 };
 

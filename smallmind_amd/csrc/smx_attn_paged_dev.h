@@ -198,7 +198,8 @@ template <bool F32> struct Query {
     float unit;            // of the products
 };
 
-template <bool F32>
+// CHECK: a row that holds a NaN or an infinity becomes NaN.
+template <bool F32, bool CHECK = true>
 __device__ __forceinline__ void load_q(const AttnPgArgs &a, const Row &r, int h, Query<F32> &Q)
 {
     const int64_t at = (int64_t)r.token * a.q_stride + (int64_t)r.head * a.c.hd;
@@ -218,13 +219,13 @@ __device__ __forceinline__ void load_q(const AttnPgArgs &a, const Row &r, int h,
                     for (int e = 0; e < 8; e++) v[e] = p[e];
                 }
             }
-#pragma unroll
-            for (int e = 0; e < 8; e++) top = max(top, (uint32_t)(v[e] & 0x7FFF));
             __builtin_memcpy(&Q.q[0][n], v, 16);
+            if constexpr (CHECK) {
+#pragma unroll
+                for (int e = 0; e < 8; e++) top = max(top, (uint32_t)(v[e] & 0x7FFF));
+            }
         }
-        // a row that holds a NaN or an infinity is NaN
-        const bool bad = max_halves(top >= (BF16 ? 0x7F80u : 0x7C00u) ? 1.0f : 0.0f) > 0.0f;
-        if (bad) Q.unit = __builtin_nanf("");
+        if (CHECK && max_halves(top >= (BF16 ? 0x7F80u : 0x7C00u) ? 1.0f : 0.0f) > 0.0f) Q.unit = __builtin_nanf("");
     } else {
         float f[NK][8];
         uint32_t top = 0;
@@ -323,12 +324,12 @@ struct Shape {
     float slope;
     bool shaped;
     Shape() = default;
-    __device__ __forceinline__ Shape(const AttnPgArgs &a, const Row &r, float unit)
+    __device__ __forceinline__ Shape(const AttnPgArgs &a, float slope_of, float unit)
     {
         shaped = a.cap_in != 0.0f || a.slopes;
         in = (a.cap_in != 0.0f ? a.cap_in : a.scale_log2e) * unit;
         c = shaped ? 1.0f : in;
-        slope = a.slopes ? a.slopes[r.head] * 1.4426950408889634f : 0.0f;
+        slope = slope_of * 1.4426950408889634f;
     }
 };
 

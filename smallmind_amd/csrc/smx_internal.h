@@ -377,7 +377,7 @@ hipError_t launch_paged_read(const PgView &c, const int32_t *places, int n_tok, 
 // How a call is cut up (the same for every content of device memory), and the call with work of plan.work_bytes bytes.
 AttnPgPlan attn_paged_plan(const PgView &c, int io, int n_tok, int n_head, int n_seq, int max_q, int max_len, int window);
 hipError_t launch_attn_paged(AttnPgArgs a, const AttnPgPlan &p, void *work, hipStream_t s);
-MassPgPlan attn_mass_plan(const PgView &c, int n_head, int n_seq, int max_q, int max_len);
+MassPgPlan attn_mass_plan(const PgView &c, int io, int n_head, int n_seq, int max_q, int max_len);
 hipError_t launch_attn_mass(AttnPgArgs a, const MassPgPlan &p, void *work, hipStream_t s);
 hipError_t launch_paged_evict(const PgEvictArgs &a, int n_seq, hipStream_t s);
 

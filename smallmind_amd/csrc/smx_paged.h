@@ -61,14 +61,15 @@ struct PgWriteArgs {
     const void *q, *k, *v;        // token t's rows at t * stride (in elements); q, k, v may be null
     int64_t q_stride, k_stride, v_stride;
     const float *q_gamma, *k_gamma;
-    float eps;
+    float eps, inv_hd;
     PgRotation rot;               // half = 0: none
     const int32_t *places;
     void *q_out, *k_out;
     int n_tok, n_head, n_kv, hd;
     int out_type;                 // of q_out and k_out
     int vec;                      // rows can be read and written 16 bytes at a time
-    int splits, group_shift;      // waves that share a token's rows; log2 of the lanes of a row
+    int splits, q_parts;          // waves that share a token's rows; the first of them that take queries only (0: all take both)
+    int group_shift;              // log2 of the lanes of a row
 };
 
 // Arguments of the eviction (k_paged_evict.hip).

@@ -850,7 +850,7 @@ def attention_mass(q, lse, cache: GpuPagedCache, starts, lens, tables, max_q: in
         out = torch.empty((n_seq, cache.n_kv_head, max(max_len, 0)), dtype=torch.float32, device=cache.device)
         if out.numel() == 0 and max_len == 0:
             return out
-        need = cache._work_bytes("smx_attention_mass_work_bytes", (n_head, n_seq, max_q, max_len))
+        need = cache._work_bytes("smx_attention_mass_work_bytes", (t, n_head, n_seq, max_q, max_len))
         work = torch.empty(need, dtype=torch.uint8, device=cache.device) if need else None
         call("smx_attention_mass", h, t, q.data_ptr(), stride, lse.data_ptr(), _opt(mass), mass_stride, width, out.data_ptr(), n_tok,
              n_head, n_seq, starts.data_ptr(), lens.data_ptr(), tables.data_ptr(), tables.shape[1], max_q, max_len,

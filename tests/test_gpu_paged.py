@@ -670,7 +670,7 @@ def test_the_same_call_twice_gives_the_same_bits(Q):
     want = Q.attention_mass(B.q, a[1], *B.args(), mass=before)
     c, st, le, ta, mq, ml = B.args()
     need = ctypes.c_int64()
-    _lib.call("smx_attention_mass_work_bytes", c._h, 8, 3, mq, ml, ctypes.byref(need))
+    _lib.call("smx_attention_mass_work_bytes", c._h, 30, 8, 3, mq, ml, ctypes.byref(need))
     work = torch.empty(max(need.value, 16), dtype=torch.uint8, device="cuda")
     _lib.call("smx_attention_mass", c._h, 30, B.q.data_ptr(), B.q.stride(0), a[1].data_ptr(), before.data_ptr(), ml, ml, before.data_ptr(),
               B.q.shape[0], 8, 3, st.data_ptr(), le.data_ptr(), ta.data_ptr(), ta.shape[1], mq, ml, None, work.data_ptr(), work.numel(),

@@ -37,7 +37,7 @@ def test_null_caches_are_refused(lib):
     assert lib.smx_paged_append(None, F32, None, 0, 0, P, 64, P, 64, None, None, 0.0, None, None, P, 1, F32, None, None) == -1
     assert lib.smx_paged_read(None, P, 1, P, P, None) == -1
     assert lib.smx_attention_paged_work_bytes(None, F32, 1, 1, 1, 1, 64, None, ctypes.byref(n)) == -1
-    assert lib.smx_attention_mass_work_bytes(None, 1, 1, 1, 64, ctypes.byref(n)) == -1
+    assert lib.smx_attention_mass_work_bytes(None, F32, 1, 1, 1, 64, ctypes.byref(n)) == -1
     assert lib.smx_attention_paged(None, F32, P, 64, P, None, 1, 1, 1, P, P, P, 1, 1, 64, None, P, 1 << 20, None) == -1
     assert lib.smx_attention_mass(None, F32, P, 64, P, None, 0, 0, P, 1, 1, 1, P, P, P, 1, 1, 64, None, P, 1 << 20, None) == -1
     assert lib.smx_paged_evict(None, P, 64, P, 1, 64, 32, 8, P, 1, P, 1, P, P, P, None) == -1
