@@ -2,14 +2,19 @@
 // those others that have received the most weight, n_keep in all, copied in their order to other pages.
 //
 // Mathematics.  With n positions, r = min(n_recent, n_keep, n) of them the last, m = min(n, n_keep) - r of the first n - r are chosen:
-// those whose weight is above the m-th largest, and of those equal to it the first.  The m-th largest is found digit
-// by digit: weights as unsigned numbers of the same order, a count of each value of the leading 8 bits, and so on down
-// the four bytes.  A NaN counts as less than every number, -0 as 0.
+// those whose weight is above the m-th largest, and of those equal to it the first.  The m-th largest is found digit by
+// digit: weights as unsigned numbers of the same order, a count of each value of the leading 11 bits, of the next 11 among
+// those that lead alike, and of the last 10; it ends early where a digit's count is the number still wanted, for weights that differ
+// mostly after two.  A NaN counts as less than every number, -0 as 0.
 //
-// Layout.  Choosing: one workgroup per (sequence, KV head); a thread owns SEG consecutive positions of each segment of
-// 1024 * SEG, so that one scan over the threads gives every position its place in order.  Up to one segment the weights
-// stay in registers through all passes; longer sequences read them again (from the L2).  Copying: a lane per
-// 16-byte unit, rows anywhere in the pages.
+// Layout.  Choosing: one workgroup per (sequence, KV head), 64 positions at a time a wave, so that loads and stores are of
+// whole lines and ballots give every position its place in order.  Up to 16384 positions the weights stay in registers;
+// longer sequences are gone through a segment at a time and read again for each digit (from the L2).  What bounds it is the workgroup's own
+// chain of loads, counts and barriers: 8.9 us for 700 positions, 18.6 us for 128 sequences and heads of 8192 (20 to 27 us when the
+// number was found bit by bit with ballots, 21 us with 8-bit digits and positions in order of the threads).
+// Copying: a lane per 16-byte unit, rows anywhere in the pages.  By the workgroup that chose where that is at most 128 KB of new
+// rows, so that a second launch is spared (64 KB: 11.2 us for 8.9 + 3.4); by a launch of its own above (1 MB: 118 us for
+// 18.6 + 52, of which 52 are 270 MB read and as much written at 5.2 TB/s, a large copy's rate).
 #include "smx_device.h"
 #include "smx_internal.h"
 
@@ -29,143 +34,114 @@ __device__ __forceinline__ uint32_t order_of(float f)
     return (u >> 31) ? ~u : u | 0x80000000u;
 }
 
-struct Choose {
-    uint32_t hist[16][256];   // a count for each wave: equal weights are common
-    uint32_t total[256];
-    uint32_t wave_gt[16], wave_eq[16];
-    uint32_t digit, above, least;
-};
-
-__global__ __launch_bounds__(kThreads) void k_paged_choose(const PgEvictArgs a)
+// Lanes before this one whose bit is set.
+__device__ __forceinline__ uint32_t before(uint64_t m)
 {
-    __shared__ Choose S;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int b = blockIdx.x / a.c.n_kv, h = blockIdx.x - b * a.c.n_kv;
-    const int n = min(max(a.lens[b], 0), a.max_len);
-    const int keep = min(n, a.n_keep), recent = min(a.n_recent, keep), cand = n - recent;
-    const uint32_t want = (uint32_t)(keep - recent);
-    const float *mass = a.mass + (int64_t)blockIdx.x * a.mass_stride;
-    int32_t *kept = a.kept + (int64_t)blockIdx.x * a.n_keep;
-    float *out = a.new_mass + (int64_t)blockIdx.x * a.n_keep;
-    if (h == 0 && tid == 0) a.new_lens[b] = keep;
-
-    uint32_t key[kSeg];
-    const auto load = [&](int s0) {
-#pragma unroll
-        for (int i = 0; i < kSeg; i++) {
-            const int p = s0 + tid * kSeg + i;
-            key[i] = p < cand ? order_of(mass[p]) : 0u;
-        }
-    };
-    load(0);
-    uint32_t least = 0, ties = 0;       // the m-th largest, and how many equal to it are kept
-    const bool all = want >= (uint32_t)cand;
-    if (want > 0 && !all) {
-        uint32_t left = want;
-        for (int shift = 24; shift >= 0; shift -= 8) {
-            for (int i = tid; i < 16 * 256; i += kThreads) (&S.hist[0][0])[i] = 0;
-            __syncthreads();
-            for (int s0 = 0; s0 < cand; s0 += kSegment) {
-                if (cand > kSegment) load(s0);
-#pragma unroll
-                for (int i = 0; i < kSeg; i++) {
-                    const bool in = s0 + tid * kSeg + i < cand && (shift == 24 || (key[i] >> (shift + 8)) == (least >> (shift + 8)));
-                    if (in) atomicAdd(&S.hist[wave][(key[i] >> shift) & 255u], 1u);
-                }
-            }
-            __syncthreads();
-            if (tid < 256) {
-                uint32_t t = 0;
-#pragma unroll
-                for (int w = 0; w < 16; w++) t += S.hist[w][tid];
-                S.total[tid] = t;
-            }
-            __syncthreads();
-            // the largest digit with `left` or more at or above it
-            if (wave == 0) {
-                uint32_t c[4], sum = 0;
-#pragma unroll
-                for (int i = 0; i < 4; i++) c[i] = S.total[4 * lane + i], sum += c[i];
-                uint32_t above = sum;   // of this lane's digits and all higher ones
-                for (int o = 1; o < 64; o <<= 1) {
-                    const uint32_t v = __shfl_down(above, o, 64);
-                    if (lane + o < 64) above += v;
-                }
-                above -= sum;
-#pragma unroll
-                for (int i = 3; i >= 0; i--) {
-                    if (above < left && above + c[i] >= left) S.digit = 4 * lane + i, S.above = above;
-                    above += c[i];
-                }
-            }
-            __syncthreads();
-            least |= S.digit << shift;
-            left -= S.above;
-            __syncthreads();
-        }
-        ties = left;
-    }
-    // in order of position: every one above `least`, and the first `ties` equal to it
-    uint32_t eq_before = 0, at_before = 0;
-    for (int s0 = 0; s0 < cand && want > 0; s0 += kSegment) {
-        if (cand > kSegment) load(s0);
-        uint32_t gt = 0, eq = 0;
-#pragma unroll
-        for (int i = 0; i < kSeg; i++) {
-            const bool in = s0 + tid * kSeg + i < cand;
-            gt += in && (all || key[i] > least);
-            eq += in && !all && key[i] == least;
-        }
-        uint32_t g = gt, e = eq;
-        for (int o = 1; o < 64; o <<= 1) {
-            const uint32_t x = __shfl_up(g, o, 64), y = __shfl_up(e, o, 64);
-            if (lane >= o) g += x, e += y;
-        }
-        if (lane == 63) S.wave_gt[wave] = g, S.wave_eq[wave] = e;
-        __syncthreads();
-        uint32_t gb = g - gt, eb = e - eq, gall = 0, eall = 0;
-#pragma unroll
-        for (int w = 0; w < 16; w++) {
-            if (w < wave) gb += S.wave_gt[w], eb += S.wave_eq[w];
-            gall += S.wave_gt[w], eall += S.wave_eq[w];
-        }
-        eb += eq_before;
-        uint32_t at = at_before + gb + min(eb, ties) - min(eq_before, ties);
-#pragma unroll
-        for (int i = 0; i < kSeg; i++) {
-            const int p = s0 + tid * kSeg + i;
-            if (p >= cand) continue;
-            const bool is_eq = !all && key[i] == least;
-            if (all || key[i] > least || (is_eq && eb < ties)) {
-                kept[at] = p;
-                out[at] = mass[p];
-                at++;
-            }
-            eb += is_eq;
-        }
-        at_before += gall + min(eq_before + eall, ties) - min(eq_before, ties);
-        eq_before += eall;
-        __syncthreads();
-    }
-    for (int i = tid; i < recent; i += kThreads) {
-        kept[want + i] = cand + i;
-        out[want + i] = mass[cand + i];
-    }
-    for (int i = keep + tid; i < a.n_keep; i += kThreads) {
-        kept[i] = -1;
-        out[i] = 0.0f;
-    }
+    return __builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0u));
 }
 
-// Rows kept[..] of the old pages to places 0 .. of the new ones.  blockIdx.y: (sequence, KV head).
-__global__ __launch_bounds__(256) void k_paged_copy(const PgEvictArgs a)
+// What a workgroup works on, and what it keeps of it.
+struct Job {
+    int b, h, n, keep, recent, cand;
+    uint32_t want;      // of the first `cand` positions
+    const float *mass;
+    int32_t *kept;
+    float *out;
+
+    __device__ __forceinline__ explicit Job(const PgEvictArgs &a)
+    {
+        b = blockIdx.x / a.c.n_kv, h = blockIdx.x - b * a.c.n_kv;
+        n = min(max(a.lens[b], 0), a.max_len);
+        keep = min(n, a.n_keep), recent = min(a.n_recent, keep), cand = n - recent;
+        want = (uint32_t)(keep - recent);
+        mass = a.mass + (int64_t)blockIdx.x * a.mass_stride;
+        kept = a.kept + (int64_t)blockIdx.x * a.n_keep;
+        out = a.new_mass + (int64_t)blockIdx.x * a.n_keep;
+        if (h == 0 && threadIdx.x == 0) a.new_lens[b] = keep;
+    }
+    // The last positions, and the places that stay empty.
+    __device__ __forceinline__ void rest(int n_keep) const
+    {
+        for (int i = threadIdx.x; i < recent; i += kThreads) {
+            kept[want + i] = cand + i;
+            out[want + i] = mass[cand + i];
+        }
+        for (int i = keep + threadIdx.x; i < n_keep; i += kThreads) {
+            kept[i] = -1;
+            out[i] = 0.0f;
+        }
+    }
+};
+
+// A wave's keys: key i of a lane is that of position first + 64 i + lane, for i < per, so that loads and stores are of whole lines
+// and a ballot has 64 positions in their order.  A place without a candidate has a NaN's key.
+struct Keys {
+    uint32_t key[kSeg];
+    int first, per, cand;
+
+    __device__ __forceinline__ void load(const float *mass, int first_, int per_, int cand_)
+    {
+        first = first_, per = per_, cand = cand_;
+#pragma unroll
+        for (int i = 0; i < kSeg; i++) {
+            const int p = first + 64 * i + (threadIdx.x & 63);
+            key[i] = i < per && p < cand ? order_of(mass[p]) : 0u;
+        }
+    }
+    __device__ __forceinline__ bool in(int i) const { return first + 64 * i + (int)(threadIdx.x & 63) < cand; }
+};
+
+// In order of position, every key above `least` and the first `ties` equal to it go to their places.  eq, at: keys equal to `least`
+// and places taken in the segments before.
+struct Counts {
+    uint32_t gt[16], eq[16];
+};
+__device__ __forceinline__ void place(Counts &S, const Keys &k, const Job &j, uint32_t least, uint32_t ties, bool all, uint32_t &eq_all, uint32_t &at_all)
 {
-    const int units = a.c.w / 8, pair = blockIdx.y;
-    const int i = (blockIdx.x * 256 + threadIdx.x) / units, u = (blockIdx.x * 256 + threadIdx.x) % units;
-    if (i >= a.n_keep) return;
-    const int p = a.kept[(int64_t)pair * a.n_keep + i];
-    if (p < 0) return;
-    const int b = pair / a.c.n_kv, h = pair - b * a.c.n_kv;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    uint32_t gt = 0, eq = 0;
+#pragma unroll
+    for (int i = 0; i < kSeg; i++) {
+        if (i < k.per) {
+            gt += (uint32_t)__popcll(__ballot(k.in(i) && (all || k.key[i] > least)));
+            eq += (uint32_t)__popcll(__ballot(k.in(i) && !all && k.key[i] == least));
+        }
+    }
+    if (lane == 0) S.gt[wave] = gt, S.eq[wave] = eq;
+    __syncthreads();
+    uint32_t gb = 0, eb = 0, gall = 0, eall = 0;
+#pragma unroll
+    for (int w = 0; w < 16; w++) {
+        if (w == wave) gb = gall, eb = eall;
+        gall += S.gt[w], eall += S.eq[w];
+    }
+    eb += eq_all;
+    uint32_t at = at_all + gb + min(eb, ties) - min(eq_all, ties);   // (of this wave's first)
+#pragma unroll
+    for (int i = 0; i < kSeg; i++) {
+        if (i < k.per) {
+            const bool is_eq = k.in(i) && !all && k.key[i] == least;
+            const uint64_t eqs = __ballot(is_eq);
+            const bool keep = (k.in(i) && (all || k.key[i] > least)) || (is_eq && eb + before(eqs) < ties);
+            const uint64_t keeps = __ballot(keep);
+            if (keep) {
+                const int p = k.first + 64 * i + lane;
+                const uint32_t to = at + before(keeps);
+                j.kept[to] = p;
+                j.out[to] = j.mass[p];
+            }
+            at += (uint32_t)__popcll(keeps);
+            eb += (uint32_t)__popcll(eqs);
+        }
+    }
+    at_all += gall + min(eq_all + eall, ties) - min(eq_all, ties);
+    eq_all += eall;
+    __syncthreads();
+}
+
+// Unit u of row p of the old pages to row i of the new ones.
+__device__ __forceinline__ void copy_unit(const PgEvictArgs &a, int b, int h, int p, int i, int u)
+{
     const int src = a.tables[(int64_t)b * a.table_stride + p / a.c.page], dst = a.new_tables[(int64_t)b * a.new_stride + i / a.c.page];
     if ((unsigned)dst >= (unsigned)a.c.n_pages) return;
     uint4 k = make_uint4(0, 0, 0, 0), v = k;
@@ -181,15 +157,110 @@ __global__ __launch_bounds__(256) void k_paged_copy(const PgEvictArgs a)
     *(uint4 *)(row + a.c.v_off()) = v;
 }
 
+// COPY: the rows too.
+template <bool COPY>
+__global__ __launch_bounds__(kThreads) void k_paged_choose(const PgEvictArgs a)
+{
+    __shared__ uint32_t hist[2048], sums[16], found[3];
+    __shared__ Counts S;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const Job j(a);
+    const bool one = j.cand <= kSegment;                     // the keys stay in registers
+    const int per = one ? (j.cand + kThreads - 1) / kThreads : kSeg, step = per * kThreads;
+    Keys k;
+    k.load(j.mass, wave * 64 * per, per, j.cand);
+    const bool all = j.want >= (uint32_t)j.cand;
+    uint32_t least = 0, ties = 0;       // the m-th largest, and how many equal to it are kept
+    if (j.want > 0 && !all) {
+        uint32_t left = j.want;
+        hist[tid] = 0, hist[tid + kThreads] = 0;
+        __syncthreads();
+#pragma unroll
+        for (int pass = 0; pass < 3; pass++) {
+            const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, above_shift = pass == 1 ? 21 : 10;
+            const uint32_t mask = pass == 2 ? 1023u : 2047u;
+            for (int s0 = 0; s0 < j.cand; s0 += step) {
+                if (!one) k.load(j.mass, s0 + wave * 64 * per, per, j.cand);
+#pragma unroll
+                for (int i = 0; i < kSeg; i++) {
+                    if (i < per && k.in(i) && (pass == 0 || ((k.key[i] ^ least) >> above_shift) == 0)) {
+                        const uint32_t digit = (k.key[i] >> shift) & mask;
+                        // (equal weights are common, and would wait for each other)
+                        const uint32_t lead = __builtin_amdgcn_readfirstlane(digit);
+                        if (digit == lead) {
+                            const uint64_t same = __ballot(true);
+                            if (before(same) == 0) atomicAdd(&hist[digit], (uint32_t)__popcll(same));
+                        } else {
+                            atomicAdd(&hist[digit], 1u);
+                        }
+                    }
+                }
+            }
+            __syncthreads();
+            // the largest digit with `left` or more at or above it: digits from the highest down, two of a thread
+            const int d0 = 2047 - 2 * tid;
+            const uint32_t c0 = hist[d0], c1 = hist[d0 - 1];
+            hist[d0] = 0, hist[d0 - 1] = 0;
+            uint32_t sum = c0 + c1;
+            for (int o = 1; o < 64; o <<= 1) {
+                const uint32_t v = __shfl_up(sum, o, 64);
+                if (lane >= o) sum += v;
+            }
+            if (lane == 63) sums[wave] = sum;
+            __syncthreads();
+            uint32_t above = sum - c0 - c1;
+#pragma unroll
+            for (int w = 0; w < 16; w++) above += w < wave ? sums[w] : 0u;
+            if (above < left && above + c0 >= left) found[0] = d0, found[1] = above, found[2] = c0;
+            above += c0;
+            if (above < left && above + c1 >= left) found[0] = d0 - 1, found[1] = above, found[2] = c1;
+            __syncthreads();
+            least |= found[0] << shift;
+            left -= found[1];
+            ties = left;
+            if (found[2] == left) {     // all with these digits are kept
+                ties = ~0u;
+                break;
+            }
+        }
+    }
+    uint32_t eq = 0, at = 0;
+    for (int s0 = 0; s0 < j.cand && j.want > 0; s0 += step) {
+        if (!one) k.load(j.mass, s0 + wave * 64 * per, per, j.cand);
+        place(S, k, j, least, ties, all, eq, at);
+    }
+    j.rest(a.n_keep);
+    if constexpr (COPY) {
+        __syncthreads();   // (what the workgroup has written, it reads)
+        const int units = a.c.w / 8;
+        for (int i = tid; i < j.keep * units; i += kThreads) copy_unit(a, j.b, j.h, j.kept[i / units], i / units, i % units);
+    }
+}
+
+// Rows kept[..] of the old pages to places 0 .. of the new ones.  blockIdx.y: (sequence, KV head).
+__global__ __launch_bounds__(256) void k_paged_copy(const PgEvictArgs a)
+{
+    const int units = a.c.w / 8, pair = blockIdx.y;
+    const int i = (blockIdx.x * 256 + threadIdx.x) / units, u = (blockIdx.x * 256 + threadIdx.x) % units;
+    if (i >= a.n_keep) return;
+    const int p = a.kept[(int64_t)pair * a.n_keep + i];
+    if (p < 0) return;
+    const int b = pair / a.c.n_kv;
+    copy_unit(a, b, pair - b * a.c.n_kv, p, i, u);
+}
+
 }  // namespace
 
 hipError_t launch_paged_evict(const PgEvictArgs &a, int n_seq, hipStream_t s)
 {
-    k_paged_choose<<<(unsigned)(n_seq * a.c.n_kv), kThreads, 0, s>>>(a);
+    const unsigned pairs = (unsigned)(n_seq * a.c.n_kv);
+    const bool copy = (int64_t)a.n_keep * a.c.w * 4 <= (128 << 10);   // K and V rows, 2 bytes a dim
+    if (copy) k_paged_choose<true><<<pairs, kThreads, 0, s>>>(a);
+    else k_paged_choose<false><<<pairs, kThreads, 0, s>>>(a);
     const hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return e;
+    if (e != hipSuccess || copy) return e;
     const int64_t n = (int64_t)a.n_keep * (a.c.w / 8);
-    k_paged_copy<<<dim3((unsigned)((n + 255) / 256), (unsigned)(n_seq * a.c.n_kv)), 256, 0, s>>>(a);
+    k_paged_copy<<<dim3((unsigned)((n + 255) / 256), pairs), 256, 0, s>>>(a);
     return hipGetLastError();
 }
 
