@@ -464,7 +464,7 @@ def _attention_q8(q, cache, prefix, slots, lens, max_len, name):
     with _on_device(index, q, slots, lens):
         out = torch.empty(q.shape, dtype=torch.float32, device=cache.device)
         need = cache._work_bytes(n_seq, n_q, n_head, prefix[1] if prefix else 0, max_len)
-        work = torch.empty(need, dtype=torch.uint8, device=cache.device) if need else None
+        work = lens.new_empty((need,), dtype=torch.uint8) if need else None
         call(name, h, q.data_ptr(), stride, out.data_ptr(), n_seq, n_q, n_head, *prefix, slots.data_ptr(), lens.data_ptr(),
              max_len, work.data_ptr() if need else None, need, _raw_stream(index))
     return out
@@ -663,7 +663,7 @@ class GpuPagedCache:
         with undefined contents).  With k_gamma or a rotation the keys are normed and turned as they are by qk_norm_rope; with q
         ([n_tok, n_head, head_dim] of k's type) so are the queries, and they are returned, of `dtype` (default: as they
         come)."""
-        torch, n, kv, hd, index = _torch(), places.numel(), self.n_kv_head, self.head_dim, self.device.index
+        n, kv, hd, index = places.numel(), self.n_kv_head, self.head_dim, self.device.index
         ks, vs = _token_rows(k, kv, hd, "k"), _token_rows(v, kv, hd, "v")
         if k.shape[0] != n or v.shape[0] != n or v.dtype is not k.dtype:
             raise ValueError(f"k and v must hold one row per token ({n}), of one type")
@@ -683,7 +683,7 @@ class GpuPagedCache:
                 _floats(g, hd, what)
         turn, rot, at = _turning(rotation, pos, n)
         with _on_device(index, k, v, places, q, q_gamma, k_gamma, *turn):
-            out = None if q is None else torch.empty(q.shape, dtype=dtype, device=self.device)
+            out = None if q is None else q.new_empty(q.shape, dtype=dtype)
             if n:
                 call("smx_paged_append", self._handle(), tin, _opt(q), qs, n_head, k.data_ptr(), ks, v.data_ptr(), vs, _opt(q_gamma),
                      _opt(k_gamma), _eps(eps), rot, at, places.data_ptr(), n, tout, _opt(out), _raw_stream(index))
@@ -696,7 +696,7 @@ class GpuPagedCache:
         _int32(places, n, "places")
         _c_int(n, "the number of tokens")
         with _on_device(index, places):
-            k = torch.empty((n, self.n_kv_head, self.head_dim), dtype=self.dtype, device=self.device)
+            k = places.new_empty((n, self.n_kv_head, self.head_dim), dtype=self.dtype)
             v = torch.empty_like(k)
             if n:
                 call("smx_paged_read", self._handle(), places.data_ptr(), n, k.data_ptr(), v.data_ptr(), _raw_stream(index))
@@ -708,7 +708,7 @@ class GpuPagedCache:
         [n_seq, pages] and new_tables [n_seq, pages] int32: the kept rows are copied in order to positions 0 .. of the new
         pages, which must be others than any sequence's old ones (smx_paged_evict).  Returns (kept [n_seq, n_kv_head, n_keep]
         int32, -1 beyond; new lens [n_seq] int32; their weights [n_seq, n_kv_head, n_keep] float32)."""
-        torch, index = _torch(), self.device.index
+        index = self.device.index
         if mass.dim() != 3 or mass.shape[1] != self.n_kv_head or mass.shape[0] < 1:
             raise ValueError(f"mass must be [n_seq, {self.n_kv_head}, max_len]")
         n_seq, kv, max_len = mass.shape
@@ -719,9 +719,8 @@ class GpuPagedCache:
         for t, what in ((tables, "tables"), (new_tables, "new_tables")):
             _table(t, n_seq, what)
         with _on_device(index, mass, lens, tables, new_tables):
-            kept = torch.empty((n_seq, kv, max(n_keep, 0)), dtype=torch.int32, device=self.device)
-            new_lens = torch.empty(n_seq, dtype=torch.int32, device=self.device)
-            new_mass = torch.empty(kept.shape, dtype=torch.float32, device=self.device)
+            shape = (n_seq, kv, max(n_keep, 0))
+            kept, new_lens, new_mass = lens.new_empty(shape), lens.new_empty((n_seq,)), mass.new_empty(shape)
             call("smx_paged_evict", self._handle(), mass.data_ptr(), stride, lens.data_ptr(), n_seq, max_len, n_keep, n_recent,
                  tables.data_ptr(), tables.shape[1], new_tables.data_ptr(), new_tables.shape[1], kept.data_ptr(),
                  new_lens.data_ptr(), new_mass.data_ptr(), _raw_stream(index))
@@ -767,6 +766,8 @@ def _mass_rows(mass) -> int:
 
 
 def _rules(n_seq, n_head, scale, cap, slopes, window, prefix):
+    if scale is None and cap == 0.0 and slopes is None and window == 0 and prefix is None:
+        return None          # (what the C side takes for these)
     if slopes is not None:
         _floats(slopes, n_head, "slopes")
     if prefix is not None:
@@ -777,7 +778,7 @@ def _rules(n_seq, n_head, scale, cap, slopes, window, prefix):
             raise ValueError(f"{what} {x} must be finite and not negative")
     if scale is not None and not scale > 0.0:
         raise ValueError("scale must be positive")
-    return _lib.AttentionRulesC(0.0 if scale is None else scale, cap, _opt(slopes), _opt(prefix), window, 0)
+    return ctypes.byref(_lib.AttentionRulesC(0.0 if scale is None else scale, cap, _opt(slopes), _opt(prefix), window, 0))
 
 
 def _paged_batch(q, cache, starts, lens, tables, max_q, max_len):
@@ -820,13 +821,12 @@ def attention_paged(q, cache: GpuPagedCache, starts, lens, tables, max_q: int, m
         raise ValueError(f"out must be contiguous {q.dtype} {tuple(q.shape)}")
     with _on_device(index, q, starts, lens, tables, slopes, prefix, out):
         if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=cache.device)
-        sums = torch.empty((n_tok, n_head), dtype=torch.float32, device=cache.device) if lse else None
+            out = q.new_empty(q.shape)
+        sums = q.new_empty((n_tok, n_head), dtype=torch.float32) if lse else None
         need = cache._work_bytes("smx_attention_paged_work_bytes", (t, n_tok, n_head, n_seq, max_q, max_len), (window,))
-        work = torch.empty(need, dtype=torch.uint8, device=cache.device) if need else None
+        work = lens.new_empty((need,), dtype=torch.uint8) if need else None
         call("smx_attention_paged", h, t, q.data_ptr(), stride, out.data_ptr(), _opt(sums), n_tok, n_head, n_seq, starts.data_ptr(),
-             lens.data_ptr(), tables.data_ptr(), tables.shape[1], max_q, max_len, ctypes.byref(rules), _opt(work), need,
-             _raw_stream(index))
+             lens.data_ptr(), tables.data_ptr(), tables.shape[1], max_q, max_len, rules, _opt(work), need, _raw_stream(index))
     return (out, sums) if lse else out
 
 
@@ -847,14 +847,14 @@ def attention_mass(q, lse, cache: GpuPagedCache, starts, lens, tables, max_q: in
         width, mass_stride = mass.shape[2], _mass_rows(mass)
         _c_int(width, "width")
     with _on_device(index, q, lse, starts, lens, tables, mass, slopes, prefix):
-        out = torch.empty((n_seq, cache.n_kv_head, max(max_len, 0)), dtype=torch.float32, device=cache.device)
+        out = lse.new_empty((n_seq, cache.n_kv_head, max(max_len, 0)))
         if out.numel() == 0 and max_len == 0:
             return out
         need = cache._work_bytes("smx_attention_mass_work_bytes", (t, n_head, n_seq, max_q, max_len))
-        work = torch.empty(need, dtype=torch.uint8, device=cache.device) if need else None
+        work = lens.new_empty((need,), dtype=torch.uint8) if need else None
         call("smx_attention_mass", h, t, q.data_ptr(), stride, lse.data_ptr(), _opt(mass), mass_stride, width, out.data_ptr(), n_tok,
              n_head, n_seq, starts.data_ptr(), lens.data_ptr(), tables.data_ptr(), tables.shape[1], max_q, max_len,
-             ctypes.byref(rules), _opt(work), need, _raw_stream(index))
+             rules, _opt(work), need, _raw_stream(index))
     return out
 
 
