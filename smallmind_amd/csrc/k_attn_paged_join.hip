@@ -131,9 +131,13 @@ AttnPgPlan attn_paged_plan(const PgView &c, int io, int n_tok, int n_head, int n
     } else {
         p.tile_blocks = (int)(n_tok * group / block + n_seq);
         units = std::max<int64_t>(1, (n_tok * group + block - 1) / block) * c.n_kv;
-        // Two groups of four waves on a block until there are 512 blocks, two for every compute unit (1024 tokens over 1024
-        // positions, 32 x 128 dims, 256 blocks: 27.8 us for 31.8 with one group; 4096 over 4096, 1024 blocks: 176 for 153).
-        if (two && units < 512) p.groups = 2;
+        // Two groups of four waves on a block, which then has a compute unit to itself, while there is one for every block (1024
+        // tokens over 1024 positions, 32 x 128 dims, 256 blocks: 27.8 us for 31.8 with one group); above that, where the
+        // blocks that must wait can start early enough to end with the longest one.  Longest first, the 257th waits for the 256th, about
+        // as long as itself; a block costs some six tiles beside its own (1536 over 1536, 384 blocks: 38.7 us for 43.6;
+        // but 1280 over 4096, 320 blocks: 128 for 115, and 6 x 256 over 512, 384 blocks: 31 for 22).
+        const double longest = span + 6.0, shortest = std::min<double>(span, (max_len - std::min(max_q, max_len)) / kPgTile) + 6.0;
+        if (two && (units <= 256 || 2 * (longest - (longest - shortest) * 256 / units) <= longest)) p.groups = 2;
         // Parts up to one workgroup for every compute unit, of no fewer than four tiles.  n parts save 1 - 1 / n of the tiles'
         // time, about a microsecond each at 128 dims, and cost a launch, 4 us, and their sums' way to memory and back, 8 bytes
         // each at 5 TB/s: the best n is where these are equal, if that gains anything (64 tokens over 32768 positions, 16
