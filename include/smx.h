@@ -327,7 +327,8 @@ SMX_API int smx_paged_read(const smx_paged_cache *c, const int32_t *places_dev, 
 /* What a score is and who sees whom.  With s = scale * q . k (scale 0: 1 / sqrt(head_dim)) of a token at position t and a
  * position p: cap > 0: s becomes cap * tanh(s / cap); slopes_dev ([n_head], or NULL): slopes[h] * |t - p| is taken off.  The token
  * sees p if p is one of its sequence's first prefix_dev[b] positions ([n_seq], NULL: none; these are seen by
- * tokens before them too), or if p <= t and, with window > 0, p > t - window. */
+ * tokens before them too), or if p <= t and, with window > 0, p > t - window.  A scale, cap or scale / cap of more than 6e36 is
+ * not supported. */
 typedef struct smx_attention_rules {
     float scale;
     float cap;
@@ -353,7 +354,7 @@ SMX_API int smx_attention_mass_work_bytes(const smx_paged_cache *c, int type, in
  * as they were; a row that sees nothing is zeros, and its lse -inf.  type: of q and out, the cache's or
  * SMX_TYPE_F32.  With fp32, queries and weights count to 22 bits over an F16 cache (the query's elements to 2^-38 of the largest
  * of their row, weights to 2^-31 of the largest where that is more) and to 24 over a BF16 one; with the cache's type weights are rounded to that.
- * Sums are fp32; scores below 2^126.  rules may be NULL.  work_dev: smx_attention_paged_work_bytes bytes, 16-byte aligned,
+ * Sums are fp32; scores below 2^126.  out_dev and lse_dev are not q's memory.  rules may be NULL.  work_dev: smx_attention_paged_work_bytes bytes, 16-byte aligned,
  * free for other use when the call's work is done; calls that may overlap, replays of captured graphs among them, need one each. */
 SMX_API int smx_attention_paged(const smx_paged_cache *c, int type, const void *q_dev, int64_t q_stride, void *out_dev,
                                 float *lse_dev, int n_tok, int n_head, int n_seq, const int32_t *starts_dev,
@@ -363,7 +364,8 @@ SMX_API int smx_attention_paged(const smx_paged_cache *c, int type, const void *
  * mass_out[b][h][p] = mass[b][h][p] + the sum over b's new tokens and h's query heads of exp(score - lse), with lse_dev as
  * smx_attention_paged gives it.  mass_dev: rows [n_seq * n_kv_head], mass_stride apart, of mass_width
  * floats (what lies beyond counts as 0), or NULL; mass_out_dev [n_seq][n_kv_head][max_len], 0 from lens_dev[b] on, may be mass_dev
- * itself where mass_stride is max_len.  Each sum's order is fixed.  work_dev: smx_attention_mass_work_bytes bytes, as above. */
+ * itself where mass_stride is max_len.  Each sum's order is fixed.  score - lse is as good as its two terms: a weight is off by
+ * some 2^-23 |lse| of itself.  work_dev: smx_attention_mass_work_bytes bytes, as above. */
 SMX_API int smx_attention_mass(const smx_paged_cache *c, int type, const void *q_dev, int64_t q_stride,
                                const float *lse_dev, const float *mass_dev, int64_t mass_stride, int mass_width,
                                float *mass_out_dev, int n_tok, int n_head, int n_seq, const int32_t *starts_dev,

@@ -190,7 +190,8 @@ __device__ __forceinline__ void each_row(const PgWriteArgs &a, const Token &k, c
     struct Raw {
         Elem8<TYPE> x, z, v;
     };
-    const E *x = (const E *)src + (int64_t)k.first * a.hd, *v = KV ? (const E *)vsrc + (int64_t)k.first * a.hd : nullptr;
+    const E *x = (const E *)src + (int64_t)k.first * a.hd;
+    const int64_t to_v = KV ? (const uint8_t *)vsrc - (const uint8_t *)src : 0;
     const int64_t stride = (int64_t)k.step * a.hd;
     const auto load = [&](Raw &r, int g) {
         if (k.on && g < rows) {
@@ -204,10 +205,9 @@ __device__ __forceinline__ void each_row(const PgWriteArgs &a, const Token &k, c
             } else if (halves && T.on) {
                 r.z = load8<TYPE>(x, T.e0, VEC);
             }
-            if (KV) r.v = load8<TYPE>(v, d0, VEC);
+            if (KV) r.v = load8<TYPE>((const uint8_t *)x + to_v, d0, VEC);
         }
         x += stride;
-        if (KV) v += stride;
     };
     Raw ahead[2] = {};   // two turns ahead
     load(ahead[0], k.first);
@@ -223,7 +223,21 @@ __device__ __forceinline__ void each_row(const PgWriteArgs &a, const Token &k, c
             for (int i = 0; i < 8; i++) sq = __builtin_fmaf((float)r.x[i], (float)r.x[i], sq);
             const float m = row_sum(sq, a.group_shift) * a.inv_hd + a.eps;
             f = __builtin_amdgcn_rsqf(m);
-            if (__any(m < 1.17549435e-38f)) f = 1.0f / sqrtf(m);   // (which takes no denormal numbers)
+            // squares that leave fp32 (fp16's do not): again, with a power of two
+            const bool far = TYPE != PG_F16 && !(m >= 1.17549435e-38f && m < __builtin_huge_valf());
+            if (__any(far)) {
+                const float by = m < 1.0f ? 4.722366482869645e21f : 2.117582368135751e-22f;
+                // (from memory, one by one: few registers for what hardly ever happens)
+                const E *p = x - 3 * stride + d0;
+                sq = 0.0f;
+#pragma unroll 1
+                for (int i = 0; k.on && i < 8; i++) {
+                    const float w = (float)p[i] * by;
+                    sq = __builtin_fmaf(w, w, sq);
+                }
+                sq = row_sum(sq, a.group_shift) * a.inv_hd + a.eps * by * by;
+                if (far) f = by / sqrtf(sq);
+            }
         }
 #pragma unroll
         for (int i = 0; i < 8; i++) {

@@ -132,11 +132,18 @@ int check_batch(const smx_paged_cache *c, int type, int n_tok, int n_head, int n
     return SMX_OK;
 }
 
-int check_rules(const smx_attention_rules *r, const char *fn)
+// The factors of the scores: products to exponents of 2, or to what tanh takes and from there.
+double scale_of(const PgView &v, const smx_attention_rules *r) { return r && r->scale > 0.0f ? (double)r->scale : 1.0 / sqrt((double)v.hd); }
+constexpr double kLog2e = 1.4426950408889634;
+
+int check_rules(const smx_paged_cache *c, const smx_attention_rules *r, const char *fn)
 {
     if (!r) return SMX_OK;
     if (!(r->scale >= 0.0f && r->scale < INFINITY) || !(r->cap >= 0.0f && r->cap < INFINITY))
         SMX_FAIL(SMX_EINVAL, "%s: scale and cap must be finite and not negative", fn);
+    const double scale = scale_of(c->view, r);
+    if (scale * kLog2e > 1e37 || r->cap * kLog2e > 1e37 || (r->cap > 0.0f && scale / r->cap > 1e37))
+        SMX_FAIL(SMX_EUNSUPPORTED, "%s: scale, cap or scale / cap is above the range of fp32", fn);
     if (r->window < 0) SMX_FAIL(SMX_EINVAL, "%s: window %d is negative", fn, r->window);
     if (r->reserved != 0) SMX_FAIL(SMX_EINVAL, "%s: reserved must be zero", fn);
     if (misaligned(r->slopes_dev, 4) || misaligned(r->prefix_dev, 4)) SMX_FAIL(SMX_EINVAL, "%s: misaligned pointer", fn);
@@ -163,10 +170,10 @@ AttnPgArgs batch_args(const smx_paged_cache *c, int type, const void *q, int64_t
     a.inv_group = (double)v.n_kv / n_head;
     a.max_q = max_q < n_tok ? max_q : n_tok, a.max_len = max_len;
     a.io = elem_type(type);
-    const double scale = r && r->scale > 0.0f ? (double)r->scale : 1.0 / sqrt((double)v.hd), log2e = 1.4426950408889634;
-    a.scale_log2e = (float)(scale * log2e);
+    const double scale = scale_of(v, r);
+    a.scale_log2e = (float)(scale * kLog2e);
     if (r) {
-        if (r->cap > 0.0f) a.cap_in = (float)(scale / r->cap), a.cap_out = (float)(r->cap * log2e);
+        if (r->cap > 0.0f) a.cap_in = (float)(scale / r->cap), a.cap_out = (float)(r->cap * kLog2e);
         a.slopes = r->slopes_dev;
         a.prefix = r->prefix_dev;
         a.window = window_of(r, max_len);
@@ -337,7 +344,7 @@ SMX_API int smx_attention_paged_work_bytes(const smx_paged_cache *c, int type, i
     const char *fn = "smx_attention_paged_work_bytes";
     if (!c || !bytes) SMX_FAIL(SMX_EINVAL, "%s: null argument", fn);
     int rc = check_batch(c, type, n_tok, n_head, n_seq, max_q, max_len, fn);
-    if (rc != SMX_OK || (rc = check_rules(rules, fn)) != SMX_OK) return rc;
+    if (rc != SMX_OK || (rc = check_rules(c, rules, fn)) != SMX_OK) return rc;
     *bytes = 0;
     if (n_tok == 0) return SMX_OK;
     AttnPgPlan p;
@@ -368,7 +375,7 @@ SMX_API int smx_attention_paged(const smx_paged_cache *c, int type, const void *
     const char *fn = "smx_attention_paged";
     if (!c || (n_tok > 0 && (!q_dev || !out_dev)) || !starts_dev || !lens_dev || (max_len > 0 && !tables_dev)) SMX_FAIL(SMX_EINVAL, "%s: null argument", fn);
     int rc = check_batch(c, type, n_tok, n_head, n_seq, max_q, max_len, fn);
-    if (rc != SMX_OK || (rc = check_rules(rules, fn)) != SMX_OK) return rc;
+    if (rc != SMX_OK || (rc = check_rules(c, rules, fn)) != SMX_OK) return rc;
     if ((rc = check_operands(c, type, q_dev, q_stride, n_head, starts_dev, lens_dev, tables_dev, table_stride, max_len, fn)) != SMX_OK) return rc;
     if (misaligned(out_dev, elem_bytes(elem_type(type))) || misaligned(lse_dev, 4)) SMX_FAIL(SMX_EINVAL, "%s: misaligned pointer", fn);
     if (n_tok == 0) return SMX_OK;
@@ -394,7 +401,7 @@ SMX_API int smx_attention_mass(const smx_paged_cache *c, int type, const void *q
     const char *fn = "smx_attention_mass";
     if (!c || (n_tok > 0 && (!q_dev || !lse_dev)) || !mass_out_dev || !starts_dev || !lens_dev || (max_len > 0 && !tables_dev)) SMX_FAIL(SMX_EINVAL, "%s: null argument", fn);
     int rc = check_batch(c, type, n_tok, n_head, n_seq, max_q, max_len, fn);
-    if (rc != SMX_OK || (rc = check_rules(rules, fn)) != SMX_OK) return rc;
+    if (rc != SMX_OK || (rc = check_rules(c, rules, fn)) != SMX_OK) return rc;
     if ((rc = check_operands(c, type, q_dev, q_stride, n_head, starts_dev, lens_dev, tables_dev, table_stride, max_len, fn)) != SMX_OK) return rc;
     if (mass_dev && (mass_width < 0 || mass_stride < mass_width)) SMX_FAIL(SMX_EINVAL, "%s: rows of mass must be at least mass_width apart", fn);
     if (mass_dev == mass_out_dev && mass_stride != max_len) SMX_FAIL(SMX_EINVAL, "%s: in place, rows of mass must be max_len apart", fn);

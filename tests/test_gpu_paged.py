@@ -155,6 +155,23 @@ def test_positions_without_an_angle(Q):
     assert np.array_equal(np.isnan(f64(gv)).all((1, 2)), [False, True, True, False, True]) and np.isnan(f64(gk[1])).all()
 
 
+@pytest.mark.parametrize("exponent,tin", [(-66, F32), (-61, BF16), (65, F32), (66, BF16), (118, F32)])
+@pytest.mark.parametrize("hd", [8, 104, 256])
+def test_norms_of_rows_whose_squares_leave_fp32(Q, hd, exponent, tin):
+    """Beside ordinary rows; eps 0, so that small rows are not lost in it."""
+    rng = np.random.default_rng([hd, 100 + exponent])
+    n = 9
+    x = rng.normal(0, 1, (n, 3, hd)) * np.exp2(np.where(rng.uniform(size=(n, 3, 1)) < 0.6, exponent, 0))
+    x = dev(x, tin)
+    g = rng.normal(1, 0.3, hd).astype(np.float32)
+    cos, sin = tables(rng, 16, hd // 2)
+    pos = rng.integers(0, 16, (1, n)).astype(np.int32)
+    q, k = Q.qk_norm_rope(x, x[:, :2], dev(g), dev(g), 0.0, Q.Rotation(cos, sin, halves=True), dev(pos), dtype=F32)
+    want, e = R.turned(f64(x), g, 0.0, cos.cpu().numpy(), sin.cpu().numpy(), pos, [hd // 2], True)
+    close(q, want, e)
+    close(k, want[:, :2], e[:, :2])
+
+
 # ---- batches ---------------------------------------------------------------------------------------
 class Batch:
     """Sequences of these lengths with `new` new tokens each, their pages shuffled in a cache whose other pages hold NaN."""
@@ -594,6 +611,16 @@ def test_refusals_with_a_cache(Q):
     B.check(out, _)             # the refused calls left nothing behind
 
 
+def test_factors_beyond_fp32_are_refused(Q):
+    from smallmind_amd._lib import SmxError
+    B = Batch(Q, np.random.default_rng(65), F16, F32, 4, 2, 64, 16, [40], [2])
+    for bad in (dict(scale=3e37), dict(cap=3e37), dict(cap=1e-40), dict(scale=10.0, cap=1e-37)):
+        with pytest.raises(SmxError, match="range of fp32"):
+            Q.attention_paged(B.q, *B.args(), **bad)
+    out, lse = Q.attention_paged(B.q, *B.args(), lse=True, scale=1e-30, cap=1e30)      # (all scores all but 0)
+    B.check(out, lse, scale=1e-30, cap=1e30)
+
+
 def test_on_another_stream(Q):
     rng = np.random.default_rng(61)
     B = Batch(Q, rng, F16, F32, 4, 2, 64, 16, [3000, 70], [1, 30])
@@ -655,6 +682,47 @@ def test_captured_calls(Q):
             for x, y in zip(step(), have):
                 assert torch.equal(x, y), rep
         torch.cuda.synchronize()
+
+
+def test_captured_evictions(Q):
+    """Two graphs of one cache, one whose rows move in the choosing launch and one with a launch for them."""
+    rng = np.random.default_rng(64)
+    for kv, hd, n, keep in ((2, 64, 700, 256), (2, 128, 900, 600)):
+        page = 64
+        pages, more = -(-n // page), -(-keep // page)
+        c = Q.GpuPagedCache(BF16, 2 * pages + 4 * more, kv, hd, page)
+        every = i32(np.arange(2 * pages * page))
+        k = dev(rng.normal(0, 1, (len(every), kv, hd)), BF16)
+        c.append(k, -k, every)
+        tab, new = i32(np.arange(2 * pages).reshape(2, pages)), [i32(2 * pages + 2 * more * i + np.arange(2 * more).reshape(2, more)) for i in (0, 1)]
+        mass, lens = dev(rng.uniform(0, 1, (2, kv, n)).astype(np.float32)), i32([n, n // 2])
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            c.evict(mass, lens, keep, 17, tab, new[0])
+        s.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s):
+            outs = c.evict(mass, lens, keep, 17, tab, new[0])
+        places = [i32((x.cpu().numpy()[:, :, None] * page + np.arange(page)).reshape(-1)) for x in new]
+        for rep in range(4):
+            mass.copy_(dev(np.floor(rng.uniform(0, 50 + rep, mass.shape)).astype(np.float32)))
+            lens.copy_(i32([n - rep, n // 3 + rep]))
+            torch.cuda.synchronize()
+            g.replay()
+            want = c.evict(mass, lens, keep, 17, tab, new[1])
+            torch.cuda.synchronize()
+            m, ln = mass.cpu().numpy(), lens.cpu().numpy()
+            for x, y in zip(outs, want):
+                assert torch.equal(x, y), rep
+            for b in range(2):
+                for h in range(kv):
+                    assert [p for p in outs[0][b, h].tolist() if p >= 0] == R.evict(m[b, h], ln[b], keep, 17)
+            for x, y in zip(c.read(places[0]), c.read(places[1])):
+                for b in range(2):          # (beyond the rows kept now lie those that an earlier call kept)
+                    rows = slice(b * more * page, b * more * page + int(outs[1][b]))
+                    assert torch.equal(x[rows], y[rows]), rep
+        c.close()
 
 
 def test_the_same_call_twice_gives_the_same_bits(Q):

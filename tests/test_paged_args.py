@@ -145,3 +145,22 @@ def test_plain_eviction():
     assert R.evict(m, 6, 8, 0) == [0, 1, 2, 3, 4, 5]
     assert R.evict(m, 6, 5, 0) == [0, 1, 2, 4, 5]
     assert R.evict(m, 8, 3, 3) == [5, 6, 7] and R.evict(m, 0, 3, 3) == []
+
+
+def test_structs_are_laid_out_as_in_the_header(tmp_path):
+    import os
+    import subprocess
+
+    from smallmind_amd import _lib
+    structs = {"smx_rotation": _lib.RotationC, "smx_attention_rules": _lib.AttentionRulesC}
+    src = tmp_path / "layout.c"
+    src.write_text("#include <stddef.h>\n#include <stdio.h>\n#include \"smx.h\"\nint main(void) {\n" + "".join(
+        f'printf("%d\\n", (int)sizeof({n}));\n' + "".join(f'printf("%d\\n", (int)offsetof({n}, {f}));\n' for f, _ in c._fields_)
+        for n, c in structs.items()) + "return 0; }\n")
+    include = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "include")
+    subprocess.run(["gcc", "-std=c99", "-I", include, str(src), "-o", str(tmp_path / "layout")], check=True, capture_output=True)
+    got = [int(x) for x in subprocess.run([str(tmp_path / "layout")], check=True, capture_output=True, text=True).stdout.split()]
+    want = []
+    for c in structs.values():
+        want += [ctypes.sizeof(c)] + [getattr(c, f).offset for f, _ in c._fields_]
+    assert got == want
