@@ -179,11 +179,12 @@ hipError_t launch_attn_paged(AttnPgArgs a, const AttnPgPlan &p, void *work, hipS
     return hipGetLastError();
 }
 
-// Row blocks that k_attn_mass lays out at a time.
+// Parts of a query's values in k_attn_mass, and row blocks that it lays out at a time.
+static int attn_mass_parts(const PgView &c, int io) { return io != PG_F32 ? 1 : c.bf16 ? 3 : 2; }
 static int attn_mass_blocks(const PgView &c, int io)
 {
-    const int parts = io != PG_F32 ? 1 : c.bf16 ? 3 : 2;
-    return parts * c.w <= 256 ? 4 : parts * c.w <= 512 ? 2 : 1;
+    const int wide = attn_mass_parts(c, io) * c.w;
+    return wide <= 256 ? 4 : wide <= 512 ? 2 : 1;
 }
 
 MassPgPlan attn_mass_plan(const PgView &c, int io, int n_head, int n_seq, int max_q, int max_len)
@@ -198,11 +199,16 @@ MassPgPlan attn_mass_plan(const PgView &c, int io, int n_head, int n_seq, int ma
         return p;
     }
     const int64_t keys = c.w <= 128 ? 256 : 128, units = pairs * ((max_len + keys - 1) / keys);
-    // parts of 1024 rows: equal work, however many rows a position is seen by (4095 tokens, 32 heads of 128: 121 us, as with
-    // 768 and 1536; 2048 and more leave the chip to the longest)
     const int nb = attn_mass_blocks(c, io);
     const int64_t blocks = (rows + 32 * nb - 1) / (32 * nb);
-    p.per = 32 / nb;
+    // Rows of a part: as many as make two workgroups for every compute unit, but 256 at least at 128 dims, which with
+    // the sum of parts take 10 us (512 tokens over 512 positions, 32 heads over 8 of 128: 43 us in parts of 1024, 21 of 256; 512 over 4096:
+    // 44, 32 of 512 and 35 of 256); 1024 are enough, so that early positions, which more rows see, do not end last (4095
+    // tokens: 130 us, 140 in parts of 2048, 358 in one); but no more parts than make 3072 workgroups, whose work memory
+    // is at most 6 MB or so (2048 over 32768: 610 us with 3 parts, 632 with 8).
+    const int64_t few = std::max<int64_t>(32768 / (c.w * attn_mass_parts(c, io)), (rows * units + 511) / 512);
+    const int64_t many = std::max<int64_t>(1024, (rows * units + 3071) / 3072);
+    p.per = (int)((std::min(few, many) + 32 * nb - 1) / (32 * nb));
     p.parts = (int)((blocks + p.per - 1) / p.per);
     p.blocks = units * p.parts;
     p.work_bytes = p.parts > 1 ? (int64_t)p.parts * pairs * max_len * 4 : 0;
