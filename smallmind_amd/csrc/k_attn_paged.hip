@@ -241,14 +241,15 @@ __device__ __forceinline__ void interleave()
     }
 }
 
-// A block of 128 rows, gone through by NG groups of four waves that take tiles in turn.
-template <bool F32, int NG>
+// A block of 128 rows, gone through by NG groups of four waves that take tiles in turn.  SPARE: without the registers for
+// another tile's scores.
+template <bool F32, int NG, bool SPARE>
 __device__ __forceinline__ void many(const AttnPgArgs &a, Many<NG> &M, const Seq &s, int head, int row0, int part)
 {
     constexpr int NP = kParts<F32>;
     // 32-position halves of a tile at once: two where registers suffice, and then the next tile's scores while this one's weigh
     constexpr int KT = W * NP > 512 ? 1 : 2;
-    constexpr bool AHEAD = KT == 2;
+    constexpr bool AHEAD = KT == 2 && !SPARE;
     const int lane = threadIdx.x & 63, h = lane >> 5, wave = wave_id() & 3, group = wave_id() >> 2;
     const int mine = row0 + wave * kPgRows;
     Tiles &T = M.t[group];
@@ -499,7 +500,7 @@ __device__ __forceinline__ void few(const AttnPgArgs &a, Few<NW> &F, const Seq &
 
 // Finds the block's sequence.  Block x belongs to the last sequence whose first block floor(start * group / 128) + b is
 // not above x: no sequence has more blocks than lie between its own first and the next one's.
-template <bool F32, int NG>
+template <bool F32, int NG, bool SPARE>
 __device__ __forceinline__ void many_rows(const AttnPgArgs &a, Many<NG> &M)
 {
     constexpr int ROWS = 4 * kPgRows;
@@ -521,24 +522,23 @@ __device__ __forceinline__ void many_rows(const AttnPgArgs &a, Many<NG> &M)
     const Seq s = seq_of(a, b);
     const int64_t row0 = (block - ((int64_t)s.start * a.group / ROWS + b)) * ROWS;
     if (row0 >= s.rows || s.rows <= a.short_rows) return;
-    many<F32, NG>(a, M, s, pair % a.c.n_kv, (int)row0, pair / a.c.n_kv);
+    many<F32, NG, SPARE>(a, M, s, pair % a.c.n_kv, (int)row0, pair / a.c.n_kv);
 }
 
-// Workgroups [0, tile_wgs): blocks of 128 rows, NG groups of four waves each; the others: a short sequence each.  NG = 0: there are
-// only these.
-template <bool F32, int NG>
-__global__ __launch_bounds__(NG == 2 ? 512 : 256, NG == 0 && W <= 128 && W * kParts<F32> <= 256 ? 2 : 1) void k_attn_paged(const AttnPgArgs a)
+// Workgroups [0, tile_wgs): blocks of 128 rows, gone through as MODE says; the others: a short sequence each.
+template <bool F32, PgMode MODE>
+__global__ __launch_bounds__(MODE == PG_TWO_GROUPS ? 512 : 256, MODE == PG_SHORT && W <= 128 && W * kParts<F32> <= 256 ? 2 : 1) void k_attn_paged(const AttnPgArgs a)
 {
-    constexpr int NW = NG == 2 ? 8 : 4;
+    constexpr int NG = MODE == PG_TWO_GROUPS ? 2 : 1, NW = 4 * NG;
     union Mem {
-        Many<NG == 2 ? 2 : 1> many;
+        Many<NG> many;
         Few<NW> few;
     };
-    __shared__ __align__(1024) char mem[NG ? sizeof(Mem) : sizeof(Few<NW>)];
+    __shared__ __align__(1024) char mem[MODE != PG_SHORT ? sizeof(Mem) : sizeof(Few<NW>)];
     Mem &M = *(Mem *)mem;
-    if constexpr (NG > 0) {
+    if constexpr (MODE != PG_SHORT) {
         if ((int)blockIdx.x < a.tile_wgs) {
-            many_rows<F32, NG>(a, M.many);
+            many_rows<F32, NG, MODE == PG_SPARE>(a, M.many);
             return;
         }
     }
@@ -550,15 +550,19 @@ __global__ __launch_bounds__(NG == 2 ? 512 : 256, NG == 0 && W <= 128 && W * kPa
 
 // Whether two groups of four waves find registers: 256 a lane.
 template <bool F32> constexpr bool kTwoGroups = W <= 128 && W * (1 + kParts<F32>) <= (kParts<F32> == 1 ? 256 : 192);
+// Whether PG_SPARE leaves room for three waves on a SIMD, where PG_ONE_GROUP has two.
+template <bool F32> constexpr bool kSpare = W * kParts<F32> <= 64;
 
 template <bool F32>
 hipError_t launch(const AttnPgArgs &a, const AttnPgPlan &p, hipStream_t s)
 {
     const unsigned n = (unsigned)p.blocks;
-    if (p.groups == 0) k_attn_paged<F32, 0><<<n, 256, 0, s>>>(a);
-    else if (p.groups == 1) k_attn_paged<F32, 1><<<n, 256, 0, s>>>(a);
-    else if constexpr (kTwoGroups<F32>) k_attn_paged<F32, 2><<<n, 512, 0, s>>>(a);
-    else return hipErrorInvalidValue;
+    if (p.mode == PG_SHORT) k_attn_paged<F32, PG_SHORT><<<n, 256, 0, s>>>(a);
+    if (p.mode == PG_ONE_GROUP) k_attn_paged<F32, PG_ONE_GROUP><<<n, 256, 0, s>>>(a);
+    if constexpr (kTwoGroups<F32>)
+        if (p.mode == PG_TWO_GROUPS) k_attn_paged<F32, PG_TWO_GROUPS><<<n, 512, 0, s>>>(a);
+    if constexpr (kSpare<F32>)
+        if (p.mode == PG_SPARE) k_attn_paged<F32, PG_SPARE><<<n, 256, 0, s>>>(a);
     return hipGetLastError();
 }
 
@@ -570,6 +574,9 @@ hipError_t SMX_PG_NAME(launch_attn_paged, SMX_PG_W, SMX_PG_BF16)(const AttnPgArg
 {
     return a.io == PG_F32 ? launch<true>(a, p, s) : launch<false>(a, p, s);
 }
-bool SMX_PG_NAME(attn_paged_two, SMX_PG_W, SMX_PG_BF16)(int io) { return io == PG_F32 ? kTwoGroups<true> : kTwoGroups<false>; }
+bool SMX_PG_NAME(attn_paged_has, SMX_PG_W, SMX_PG_BF16)(int io, PgMode m)
+{
+    return m == PG_TWO_GROUPS ? (io == PG_F32 ? kTwoGroups<true> : kTwoGroups<false>) : m != PG_SPARE || (io == PG_F32 ? kSpare<true> : kSpare<false>);
+}
 
 }  // namespace smx

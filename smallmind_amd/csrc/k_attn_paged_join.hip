@@ -102,7 +102,7 @@ __global__ __launch_bounds__(256) void k_attn_mass_join(const AttnPgArgs a)
 #define SMX_DECL(w, b)                                                                                      \
     hipError_t launch_attn_paged_w##w##_b##b(const AttnPgArgs &a, const AttnPgPlan &p, hipStream_t s);      \
     hipError_t launch_attn_mass_w##w##_b##b(const AttnPgArgs &a, const MassPgPlan &p, hipStream_t s);       \
-    bool attn_paged_two_w##w##_b##b(int io);
+    bool attn_paged_has_w##w##_b##b(int io, PgMode m);
 SMX_ALL(SMX_DECL)
 #undef SMX_DECL
 
@@ -111,17 +111,17 @@ AttnPgPlan attn_paged_plan(const PgView &c, int io, int n_tok, int n_head, int n
     AttnPgPlan p{};
     const int64_t group = n_head / c.n_kv, rows = max_q * group;
     const int64_t tiles = std::max(1, (max_len + kPgTile - 1) / kPgTile);
-    bool two = false;
-#define SMX_CASE(w_, b) if (c.w == w_ && c.bf16 == b) two = attn_paged_two_w##w_##_b##b(io);
+    bool two = false, spare = false;
+#define SMX_CASE(w_, b) if (c.w == w_ && c.bf16 == b) two = attn_paged_has_w##w_##_b##b(io, PG_TWO_GROUPS), spare = attn_paged_has_w##w_##_b##b(io, PG_SPARE);
     SMX_ALL(SMX_CASE)
 #undef SMX_CASE
     constexpr int block = 4 * kPgRows;
-    p.groups = rows <= kPgRows ? 0 : 1;
+    p.mode = rows <= kPgRows ? PG_SHORT : PG_ONE_GROUP;
     // what a block goes through at most, where the window says so, and how many blocks that is done by
-    const int64_t span = window > 0 ? std::min<int64_t>(tiles, (window + (p.groups ? block / group + 1 : (int64_t)max_q)) / kPgTile + 2) : tiles;
+    const int64_t span = window > 0 ? std::min<int64_t>(tiles, (window + (p.mode != PG_SHORT ? block / group + 1 : (int64_t)max_q)) / kPgTile + 2) : tiles;
     int64_t units = (int64_t)n_seq * c.n_kv, n = 1;
-    p.chunk = p.groups ? 1 : 4;
-    if (p.groups == 0) {
+    p.chunk = p.mode != PG_SHORT ? 1 : 4;
+    if (p.mode == PG_SHORT) {
         // two workgroups for every compute unit, of four tiles at least, or two where that leaves most of the chip idle; but one
         // part, which needs no second launch, up to 1024 positions of 64 dims or 512 of 128 (700 of 64, 4 heads: 10.7 us for 6.9 + 4.2
         // in six parts, and 4 us less for the host to do)
@@ -137,7 +137,10 @@ AttnPgPlan attn_paged_plan(const PgView &c, int io, int n_tok, int n_head, int n
         // as long as itself; a block costs some six tiles beside its own (1536 over 1536, 384 blocks: 38.7 us for 43.6;
         // but 1280 over 4096, 320 blocks: 128 for 115, and 6 x 256 over 512, 384 blocks: 31 for 22).
         const double longest = span + 6.0, shortest = std::min<double>(span, (max_len - std::min(max_q, max_len)) / kPgTile) + 6.0;
-        if (two && (units <= 256 || 2 * (longest - (longest - shortest) * 256 / units) <= longest)) p.groups = 2;
+        if (two && (units <= 256 || 2 * (longest - (longest - shortest) * 256 / units) <= longest)) p.mode = PG_TWO_GROUPS;
+        // More than two blocks for every compute unit: three at a time where their registers allow it (64 dims, 16 prompts of 1023,
+        // 12 heads: 61 us for 71; 4096 over 4096, 32 heads over 8: 99 for 111; but 2048 over 8192, 512 blocks: 182 for 175).
+        if (spare && units > 512) p.mode = PG_SPARE;
         // Parts up to one workgroup for every compute unit, of no fewer than four tiles.  n parts save 1 - 1 / n of the tiles'
         // time, about a microsecond each at 128 dims, and cost a launch, 4 us, and their sums' way to memory and back, 8 bytes
         // each at 5 TB/s: the best n is where these are equal, if that gains anything (64 tokens over 32768 positions, 16
@@ -148,10 +151,10 @@ AttnPgPlan attn_paged_plan(const PgView &c, int io, int n_tok, int n_head, int n
         if (n > 1 && save * (1 - 1.0 / n) < 4 + part * n) n = 1;
     }
     p.parts = (int)std::max<int64_t>(n, 1);
-    const int64_t shares = p.groups ? (p.tile_blocks + n_seq - 1) / n_seq * (int64_t)n_seq : 0;   // (blocks in equal shares)
+    const int64_t shares = p.mode != PG_SHORT ? (p.tile_blocks + n_seq - 1) / n_seq * (int64_t)n_seq : 0;   // (blocks in equal shares)
     p.tile_wgs = shares * c.n_kv * p.parts;
     // short sequences of a batch with longer ones go their own way
-    p.blocks = p.tile_wgs + (p.groups == 0 || n_seq > 1 ? (int64_t)n_seq * c.n_kv * p.parts : 0);
+    p.blocks = p.tile_wgs + (p.mode == PG_SHORT || n_seq > 1 ? (int64_t)n_seq * c.n_kv * p.parts : 0);
     p.work_bytes = p.parts > 1 ? (int64_t)p.parts * n_tok * n_head * (c.hd + 2) * 4 : 0;
     return p;
 }
@@ -160,7 +163,7 @@ hipError_t launch_attn_paged(AttnPgArgs a, const AttnPgPlan &p, void *work, hipS
 {
     a.tile_wgs = (int)p.tile_wgs;
     a.tile_blocks = p.tile_blocks;
-    a.short_rows = p.groups && a.n_seq > 1 ? kPgRows : 0;
+    a.short_rows = p.mode != PG_SHORT && a.n_seq > 1 ? kPgRows : 0;
     a.chunk = p.chunk;
     a.parts = p.parts;
     const int64_t rows = (int64_t)a.n_tok * a.n_head;

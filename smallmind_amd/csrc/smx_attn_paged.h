@@ -44,9 +44,13 @@ struct AttnPgArgs {
     int chunk, parts;            // tiles that a part has at least; parts (1: the outputs are written at once)
 };
 
+// How blocks of 128 rows are gone through: by four waves, or by two groups of four that take tiles in turn; in PG_SPARE by
+// four waves that leave registers for more blocks on a compute unit.  PG_SHORT: no sequence has more than 32 rows per KV head.
+enum PgMode { PG_SHORT, PG_ONE_GROUP, PG_TWO_GROUPS, PG_SPARE };
+
 // How a call is cut up.
 struct AttnPgPlan {
-    int groups;                  // of four waves that share a block of 128 rows; 0: every sequence is short
+    PgMode mode;
     int chunk, parts, tile_blocks;
     int64_t tile_wgs, blocks;
     int64_t work_bytes;

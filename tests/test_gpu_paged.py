@@ -212,24 +212,24 @@ class Batch:
     def args(self):
         return self.c, i32(self.starts), i32(self.lens), i32(self.tables), self.max_q, self.max_len
 
-    def rows(self, b, scale=None, cap=0.0, slopes=None, window=0, prefix=None):
-        """For each KV head of sequence b: (head, query heads, Scores of tokens x heads, seen)."""
+    def rows(self, b, scale=None, cap=0.0, slopes=None, window=0, prefix=None, every=1):
+        """For every `every`th KV head of sequence b: (head, query heads, Scores of tokens x heads, seen)."""
         n, m, G = self.lens[b], self.new[b], self.H // self.kv
         qb = f64(self.q[self.starts[b]:self.starts[b + 1]])
         t = np.arange(n - m, n)
         see = R.visible(n - m, m, n, min(prefix[b], n) if prefix is not None else 0, window)
-        for h in range(self.kv):
+        for h in range(b % every, self.kv, every):
             for g in range(G):
                 yield h, h * G + g, R.Scores(qb[:, h * G + g], self.k[b][:, h], t, self.io, self.cache_type, scale, cap,
                                              0.0 if slopes is None else slopes[h * G + g]), see
 
-    def check(self, out, lse, skip=(), **rules):
+    def check(self, out, lse, skip=(), every=1, **rules):
         out, lse = out.cpu(), lse.cpu()
         for b in range(len(self.lens)):
             if b in skip or not self.new[b]:
                 continue
             at = slice(self.starts[b], self.starts[b + 1])
-            for h, head, S, see in self.rows(b, **rules):
+            for h, head, S, see in self.rows(b, every=every, **rules):
                 o, e, l, le = R.attention(S, self.v[b][:, h], see, self.io, self.cache_type)
                 close(out[at, head], o, e)
                 got = f64(lse[at, head])
@@ -325,6 +325,17 @@ def mass(Q, B, rules, before=None):
             want[:, B.lens[b]:] = 0
         bad = np.isnan(want) != np.isnan(got[b])
         assert not bad.any() and (np.nan_to_num(np.abs(got[b] - want)) <= np.nan_to_num(bound)).all(), (b, np.nanmax(np.abs(got[b] - want) - bound))
+
+
+@pytest.mark.parametrize("cache,io,hd", [(F16, F16, 64), (BF16, BF16, 32), (BF16, BF16, 128), (F16, F32, 32), (F16, F16, 96), (BF16, BF16, 256)])
+@pytest.mark.parametrize("heads", [150, 300])
+def test_many_blocks(Q, cache, io, hd, heads):
+    """More blocks of rows than compute units, and more than two for each."""
+    rng = np.random.default_rng([hd, heads])
+    B = Batch(Q, rng, cache, io, heads, heads, hd, 16, [200, 90, 33], [170, 40, 1])
+    for rules in ({}, dict(window=37, prefix=[20, 0, 33], slopes=rng.uniform(0.01, 0.3, heads))):
+        out, lse = run(Q, B, rules)
+        B.check(out, lse, every=7, **rules)
 
 
 def test_rows_that_see_nothing_and_rows_of_no_sequence(Q):
