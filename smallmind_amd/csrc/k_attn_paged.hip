@@ -14,10 +14,19 @@
 // read out of LDS transposed, in that order: weights do not move between lanes, a row's maximum and sum take one exchange.
 //
 // Two ways through the positions, in chunks of one workgroup each; k_attn_paged_join adds up what the chunks found.
-//   many rows: a block of 128 or 256 rows of one sequence and KV head (the group's heads of a token are neighbouring rows), 32 per
-//     wave; all walk the same tiles of 64 positions, which go from memory to LDS one tile ahead.
+//   many rows: a block of 128 rows of one sequence and KV head (the group's heads of a token are neighbouring rows), 32 per
+//     wave; all walk the same tiles of 64 positions, which go from memory to LDS one tile ahead (PgMode).
 //   few rows (up to 32 per KV head): every wave holds all of them and takes tiles of 32 positions in turn, K from memory to
 //     registers, V to LDS of its own; the waves join their sums at the end.
+//
+// What bounds it.  Many rows of 128 dims: the matrix cores, at the clock that the card's power leaves them (2048 tokens over 32768
+// positions, 32 heads over 8, bf16: 980 to 1090 us, 980 to 1090 TFLOP/s, where the library's product of 8192^3 reaches 1160 to
+// 1220).  64 dims: the vector unit's 32 exponentials and some 110 other instructions of a wave's tile beside 16 matrix
+// instructions (4096 over 16384, 32 heads over 8: 620 us, 780 TFLOP/s); a cap adds 5 instructions, two of them transcendental, to each of 32
+// scores, slopes 3.  Short prompts: the way in and out of a block and the tiles that the diagonal cuts (4 of 1023, 12
+// heads of 64: 28 us).  fp32 queries over an F16 cache: twice the matrix instructions and the splitting of weights (512 over
+// 4096, 32 heads over 4 of 64: 49 us and 6 of the join).  Few rows: memory (64 sequences of up to 8192 positions, 8 heads
+// of 128: 245 us, 5.5 TB/s), in short contexts the chain from page table to rows to the waves' joining (700 positions: 10.6 us).
 #include "smx_attn_paged_dev.h"
 
 namespace smx {
