@@ -207,10 +207,10 @@ MassPgPlan attn_mass_plan(const PgView &c, int io, int n_head, int n_seq, int ma
     // Rows of a part: as many as make two workgroups for every compute unit, but 256 at least at 128 dims, which with
     // the sum of parts take 10 us (512 tokens over 512 positions, 32 heads over 8 of 128: 43 us in parts of 1024, 21 of 256; 512 over 4096:
     // 44, 32 of 512 and 35 of 256); 1024 are enough, so that early positions, which more rows see, do not end last (4095
-    // tokens: 130 us, 140 in parts of 2048, 358 in one); but no more parts than make 3072 workgroups, whose work memory
+    // tokens: 130 us, 140 in parts of 2048, 358 in one); but no more parts than make 3000 workgroups, whose work memory
     // is at most 6 MB or so (2048 over 32768: 610 us with 3 parts, 632 with 8).
     const int64_t few = std::max<int64_t>(32768 / (c.w * attn_mass_parts(c, io)), (rows * units + 511) / 512);
-    const int64_t many = std::max<int64_t>(1024, (rows * units + 3071) / 3072);
+    const int64_t many = std::max<int64_t>(1024, (rows * units + 2999) / 3000);
     p.per = (int)((std::min(few, many) + 32 * nb - 1) / (32 * nb));
     p.parts = (int)((blocks + p.per - 1) / p.per);
     p.blocks = units * p.parts;
