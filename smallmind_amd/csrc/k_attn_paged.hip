@@ -26,7 +26,7 @@
 // scores, slopes 3.  Short prompts: the way in and out of a block and the tiles that the diagonal cuts (4 of 1023, 12
 // heads of 64: 28 us).  fp32 queries over an F16 cache: twice the matrix instructions and the splitting of weights (512 over
 // 4096, 32 heads over 4 of 64: 49 us and 6 of the join).  Few rows: memory (64 sequences of up to 8192 positions, 8 heads
-// of 128: 245 us, 5.5 TB/s), in short contexts the chain from page table to rows to the waves' joining (700 positions: 10.6 us).
+// of 128: 250 us, 5.4 TB/s), in short contexts the chain from page table to rows to the waves' joining (700 positions: 10.6 us).
 #include "smx_attn_paged_dev.h"
 
 namespace smx {

@@ -122,11 +122,14 @@ AttnPgPlan attn_paged_plan(const PgView &c, int io, int n_tok, int n_head, int n
     int64_t units = (int64_t)n_seq * c.n_kv, n = 1;
     p.chunk = p.mode != PG_SHORT ? 1 : 4;
     if (p.mode == PG_SHORT) {
-        // two workgroups for every compute unit, of four tiles at least, or two where that leaves most of the chip idle; but one
-        // part, which needs no second launch, up to 1024 positions of 64 dims or 512 of 128 (700 of 64, 4 heads: 10.7 us for 6.9 + 4.2
-        // in six parts, and 4 us less for the host to do)
+        // Two workgroups for every compute unit, of four tiles at least, or two where that leaves most of the chip idle; up to
+        // eight for long contexts, which differ in length, while 32 tiles are left for each (8 heads of 128 dims, 64 sequences of 2048 to
+        // 8192 at random: 251 us for 260, 32 of 8000 to 32768: 441 for 493; where lengths happen to end evenly 250 for 246); but one part,
+        // which needs no second launch, up to 1024 positions of 64 dims or 512 of 128 (700 of 64, 4 heads: 10.7 us for 6.9 + 4.2 in
+        // six parts, and 4 us less for the host to do).
         n = std::min((512 + units - 1) / units, (span + 3) / 4);
         if (n * units < 128) n = std::max(n, std::min((128 + units - 1) / units, (span + 1) / 2)), p.chunk = 2;
+        n = std::max(n, std::min((2048 + units - 1) / units, span / 32));
         if (span * c.w <= 1024) n = 1;
     } else {
         p.tile_blocks = (int)(n_tok * group / block + n_seq);
