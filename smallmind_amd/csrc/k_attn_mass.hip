@@ -97,8 +97,8 @@ __global__ __launch_bounds__(kWaves * 64) void k_attn_mass_few(const AttnPgArgs 
     int at = 32 * (kWaves * share + wave);
     elem8 k[2][NK];
     bool there[2][2];
-    const bool any = s.rows > 0 && at < s.len;
-    if (any) {
+    const bool any_rows = s.rows > 0;
+    if (any_rows && at < s.len) {
         Pages P(a, s, head, at / kPgGroup);
         load_k(a, s, P, at, lane, k[0], there[0][0], there[0][1]);
         const Row r = row_of(a, s, head, lane & 31);
@@ -133,8 +133,9 @@ __global__ __launch_bounds__(kWaves * 64) void k_attn_mass_few(const AttnPgArgs 
             if (at < s.len) go(k[1], there[1][0], there[1][1], k[0], there[0]);
         }
     }
-    // positions that nobody sees: what they had, 0 beyond the sequence
-    for (; at < a.max_len; at += step) Giving(a, pair, at, lane).give(a, s, pair, 0, 0.0f);
+    // positions that nobody is there to see: what they had; 0 beyond the sequence
+    for (int p = (any_rows ? (s.len + 31) / 32 * 32 : 0) + share * kWaves * 64 + (int)threadIdx.x; p < a.max_len; p += (int)(gridDim.x / pairs) * kWaves * 64)
+        a.mass_out[(int64_t)pair * a.max_len + p] = p < s.len && a.mass && p < a.mass_width ? a.mass[pair * a.mass_stride + p] : 0.0f;
 }
 
 // ---- many rows ---------------------------------------------------------------------------------------
