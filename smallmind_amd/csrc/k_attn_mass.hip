@@ -90,10 +90,11 @@ template <bool F32>
 __global__ __launch_bounds__(kWaves * 64) void k_attn_mass_few(const AttnPgArgs a)
 {
     const int lane = threadIdx.x & 63, h = lane >> 5, wave = wave_id();
-    const int pairs = a.n_seq * a.c.n_kv, pair = blockIdx.x % pairs, share = blockIdx.x / pairs;
-    const int b = pair / a.c.n_kv, head = pair - b * a.c.n_kv;
+    const int pairs = a.n_seq * a.c.n_kv, shares = gridDim.x / pairs, head = blockIdx.x % a.c.n_kv, rest = blockIdx.x / a.c.n_kv;
+    const int b = a.ranked ? nth_longest(a, rest / shares) : rest % a.n_seq, share = a.ranked ? rest % shares : rest / a.n_seq;
+    const int pair = b * a.c.n_kv + head;
     const Seq s = seq_of(a, b);
-    const int step = 32 * kWaves * (gridDim.x / pairs);
+    const int step = 32 * kWaves * shares;
     int at = 32 * (kWaves * share + wave);
     elem8 k[2][NK];
     bool there[2][2];
@@ -134,7 +135,7 @@ __global__ __launch_bounds__(kWaves * 64) void k_attn_mass_few(const AttnPgArgs 
         }
     }
     // positions that nobody is there to see: what they had; 0 beyond the sequence
-    for (int p = (any_rows ? (s.len + 31) / 32 * 32 : 0) + share * kWaves * 64 + (int)threadIdx.x; p < a.max_len; p += (int)(gridDim.x / pairs) * kWaves * 64)
+    for (int p = (any_rows ? (s.len + 31) / 32 * 32 : 0) + share * kWaves * 64 + (int)threadIdx.x; p < a.max_len; p += shares * kWaves * 64)
         a.mass_out[(int64_t)pair * a.max_len + p] = p < s.len && a.mass && p < a.mass_width ? a.mass[pair * a.mass_stride + p] : 0.0f;
 }
 

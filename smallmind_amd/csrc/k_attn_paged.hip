@@ -26,7 +26,7 @@
 // scores, slopes 3.  Short prompts: the way in and out of a block and the tiles that the diagonal cuts (4 of 1023, 12
 // heads of 64: 28 us).  fp32 queries over an F16 cache: twice the matrix instructions and the splitting of weights (512 over
 // 4096, 32 heads over 4 of 64: 49 us and 6 of the join).  Few rows: memory (64 sequences of up to 8192 positions, 8 heads
-// of 128: 250 us, 5.4 TB/s), in short contexts the chain from page table to rows to the waves' joining (700 positions: 10.6 us).
+// of 128: 242 us, 5.6 TB/s), in short contexts the chain from page table to rows to the waves' joining (700 positions: 10.6 us).
 #include "smx_attn_paged_dev.h"
 
 namespace smx {
@@ -551,10 +551,13 @@ __global__ __launch_bounds__(MODE == PG_TWO_GROUPS ? 512 : 256, MODE == PG_SHORT
             return;
         }
     }
-    const int i = blockIdx.x - a.tile_wgs, units = a.n_seq * a.c.n_kv, unit = i % units;
-    const Seq s = seq_of(a, unit / a.c.n_kv);
+    // (KV heads fastest: one's pages are read through one XCD's L2 where there are eight)
+    const int i = blockIdx.x - a.tile_wgs, head = i % a.c.n_kv, rest = i / a.c.n_kv;
+    const bool ranked = MODE == PG_SHORT && a.ranked;
+    const int b = ranked ? nth_longest(a, rest / a.parts) : rest % a.n_seq, part = ranked ? rest % a.parts : rest / a.n_seq;
+    const Seq s = seq_of(a, b);
     if (s.rows <= 0 || s.rows > kPgRows) return;
-    few<F32, NW>(a, M.few, s, unit % a.c.n_kv, i / units);
+    few<F32, NW>(a, M.few, s, head, part);
 }
 
 // Whether two groups of four waves find registers: 256 a lane.

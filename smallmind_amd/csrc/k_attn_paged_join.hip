@@ -123,10 +123,11 @@ AttnPgPlan attn_paged_plan(const PgView &c, int io, int n_tok, int n_head, int n
     p.chunk = p.mode != PG_SHORT ? 1 : 4;
     if (p.mode == PG_SHORT) {
         // Two workgroups for every compute unit, of four tiles at least, or two where that leaves most of the chip idle; up to
-        // eight for long contexts, which differ in length, while 32 tiles are left for each (8 heads of 128 dims, 64 sequences of 2048 to
-        // 8192 at random: 251 us for 260, 32 of 8000 to 32768: 441 for 493; where lengths happen to end evenly 250 for 246); but one part,
-        // which needs no second launch, up to 1024 positions of 64 dims or 512 of 128 (700 of 64, 4 heads: 10.7 us for 6.9 + 4.2 in
-        // six parts, and 4 us less for the host to do).
+        // eight for long contexts while 32 tiles are left for each, the longest sequences' first, so that all end together (8
+        // heads of 128 dims, 64 sequences of 2048 to 8192: 241 us for 252 in their own order and 260 in one part, 32 of 8000 to
+        // 32768: 417 for 442 and 493; 64 of 8192: 376 for 367 in one part); but one part, which needs no second launch, up to 1024
+        // positions of 64 dims or 512 of 128 (700 of 64, 4 heads: 10.7 us for 6.9 + 4.2 in six parts, and 4 us less for the
+        // host to do).
         n = std::min((512 + units - 1) / units, (span + 3) / 4);
         if (n * units < 128) n = std::max(n, std::min((128 + units - 1) / units, (span + 1) / 2)), p.chunk = 2;
         n = std::max(n, std::min((2048 + units - 1) / units, span / 32));
@@ -158,6 +159,8 @@ AttnPgPlan attn_paged_plan(const PgView &c, int io, int n_tok, int n_head, int n
     p.tile_wgs = shares * c.n_kv * p.parts;
     // short sequences of a batch with longer ones go their own way
     p.blocks = p.tile_wgs + (p.mode == PG_SHORT || n_seq > 1 ? (int64_t)n_seq * c.n_kv * p.parts : 0);
+    // (up to 512 workgroups all start at once)
+    p.ranked = p.mode == PG_SHORT && n_seq > 1 && p.blocks > 512;
     p.work_bytes = p.parts > 1 ? (int64_t)p.parts * n_tok * n_head * (c.hd + 2) * 4 : 0;
     return p;
 }
@@ -168,6 +171,7 @@ hipError_t launch_attn_paged(AttnPgArgs a, const AttnPgPlan &p, void *work, hipS
     a.tile_blocks = p.tile_blocks;
     a.short_rows = p.mode != PG_SHORT && a.n_seq > 1 ? kPgRows : 0;
     a.chunk = p.chunk;
+    a.ranked = p.ranked;
     a.parts = p.parts;
     const int64_t rows = (int64_t)a.n_tok * a.n_head;
     a.part_acc = (float *)work;
@@ -200,8 +204,13 @@ MassPgPlan attn_mass_plan(const PgView &c, int io, int n_head, int n_seq, int ma
     p.parts = 1;
     p.few = rows <= kPgRows;
     if (p.few) {
-        // positions of a pair over enough workgroups for four of each compute unit, 128 at a time
-        p.blocks = pairs * std::max<int64_t>(1, std::min<int64_t>((512 + pairs - 1) / pairs, (max_len + 127) / 128));
+        // positions of a pair over enough workgroups for two on each compute unit, 128 at a time; over twice as many, the longest
+        // sequences' first, where 2048 positions are left for each (8 heads of 128 dims, 64 sequences of 2048 to 8192: 145 us
+        // for 162, 32 of 8000 to 32768: 263 for 320; 64 of 8192: 220 for 215; 16 of 8192 would take 48 for 43)
+        const int64_t shares = std::max<int64_t>(std::min<int64_t>((1024 + pairs - 1) / pairs, max_len / 2048),
+                                                 std::min<int64_t>((512 + pairs - 1) / pairs, (max_len + 127) / 128));
+        p.blocks = pairs * std::max<int64_t>(1, shares);
+        p.ranked = n_seq > 1 && p.blocks > 512;
         return p;
     }
     const int64_t keys = c.w <= 128 ? 256 : 128, units = pairs * ((max_len + keys - 1) / keys);
@@ -225,6 +234,7 @@ hipError_t launch_attn_mass(AttnPgArgs a, const MassPgPlan &p, void *work, hipSt
 {
     a.mass_parts = p.parts;
     a.mass_per = p.per;
+    a.ranked = p.ranked;
     a.mass_part = (float *)work;
     hipError_t e = hipErrorInvalidValue;
 #define SMX_CASE(w_, b) if (a.c.w == w_ && a.c.bf16 == b) e = launch_attn_mass_w##w_##_b##b(a, p, s);

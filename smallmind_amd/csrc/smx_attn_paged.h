@@ -42,6 +42,7 @@ struct AttnPgArgs {
     int tile_wgs, tile_blocks;   // workgroups (blocks of rows) of the many-row path; the rest take short sequences
     int short_rows;              // sequences of up to this many rows go the short way (0: none do)
     int chunk, parts;            // tiles that a part has at least; parts (1: the outputs are written at once)
+    int ranked;                  // few rows: the longest sequences first
 };
 
 // How blocks of 128 rows are gone through: by four waves, or by two groups of four that take tiles in turn; in PG_SPARE by
@@ -51,14 +52,14 @@ enum PgMode { PG_SHORT, PG_ONE_GROUP, PG_TWO_GROUPS, PG_SPARE };
 // How a call is cut up.
 struct AttnPgPlan {
     PgMode mode;
-    int chunk, parts, tile_blocks;
+    int chunk, parts, tile_blocks, ranked;
     int64_t tile_wgs, blocks;
     int64_t work_bytes;
 };
 
 struct MassPgPlan {
     bool few;                    // every sequence has up to 32 rows per KV head
-    int parts, per;
+    int parts, per, ranked;
     int64_t blocks, work_bytes;
 };
 

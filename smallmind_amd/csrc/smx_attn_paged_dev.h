@@ -86,6 +86,19 @@ __device__ __forceinline__ Seq seq_of(const AttnPgArgs &a, int b)
     return s;
 }
 
+// The sequence that is n-th by length, the longest first, among the 64 that n is one of.
+__device__ __forceinline__ int nth_longest(const AttnPgArgs &a, int n)
+{
+    const int lane = threadIdx.x & 63, b0 = n & ~63, count = min(64, a.n_seq - b0);
+    const int len = lane < count ? a.lens[b0 + lane] : 0;
+    int rank = lane < count ? 0 : 64;
+    for (int j = 0; j < count; j++) {
+        const int l = __builtin_amdgcn_readlane(len, j);
+        rank += l > len || (l == len && j < lane);
+    }
+    return b0 + __builtin_ctzll(__ballot(rank == n - b0));
+}
+
 // What the rows of tokens at positions t0 .. t1 go through: tiles [0, pre) and [from, end), `count` in all.
 struct Range {
     int pre, from, end, count;

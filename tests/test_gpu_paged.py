@@ -808,3 +808,17 @@ def test_a_conversation(Q):
     step([1, 1, 1])
     step([1, 20, 1])
     c.close()
+
+
+@pytest.mark.parametrize("n_seq", [130, 64, 70])
+def test_many_sequences_of_different_lengths(Q, n_seq):
+    """More workgroups than start at once: the longest sequences go first, equal ones and empty ones among them."""
+    rng = np.random.default_rng(n_seq)
+    lens = [int(n) for n in rng.integers(0, 90, n_seq)]
+    lens[3], lens[-1], lens[10], lens[11] = 0, 4200, 77, 77
+    new = [min(n, 1) for n in lens]
+    B = Batch(Q, rng, F16, F32, 8, 8, 64, 16, lens, new, pad=2)
+    out, lse = run(Q, B)
+    B.check(out, lse, every=5)
+    before = dev(rng.uniform(0, 1, (n_seq, 8, 100)).astype(np.float32))
+    mass(Q, B, {}, before)
