@@ -529,6 +529,11 @@ def verify_draft(target, draft, tokens, u_accept, u_draw, lens=None):
 _ELEM = None
 
 
+def _rows_like(t, dtype):
+    """A contiguous tensor of t's shape and device (empty_like, the quickest way there, keeps strides)."""
+    return _torch().empty_like(t) if dtype is t.dtype and t.is_contiguous() else t.new_empty(t.shape, dtype=dtype)
+
+
 def _elem_type(dtype, what: str) -> int:
     """The smx_type of rows of this torch type."""
     global _ELEM
@@ -608,7 +613,7 @@ def qk_norm_rope(q, k, q_gamma=None, k_gamma=None, eps: float = 1e-6, rotation: 
     head_dim] and k [n_tok, n_kv_head, head_dim] float32, float16 or bfloat16 (tokens may be rows of a fused projection);
     gammas [head_dim] float32 (None: no norm); pos [n_tok], or [n_axes, n_tok], int32.  Returns (q, k) of `dtype` (default:
     as they come), rounded once."""
-    torch, index = _torch(), q.get_device()
+    index = q.get_device()
     if index < 0:
         raise ValueError("operands must be device (cuda) tensors")
     if q.dim() != 3 or k.dtype is not q.dtype or k.dim() != 3 or q.shape[0] != k.shape[0]:
@@ -683,7 +688,7 @@ class GpuPagedCache:
                 _floats(g, hd, what)
         turn, rot, at = _turning(rotation, pos, n)
         with _on_device(index, k, v, places, q, q_gamma, k_gamma, *turn):
-            out = None if q is None else q.new_empty(q.shape, dtype=dtype)
+            out = None if q is None else _rows_like(q, dtype)
             if n:
                 call("smx_paged_append", self._handle(), tin, _opt(q), qs, n_head, k.data_ptr(), ks, v.data_ptr(), vs, _opt(q_gamma),
                      _opt(k_gamma), _eps(eps), rot, at, places.data_ptr(), n, tout, _opt(out), _raw_stream(index))
@@ -821,7 +826,7 @@ def attention_paged(q, cache: GpuPagedCache, starts, lens, tables, max_q: int, m
         raise ValueError(f"out must be contiguous {q.dtype} {tuple(q.shape)}")
     with _on_device(index, q, starts, lens, tables, slopes, prefix, out):
         if out is None:
-            out = q.new_empty(q.shape)
+            out = _rows_like(q, q.dtype)
         sums = q.new_empty((n_tok, n_head), dtype=torch.float32) if lse else None
         need = cache._work_bytes("smx_attention_paged_work_bytes", (t, n_tok, n_head, n_seq, max_q, max_len), (window,))
         work = lens.new_empty((need,), dtype=torch.uint8) if need else None
