@@ -629,8 +629,8 @@ def qk_norm_rope(q, k, q_gamma=None, k_gamma=None, eps: float = 1e-6, rotation: 
         _c_int(x, what)
     turn, rot, at = _turning(rotation, pos, n)
     with _on_device(index, k, q_gamma, k_gamma, *turn):
-        qo = torch.empty(q.shape, dtype=dtype, device=q.device)
-        ko = torch.empty(k.shape, dtype=dtype, device=q.device)
+        qo = _rows_like(q, dtype)
+        ko = _rows_like(k, dtype)
         if n and n_head + k.shape[1]:
             call("smx_qk_norm_rope", tin, q.data_ptr(), qs, n_head, k.data_ptr(), ks, k.shape[1], hd, _opt(q_gamma), _opt(k_gamma),
                  _eps(eps), rot, at, n, tout, qo.data_ptr(), ko.data_ptr(), _raw_stream(index))
