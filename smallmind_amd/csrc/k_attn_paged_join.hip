@@ -141,7 +141,8 @@ AttnPgPlan attn_paged_plan(const PgView &c, int io, int n_tok, int n_head, int n
         // as long as itself; a block costs some six tiles beside its own (1536 over 1536, 384 blocks: 38.7 us for 43.6;
         // but 1280 over 4096, 320 blocks: 128 for 115, and 6 x 256 over 512, 384 blocks: 31 for 22).
         const double longest = span + 6.0, shortest = std::min<double>(span, (max_len - std::min(max_q, max_len)) / kPgTile) + 6.0;
-        if (two && (units <= 256 || 2 * (longest - (longest - shortest) * 256 / units) <= longest)) p.mode = PG_TWO_GROUPS;
+        const double wgs = (double)((p.tile_blocks + n_seq - 1) / n_seq * (int64_t)n_seq * c.n_kv);   // (those that find no rows among them)
+        if (two && (units <= 256 || 2 * (longest - (longest - shortest) * 256 / wgs) <= longest)) p.mode = PG_TWO_GROUPS;
         // More than two blocks for every compute unit: three at a time where their registers allow it (64 dims, 16 prompts of 1023,
         // 12 heads: 61 us for 71; 4096 over 4096, 32 heads over 8: 99 for 111; but 2048 over 8192, 512 blocks: 182 for 175).
         if (spare && units > 512) p.mode = PG_SPARE;
