@@ -211,7 +211,8 @@ template <bool F32> struct Query {
     float unit;            // of the products
 };
 
-// CHECK: a row that holds a NaN or an infinity becomes NaN.
+// CHECK: a row that holds a NaN or an infinity becomes NaN throughout, so that its products are NaN, and only they: what the row does
+// not see is masked as ever, and a row that sees nothing stays one.
 template <bool F32, bool CHECK = true>
 __device__ __forceinline__ void load_q(const AttnPgArgs &a, const Row &r, int h, Query<F32> &Q)
 {
@@ -238,7 +239,15 @@ __device__ __forceinline__ void load_q(const AttnPgArgs &a, const Row &r, int h,
                 for (int e = 0; e < 8; e++) top = max(top, (uint32_t)(v[e] & 0x7FFF));
             }
         }
-        if (CHECK && max_halves(top >= (BF16 ? 0x7F80u : 0x7C00u) ? 1.0f : 0.0f) > 0.0f) Q.unit = __builtin_nanf("");
+        if constexpr (CHECK) {
+            const bool bad = max_halves(top >= (BF16 ? 0x7F80u : 0x7C00u) ? 1.0f : 0.0f) > 0.0f;
+            if (__any(bad)) {
+#pragma unroll
+                for (int n = 0; n < NK; n++)
+#pragma unroll
+                    for (int e = 0; e < 8; e++) Q.q[0][n][e] = bad ? (elem)__builtin_nanf("") : Q.q[0][n][e];
+            }
+        }
     } else {
         float f[NK][8];
         uint32_t top = 0;
@@ -268,7 +277,7 @@ __device__ __forceinline__ void load_q(const AttnPgArgs &a, const Row &r, int h,
             mul = __uint_as_float((268u << 23) - e);
             Q.unit = __uint_as_float(e) * (1.0f / 16384.0f);
         }
-        if (bad) Q.unit = __builtin_nanf("");
+        if (bad) mul = __builtin_nanf("");
 #pragma unroll
         for (int n = 0; n < NK; n++)
 #pragma unroll

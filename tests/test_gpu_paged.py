@@ -822,3 +822,33 @@ def test_many_sequences_of_different_lengths(Q, n_seq):
     B.check(out, lse, every=5)
     before = dev(rng.uniform(0, 1, (n_seq, 8, 100)).astype(np.float32))
     mass(Q, B, {}, before)
+
+
+@pytest.mark.parametrize("cache,io", [(F16, F32), (BF16, BF16), (F16, F16), (BF16, F32)])
+@pytest.mark.parametrize("H,kv", [(4, 2), (40, 1)])
+def test_rows_that_see_nothing_whatever_their_query(Q, cache, io, H, kv):
+    """Tokens before position 0, and one whose only position lies on a page that does not exist."""
+    rng = np.random.default_rng(H)
+    B = Batch(Q, rng, cache, io, H, kv, 64, 16, [3, 40], [7, 2])
+    B.tables[1, 2] = -1
+    B.q[2, 0, 3], B.q[3, H - 1, 0], B.q[8, 1, 9] = math.nan, math.inf, math.nan
+    out, lse = run(Q, B, dict(window=1))
+    blind = np.array([True] * 4 + [False] * 3 + [True] * 2)
+    assert not out[blind].any() and bool((lse[blind] == -math.inf).all())
+    assert np.isfinite(f64(out)[~blind]).all() and np.isfinite(f64(lse)[~blind]).all()
+    B.c.close()
+
+
+@pytest.mark.parametrize("cache,io,hd", [(BF16, BF16, 128), (F16, F16, 64), (F16, F32, 64), (BF16, F32, 128)])
+@pytest.mark.parametrize("lens,new", [([5000, 30], [1, 1]), ([4000, 50], [40, 3]), ([300, 40], [200, 2])])
+def test_queries_that_are_not_finite_in_contexts_of_parts(Q, cache, io, hd, lens, new):
+    """Each its own row alone, whatever number of workgroups goes through the positions."""
+    rng = np.random.default_rng([hd, lens[0]])
+    B = Batch(Q, rng, cache, io, 4, 1, hd, 32, lens, new)
+    clean, sums = (f64(x) for x in run(Q, B))
+    for t, head, d, what in ((0, 1, 7, math.inf), (sum(new) - 1, 0, 0, -math.inf), (new[0] - 1, 3, hd - 1, math.nan), (new[0], 2, 5, math.inf)):
+        B.q[t, head, d] = what
+        clean[t, head], sums[t, head] = np.nan, np.nan
+    out, lse = (f64(x) for x in run(Q, B))
+    assert np.array_equal(out, clean, equal_nan=True) and np.array_equal(lse, sums, equal_nan=True)
+    B.c.close()
