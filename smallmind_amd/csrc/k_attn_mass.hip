@@ -84,6 +84,16 @@ __device__ __forceinline__ float lse_of(const Row &r, float l)
     return !r.valid ? __builtin_huge_valf() : l == -__builtin_huge_valf() ? 0.0f : l * 1.4426950408889634f;
 }
 
+// A row whose lse is NaN (its query, or a position that it sees, is not finite) gives NaN to what it sees and nothing to the rest:
+// its products are NaN, and masked before lse is taken off.
+template <bool F32>
+__device__ __forceinline__ void settle(Query<F32> &Q, float &lse)
+{
+    const bool bad = lse != lse;
+    spoil(Q, bad);
+    if (bad) lse = 0.0f;
+}
+
 // ---- few rows ----------------------------------------------------------------------------------------
 // A workgroup takes a share of a sequence's positions, 32 at a time in turn with its other waves.
 template <bool F32>
@@ -103,9 +113,11 @@ __global__ __launch_bounds__(kWaves * 64) void k_attn_mass_few(const AttnPgArgs 
         Pages P(a, s, head, at / kPgGroup);
         load_k(a, s, P, at, lane, k[0], there[0][0], there[0][1]);
         const Row r = row_of(a, s, head, lane & 31);
-        const float lse = lse_of(r, a.lse_in[(int64_t)r.token * a.n_head + r.head]);
+        float lse = a.lse_in[(int64_t)r.token * a.n_head + r.head];
         Query<F32> Q;
         load_q<F32, false>(a, r, h, Q);   // (a row that is not finite has an lse of NaN)
+        settle(Q, lse);
+        lse = lse_of(r, lse);
         const Shape S(a, a.slopes ? a.slopes[r.head] : 0.0f, Q.unit);
         const Bounds B = bounds_of(a, s, s.first, row_of(a, s, head, s.rows - 1).t);
         const auto go = [&](const elem8 (&kk)[NK], bool th0, bool th1, elem8 (&next)[NK], bool (&th)[2]) {
@@ -197,6 +209,7 @@ __global__ __launch_bounds__(kWaves * 64) void k_attn_mass(const AttnPgArgs a)
         for (int st = s0; st < s1; st++) {
             __syncthreads();   // the rows before have been read
             if (wave < NB) {
+                settle(Q, lse);
 #pragma unroll
                 for (int q = 0; q < NP; q++)
 #pragma unroll

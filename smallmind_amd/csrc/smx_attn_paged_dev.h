@@ -211,8 +211,15 @@ template <bool F32> struct Query {
     float unit;            // of the products
 };
 
-// CHECK: a row that holds a NaN or an infinity becomes NaN throughout, so that its products are NaN, and only they: what the row does
-// not see is masked as ever, and a row that sees nothing stays one.
+// A row that gives NaN: its products become that, and only they, so that what the row does not see is masked as ever, and a row that sees
+// nothing stays one.  (One element is enough: NaN times 0 is NaN.)
+template <bool F32>
+__device__ __forceinline__ void spoil(Query<F32> &Q, bool bad)
+{
+    Q.q[0][0][0] = bad ? (elem)__builtin_nanf("") : Q.q[0][0][0];
+}
+
+// CHECK: a row that holds a NaN or an infinity is spoilt.
 template <bool F32, bool CHECK = true>
 __device__ __forceinline__ void load_q(const AttnPgArgs &a, const Row &r, int h, Query<F32> &Q)
 {
@@ -239,15 +246,7 @@ __device__ __forceinline__ void load_q(const AttnPgArgs &a, const Row &r, int h,
                 for (int e = 0; e < 8; e++) top = max(top, (uint32_t)(v[e] & 0x7FFF));
             }
         }
-        if constexpr (CHECK) {
-            const bool bad = max_halves(top >= (BF16 ? 0x7F80u : 0x7C00u) ? 1.0f : 0.0f) > 0.0f;
-            if (__any(bad)) {
-#pragma unroll
-                for (int n = 0; n < NK; n++)
-#pragma unroll
-                    for (int e = 0; e < 8; e++) Q.q[0][n][e] = bad ? (elem)__builtin_nanf("") : Q.q[0][n][e];
-            }
-        }
+        if constexpr (CHECK) spoil(Q, max_halves(top >= (BF16 ? 0x7F80u : 0x7C00u) ? 1.0f : 0.0f) > 0.0f);
     } else {
         float f[NK][8];
         uint32_t top = 0;
@@ -277,7 +276,6 @@ __device__ __forceinline__ void load_q(const AttnPgArgs &a, const Row &r, int h,
             mul = __uint_as_float((268u << 23) - e);
             Q.unit = __uint_as_float(e) * (1.0f / 16384.0f);
         }
-        if (bad) mul = __builtin_nanf("");
 #pragma unroll
         for (int n = 0; n < NK; n++)
 #pragma unroll
@@ -287,6 +285,7 @@ __device__ __forceinline__ void load_q(const AttnPgArgs &a, const Row &r, int h,
 #pragma unroll
                 for (int k = 0; k < kParts<F32>; k++) Q.q[k][n][e] = p[k][0], Q.q[k][n][e + 1] = p[k][1];
             }
+        spoil(Q, bad);
     }
 }
 

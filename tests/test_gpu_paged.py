@@ -852,3 +852,54 @@ def test_queries_that_are_not_finite_in_contexts_of_parts(Q, cache, io, hd, lens
     out, lse = (f64(x) for x in run(Q, B))
     assert np.array_equal(out, clean, equal_nan=True) and np.array_equal(lse, sums, equal_nan=True)
     B.c.close()
+
+
+# ---- what is not finite, and the ends of the ranges ---------------------------------------------------
+def received(Q, B, lse, hidden=None, **rules):
+    """attention_mass against the plain form with this lse; hidden: positions of sequence 0 that lie on pages that do not exist."""
+    got = f64(Q.attention_mass(B.q, lse, *B.args(), **kernel_rules(rules)))
+    l64 = f64(lse)
+    for b in range(len(B.lens)):
+        want, bound = np.zeros((B.kv, B.max_len)), np.zeros((B.kv, B.max_len))
+        for h, head, S, see in B.rows(b, **rules):
+            if hidden is not None and b == 0:
+                see = see & ~hidden
+            l = l64[B.starts[b]:B.starts[b + 1], head]
+            w, e = R.received(S, np.where(np.isneginf(l), np.inf, l), see)
+            want[h, :B.lens[b]] += w
+            bound[h, :B.lens[b]] += e + 2.0 ** -24 * np.nan_to_num(w) * 4
+        close(torch.from_numpy(got[b]), want, np.nan_to_num(bound))
+
+
+@pytest.mark.parametrize("cache,io,hd", [(F16, F32, 64), (BF16, BF16, 128), (F16, F16, 64), (BF16, F32, 192)])
+@pytest.mark.parametrize("rules", [{}, dict(window=37), dict(window=20, prefix=True), dict(window=50, cap=20.0), dict(window=90, slopes=True)])
+@pytest.mark.parametrize("lens,new", [([100, 333], [1, 3]), ([200, 131], [150, 64]), ([900, 20], [700, 5])])
+def test_received_weights_of_rows_that_are_not_finite(Q, cache, io, hd, rules, lens, new):
+    """A query that is not finite, and positions that are not, count where they are seen and nowhere else."""
+    rng = np.random.default_rng([hd, lens[0]])
+    H, kv = 4, 2
+    B = Batch(Q, rng, cache, io, H, kv, hd, 16, lens, new)
+    rules = dict(rules)
+    if rules.get("slopes"):
+        rules["slopes"] = np.array([0.3, 0.1, 0.02, 0.0], np.float32)
+    if rules.get("prefix"):
+        rules["prefix"] = [9, 3]
+    # a page that the cache does not have, before the last tokens of sequence 0
+    gone = (lens[0] - 20) // 16
+    B.tables[0, gone] = -1
+    hidden = np.arange(lens[0]) // 16 == gone
+    B.q[new[0] // 3, 1, 5] = math.nan
+    B.q[B.starts[1], 2, 0] = math.inf
+    B.q[new[0] // 2, 3, hd - 1] = -math.inf
+
+    def check():
+        _, lse = run(Q, B, rules)
+        l = f64(lse)
+        assert np.isnan(l[new[0] // 3, 1]) and np.isnan(l[B.starts[1], 2]) and np.isnan(l[new[0] // 2, 3])
+        received(Q, B, lse, hidden, **rules)
+    check()
+    for b, p, h in ((0, lens[0] - new[0] // 2 - 1, 0), (1, lens[1] - 2, 1)):
+        B.k[b][p, h] = B.v[b][p, h] = math.nan
+        B.c.append(dev(B.k[b][p:p + 1], cache), dev(B.v[b][p:p + 1], cache), B.places(b, np.array([p])))
+    check()
+    B.c.close()
