@@ -172,6 +172,9 @@ AttnPgArgs batch_args(const smx_paged_cache *c, int type, const void *q, int64_t
     a.io = elem_type(type);
     const double scale = scale_of(v, r);
     a.scale_log2e = (float)(scale * kLog2e);
+    // (the unit is some 2^-14 of the largest of a row: with a factor of 0 what is masked, -inf, would be NaN; scores of rows below this are
+    // below 2^-70, as good as 0)
+    a.q_least = (float)fmax(ldexp(1.0, -100), ldexp(1.0, -112) / (scale * kLog2e));
     if (r) {
         if (r->cap > 0.0f) a.cap_in = (float)(scale / r->cap), a.cap_out = (float)(r->cap * kLog2e);
         a.slopes = r->slopes_dev;

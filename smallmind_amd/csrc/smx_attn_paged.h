@@ -43,6 +43,7 @@ struct AttnPgArgs {
     int short_rows;              // sequences of up to this many rows go the short way (0: none do)
     int chunk, parts;            // tiles that a part has at least; parts (1: the outputs are written at once)
     int ranked;                  // few rows: the longest sequences first
+    float q_least;               // fp32 queries over F16: a row counts as no smaller, so that its unit times scale_log2e is not 0
 };
 
 // How blocks of 128 rows are gone through: by four waves, or by two groups of four that take tiles in turn; in PG_SPARE by

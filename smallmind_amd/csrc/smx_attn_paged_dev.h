@@ -271,7 +271,7 @@ __device__ __forceinline__ void load_q(const AttnPgArgs &a, const Row &r, int h,
         float mul = 1.0f;
         if constexpr (!BF16) {
             // the power of two that brings the row's largest below 2^15
-            const float amax = fmaxf(max_halves(__uint_as_float(min(top, 0x7F7FFFFFu))), 7.8886090522101181e-31f);
+            const float amax = fmaxf(max_halves(__uint_as_float(min(top, 0x7F7FFFFFu))), a.q_least);
             const uint32_t e = __float_as_uint(amax) & 0x7F800000u;
             mul = __uint_as_float((268u << 23) - e);
             Q.unit = __uint_as_float(e) * (1.0f / 16384.0f);

@@ -903,3 +903,17 @@ def test_received_weights_of_rows_that_are_not_finite(Q, cache, io, hd, rules, l
         B.c.append(dev(B.k[b][p:p + 1], cache), dev(B.v[b][p:p + 1], cache), B.places(b, np.array([p])))
     check()
     B.c.close()
+
+
+@pytest.mark.parametrize("new", [[1, 2], [70, 30]])
+@pytest.mark.parametrize("scale", [1e-12, 1e-30, 1e-44])
+def test_scores_below_fp32(Q, new, scale):
+    """Queries of nothing, or all but nothing, and a scale that together leave fp32: every position counts alike."""
+    rng = np.random.default_rng(77)
+    for cache, io in ((F16, F32), (F16, F16), (BF16, F32)):
+        B = Batch(Q, rng, cache, io, 4, 2, 64, 16, [100, 45], new)
+        B.q[::2] = 0.0
+        B.q[1::2] *= 2.0 ** -20
+        B.check(*run(Q, B, dict(scale=scale)), scale=scale)
+        mass(Q, B, dict(scale=scale))
+        B.c.close()
