@@ -132,7 +132,7 @@ __global__ __launch_bounds__(kWaves * 64) void k_attn_mass_few(const AttnPgArgs 
                 for (int n = 0; n < NK; n++)
 #pragma unroll
                     for (int q = 0; q < kParts<F32>; q++) x = mfma(kk[n], Q.q[q][n], n || q ? x : float16v(0.0f));
-                if (S.shaped) shape<true>(a, S, x, r.t, at, h);   // (the sums are fp32 whatever the queries)
+                if (S.shaped) shape<false>(a, S, x, r.t, at, h);   // (the sums are fp32 whatever the queries)
                 if (!th0 || !th1 || !B.whole(s.pre, at, 32)) mask(x, seen(a, s, r.t, at, h, th0, th1));
 #pragma unroll
                 for (int i = 0; i < 16; i++) x[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i], S.c, -lse));
@@ -275,7 +275,7 @@ __global__ __launch_bounds__(kWaves * 64) void k_attn_mass(const AttnPgArgs a)
                 scores(x, j);
                 if (shaped) {
 #pragma unroll
-                    for (int u = 0; u < KT; u++) shape<true>(a, S, x[u], t, at + 32 * u, h);   // (the sums are fp32 whatever the queries)
+                    for (int u = 0; u < KT; u++) shape<false>(a, S, x[u], t, at + 32 * u, h);   // (the sums are fp32 whatever the queries)
                 }
                 if (!all || !B.whole(s.pre, at, 32 * KT)) {
 #pragma unroll

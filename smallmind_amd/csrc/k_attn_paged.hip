@@ -253,7 +253,7 @@ __device__ __forceinline__ void interleave()
 
 // A block of 128 rows, gone through by NG groups of four waves that take tiles in turn.  SPARE: without the registers for
 // another tile's scores.
-template <bool F32, int NG, bool SPARE>
+template <bool F32, int NG, bool SPARE, bool QUICK>
 __device__ __forceinline__ void many(const AttnPgArgs &a, Many<NG> &M, const Seq &s, int head, int row0, int part)
 {
     constexpr int NP = kParts<F32>;
@@ -346,7 +346,7 @@ __device__ __forceinline__ void many(const AttnPgArgs &a, Many<NG> &M, const Seq
                 if (!AHEAD) scores(x, T.k[at], t0);
                 if (S.shaped) {
 #pragma unroll
-                    for (int t = 0; t < KT; t++) shape<F32>(a, S, x[t], r.t, pos + 32 * (t0 + t), h);
+                    for (int t = 0; t < KT; t++) shape<QUICK>(a, S, x[t], r.t, pos + 32 * (t0 + t), h);
                 }
                 if (cut) {
 #pragma unroll
@@ -417,7 +417,7 @@ template <int NW> union Few {
     Handed<NW / 2> j;
 };
 
-template <bool F32, int NW>
+template <bool F32, int NW, bool QUICK>
 __device__ __forceinline__ void few(const AttnPgArgs &a, Few<NW> &F, const Seq &s, int head, int part)
 {
     const int lane = threadIdx.x & 63, h = lane >> 5, wave = wave_id();
@@ -483,7 +483,7 @@ __device__ __forceinline__ void few(const AttnPgArgs &a, Few<NW> &F, const Seq &
             for (int p = 0; p < kParts<F32>; p++) x[0] = mfma(k[n], Q.q[p][n], n || p ? x[0] : float16v(0.0f));
         if (more) fetch_k();
         if (B.none(s.pre, at, 32)) continue;
-        if (S.shaped) shape<F32>(a, S, x[0], r.t, at, h);
+        if (S.shaped) shape<QUICK>(a, S, x[0], r.t, at, h);
         if (cut) mask(x[0], seen(a, s, r.t, at, h, th0, th1));
         elem8 w[kParts<F32>][2];
         const float e = R.refer<1>(x, S.c);
@@ -510,7 +510,7 @@ __device__ __forceinline__ void few(const AttnPgArgs &a, Few<NW> &F, const Seq &
 
 // Finds the block's sequence.  Block x belongs to the last sequence whose first block floor(start * group / 128) + b is
 // not above x: no sequence has more blocks than lie between its own first and the next one's.
-template <bool F32, int NG, bool SPARE>
+template <bool F32, int NG, bool SPARE, bool QUICK>
 __device__ __forceinline__ void many_rows(const AttnPgArgs &a, Many<NG> &M)
 {
     constexpr int ROWS = 4 * kPgRows;
@@ -532,11 +532,12 @@ __device__ __forceinline__ void many_rows(const AttnPgArgs &a, Many<NG> &M)
     const Seq s = seq_of(a, b);
     const int64_t row0 = (block - ((int64_t)s.start * a.group / ROWS + b)) * ROWS;
     if (row0 >= s.rows || s.rows <= a.short_rows) return;
-    many<F32, NG, SPARE>(a, M, s, pair % a.c.n_kv, (int)row0, pair / a.c.n_kv);
+    many<F32, NG, SPARE, QUICK>(a, M, s, pair % a.c.n_kv, (int)row0, pair / a.c.n_kv);
 }
 
-// Workgroups [0, tile_wgs): blocks of 128 rows, gone through as MODE says; the others: a short sequence each.
-template <bool F32, PgMode MODE>
+// Workgroups [0, tile_wgs): blocks of 128 rows, gone through as MODE says; the others: a short sequence each.  QUICK: how a cap's tanh is
+// computed.
+template <bool F32, PgMode MODE, bool QUICK = !F32>
 __global__ __launch_bounds__(MODE == PG_TWO_GROUPS ? 512 : 256, MODE == PG_SHORT && W <= 128 && W * kParts<F32> <= 256 ? 2 : 1) void k_attn_paged(const AttnPgArgs a)
 {
     constexpr int NG = MODE == PG_TWO_GROUPS ? 2 : 1, NW = 4 * NG;
@@ -548,7 +549,7 @@ __global__ __launch_bounds__(MODE == PG_TWO_GROUPS ? 512 : 256, MODE == PG_SHORT
     Mem &M = *(Mem *)mem;
     if constexpr (MODE != PG_SHORT) {
         if ((int)blockIdx.x < a.tile_wgs) {
-            many_rows<F32, NG, MODE == PG_SPARE>(a, M.many);
+            many_rows<F32, NG, MODE == PG_SPARE, QUICK>(a, M.many);
             return;
         }
     }
@@ -558,7 +559,7 @@ __global__ __launch_bounds__(MODE == PG_TWO_GROUPS ? 512 : 256, MODE == PG_SHORT
     const int b = ranked ? nth_longest(a, rest / a.parts) : rest % a.n_seq, part = ranked ? rest % a.parts : rest / a.n_seq;
     const Seq s = seq_of(a, b);
     if (s.rows <= 0 || s.rows > kPgRows) return;
-    few<F32, NW>(a, M.few, s, head, part);
+    few<F32, NW, QUICK>(a, M.few, s, head, part);
 }
 
 // Whether two groups of four waves find registers: 256 a lane.
@@ -570,6 +571,15 @@ template <bool F32>
 hipError_t launch(const AttnPgArgs &a, const AttnPgPlan &p, hipStream_t s)
 {
     const unsigned n = (unsigned)p.blocks;
+    if constexpr (!F32) {
+        // (a large cap is rare: one group of waves on every block, so that the other instances need not hold its tanh as well, which
+        // takes registers of theirs: mixed chunks and decodes with a window 41 us for 38)
+        if (a.cap_in != 0.0f && a.cap_out > kQuickCap) {
+            if (p.mode == PG_SHORT) k_attn_paged<F32, PG_SHORT, false><<<n, 256, 0, s>>>(a);
+            else k_attn_paged<F32, PG_ONE_GROUP, false><<<n, 256, 0, s>>>(a);
+            return hipGetLastError();
+        }
+    }
     if (p.mode == PG_SHORT) k_attn_paged<F32, PG_SHORT><<<n, 256, 0, s>>>(a);
     if (p.mode == PG_ONE_GROUP) k_attn_paged<F32, PG_ONE_GROUP><<<n, 256, 0, s>>>(a);
     if constexpr (kTwoGroups<F32>)

@@ -176,7 +176,8 @@ AttnPgArgs batch_args(const smx_paged_cache *c, int type, const void *q, int64_t
     // below 2^-70, as good as 0)
     a.q_least = (float)fmax(ldexp(1.0, -100), ldexp(1.0, -112) / (scale * kLog2e));
     if (r) {
-        if (r->cap > 0.0f) a.cap_in = (float)(scale / r->cap), a.cap_out = (float)(r->cap * kLog2e);
+        // (a cap so large that scale / cap leaves fp32's normal numbers changes no score of products below 2^113 by 2^-24 of itself)
+        if (r->cap > 0.0f && scale / r->cap >= 1.17549435e-38) a.cap_in = (float)(scale / r->cap), a.cap_out = (float)(r->cap * kLog2e);
         a.slopes = r->slopes_dev;
         a.prefix = r->prefix_dev;
         a.window = window_of(r, max_len);

@@ -357,14 +357,15 @@ struct Shape {
 // Position (of 32) of a lane's element i.
 __device__ __forceinline__ int pos32(int i, int h) { return 8 * (i >> 2) + 4 * h + (i & 3); }
 
-// x of 32 positions from `at` on.  With 16-bit outputs tanh is 1 - 2 / (1 + e^2y), off by up to 2^-21 where the series keeps
-// small values to 2^-24 of themselves: 2^-21 of the cap in a score, which a weight's 8 or 11 bits do not notice, for 5
-// instructions in place of 19.
-template <bool F32>
+// x of 32 positions from `at` on.  QUICK, for 16-bit outputs and caps up to kQuickCap: tanh is 1 - 2 / (1 + e^2y), off by up to 2^-21
+// where the series keeps small values to 2^-24 of themselves: 2^-21 of the cap in a score, 2^-14 at most, which a weight's 8 or 11
+// bits do not notice, for 5 instructions in place of 19.
+constexpr float kQuickCap = 128.0f * 1.4426950408889634f;   // (as an exponent of 2)
+template <bool QUICK>
 __device__ __forceinline__ void shape(const AttnPgArgs &a, const Shape &S, float16v &x, int t, int at, int h)
 {
     const float away = (float)(t - at - 4 * h);   // (exact: positions are below 2^24)
-    if (!F32 && a.cap_in != 0.0f) {
+    if (QUICK && a.cap_in != 0.0f) {
         const float in = S.in * 2.8853900817779268f;
 #pragma unroll
         for (int i = 0; i < 16; i++)
@@ -373,7 +374,7 @@ __device__ __forceinline__ void shape(const AttnPgArgs &a, const Shape &S, float
 #pragma unroll
             for (int i = 0; i < 16; i++) x[i] = __builtin_fmaf(-S.slope, fabsf(away - (float)pos32(i, 0)), x[i]);
         }
-    } else if (F32 && a.cap_in != 0.0f) {
+    } else if (!QUICK && a.cap_in != 0.0f) {
 #pragma unroll
         for (int i = 0; i < 16; i++) {
             x[i] = tanh_of(x[i] * S.in) * a.cap_out;

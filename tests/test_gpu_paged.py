@@ -917,3 +917,45 @@ def test_scores_below_fp32(Q, new, scale):
         B.check(*run(Q, B, dict(scale=scale)), scale=scale)
         mass(Q, B, dict(scale=scale))
         B.c.close()
+
+
+@pytest.mark.parametrize("cache,io", [(F16, F16), (BF16, BF16), (F16, F32)])
+@pytest.mark.parametrize("cap,scale", [(130.0, None), (5000.0, None), (1e6, None), (1e30, None), (1e36, 1e-6)])
+@pytest.mark.parametrize("lens,new", [([300, 65], [1, 3]), ([260, 97], [130, 40])])
+def test_caps_far_above_the_scores(Q, cache, io, cap, scale, lens, new):
+    """The cap then changes little, and is off by little: 2^-20 of the score where tanh is computed, whatever the cap."""
+    rng = np.random.default_rng(int(math.log2(cap)))
+    if scale:
+        cache = io = BF16
+    B = Batch(Q, rng, cache, io, 4, 2, 64, 16, lens, new)
+    if scale:
+        B.q *= 2.0 ** 17     # (products of some 10^6 to 10^7)
+    rules = dict(cap=cap) if scale is None else dict(cap=cap, scale=scale)
+    out, lse = run(Q, B, rules)
+    for b in range(len(lens)):
+        at = slice(B.starts[b], B.starts[b + 1])
+        for h, head, S, see in B.rows(b, **rules):
+            if io == cache:
+                # (that of the score without a cap, and the tanh's)
+                S.e = R.Scores(f64(B.q[at, head]), B.k[b][:, h], None, io, cache, scale).e + np.abs(S.s) * 2.0 ** -20
+            o, e, l, le = R.attention(S, B.v[b][:, h], see, io, cache)
+            close(out[at, head], o, e)
+            close(lse[at, head], l, le)
+    B.c.close()
+
+
+@pytest.mark.parametrize("cap", [128.0, 3000.0])
+def test_large_caps_of_many_blocks(Q, cap):
+    """More than two blocks for every compute unit, with a cap at and above the quick tanh's."""
+    rng = np.random.default_rng(79)
+    for cache, hd in ((F16, 64), (BF16, 32)):
+        B = Batch(Q, rng, cache, cache, 300, 300, hd, 16, [200, 90, 33], [170, 40, 1])
+        out, lse = run(Q, B, dict(cap=cap))
+        for b in range(3):
+            at = slice(B.starts[b], B.starts[b + 1])
+            for h, head, S, see in B.rows(b, cap=cap, every=17):
+                S.e = R.Scores(f64(B.q[at, head]), B.k[b][:, h], None, cache, cache).e + (np.abs(S.s) * 2.0 ** -20 if cap > 128 else cap * 2.0 ** -21)
+                o, e, l, le = R.attention(S, B.v[b][:, h], see, cache, cache)
+                close(out[at, head], o, e)
+                close(lse[at, head], l, le)
+        B.c.close()
