@@ -175,7 +175,7 @@ struct Token {
 };
 
 // One kind of rows of a token: queries, or keys with their values (KV).  put(row, y, v): the row normed and turned, its V row.
-// f (x A + z B) with A = gamma c and B = gamma' s: the norm's factor f last.
+// x f A + z f B with A = gamma c and B = gamma' s: the norm's factor f first, since x gamma may leave fp32 where x f gamma does not.
 template <int TYPE, bool VEC, bool KV, typename Put>
 __device__ __forceinline__ void each_row(const PgWriteArgs &a, const Token &k, const void *src, const void *vsrc, int rows, const float *gamma,
                                          bool norm, Put put)
@@ -220,17 +220,19 @@ __device__ __forceinline__ void each_row(const PgWriteArgs &a, const Token &k, c
         const Raw r = ahead[0];
         ahead[0] = ahead[1];
         load(ahead[1], g + 2 * k.step);
-        float y[8], f = 1.0f;
+        float y[8], xs[8], zs[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) xs[i] = (float)r.x[i], zs[i] = halves ? (float)r.z[i] : 0.0f;
         if (norm) {
             float sq = 0.0f;
 #pragma unroll
-            for (int i = 0; i < 8; i++) sq = __builtin_fmaf((float)r.x[i], (float)r.x[i], sq);
+            for (int i = 0; i < 8; i++) sq = __builtin_fmaf(xs[i], xs[i], sq);
             const float m = row_sum(sq, a.group_shift) * a.inv_hd + a.eps;
-            f = __builtin_amdgcn_rsqf(m);
+            float f = __builtin_amdgcn_rsqf(m);
             // squares that leave fp32 (fp16's do not): again, with a power of two
             const bool far = TYPE != PG_F16 && !(m >= 1.17549435e-38f && m < __builtin_huge_valf());
             if (__any(far)) {
-                const float by = m < 1.0f ? 4.722366482869645e21f : 2.117582368135751e-22f;
+                const float by = m < 1.0f ? 0x1p96f : 0x1p-72f;
                 // (from memory, one by one: few registers for what hardly ever happens)
                 const E *p = x - 3 * stride + d0;
                 sq = 0.0f;
@@ -239,16 +241,22 @@ __device__ __forceinline__ void each_row(const PgWriteArgs &a, const Token &k, c
                     const float w = (float)p[i] * by;
                     sq = __builtin_fmaf(w, w, sq);
                 }
-                sq = row_sum(sq, a.group_shift) * a.inv_hd + a.eps * by * by;
-                if (far) f = by / sqrtf(sq);
+                const float root = 1.0f / sqrtf(row_sum(sq, a.group_shift) * a.inv_hd + a.eps * by * by);
+                // x by root, in the order that leaves no product outside: small rows times `by` first, large ones last
+                const float last = !far ? 1.0f : m < 1.0f ? root : by;
+                if (far) f = m < 1.0f ? by : root;
+#pragma unroll
+                for (int i = 0; i < 8; i++) xs[i] *= f, zs[i] *= f;
+                f = last;
             }
+#pragma unroll
+            for (int i = 0; i < 8; i++) xs[i] *= f, zs[i] *= f;
         }
 #pragma unroll
         for (int i = 0; i < 8; i++) {
-            float z = halves ? (float)r.z[i] : (float)r.x[i ^ 1];
+            float z = halves ? zs[i] : xs[i ^ 1];
             if (partial) z = i < T.on ? z : 0.0f;
-            y[i] = __builtin_fmaf(z, B[i], (float)r.x[i] * A[i]);
-            if (norm) y[i] *= f;
+            y[i] = __builtin_fmaf(z, B[i], xs[i] * A[i]);
         }
         put(g, y, r.v);
     }

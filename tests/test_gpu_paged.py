@@ -959,3 +959,27 @@ def test_large_caps_of_many_blocks(Q, cap):
                 close(out[at, head], o, e)
                 close(lse[at, head], l, le)
         B.c.close()
+
+
+@pytest.mark.parametrize("exponent,gamma,tin", [(126, 1, F32), (126, 1, BF16), (60, 72, F32), (60, 72, BF16), (-60, -80, F32), (-60, -80, BF16),
+                                                (-132, 0, F32), (-140, 3, F32), (-132, 0, BF16)])
+@pytest.mark.parametrize("hd,halves", [(8, True), (104, False), (128, True), (256, False)])
+def test_norms_at_the_ends_of_the_range(Q, hd, halves, exponent, gamma, tin):
+    """Rows, and weights, whose products leave fp32 though what they come to does not; beside ordinary rows."""
+    rng = np.random.default_rng([hd, 300 + exponent])
+    n = 9
+    x = np.clip(rng.normal(0, 0.6, (n, 3, hd)), -1.9, 1.9) * np.exp2(np.where(rng.uniform(size=(n, 3, 1)) < 0.6, exponent, 0))
+    x = dev(x, tin)
+    assert bool(torch.isfinite(x).all()) and bool((x.double().abs().amax(2) > 0).all())
+    g = (rng.normal(1, 0.3, hd) * 2.0 ** gamma).astype(np.float32)
+    cos, sin = tables(rng, 16, hd // 2)
+    pos = rng.integers(0, 16, (1, n)).astype(np.int32)
+    a = dev(g), dev(g), 0.0, Q.Rotation(cos, sin, halves=halves), dev(pos)
+    q, k = Q.qk_norm_rope(x, x[:, :2], *a, dtype=F32)
+    want, e = R.turned(f64(x), g, 0.0, cos.cpu().numpy(), sin.cpu().numpy(), pos, [hd // 2], halves)
+    close(q, want, e)
+    close(k, want[:, :2], e[:, :2])
+    c = Q.GpuPagedCache(BF16, 1, 2, hd, 16)
+    c.append(x[:, :2], torch.ones_like(x[:, :2]), i32(np.arange(n)), q_gamma=a[0], k_gamma=a[1], eps=0.0, rotation=a[3], pos=a[4])
+    close(c.read(i32(np.arange(n)))[0], want[:, :2], e[:, :2] + R.HALF_STEP[BF16] * (np.abs(want) + e)[:, :2])
+    c.close()
