@@ -229,8 +229,8 @@ __device__ __forceinline__ void each_row(const PgWriteArgs &a, const Token &k, c
             for (int i = 0; i < 8; i++) sq = __builtin_fmaf(xs[i], xs[i], sq);
             const float m = row_sum(sq, a.group_shift) * a.inv_hd + a.eps;
             float f = __builtin_amdgcn_rsqf(m);
-            // squares that leave fp32 (fp16's do not): again, with a power of two
-            const bool far = TYPE != PG_F16 && !(m >= 1.17549435e-38f && m < __builtin_huge_valf());
+            // squares that leave fp32 (fp16's do not, but the least eps beside zeros does): again, with a power of two
+            const bool far = !(m >= 1.17549435e-38f && m < __builtin_huge_valf());
             if (__any(far)) {
                 const float by = m < 1.0f ? 0x1p96f : 0x1p-72f;
                 // (from memory, one by one: few registers for what hardly ever happens)

@@ -983,3 +983,12 @@ def test_norms_at_the_ends_of_the_range(Q, hd, halves, exponent, gamma, tin):
     c.append(x[:, :2], torch.ones_like(x[:, :2]), i32(np.arange(n)), q_gamma=a[0], k_gamma=a[1], eps=0.0, rotation=a[3], pos=a[4])
     close(c.read(i32(np.arange(n)))[0], want[:, :2], e[:, :2] + R.HALF_STEP[BF16] * (np.abs(want) + e)[:, :2])
     c.close()
+
+
+@pytest.mark.parametrize("tin", [F16, BF16, F32])
+def test_rows_of_zeros_with_the_least_eps(Q, tin):
+    x = torch.zeros(3, 2, 64, dtype=tin, device="cuda")
+    x[1] = 1.0
+    g = torch.ones(64, device="cuda")
+    q, _ = Q.qk_norm_rope(x, x, g, g, 1e-40, dtype=F32)
+    close(q, f64(x), 72 * 2.0 ** -24)
