@@ -41,6 +41,15 @@ int elem_bytes(int pg) { return pg == PG_F32 ? 4 : 2; }
 int cache_type(const PgView &v) { return v.bf16 ? PG_BF16 : PG_F16; }
 bool misaligned(const void *p, int bytes) { return (uintptr_t)p % bytes != 0; }
 
+// Whether `bytes` bytes from p on meet one of the n rows of `row` elements of `size` bytes, `stride` elements apart, from q on.  (All are
+// positive, and stride no less than row; of one row it may be anything.)
+bool meet(const void *p, int64_t bytes, const void *q, int64_t n, int64_t stride, int64_t row, int size)
+{
+    const __int128 step = (__int128)stride * size, at = (__int128)(uintptr_t)p - (uintptr_t)q, far = at - row * size;
+    const __int128 i = far < 0 ? 0 : far / step + 1;   // the first row that ends behind p
+    return i < n && i * step < at + bytes;
+}
+
 // The cache's memory is on its device, so the call's stream has to be too.
 int check_device(const smx_paged_cache *c, const char *fn)
 {
@@ -114,6 +123,21 @@ int check_rows(int in_type, const void *q, int64_t q_stride, int n_head, const v
              (!k || (!misaligned(k, 16) && k_stride % piece == 0 && (cache || !misaligned(k_out, 16)))) &&
              (!v || (!misaligned(v, 16) && v_stride % piece == 0));
     return check_rotation(rot, pos, hd, fn, &a->rot);
+}
+
+// Outputs where inputs lie: other waves may still read there.
+int check_apart(const PgWriteArgs &a, int type, const char *fn)
+{
+    const int in = elem_bytes(type);
+    const int64_t out = elem_bytes(a.out_type), hd = a.hd;
+    const auto met = [&](const void *o, int64_t heads) {
+        const int64_t n = o ? a.n_tok * heads * hd * out : 0;
+        return n && ((a.q && meet(o, n, a.q, a.n_tok, a.q_stride, a.n_head * hd, in)) ||
+                     (a.k && meet(o, n, a.k, a.n_tok, a.k_stride, a.n_kv * hd, in)) ||
+                     (a.v && meet(o, n, a.v, a.n_tok, a.v_stride, a.n_kv * hd, in)));
+    };
+    if (met(a.q ? a.q_out : nullptr, a.n_head) || met(a.k_out, a.n_kv)) SMX_FAIL(SMX_EINVAL, "%s: an output lies in the inputs' memory", fn);
+    return SMX_OK;
 }
 
 // What an attention call and one for received weights have in common; `a` gets it.
@@ -301,9 +325,9 @@ SMX_API int smx_qk_norm_rope(int in_type, const void *q_dev, int64_t q_stride, i
     if ((!q_dev && !k_dev) || (q_dev && !q_out_dev) || (k_dev && !k_out_dev)) SMX_FAIL(SMX_EINVAL, "%s: null argument", fn);
     PgWriteArgs a;
     int type;
-    const int rc = check_rows(in_type, q_dev, q_stride, n_head, k_dev, k_stride, nullptr, 0, n_kv_head, head_dim, q_gamma_dev,
+    int rc = check_rows(in_type, q_dev, q_stride, n_head, k_dev, k_stride, nullptr, 0, n_kv_head, head_dim, q_gamma_dev,
                               k_gamma_dev, eps, rot, pos_dev, n_tok, out_type, q_out_dev, k_out_dev, false, fn, &a, &type);
-    if (rc != SMX_OK || n_tok == 0) return rc;
+    if (rc != SMX_OK || n_tok == 0 || (rc = check_apart(a, type, fn)) != SMX_OK) return rc;
     SMX_HIP(launch_paged_write(a, type, (hipStream_t)stream));
     return SMX_OK;
 }
@@ -321,7 +345,7 @@ SMX_API int smx_paged_append(smx_paged_cache *c, int in_type, const void *q_dev,
     if (rc != SMX_OK) return rc;
     if (misaligned(places_dev, 4)) SMX_FAIL(SMX_EINVAL, "%s: misaligned pointer", fn);
     if (n_tok == 0) return SMX_OK;
-    if ((rc = check_device(c, fn)) != SMX_OK) return rc;
+    if ((rc = check_apart(a, type, fn)) != SMX_OK || (rc = check_device(c, fn)) != SMX_OK) return rc;
     a.c = c->view;
     a.places = places_dev;
     SMX_HIP(launch_paged_write(a, type, (hipStream_t)stream));
@@ -386,6 +410,11 @@ SMX_API int smx_attention_paged(const smx_paged_cache *c, int type, const void *
     AttnPgPlan p;
     if ((rc = plan_attention(c, type, n_tok, n_head, n_seq, max_q, max_len, rules, fn, &p)) != SMX_OK) return rc;
     if ((rc = check_work(work_dev, work_bytes, p.work_bytes, fn)) != SMX_OK) return rc;
+    const int size = elem_bytes(elem_type(type));
+    const int64_t rows = (int64_t)n_tok * n_head, hd = c->view.hd;
+    if (meet(out_dev, rows * hd * size, q_dev, n_tok, q_stride, n_head * hd, size) ||
+        (lse_dev && meet(lse_dev, rows * 4, q_dev, n_tok, q_stride, n_head * hd, size)))
+        SMX_FAIL(SMX_EINVAL, "%s: an output lies in q's memory", fn);
     if ((rc = check_device(c, fn)) != SMX_OK) return rc;
     AttnPgArgs a = batch_args(c, type, q_dev, q_stride, n_tok, n_head, n_seq, starts_dev, lens_dev, tables_dev, table_stride, max_q,
                               max_len, rules);

@@ -818,7 +818,7 @@ def attention_paged(q, cache: GpuPagedCache, starts, lens, tables, max_q: int, m
     tanh(score / cap) where cap > 0, less slopes[h] * |t - p| ([n_head] float32).
     Returns [n_tok, n_head, head_dim] of q's type, or that and, with lse, the logarithms of the sums of exponentials
     [n_tok, n_head] float32.  Rows that see nothing are zeros (lse -inf).  Rows of no sequence are left as they are in
-    `out`, undefined where that is not given."""
+    `out`, undefined where that is not given.  `out` must not lie in q's memory."""
     torch, h, index = _torch(), cache._handle(), cache.device.index
     n_tok, n_head, n_seq, stride, t, max_len = _paged_batch(q, cache, starts, lens, tables, max_q, max_len)
     rules = _rules(n_seq, n_head, scale, cap, slopes, window, prefix)

@@ -992,3 +992,43 @@ def test_rows_of_zeros_with_the_least_eps(Q, tin):
     g = torch.ones(64, device="cuda")
     q, _ = Q.qk_norm_rope(x, x, g, g, 1e-40, dtype=F32)
     close(q, f64(x), 72 * 2.0 ** -24)
+
+
+def test_outputs_in_the_inputs_memory_are_refused(Q):
+    from smallmind_amd._lib import SmxError
+    rng = np.random.default_rng(80)
+    B = Batch(Q, rng, F16, F16, 4, 2, 64, 16, [40, 9], [3, 1])
+    n, row = 4, 4 * 64
+    buf = torch.zeros(8 * n * row, dtype=F16, device="cuda")
+    q = buf[n * row:2 * n * row].view(n, 4, 64).copy_(B.q)
+    for at in (n * row, row, 2 * n * row - 8):                        # on q, from before it into it, on its end
+        with pytest.raises(SmxError, match="lies in q's memory"):
+            Q.attention_paged(q, *B.args(), out=buf[at:at + n * row].view(n, 4, 64))
+    for at in (0, 2 * n * row):                                       # right before it, right behind
+        out, lse = Q.attention_paged(q, *B.args(), out=buf[at:at + n * row].view(n, 4, 64), lse=True)
+        assert out.data_ptr() == buf.data_ptr() + 2 * at
+        B.check(out, lse)
+    # between rows of q that lie far apart
+    wide = buf.view(n, -1)[:, :row].unflatten(1, (4, 64)).copy_(B.q)
+    B.check(*Q.attention_paged(wide, *B.args(), out=buf[row:row + n * row].view(n, 4, 64), lse=True))
+    with pytest.raises(SmxError, match="lies in q's memory"):
+        Q.attention_paged(wide, *B.args(), out=buf[5 * row:9 * row].view(n, 4, 64))
+    B.c.close()
+
+
+def test_appends_into_their_inputs_are_refused(Q):
+    from smallmind_amd import _lib
+    lib, s = _lib.load(), torch.cuda.current_stream().cuda_stream
+    c = Q.GpuPagedCache(F16, 1, 1, 64, 16)
+    f = torch.randn(3, 256, device="cuda")                 # rows of 2 + 1 + 1 heads
+    out, at = torch.zeros(3, 2, 64, device="cuda"), i32([0, 1, 2])
+
+    def append(to):
+        return lib.smx_paged_append(c._h, 0, f.data_ptr(), 256, 2, f.data_ptr() + 512, 256, f.data_ptr() + 768, 256, None, None, 0.0, None, None,
+                                    at.data_ptr(), 3, 0, to, s)
+    for off in (0, 512, 764, 2 * 1024 + 1020, -4):
+        assert append(f.data_ptr() + off) == -1 and b"lies in the inputs' memory" in lib.smx_last_error()
+    assert append(out.data_ptr()) == 0
+    assert torch.equal(out.flatten(1), f[:, :128])
+    assert torch.equal(c.read(at)[1].flatten(1), f[:, 192:].half())
+    c.close()

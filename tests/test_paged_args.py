@@ -70,6 +70,19 @@ def test_qk_norm_rope_refuses(lib):
         assert run(**bad) == -5, bad
 
 
+def test_writes_into_their_inputs_are_refused(lib):
+    """3 tokens of 2 heads of queries and 1 of keys, 64 fp32 values each, in rows of a fused projection 1024 bytes apart."""
+    base, end = 1 << 20, (1 << 20) + 3 * 1024
+    for qo, ko in ((base, end), (base + 1024 * 2 + 508, end), (base - 1532, end), (end, base + 512), (end, base + 1024 * 2 + 764),
+                   (end, base - 764), (end, base + 256)):
+        p = [ctypes.c_void_p(x) for x in (base, base + 512, qo, ko)]
+        assert lib.smx_qk_norm_rope(F32, p[0], 256, 2, p[1], 256, 1, 64, None, None, 0.0, None, None, 3, F32, p[2], p[3], None) == -1, (qo, ko)
+        assert b"lies in the inputs' memory" in lib.smx_last_error()
+    # one token's stride may be anything
+    p = [ctypes.c_void_p(x) for x in (base, base + 512, base + 252, end)]
+    assert lib.smx_qk_norm_rope(F32, p[0], 1 << 62, 2, p[1], 1 << 62, 1, 64, None, None, 0.0, None, None, 1, F32, p[2], p[3], None) == -1
+
+
 def test_python_refuses_before_any_call():
     import types
 
