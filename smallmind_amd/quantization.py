@@ -781,6 +781,8 @@ def _rules(n_seq, n_head, scale, cap, slopes, window, prefix):
     for x, what in ((0.0 if scale is None else scale, "scale"), (cap, "cap")):
         if not 0.0 <= x < 3.4e38:
             raise ValueError(f"{what} {x} must be finite and not negative")
+        if 0.0 < x < 1.4e-45:      # (0 in fp32, which stands for the default scale and for no cap)
+            raise ValueError(f"{what} {x} is below the range of float32")
     if scale is not None and not scale > 0.0:
         raise ValueError("scale must be positive")
     return ctypes.byref(_lib.AttentionRulesC(0.0 if scale is None else scale, cap, _opt(slopes), _opt(prefix), window, 0))

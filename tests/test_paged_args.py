@@ -124,6 +124,16 @@ def test_python_refuses_before_any_call():
         Q.attention_paged(q, cache, two, one, tab, 1, 64, out=torch.zeros(1, 1, 64).half())
 
 
+def test_factors_below_fp32_are_refused_in_python():
+    """0 in fp32, which would be taken for the default scale and for no cap."""
+    from smallmind_amd import quantization as Q
+    for bad in (dict(scale=1e-46), dict(scale=1e-300), dict(cap=1e-46), dict(cap=5e-324)):
+        with pytest.raises(ValueError, match="below the range"):
+            Q._rules(1, 1, **{**dict(scale=None, cap=0.0, slopes=None, window=0, prefix=None), **bad})
+    for scale in (1.4e-45, 2e-45, 1.0):
+        assert Q._rules(1, 1, scale, 0.0, None, 0, None)._obj.scale > 0.0
+
+
 def test_plain_rotation_keeps_lengths_and_turns_by_axes():
     rng = np.random.default_rng(0)
     x = rng.normal(0, 1, (5, 2, 16))
