@@ -201,7 +201,8 @@ static int attn_mass_blocks(const PgView &c, int io)
 MassPgPlan attn_mass_plan(const PgView &c, int io, int n_head, int n_seq, int max_q, int max_len)
 {
     MassPgPlan p{};
-    const int64_t rows = (int64_t)max_q * (n_head / c.n_kv), pairs = (int64_t)n_seq * c.n_kv;
+    // (max_q is a bound, and may be any: no call has rows of more than 2^31 - 1 values in all)
+    const int64_t rows = std::min<int64_t>((int64_t)max_q * (n_head / c.n_kv), 0x7FFFFFFF / (c.n_kv * c.hd)), pairs = (int64_t)n_seq * c.n_kv;
     p.parts = 1;
     p.few = rows <= kPgRows;
     if (p.few) {
@@ -224,7 +225,7 @@ MassPgPlan attn_mass_plan(const PgView &c, int io, int n_head, int n_seq, int ma
     // is at most 6 MB or so (2048 over 32768: 610 us with 3 parts, 632 with 8).
     const int64_t few = std::max<int64_t>(32768 / (c.w * attn_mass_parts(c, io)), (rows * units + 511) / 512);
     const int64_t many = std::max<int64_t>(1024, (rows * units + 2999) / 3000);
-    p.per = (int)((std::min(few, many) + 32 * nb - 1) / (32 * nb));
+    p.per = (int)std::min((std::min(few, many) + 32 * nb - 1) / (32 * nb), blocks);
     p.parts = (int)((blocks + p.per - 1) / p.per);
     p.blocks = units * p.parts;
     p.work_bytes = p.parts > 1 ? (int64_t)p.parts * pairs * max_len * 4 : 0;

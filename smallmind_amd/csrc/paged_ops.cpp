@@ -242,8 +242,9 @@ int plan_attention(const smx_paged_cache *c, int type, int n_tok, int n_head, in
 
 int plan_mass(const smx_paged_cache *c, int type, int n_head, int n_seq, int max_q, int max_len, const char *fn, MassPgPlan *p)
 {
-    *p = attn_mass_plan(c->view, elem_type(type), n_head, n_seq, max_q, max_len);
-    if (p->blocks > kMaxBlocks || (double)n_seq * c->view.n_kv * max_len > (double)kMaxOutputs)
+    const bool fits = (double)n_seq * c->view.n_kv * max_len <= (double)kMaxOutputs;   // (the plan's numbers then do as well)
+    if (fits) *p = attn_mass_plan(c->view, elem_type(type), n_head, n_seq, max_q, max_len);
+    if (!fits || p->blocks > kMaxBlocks)
         SMX_FAIL(SMX_EUNSUPPORTED, "%s: %d sequences of %d positions are too many outputs", fn, n_seq, max_len);
     return SMX_OK;
 }

@@ -1032,3 +1032,21 @@ def test_appends_into_their_inputs_are_refused(Q):
     assert torch.equal(out.flatten(1), f[:, :128])
     assert torch.equal(c.read(at)[1].flatten(1), f[:, 192:].half())
     c.close()
+
+
+def test_a_bound_of_new_tokens_that_says_nothing(Q):
+    """max_q 2^31 - 1, for 4096 sequences of up to 2048 positions, all but three of them empty: the plan's numbers stay in range."""
+    rng = np.random.default_rng(81)
+    n = 4096
+    B = Batch(Q, rng, BF16, BF16, 64, 8, 128, 1024, [40, 900, 0] + [0] * (n - 4) + [77], [5, 60, 0] + [0] * (n - 4) + [1])
+    tab = i32(np.concatenate([B.tables, np.full((n, 1), -1)], 1))
+    a = B.c, i32(B.starts), i32(B.lens), tab
+    want, lse = Q.attention_paged(B.q, *a, 60, 900, lse=True)
+    out, got = Q.attention_paged(B.q, *a, 2 ** 31 - 1, 2048, lse=True)
+    B.check(out, got, every=8)
+    B.check(want, lse, every=8)
+    few, many = (f64(Q.attention_mass(B.q, lse, *a, q, 2048)[[0, 1, 2, n - 1]]) for q in (60, 2 ** 31 - 1))
+    # (both add up each position's up to 480 weights in some order)
+    assert not few[2].any() and (few[1].sum() > 0) and (np.abs(few - many) <= (480 + 70) * 2.0 ** -24 * 2 * few).all()
+    assert not many[:, :, 900:].any()
+    B.c.close()
