@@ -351,10 +351,11 @@ SMX_API int smx_attention_mass_work_bytes(const smx_paged_cache *c, int type, in
  * max_len) names the pages of its positions; a page that the cache does not have is not seen.
  * q: token t at q_dev + t * q_stride, [n_head][head_dim] (n_head a multiple of n_kv_head); out_dev [n_tok][n_head][head_dim];
  * lse_dev [n_tok][n_head] or NULL: the logarithm of the sum of the exponentials of the scores seen.  Rows of no sequence are left
- * as they were; a row that sees nothing is zeros, and its lse -inf.  type: of q and out, the cache's or
+ * as they were; a row that sees nothing is zeros, and its lse -inf; any other whose query is not finite is NaN.  type: of q and out, the cache's or
  * SMX_TYPE_F32.  With fp32, queries and weights count to 22 bits over an F16 cache (the query's elements to 2^-38 of the largest
- * of their row, weights to 2^-31 of the largest where that is more) and to 24 over a BF16 one; with the cache's type weights are rounded to that.
- * Sums are fp32; scores below 2^126.  out_dev and lse_dev are not q's memory.  rules may be NULL.  work_dev: smx_attention_paged_work_bytes bytes, 16-byte aligned,
+ * of their row, weights to 2^-31 of the largest where that is more) and to 24 over a BF16 one; with the cache's type weights are rounded to that,
+ * and a cap up to 128 leaves scores off by up to 2^-21 of the cap (otherwise by some 2^-20 of themselves).
+ * Sums are fp32; scores below 2^126, and 2^8 times the sum of the values seen below 2^128.  out_dev and lse_dev are not q's memory.  rules may be NULL.  work_dev: smx_attention_paged_work_bytes bytes, 16-byte aligned,
  * free for other use when the call's work is done; calls that may overlap, replays of captured graphs among them, need one each. */
 SMX_API int smx_attention_paged(const smx_paged_cache *c, int type, const void *q_dev, int64_t q_stride, void *out_dev,
                                 float *lse_dev, int n_tok, int n_head, int n_seq, const int32_t *starts_dev,
@@ -365,7 +366,8 @@ SMX_API int smx_attention_paged(const smx_paged_cache *c, int type, const void *
  * smx_attention_paged gives it.  mass_dev: rows [n_seq * n_kv_head], mass_stride apart, of mass_width
  * floats (what lies beyond counts as 0), or NULL; mass_out_dev [n_seq][n_kv_head][max_len], 0 from lens_dev[b] on, may be mass_dev
  * itself where mass_stride is max_len.  Each sum's order is fixed.  score - lse is as good as its two terms: a weight is off by
- * some 2^-23 |lse| of itself.  work_dev: smx_attention_mass_work_bytes bytes, as above. */
+ * some 2^-23 |lse| of itself, and by 2^-21 of the cap where lse_dev is of queries of the cache's type with a cap up to 128 (the scores here
+ * are not off by that).  A row whose lse is NaN makes NaN of what it sees.  work_dev: smx_attention_mass_work_bytes bytes, as above. */
 SMX_API int smx_attention_mass(const smx_paged_cache *c, int type, const void *q_dev, int64_t q_stride,
                                const float *lse_dev, const float *mass_dev, int64_t mass_stride, int mass_width,
                                float *mass_out_dev, int n_tok, int n_head, int n_seq, const int32_t *starts_dev,
@@ -376,8 +378,9 @@ SMX_API int smx_attention_mass(const smx_paged_cache *c, int type, const void *q
  * first of equals; NaN counts as less than any number), all where there are no more.  Their rows are copied in
  * order to positions 0 .. of the pages that new_tables_dev names (new_stride * page_size >= n_keep; pages that no sequence of tables_dev reads, no
  * page twice), kept_dev [n_seq][n_kv_head][n_keep] receives which they were (-1 beyond), new_lens_dev [n_seq] how
- * many, new_mass_dev as kept_dev their weights (0 beyond).  The old pages are left as they are.  Positions then
- * no longer say how far apart tokens are: a window or slopes count in what was kept. */
+ * many, new_mass_dev as kept_dev their weights (0 beyond).  The old pages are left as they are.  Rows of a page that the cache does not have are
+ * copied as zeros, which are seen from then on; rows to one are not written.  Positions then
+ * no longer say how far apart tokens are: a window, a prefix or slopes count in what was kept. */
 SMX_API int smx_paged_evict(smx_paged_cache *c, const float *mass_dev, int64_t mass_stride, const int32_t *lens_dev,
                             int n_seq, int max_len, int n_keep, int n_recent, const int32_t *tables_dev, int table_stride,
                             const int32_t *new_tables_dev, int new_stride, int32_t *kept_dev, int32_t *new_lens_dev,

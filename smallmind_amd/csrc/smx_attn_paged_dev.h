@@ -323,7 +323,7 @@ struct LaneAt {
 static_assert(W % 64 == 0 || W == 32 || W == 96, "pg_unit turns whole sets of units");
 
 // ---- scores ----------------------------------------------------------------------------------------
-// tanh: its series below 0.4 (the next term is less than 2^-24 of the value there), else by an exponential.
+// tanh: its series below 0.4 (the next term is 6.4e-8, some 2^-24, of the value there), else by an exponential.
 __device__ __forceinline__ float tanh_of(float y)
 {
     const float t = fabsf(y), z = y * y;

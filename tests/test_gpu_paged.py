@@ -1050,3 +1050,24 @@ def test_a_bound_of_new_tokens_that_says_nothing(Q):
     assert not few[2].any() and (few[1].sum() > 0) and (np.abs(few - many) <= (480 + 70) * 2.0 ** -24 * 2 * few).all()
     assert not many[:, :, 900:].any()
     B.c.close()
+
+
+@pytest.mark.parametrize("cache,io", [(F16, F16), (BF16, BF16), (F16, F32)])
+@pytest.mark.parametrize("lens,new", [([300, 65], [1, 3]), ([260, 97], [130, 40])])
+def test_received_weights_by_the_attentions_own_sums(Q, cache, io, lens, new):
+    """With a cap, 16-bit queries' lse is off by 2^-21 of it where the weights' scores are not: a weight by as much of itself."""
+    rng = np.random.default_rng(78)
+    for rules in (dict(cap=50.0), dict(cap=30.0, scale=0.5, window=60), dict(slopes=np.array([0.3, 0.1, 0.02, 0.0], np.float32))):
+        B = Batch(Q, rng, cache, io, 4, 2, 64, 16, lens, new)
+        _, lse = run(Q, B, rules)
+        got = f64(Q.attention_mass(B.q, lse, *B.args(), **kernel_rules(rules)))
+        for b in range(len(lens)):
+            want, bound = np.zeros((2, B.max_len)), np.zeros((2, B.max_len))
+            for h, head, S, see in B.rows(b, **rules):
+                _, _, l, le = R.attention(S, B.v[b][:, h], see, io, cache)
+                w, e = R.received(S, l, see)
+                each = np.where(see, np.exp(S.s - l[:, None]), 0.0)
+                want[h, :lens[b]] += w
+                bound[h, :lens[b]] += e + le @ each + 2.0 ** -24 * w * 4
+            close(torch.from_numpy(got[b]), want, bound)
+        B.c.close()
