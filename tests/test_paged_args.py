@@ -187,3 +187,28 @@ def test_structs_are_laid_out_as_in_the_header(tmp_path):
     for c in structs.values():
         want += [ctypes.sizeof(c)] + [getattr(c, f).offset for f, _ in c._fields_]
     assert got == want
+
+
+def test_the_documented_calls_fit_the_binding():
+    """The C# sample of the paged operators: each call's arguments by number and kind, and names that the binding has."""
+    import os
+    import re
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    cs = open(os.path.join(root, "smallmind_amd", "bindings", "csharp", "Smx.cs")).read()
+    text = open(os.path.join(root, "INTEGRATION.md")).read()
+    block = next(b for b in re.findall(r"```csharp\n(.*?)```", text, re.S) if "smx_paged_cache_create" in b)
+    block = re.sub(r"//[^\n]*", "", block)
+    assert "SMX_TYPE" not in block
+    for struct, field in (("Rotation", "CosDev SinDev NPos NRot Halves NAxes"), ("AttentionRules", "Window")):
+        body = re.search(r"public struct %s\b.*?\n        \}" % struct, cs, re.S).group(0)
+        used = re.search(r"new %s \{(.*?)\}" % struct, block).group(1)
+        assert re.findall(r"(\w+) =", used) == field.split() and all(re.search(r"\b%s\b" % f, body) for f in field.split())
+    calls = re.findall(r"(smx_\w+)\((.*?)\);", block, re.S)
+    assert len(calls) == 7
+    for name, args in calls:
+        params = re.search(r"extern int %s\((.*?)\);" % name, cs, re.S).group(1).split(",")
+        args = args.split(",")
+        assert len(args) == len(params), name
+        for a, p in zip(args, params):
+            kinds = [w for w in ("ref", "out", "in") if w in p.split()], [w for w in ("ref", "out", "in") if w in a.split()]
+            assert kinds[0] == kinds[1], (name, a, p)
