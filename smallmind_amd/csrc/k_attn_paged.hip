@@ -20,12 +20,12 @@
 //     registers, V to LDS of its own; the waves join their sums at the end.
 //
 // What bounds it.  Many rows of 128 dims: the matrix cores, at the clock that the card's power leaves them (2048 tokens over
-// 32768 positions, 32 heads over 8, bf16: 980 to 1090 us, 980 to 1090 TFLOP/s, where the library's product of 8192^3 reaches
-// 1160 to 1220).  64 dims: the vector unit's 32 exponentials and some 110 other instructions of a wave's tile beside 16 matrix
-// instructions (4096 over 16384, 32 heads over 8: 620 us, 780 TFLOP/s); a cap adds 5 instructions, two of them transcendental,
+// 32768 positions, 32 heads over 8, bf16: 970 to 1090 us, 980 to 1100 TFLOP/s, where the library's product of 8192^3 reaches
+// 1160 to 1225).  64 dims: the vector unit's 32 exponentials and some 110 other instructions of a wave's tile beside 16 matrix
+// instructions (4096 over 16384, 32 heads over 8: 585 to 620 us, 780 to 820 TFLOP/s); a cap adds 5 instructions, two of them transcendental,
 // to each of 32 scores, slopes 3.  Short prompts: the way in and out of a block and the tiles that the diagonal cuts (4 of
-// 1023, 12 heads of 64: 28 us).  fp32 queries over an F16 cache: twice the matrix instructions and the splitting of weights
-// (512 over 4096, 32 heads over 4 of 64: 49 us and 6 of the join).  Few rows: memory (64 sequences of up to 8192 positions, 8
+// 1023, 12 heads of 64: 23 us).  fp32 queries over an F16 cache: twice the matrix instructions and the splitting of weights
+// (512 over 4096, 32 heads over 4 of 64: 49 us with the join's 6; over a BF16 cache, three times, 71).  Few rows: memory (64 sequences of up to 8192 positions, 8
 // heads of 128: 242 us, 5.6 TB/s), in short contexts the chain from page table to rows to the waves' joining (700 positions:
 // 10.6 us).
 #include "smx_attn_paged_dev.h"

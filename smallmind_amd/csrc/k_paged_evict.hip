@@ -14,7 +14,7 @@
 // number was found bit by bit with ballots, 21 us with 8-bit digits and positions in order of the threads).
 // Copying: a lane per 16-byte unit, rows anywhere in the pages.  By the workgroup that chose where that is at most 128 KB of new
 // rows, so that a second launch is spared (64 KB: 11.2 us for 8.9 + 3.4); by a launch of its own above (1 MB: 118 us for
-// 18.6 + 52, of which 52 are 270 MB read and as much written at 5.2 TB/s, a large copy's rate).
+// 18.6 + 52, of which 52 are 134 MB read and as much written at 5.2 TB/s, a large copy's rate).
 #include "smx_device.h"
 #include "smx_internal.h"
 

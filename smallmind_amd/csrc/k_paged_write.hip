@@ -10,8 +10,8 @@
 // L1 they have just come to), which leaves head_dim and the rotated width free of any rule on lanes.  A work item is one
 // query row, or one K row with its V row: whether V is finite decides what K holds.
 //
-// What bounds it.  Memory (16383 tokens, 32 + 8 + 8 heads of 128, bf16: 97 to 101 us for 403 MB, 4.0 to 4.2 TB/s, where a large
-// copy reaches 4.85; reading back 134 MB 21.7 us).  Few tokens: the chain from position to angle to row (16 tokens, 32 + 4 + 4
+// What bounds it.  Memory (16383 tokens, 32 + 8 + 8 heads of 128, bf16: 95 to 100 us for 403 MB, 4.0 to 4.2 TB/s, where a large
+// copy reaches 4.9; reading back 134 MB 21.7 us; queries and keys without a cache 86 us for 336 MB).  Few tokens: the chain from position to angle to row (16 tokens, 32 + 4 + 4
 // heads of 64: 5.6 us).  bf16 rows leave registers for four waves on a SIMD; with three the first takes 13 us more.
 #include <algorithm>
 
