@@ -136,7 +136,7 @@ int check_apart(const PgWriteArgs &a, int type, const char *fn)
                      (a.k && meet(o, n, a.k, a.n_tok, a.k_stride, a.n_kv * hd, in)) ||
                      (a.v && meet(o, n, a.v, a.n_tok, a.v_stride, a.n_kv * hd, in)));
     };
-    if (met(a.q ? a.q_out : nullptr, a.n_head) || met(a.k_out, a.n_kv)) SMX_FAIL(SMX_EINVAL, "%s: an output lies in the inputs' memory", fn);
+    if (met(a.q ? a.q_out : nullptr, a.n_head) || met(a.k ? a.k_out : nullptr, a.n_kv)) SMX_FAIL(SMX_EINVAL, "%s: an output lies in the inputs' memory", fn);
     return SMX_OK;
 }
 

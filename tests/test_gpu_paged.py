@@ -1016,6 +1016,17 @@ def test_outputs_in_the_inputs_memory_are_refused(Q):
     B.c.close()
 
 
+def test_outputs_of_rows_that_are_not_there_are_not_looked_at(Q):
+    from smallmind_amd import _lib
+    f, out = torch.randn(3, 2, 64, device="cuda"), torch.zeros(3, 2, 64, device="cuda")
+    s = torch.cuda.current_stream().cuda_stream
+    for q, k in ((f.data_ptr(), None), (None, f.data_ptr())):     # (the other's output names the input)
+        qo, ko = (out.data_ptr(), f.data_ptr()) if q else (f.data_ptr(), out.data_ptr())
+        out.zero_()
+        _lib.call("smx_qk_norm_rope", 0, q, 128, 2, k, 128, 2, 64, None, None, 0.0, None, None, 3, 0, qo, ko, s)
+        assert torch.equal(out, f)
+
+
 def test_appends_into_their_inputs_are_refused(Q):
     from smallmind_amd import _lib
     lib, s = _lib.load(), torch.cuda.current_stream().cuda_stream
