@@ -365,7 +365,7 @@ SMX_API int smx_attention_paged(const smx_paged_cache *c, int type, const void *
  * mass_out[b][h][p] = mass[b][h][p] + the sum over b's new tokens and h's query heads of exp(score - lse), with lse_dev as
  * smx_attention_paged gives it.  mass_dev: rows [n_seq * n_kv_head], mass_stride apart, of mass_width
  * floats (what lies beyond counts as 0), or NULL; mass_out_dev [n_seq][n_kv_head][max_len], 0 from lens_dev[b] on, may be mass_dev
- * itself where mass_stride is max_len.  Each sum's order is fixed.  score - lse is as good as its two terms: a weight is off by
+ * itself where mass_stride is max_len (and not otherwise overlap it).  Each sum's order is fixed.  score - lse is as good as its two terms: a weight is off by
  * some 2^-23 |lse| of itself, and by 2^-21 of the cap where lse_dev is of queries of the cache's type with a cap up to 128 (the scores here
  * are not off by that).  A row whose lse is NaN makes NaN of what it sees.  work_dev: smx_attention_mass_work_bytes bytes, as above. */
 SMX_API int smx_attention_mass(const smx_paged_cache *c, int type, const void *q_dev, int64_t q_stride,
@@ -378,7 +378,8 @@ SMX_API int smx_attention_mass(const smx_paged_cache *c, int type, const void *q
  * first of equals; NaN counts as less than any number), all where there are no more.  Their rows are copied in
  * order to positions 0 .. of the pages that new_tables_dev names (new_stride * page_size >= n_keep; pages that no sequence of tables_dev reads, no
  * page twice), kept_dev [n_seq][n_kv_head][n_keep] receives which they were (-1 beyond), new_lens_dev [n_seq] how
- * many, new_mass_dev as kept_dev their weights (0 beyond).  The old pages are left as they are.  Rows of a page that the cache does not have are
+ * many, new_mass_dev as kept_dev their weights (0 beyond).  The outputs are not the inputs' memory
+ * (new_lens_dev not lens_dev).  The old pages are left as they are.  Rows of a page that the cache does not have are
  * copied as zeros, which are seen from then on; rows to one are not written.  Positions then
  * no longer say how far apart tokens are: a window, a prefix or slopes count in what was kept. */
 SMX_API int smx_paged_evict(smx_paged_cache *c, const float *mass_dev, int64_t mass_stride, const int32_t *lens_dev,

@@ -441,6 +441,9 @@ SMX_API int smx_attention_mass(const smx_paged_cache *c, int type, const void *q
     if (mass_dev == mass_out_dev && mass_stride != max_len) SMX_FAIL(SMX_EINVAL, "%s: in place, rows of mass must be max_len apart", fn);
     if (misaligned(lse_dev, 4) || misaligned(mass_dev, 4) || misaligned(mass_out_dev, 4)) SMX_FAIL(SMX_EINVAL, "%s: misaligned pointer", fn);
     if (max_len == 0) return SMX_OK;
+    const int64_t pairs = (int64_t)n_seq * c->view.n_kv;
+    if (mass_dev && mass_dev != mass_out_dev && mass_width > 0 && meet(mass_out_dev, pairs * max_len * 4, mass_dev, pairs, mass_stride, mass_width, 4))
+        SMX_FAIL(SMX_EINVAL, "%s: mass and mass_out overlap", fn);
     MassPgPlan p;
     if ((rc = plan_mass(c, type, n_head, n_seq, max_q, max_len, fn, &p)) != SMX_OK) return rc;
     if ((rc = check_work(work_dev, work_bytes, p.work_bytes, fn)) != SMX_OK) return rc;
@@ -474,6 +477,15 @@ SMX_API int smx_paged_evict(smx_paged_cache *c, const float *mass_dev, int64_t m
     if (misaligned(mass_dev, 4) || misaligned(lens_dev, 4) || misaligned(tables_dev, 4) || misaligned(new_tables_dev, 4) ||
         misaligned(kept_dev, 4) || misaligned(new_lens_dev, 4) || misaligned(new_mass_dev, 4))
         SMX_FAIL(SMX_EINVAL, "%s: misaligned pointer", fn);
+    // (a head's workgroup may be done before another of the same sequence begins)
+    const int64_t pairs = (int64_t)n_seq * c->view.n_kv, kept = pairs * n_keep * 4;
+    const auto met = [&](const void *o, int64_t bytes) {
+        return meet(o, bytes, mass_dev, pairs, mass_stride, max_len, 4) || meet(o, bytes, lens_dev, 1, n_seq, n_seq, 4) ||
+               meet(o, bytes, tables_dev, 1, 1, (int64_t)n_seq * table_stride, 4) ||
+               meet(o, bytes, new_tables_dev, 1, 1, (int64_t)n_seq * new_stride, 4);
+    };
+    if (met(kept_dev, kept) || met(new_lens_dev, (int64_t)n_seq * 4) || met(new_mass_dev, kept))
+        SMX_FAIL(SMX_EINVAL, "%s: an output lies in the inputs' memory", fn);
     const int rc = check_device(c, fn);
     if (rc != SMX_OK) return rc;
     PgEvictArgs a{};

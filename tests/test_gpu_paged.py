@@ -1082,3 +1082,39 @@ def test_received_weights_by_the_attentions_own_sums(Q, cache, io, lens, new):
                 bound[h, :lens[b]] += e + le @ each + 2.0 ** -24 * w * 4
             close(torch.from_numpy(got[b]), want, bound)
         B.c.close()
+
+
+def test_evictions_and_received_weights_over_their_inputs_are_refused(Q):
+    from smallmind_amd import _lib
+    lib, s = _lib.load(), torch.cuda.current_stream().cuda_stream
+    rng = np.random.default_rng(82)
+    B = Batch(Q, rng, F16, F16, 4, 2, 64, 16, [40, 30], [2, 1], extra_pages=8)
+    i = i32(np.zeros(256))
+    m = dev(rng.uniform(0, 1, (2, 2, 48)).astype(np.float32))
+    lens, tab, new = i32(B.lens), i32(B.tables), i32(np.full((2, 1), -1))
+
+    def evict(kept=i.data_ptr(), left=i.data_ptr() + 512, mass=i.data_ptr() + 600):
+        return lib.smx_paged_evict(B.c._h, m.data_ptr(), 48, lens.data_ptr(), 2, 40, 8, 2, tab.data_ptr(), 3, new.data_ptr(), 1, kept, left, mass, s)
+    for bad in (dict(left=lens.data_ptr()), dict(mass=m.data_ptr()), dict(mass=m.data_ptr() + 4 * (3 * 48 + 39)), dict(kept=tab.data_ptr()),
+                dict(kept=new.data_ptr()), dict(kept=lens.data_ptr() - 124)):
+        assert evict(**bad) == -1 and b"lies in the inputs' memory" in lib.smx_last_error(), bad
+    assert evict() == 0
+    got = i.cpu().numpy()
+    assert got[128:130].tolist() == [8, 8]
+    for b in range(2):
+        for h in range(2):
+            assert got[:32].reshape(2, 2, 8)[b, h].tolist() == R.evict(m[b, h].cpu().numpy(), B.lens[b], 8, 2)
+
+    _, lse = run(Q, B)
+    c, st, le, ta, mq, ml = B.args()
+    out = torch.zeros(2 * 2 * 40 + 64, device="cuda")
+    was = out[:2 * 2 * 30]
+
+    def mass(to, width=30, stride=30):
+        return lib.smx_attention_mass(B.c._h, 1, B.q.data_ptr(), B.q.stride(0), lse.data_ptr(), was.data_ptr(), stride, width, to, 3, 4, 2, st.data_ptr(),
+                                      le.data_ptr(), ta.data_ptr(), ta.shape[1], mq, ml, None, None, 0, s)
+    for to in (was.data_ptr() + 4, was.data_ptr() + 4 * 119):
+        assert mass(to) == -1 and b"overlap" in lib.smx_last_error()
+    assert mass(m.data_ptr()) == 0 and mass(was.data_ptr(), 40, 40) == 0
+    assert torch.equal(m.flatten()[:160], out[:160])
+    B.c.close()
